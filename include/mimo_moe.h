@@ -50,7 +50,8 @@ enum {
   MIMO_ERR_SLOT = -4,             /* an expert has no resident slot / slot id out of range */
   MIMO_ERR_WORKSPACE = -5,        /* workspace missing or too small */
   MIMO_ERR_HIP = -6,              /* a HIP runtime call or kernel launch failed */
-  MIMO_ERR_ARG = -7               /* null pointer or invalid argument */
+  MIMO_ERR_ARG = -7,              /* null pointer or invalid argument */
+  MIMO_ERR_PAGES = -8             /* a step needs more pages than are free (device status) */
 };
 
 /* One MoE layer's expert slot pool (model.py:32-45 alloc_bank; pool dict keys of kernels.py:176-193). */
@@ -225,6 +226,66 @@ int mimo_moe_layer_decode_noalloc(const uint16_t* x, int M, const uint16_t* norm
                                   const float* bias, const int32_t* slot_of, int E, int k, const mimo_bank* bank,
                                   uint16_t* h, uint16_t* r_out, int32_t* inds_out, float* w_out,
                                   int32_t* status_out, void* stream);
+
+/* ---------------------------------------------------------------- the attention half's paged cache */
+
+/* One layer's K/V cache: n_pages pages of page_size tokens (a power of two, 16 to 1024), each page with one contiguous
+ * [page_size, dim] block per K/V head.  A slot is page * page_size + row, at most 2^31 - 1 of them.  Head dimensions
+ * (k_dim / v_dim): 64/64, 128/128, 192/128.  An E4M3 cache holds value / scale, scales fp32 [kv_heads].  (The reference's
+ * KVCache and RotatingKVCache, engine/mimo_stream/model.py:169-170, hold one request each.) */
+enum { MIMO_KV_BF16 = 0, MIMO_KV_E4M3 = 1 };
+typedef struct mimo_kv_cache {
+  void* k;                 /* [n_pages, kv_heads, page_size, k_dim] bf16 or E4M3 */
+  void* v;                 /* [n_pages, kv_heads, page_size, v_dim] */
+  const float* k_scale;    /* fp32 [kv_heads], E4M3 only */
+  const float* v_scale;
+  int32_t dtype, n_pages, page_size, kv_heads, k_dim, v_dim;
+} mimo_kv_cache;
+
+/* Page tables, slots and positions of one step from request lengths, on the device.  State: lens [B] (B up to 4096),
+ * table [B, max_pages] page ids (entry j holds tokens j * page_size ..), free_pages [n_pages] a stack of which the first
+ * n_free [1] entries are free.  Request b goes from lens[b] to target[b] tokens: growing takes pages off the stack (requests
+ * in order), shrinking (0 ends a request) puts pages back first, so that a step and its inverse leave the stack as it was.
+ * Outputs: lens_out [B], n_free_out [1], starts [B + 1] (the new tokens of request b are rows starts[b] .. starts[b + 1] - 1
+ * of the step), slots [N] and positions [N] of the new tokens, rows behind the last one -1 and 0.  table entries of grown
+ * requests and stack entries at and above n_free are written in place; they mean nothing under the old lengths, so a step
+ * whose outputs are dropped leaves the state as it was.  commit_lens / commit_n_free (both or neither; lens and n_free
+ * themselves, as a rule) receive the new lengths and count after everything else.  status [1] is overwritten: MIMO_OK,
+ * MIMO_ERR_PAGES when too few pages are free, MIMO_ERR_SHAPE when a length is outside [0, max_pages * page_size], a request
+ * grows by more than max_new, the new tokens are more than N (at most 2^20) or n_free and the table disagree; then starts
+ * are 0, slots -1, and lens_out / n_free_out the old state. */
+int mimo_cache_step(const int32_t* lens, const int32_t* target, int B, int32_t* table, int max_pages,
+                    int32_t* free_pages, const int32_t* n_free, int n_pages, int page_size, int N, int max_new,
+                    int32_t* lens_out, int32_t* n_free_out, int32_t* starts, int32_t* slots, int32_t* positions,
+                    int32_t* commit_lens, int32_t* commit_n_free, int32_t* status, void* stream);
+
+/* Rotary positions on q and k (the first rotary_dim dimensions of a head, pairs (i, i + rotary_dim / 2); the reference's
+ * partial RoPE, engine/mimo_stream/mimo_v2.py:66-150) and the write of k and v to their slots.  q bf16 [N, heads, k_dim] (NULL:
+ * none), k [N, kv_heads, k_dim], v [N, kv_heads, v_dim], tokens *_stride elements apart (multiples of 8); turns fp64
+ * [rotary_dim / 2]: turns per position of each pair (frequency / 2 pi).  q_out bf16 [N, heads, k_dim] may not alias q.  A slot
+ * below 0 writes no k and v; slots are distinct otherwise.  Rotated values are rounded once, to bf16 or (divided by their
+ * head's scale, clamped to +-448) to E4M3.  status (optional) receives MIMO_ERR_SLOT for a slot past the cache, which is
+ * skipped; it is not cleared. */
+int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k, int64_t k_stride,
+                      const uint16_t* v, int64_t v_stride, int N, const int32_t* positions, const int32_t* slots,
+                      const mimo_kv_cache* cache, int rotary_dim, const double* turns, uint16_t* q_out,
+                      int32_t* status, void* stream);
+
+/* Attention of a step's new tokens over the paged cache that already holds their keys and values (the reference's
+ * Attention with its causal and sliding-window masks and sinks, engine/mimo_stream/mimo_v2.py:110-150).  Row n of request b
+ * (starts[b] <= n < starts[b + 1]) is position p = lens[b] - starts[b + 1] + n and sees the keys j <= p of its request; with
+ * window > 0 those with p - j < window, and the first sink_tokens.  out[n, h] = sum_j w_j v_j / (sum_j w_j + w_sink), w_j =
+ * exp(scale q.k_j - m), w_sink = exp(sink_logits[h] - m) (NULL: none); a row whose weights sum to 0 gives 0.  Masked keys and
+ * values are not looked at: they may be NaN.  heads is a multiple of kv_heads, q bf16 [N, heads, k_dim] with tokens q_stride
+ * elements apart, out bf16 [N, heads, v_dim]; rows that belong to no request are set to 0.  max_new: no request has more new
+ * tokens (it picks the kernel; results do not depend on it).  status (optional, not cleared) receives MIMO_ERR_SLOT for a
+ * page id outside the cache (page 0 is read) and MIMO_ERR_SHAPE for a request whose lens is below its rows or past max_pages
+ * (its rows are 0). */
+int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, const mimo_kv_cache* cache, int B,
+                      const int32_t* starts, const int32_t* lens, const int32_t* table, int max_pages, int max_new,
+                      float scale, int window, int sink_tokens, const float* sink_logits, uint16_t* out,
+                      int32_t* status, void* ws, size_t ws_bytes, void* stream);
+size_t mimo_cache_attend_workspace_size(int N, int heads, int kv_heads, int v_dim);
 
 /* ---------------------------------------------------------------- measurement */
 

@@ -14,7 +14,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "mimo_stream", "libmimo_moe.so")
-SOURCES = ["codec.hip", "router.hip", "decode.hip", "prefill.hip", "layer.hip"]
+SOURCES = ["codec.hip", "router.hip", "decode.hip", "prefill.hip", "layer.hip", "cache.hip", "attend.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # -fconstexpr-steps: the bf16 sigmoid table (csrc/sigmoid_table.h) is evaluated by the compiler, ~7M steps
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fconstexpr-steps=100000000",

@@ -13,6 +13,7 @@ ABI_VERSION = 2
 
 MIMO_OK = 0
 ERR_SHAPE, ERR_ALIGN, ERR_ROWS_PER_EXPERT, ERR_SLOT, ERR_WORKSPACE, ERR_HIP, ERR_ARG = -1, -2, -3, -4, -5, -6, -7
+ERR_PAGES = -8
 _VALUE_ERRORS = {ERR_SHAPE, ERR_ALIGN, ERR_ROWS_PER_EXPERT, ERR_SLOT, ERR_WORKSPACE, ERR_ARG}
 
 
@@ -24,6 +25,14 @@ class MimoBank(ctypes.Structure):
                 ("n_slots", ctypes.c_int32), ("hidden", ctypes.c_int32), ("inter", ctypes.c_int32)]
 
 
+class MimoKvCache(ctypes.Structure):
+    """struct mimo_kv_cache (include/mimo_moe.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+                ("dtype", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("kv_heads", ctypes.c_int32), ("k_dim", ctypes.c_int32), ("v_dim", ctypes.c_int32)]
+
+
 P = ctypes.c_void_p
 I32 = ctypes.c_int32
 I64 = ctypes.c_int64
@@ -31,6 +40,7 @@ U64 = ctypes.c_uint64
 F32 = ctypes.c_float
 SZ = ctypes.c_size_t
 BANKP = ctypes.POINTER(MimoBank)
+CACHEP = ctypes.POINTER(MimoKvCache)
 
 SIGNATURES = {
     "mimo_abi_version": (I32, []),
@@ -63,6 +73,10 @@ SIGNATURES = {
     "mimo_moe_layer_prefill": (I32, [P, I32, P, F32, P, P, P, I32, I32, BANKP, P, P, P, P, P, P, SZ, P]),
     "mimo_moe_layer_prefill_workspace_size": (SZ, [I32, I32, I32, I32, I32, I32]),
     "mimo_moe_layer_decode_noalloc": (I32, [P, I32, P, F32, P, P, P, I32, I32, BANKP, P, P, P, P, P, P]),
+    "mimo_cache_step": (I32, [P, P, I32, P, I32, P, P, I32, I32, I32, I32, P, P, P, P, P, P, P, P, P]),
+    "mimo_cache_append": (I32, [P, I64, I32, P, I64, P, I64, I32, P, P, CACHEP, I32, P, P, P, P]),
+    "mimo_cache_attend": (I32, [P, I64, I32, I32, CACHEP, I32, P, P, P, I32, I32, F32, I32, I32, P, P, P, P, SZ, P]),
+    "mimo_cache_attend_workspace_size": (SZ, [I32, I32, I32, I32]),
     "mimo_profile_enable": (I32, [I32]),
     "mimo_profile_read": (I32, [I32, P, P, P]),
 }

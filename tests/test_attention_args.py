@@ -1,0 +1,146 @@
+"""Refusals of the paged-cache operators that need no GPU: wrong shapes, types and devices never reach a launch."""
+import ctypes
+import os
+
+import pytest
+import torch
+
+from mimo_stream import KVCache, PageTable, Rotary, StepPlan, _lib, append, attend
+
+pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libmimo_moe.so not built")
+
+BF = torch.bfloat16
+
+
+def _cache(**kw):
+    return KVCache(3, 16, 2, 64, 64, device="cpu", **kw)
+
+
+def test_page_table_arguments():
+    for bad in (dict(page_size=8), dict(page_size=48), dict(page_size=2048), dict(max_seqs=0), dict(max_pages=0), dict(n_pages=0)):
+        with pytest.raises(ValueError):
+            PageTable(**{**dict(max_seqs=2, max_pages=4, n_pages=8, page_size=16, device="cpu"), **bad})
+    pt = PageTable(2, 4, 8, 16, device="cpu")
+    assert pt.n_free.item() == 8 and sorted(pt.free.tolist()) == list(range(8))
+    with pytest.raises(ValueError, match="device tensors"):
+        pt.step(torch.zeros(2, dtype=torch.int32), 1)
+
+
+def test_cache_arguments():
+    with pytest.raises(ValueError):
+        KVCache(3, 16, 2, 64, 128, device="cpu")
+    with pytest.raises(ValueError):
+        KVCache(3, 24, 2, 64, 64, device="cpu")
+    with pytest.raises(ValueError):
+        KVCache(3, 16, 2, 64, 64, dtype=torch.float16, device="cpu")
+    with pytest.raises(ValueError, match="scale"):
+        KVCache(3, 16, 2, 64, 64, dtype=torch.float8_e4m3fn, device="cpu")
+    with pytest.raises(ValueError, match="scales"):
+        _cache(k_scale=1.0, v_scale=1.0)
+    c = KVCache(3, 16, 2, 64, 64, dtype=torch.float8_e4m3fn, k_scale=0.5, v_scale=[0.25, 1.0], device="cpu")
+    assert c.k.dtype == torch.float8_e4m3fn and c.k_scale.tolist() == [0.5, 0.5] and c.v_scale.tolist() == [0.25, 1.0]
+    k = torch.zeros(3, 2, 16, 64, dtype=BF)
+    with pytest.raises(ValueError):
+        KVCache.of(k, torch.zeros(3, 2, 32, 64, dtype=BF))
+    with pytest.raises(ValueError, match="contiguous"):
+        KVCache.of(k.transpose(1, 2).contiguous().transpose(1, 2), k)
+
+
+def test_rotary_arguments():
+    for dim in (0, 8, 24, 272):
+        with pytest.raises(ValueError):
+            Rotary(dim, device="cpu")
+    with pytest.raises(ValueError):
+        Rotary(64, theta=0.0, device="cpu")
+
+
+def test_cpu_tensors_are_refused():
+    c = _cache()
+    plan = StepPlan(starts=torch.zeros(2, dtype=torch.int32), lens=torch.zeros(1, dtype=torch.int32),
+                    table=torch.zeros(1, 1, dtype=torch.int32), slots=torch.zeros(1, dtype=torch.int32),
+                    positions=torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="device tensors"):
+        append(c, plan, torch.zeros(1, 2, 64, dtype=BF), torch.zeros(1, 2, 64, dtype=BF))
+    with pytest.raises(ValueError, match="device tensors"):
+        attend(torch.zeros(1, 2, 64, dtype=BF), c, plan)
+
+
+# ---- the C entries check on the host before any HIP call
+HOST = ctypes.create_string_buffer(4096)
+ADDR = (ctypes.addressof(HOST) + 255) // 256 * 256
+
+
+def _kv(**kw):
+    f = dict(k=ADDR, v=ADDR, k_scale=None, v_scale=None, dtype=0, n_pages=4, page_size=16, kv_heads=2, k_dim=64, v_dim=64)
+    f.update(kw)
+    return _lib.MimoKvCache(*(f[n] for n, _ in _lib.MimoKvCache._fields_))
+
+
+BAD_CACHES = [(dict(k=None), "ARG"), (dict(dtype=2), "ARG"), (dict(dtype=1), "ARG"), (dict(k_dim=96), "SHAPE"), (dict(v_dim=128), "SHAPE"),
+              (dict(page_size=8), "SHAPE"), (dict(page_size=100), "SHAPE"), (dict(kv_heads=0), "SHAPE"), (dict(n_pages=0), "SHAPE"),
+              (dict(n_pages=1 << 28), "SHAPE"), (dict(v=ADDR + 2), "ALIGN")]
+
+
+def _step(**kw):
+    f = dict(lens=ADDR, target=ADDR, B=1, table=ADDR, max_pages=1, free=ADDR, n_free=ADDR, n_pages=1, page_size=16, N=1, max_new=1,
+             lens_out=ADDR + 64, n_free_out=ADDR + 64, starts=ADDR, slots=ADDR, positions=ADDR, cl=None, cn=None, status=ADDR, stream=None)
+    f.update(kw)
+    return _lib.load().mimo_cache_step(*f.values())
+
+
+@pytest.mark.parametrize("bad,code", [(dict(lens=None), "ARG"), (dict(status=None), "ARG"), (dict(slots=None), "ARG"), (dict(B=0), "SHAPE"),
+                                      (dict(B=4097), "SHAPE"), (dict(N=-1), "SHAPE"), (dict(N=(1 << 20) + 1), "SHAPE"),
+                                      (dict(max_new=-1), "SHAPE"), (dict(page_size=17), "SHAPE"), (dict(n_pages=1 << 28), "SHAPE"),
+                                      (dict(lens_out=ADDR), "ARG"), (dict(cl=ADDR), "ARG"), (dict(max_pages=1 << 28), "SHAPE")])
+def test_step_refusals(bad, code):
+    assert _step(**bad) == getattr(_lib, "ERR_" + code)
+
+
+def _append(cache=None, **kw):
+    f = dict(q=ADDR, qs=128, heads=2, k=ADDR, ks=128, v=ADDR, vs=128, N=1, positions=ADDR, slots=ADDR, cache=cache or _kv(), dim=16,
+             turns=ADDR, q_out=ADDR, status=None, stream=None)
+    f.update(kw)
+    return _lib.load().mimo_cache_append(*f.values())
+
+
+@pytest.mark.parametrize("bad,code", [(dict(k=None), "ARG"), (dict(q_out=None), "ARG"), (dict(turns=None), "ARG"), (dict(dim=24), "SHAPE"),
+                                      (dict(dim=80), "SHAPE"), (dict(N=-1), "SHAPE"), (dict(ks=120), "SHAPE"), (dict(vs=132), "ALIGN"),
+                                      (dict(q=ADDR + 8), "ALIGN"), (dict(heads=0), "SHAPE")])
+def test_append_refusals(bad, code):
+    assert _append(**bad) == getattr(_lib, "ERR_" + code)
+
+
+def _attend(cache=None, **kw):
+    f = dict(q=ADDR, qs=128, N=1, heads=2, cache=cache or _kv(), B=1, starts=ADDR, lens=ADDR, table=ADDR, max_pages=1, max_new=1, scale=1.0,
+             window=0, sinks=0, logits=None, out=ADDR, status=None, ws=ADDR, bytes=1 << 40, stream=None)
+    f.update(kw)
+    return _lib.load().mimo_cache_attend(*f.values())
+
+
+@pytest.mark.parametrize("bad,code", [(dict(q=None), "ARG"), (dict(table=None), "ARG"), (dict(heads=3), "SHAPE"), (dict(heads=0), "SHAPE"),
+                                      (dict(N=-1), "SHAPE"), (dict(B=0), "SHAPE"), (dict(max_pages=0), "SHAPE"), (dict(window=-1), "SHAPE"),
+                                      (dict(sinks=-1), "SHAPE"), (dict(scale=float("nan")), "ARG"), (dict(scale=float("inf")), "ARG"),
+                                      (dict(qs=64), "SHAPE"), (dict(out=ADDR + 8), "ALIGN"), (dict(ws=None), "WORKSPACE"),
+                                      (dict(bytes=0), "WORKSPACE")])
+def test_attend_refusals(bad, code):
+    assert _attend(**bad) == getattr(_lib, "ERR_" + code)
+
+
+@pytest.mark.parametrize("bad,code", BAD_CACHES)
+def test_cache_refusals(bad, code):
+    assert _append(_kv(**bad)) == getattr(_lib, "ERR_" + code)
+    assert _attend(_kv(**bad)) == getattr(_lib, "ERR_" + code)
+
+
+def test_empty_calls_need_no_gpu():
+    assert _append(N=0) == 0 and _attend(N=0) == 0
+
+
+def test_attend_workspace_never_falls():
+    size = _lib.load().mimo_cache_attend_workspace_size
+    for heads, kv, dv in ((64, 4, 128), (5, 5, 64), (64, 1, 128)):
+        last = 0
+        for n in list(range(1, 70)) + [127, 128, 129, 1000, 4096, 65536]:
+            need = size(n, heads, kv, dv)
+            assert need >= last
+            last = need
