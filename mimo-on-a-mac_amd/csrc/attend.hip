@@ -1,77 +1,793 @@
-// Attention of a step's new tokens over the paged K/V cache (mimo_cache_attend).
+// Attention of a step's new tokens over the paged K/V cache (mimo_cache_attend; the reference's Attention,
+// engine/mimo_stream/mimo_v2.py:110-150, on one request's cache).
+//
+// Rows.  The queries that share a K/V head (its G heads, one after another, of consecutive tokens) are the rows of a tile, so
+// a key or value is read once for all of them: narrow tiles of 32 rows for requests with few rows (decode), wide tiles of 128.
+//
+// One pass over the keys with the running maximum m and sum l of each row (exp(x) = 2^(x log2 e) throughout):
+//   S^T = K Q^T      v_mfma_f32_32x32x16_bf16, K rows as the A operand: lane (r, h) = (l % 32, l / 32) then holds, for
+//                    query row r, the keys 8 (i / 4) + 4 h + i % 4 of a block of 32 in registers i = 0 .. 15
+//   P = 2^(c S - m)  in registers; the row maximum needs one exchange between the lane halves
+//   O^T += V^T P^T   the P registers 8 s .. 8 s + 7, rounded to bf16, are the B operand of keys 16 s .. as they stand: the
+//                    order of keys inside a product is free, so V^T is read in the same order, by transposing LDS reads
+// so neither S nor P leaves its lane, and m, l and the rescaling of O are per lane too.  P is rounded to bf16 because V is;
+// l sums the unrounded values.
+//
+// K and V go from HBM to LDS without passing registers, 16 bytes a lane; in LDS a tile is [64-element column block][key][128
+// bytes, E4M3 64] with the 16-byte cells of a row permuted by its number, which keeps the operand reads free of bank conflicts.
+// E4M3 becomes bf16 (exactly) after the LDS read; the scales multiply c and the result.
+//
+// Masks.  A tile's loads touch only keys that some row of the tile sees: others (past the last position, between the first
+// tokens and the window) read a visible row again, and their weights are set to 0.  A key that one row sees and another does
+// not still meets the other's weight 0 in the product, and 0 * NaN is NaN: tiles with such masks look for non-finite V
+// operands, and a wave that found one takes its sums again key by key.
+//
+// Work is cut so that the card is full: a device-side count of all requests' tiles gives the number of key tiles per block
+// (chunk); a row tile with more is split over several blocks, whose (O, m, l) a second kernel joins in a fixed order.
+#include <algorithm>
+#include <atomic>
+
 #include "cache.h"
 #include "device.h"
 
 namespace mimo {
 
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef int v2i __attribute__((ext_vector_type(2)));
+
 struct AttendArgs {
   const uint16_t* q;
   int64_t q_stride;
-  int N, Hq, Hkv, G, Dk, Dv, B, max_pages, n_pages, page_shift, window, sinks;
+  int N, Hq, Hkv, G, B, max_pages, n_pages, page_shift, window, sinks;
   const int32_t *starts, *lens, *table;
-  const void *k, *v;
+  const uint8_t *k, *v;
   const float *k_scale, *v_scale, *sink_logits;
   float scale;
   uint16_t* out;
   int32_t* status;
+  // rows of a tile: TQ tokens of HT heads (HG groups of HT heads cover G), Hh = Hkv * HG
+  int TQ, HT, HG, Hh, chunk_min, target;
+  // split tiles: per block TQ * HT rows of O (fp32 [Dv]) and (m, l); per (token, head group) the first block's slot and
+  // blocks | token's place << 16.  meta is null when no tile can be split.
+  float *part_o, *part_ml;
+  int2* meta;
 };
 
-// The simple form: one block per (token, head), each wave takes every fourth key, lanes along the head dimension.
-template <bool E4M3>
-__global__ void __launch_bounds__(256) attend_simple_kernel(AttendArgs a) {
-  const int n = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint16_t* o = a.out + ((size_t)n * a.Hq + h) * a.Dv;
-  int lo = 0, hi = a.B;                              // the last request that starts at or before n
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.starts[mid] <= n) lo = mid; else hi = mid;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int AT_THREADS = 256;
+constexpr int AT_WIDE_TARGET = 512, AT_WIDE_MIN = 4;      // blocks wanted, least 64-key tiles of a block
+constexpr int AT_NARROW_TARGET = 1024, AT_NARROW_MIN = 2; // the same in 128-key units
+
+template <int DK_, int DV_, bool F8_, bool WIDE_> struct AtCfg {
+  static constexpr int DK = DK_, DV = DV_;
+  static constexpr bool F8 = F8_, WIDE = WIDE_;
+  static constexpr int CBB = F8 ? 64 : 128;                // bytes of a row in one 64-element column block
+  static constexpr int KCB = DK / 64, VCB = DV / 64;
+  static constexpr int KEYS = WIDE ? 64 : 32;              // keys of one LDS tile (narrow: one wave's)
+  static constexpr int NB = KEYS / 32;
+  static constexpr int UNIT = WIDE ? 64 : 128;             // keys per iteration of the block
+  static constexpr int ROWS = WIDE ? 128 : 32;
+  static constexpr int KBYTES = KEYS * CBB * KCB, VBYTES = KEYS * CBB * VCB;
+  static constexpr int STAGE = KBYTES + VBYTES;
+  static constexpr int GR = 1024 / CBB;                    // rows of one copy instruction (64 lanes of 16 bytes)
+  static constexpr int LR = (WIDE ? 16 : 32) / GR;         // row groups that a wave copies per tile
+  static constexpr int MERGE = WIDE ? 0 : 4 * 32 * DV * 4 + 4 * 32 * 8;   // narrow: the waves' O, m, l joined at the end
+  static constexpr int LDS = (WIDE ? 2 * STAGE : 4 * STAGE) > MERGE ? (WIDE ? 2 * STAGE : 4 * STAGE) : MERGE;
+  static constexpr int WGS = 2;                            // blocks per CU
+  static_assert(WGS * LDS <= 163840, "LDS of the blocks of a CU");
+};
+
+__device__ __forceinline__ void at_wait_vm(int n) {
+  switch (n) {
+    case 0: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
+    case 2: asm volatile("s_waitcnt vmcnt(2)" ::: "memory"); break;
+    case 4: asm volatile("s_waitcnt vmcnt(4)" ::: "memory"); break;
+    case 6: asm volatile("s_waitcnt vmcnt(6)" ::: "memory"); break;
+    case 8: asm volatile("s_waitcnt vmcnt(8)" ::: "memory"); break;
+    case 12: asm volatile("s_waitcnt vmcnt(12)" ::: "memory"); break;
+    default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
   }
-  const int b = lo, s0 = a.starts[b], s1 = a.starts[b + 1], len = a.lens[b];
-  const bool mine = n >= s0 && n < s1;
-  const bool bad = mine && (len < s1 - s0 || len > (a.max_pages << a.page_shift));
-  if (!mine || bad) {
-    if (bad && a.status && threadIdx.x == 0) a.status[0] = MIMO_ERR_SHAPE;
-    for (int d = threadIdx.x; d < a.Dv; d += 256) o[d] = 0;
+}
+__device__ __forceinline__ void at_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// 16 bytes from every lane's address to lds + 16 * lane (lds: LDS byte offset, wave-uniform); the caller waits on vmcnt
+__device__ __forceinline__ void at_copy16(const uint8_t* src, uint32_t lds) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+__device__ __forceinline__ float at_swap_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float at_swap_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// four / two E4M3 codes of a dword to bf16, exact
+__device__ __forceinline__ bf16x8 at_f8_bf16x8(uint32_t a, uint32_t b) {
+  const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
+  const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+  return bf16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
+}
+
+// ------------------------------------------------------------------ the work of a block
+// The keys a row tile sees: positions p_min .. p_max, keys lo .. p_max and the first `sinks`; it walks the 64- or 128-key
+// units 0 .. st - 1 (first tokens) and ws .. (window), I in all.
+struct AtRange {
+  int p_min, p_max, lo, sinks, st, ws, I;
+};
+__device__ __forceinline__ AtRange at_range(int p_min, int p_max, int window, int sinks, int unit) {
+  AtRange r;
+  r.p_min = p_min, r.p_max = p_max;
+  r.lo = window && p_min >= window ? p_min - window + 1 : 0;
+  r.sinks = r.lo ? min(sinks, r.lo) : 0;
+  r.ws = r.lo / unit;
+  r.st = (r.sinks + unit - 1) / unit;
+  if (r.st >= r.ws) r.st = r.ws = 0;
+  r.I = r.st + p_max / unit - r.ws + 1;
+  return r;
+}
+// the most units any row tile of a request of `len` tokens walks
+__device__ __forceinline__ int at_most(int len, int window, int sinks, int TQ, int unit) {
+  if (len <= 0) return 0;
+  const int all = (len - 1) / unit + 1;
+  if (!window) return all;
+  const long long w = ((long long)window + TQ - 2) / unit + 2 + ((long long)min(sinks, len) + unit - 1) / unit;
+  return (int)min((long long)all, w);
+}
+
+struct AtItem {
+  int b, s0, n, len, tt, hh, split, chunk, slot0;   // slot0: of the tile's first block; -1 when the request is not split
+};
+
+// Block blockIdx.x's item: every block counts all requests' work for itself (a few KB from L2) and takes its place in the
+// list of (request, row tile from the last to the first, split) x head group, head groups fastest: neighbouring blocks, on
+// different XCDs, work on different heads, and an XCD keeps meeting the same ones.  false: past the end of the list.
+__device__ __forceinline__ bool at_find(const AttendArgs& a, int unit, int* sh, AtItem& it) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int per = (a.B + AT_THREADS - 1) / AT_THREADS;
+  const int b0 = min(a.B, t * per), b1 = min(a.B, b0 + per);
+  const long long cap = (long long)a.max_pages << a.page_shift;
+  auto request = [&](int b, int& s0, int& n, int& len) {   // clamped: whatever starts and lens hold, nothing is out of range
+    s0 = min(max(a.starts[b], 0), a.N);
+    n = min(max(a.starts[b + 1], s0), a.N) - s0;
+    len = a.lens[b];
+    if (n && (len < n || len > cap)) len = 0;              // refused: its rows are set to 0
+  };
+  long long work = 0;
+  int s0, n, len;
+  for (int b = b0; b < b1; ++b) {
+    request(b, s0, n, len);
+    if (n) work += (long long)((n + a.TQ - 1) / a.TQ) * at_most(len, a.window, a.sinks, a.TQ, unit);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
+  long long* shl = reinterpret_cast<long long*>(sh);
+  if (lane == 0) shl[wave] = work;
+  if (t == 0) sh[20] = -1;
+  __syncthreads();
+  work = min(shl[0] + shl[1] + shl[2] + shl[3], 1ll << 50);   // starts that overlap may ask for anything: then nothing is split
+  const long long fair = (work * a.Hh + a.target - 1) / a.target;
+  const int chunk = (int)min((long long)0x3fffffff, max((long long)a.chunk_min, fair));
+  long long units = 0;
+  int parts = 0;
+  for (int b = b0; b < b1; ++b) {
+    request(b, s0, n, len);
+    if (!n) continue;
+    const int nt = (n + a.TQ - 1) / a.TQ, ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, unit) + chunk - 1) / chunk);
+    units += (long long)nt * ns;
+    parts += ns > 1 ? nt * ns : 0;
+  }
+  long long iu = units;
+  int ip = parts;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const long long x = __shfl_up(iu, d, 64);
+    const int y = __shfl_up(ip, d, 64);
+    if (lane >= d) iu += x, ip += y;
+  }
+  if (lane == 63) shl[4 + wave] = iu, sh[16 + wave] = ip;
+  __syncthreads();
+  long long ub = iu - units;
+  int pb = ip - parts;
+  for (int w = 0; w < wave; ++w) ub += shl[4 + w], pb += sh[16 + w];
+  const int u = blockIdx.x / a.Hh;
+  if (u >= ub && u < ub + units) {
+    for (int b = b0; b < b1; ++b) {
+      request(b, s0, n, len);
+      if (!n) continue;
+      const int nt = (n + a.TQ - 1) / a.TQ, ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, unit) + chunk - 1) / chunk);
+      if (u < ub + (long long)nt * ns) {
+        const int at = (int)(u - ub) / ns;
+        sh[20] = b, sh[21] = s0, sh[22] = n, sh[23] = len, sh[24] = nt - 1 - at, sh[25] = (int)(u - ub) - at * ns;
+        sh[26] = ns > 1 ? (pb + at * ns) * a.Hh + blockIdx.x % a.Hh : -1;
+        break;
+      }
+      ub += (long long)nt * ns;
+      pb += ns > 1 ? nt * ns : 0;
+    }
+  }
+  __syncthreads();
+  it.b = sh[20], it.s0 = sh[21], it.n = sh[22], it.len = sh[23], it.tt = sh[24], it.split = sh[25], it.slot0 = sh[26];
+  it.hh = blockIdx.x % a.Hh;
+  it.chunk = chunk;
+  __syncthreads();                                         // the scratch is free
+  return it.b >= 0;
+}
+
+// 16 keys from a multiple of 16 on, of which a tile may load: their page and what hidden keys read instead
+struct AtKeys {
+  int g0, fb, id;
+};
+__device__ __forceinline__ AtKeys at_keys(const AttendArgs& a, const AtRange& r, int b, int g0) {
+  AtKeys g;
+  if (g0 > r.p_max || (g0 >= r.sinks && g0 + 15 < r.lo)) g0 = r.p_max & ~15;
+  g.g0 = g0;
+  g.fb = g0 >= r.lo || g0 < r.sinks ? g0 : r.lo;
+  const int at = __builtin_amdgcn_readfirstlane(b * a.max_pages + (g0 >> a.page_shift));
+  // the table is constant while the kernel runs: a scalar load, whose wait is not the vector loads'
+  g.id = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(a.table))[at];
+  return g;
+}
+__device__ __forceinline__ int at_page(const AttendArgs& a, int id) {
+  if ((uint32_t)id < (uint32_t)a.n_pages) return id;
+  if (a.status && (threadIdx.x & 63) == 0) a.status[0] = MIMO_ERR_SLOT;
+  return 0;
+}
+// cache row (of [page, head, row in page]) of key g0 + r
+__device__ __forceinline__ size_t at_row(const AttendArgs& a, const AtRange& r, const AtKeys& g, int page, int kv, int row) {
+  const int j = g.g0 + row;
+  const int key = j <= r.p_max && (j >= r.lo || j < r.sinks) ? j : g.fb;
+  return (((size_t)page * a.Hkv + kv) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+}
+
+// One wave's 32 query rows against its keys, one after another in plain 32-bit arithmetic, a hidden key never touched: the
+// sums of a wave that met a NaN or an infinity in a value that not all of its rows see.
+template <class C>
+__device__ __forceinline__ void at_slow(const AttendArgs& a, const AtRange& r, int b, int kv, int it0, int it1, int first, int count,
+                                        const bf16x8 (&Q)[C::DK / 16], int p, bool valid, float c, v16f (&O)[C::DV / 32], float& m,
+                                        float& l) {
+  const int h = (threadIdx.x >> 5) & 1;
+#pragma unroll
+  for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) O[d][i] = 0.0f;
+  m = -INFINITY, l = 0.0f;
+#pragma unroll 1
+  for (int it = it0; it < it1; ++it) {
+    const int base = (it < r.st ? it : r.ws + it - r.st) * C::UNIT + first;
+#pragma unroll 1
+    for (int j = base; j < base + count; ++j) {
+      if (j > r.p_max || (j < r.lo && j >= r.sinks)) continue;
+      const bool seen = valid && j <= p && (!a.window || j > p - a.window || j < a.sinks);
+      const int page = at_page(a, a.table[(size_t)b * a.max_pages + (j >> a.page_shift)]);
+      const size_t row = (((size_t)page * a.Hkv + kv) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
+      float s = 0.0f;
+#pragma unroll
+      for (int e = 0; e < C::DK / 16; ++e) {
+        bf16x8 x;
+        if constexpr (C::F8) {
+          const uint2 w = *reinterpret_cast<const uint2*>(a.k + row * C::DK + 16 * e + 8 * h);
+          x = at_f8_bf16x8(w.x, w.y);
+        } else {
+          x = *reinterpret_cast<const bf16x8*>(a.k + (row * C::DK + 16 * e + 8 * h) * 2);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += (float)x[i] * (float)Q[e][i];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      s = at_swap_sum(s) * c;
+      if (!seen) s = -INFINITY;
+      const float top = fmaxf(m, s), ref = top == -INFINITY ? 0.0f : top;
+      const float was = at_exp2(m - ref), w = seen ? at_exp2(s - ref) : 0.0f;
+      m = top;
+      l = l * was + (h ? 0.0f : w);                        // the halves' sums are added at the end
+#pragma unroll
+      for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const size_t at = row * C::DV + 32 * d + 8 * (i / 4) + 4 * h + i % 4;
+          const float x = C::F8 ? e4m3_unpack2(a.v[at]).x : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.v)[at]);
+          O[d][i] = O[d][i] * was + (w > 0.0f || w != w ? w * x : 0.0f);
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+  }
+}
+
+template <class C>
+__global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int t = threadIdx.x, lane = t & 63, r32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  {                                                        // rows of no request
+    const int first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N);
+    const int gap = first + a.N - last, row = a.Hq * C::DV / 8;
+    for (int i = blockIdx.x; i < gap; i += gridDim.x) {
+      uint4* o = reinterpret_cast<uint4*>(a.out) + (size_t)(i < first ? i : last + i - first) * row;
+      for (int d = t; d < row; d += AT_THREADS) o[d] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  AtItem item;
+  if (!at_find(a, C::UNIT, reinterpret_cast<int*>(lds), item)) return;
+  const int b = __builtin_amdgcn_readfirstlane(item.b), hg = item.hh % a.HG, kv = item.hh / a.HG;
+  const int tok0 = item.tt * a.TQ, toks = min(a.TQ, item.n - tok0);
+  const int heads = min(a.HT, a.G - hg * a.HT);
+  const int qrow = (C::WIDE ? 32 * wave : 0) + r32;        // this lane's query row
+  const int qt = qrow / a.HT, qh = qrow - qt * a.HT;
+  const bool valid = qt < toks && qh < heads;
+  const int head = kv * a.G + hg * a.HT + qh;
+  const size_t out_at = ((size_t)(item.s0 + tok0 + qt) * a.Hq + head) * C::DV;
+  const int base_pos = item.len - item.n + tok0;
+  if (item.len == 0) {                                     // a refused request (it is never split)
+    if (a.status && t == 0) a.status[0] = MIMO_ERR_SHAPE;
+    if (valid && (C::WIDE || wave == 0))
+      for (int d = 0; d < C::DV / 2; d += 8) *reinterpret_cast<uint4*>(a.out + out_at + h * (C::DV / 2) + d) = make_uint4(0, 0, 0, 0);
+    if (a.meta && t < toks) a.meta[(size_t)(item.s0 + tok0 + t) * a.Hh + item.hh] = make_int2(0, 1);
     return;
   }
-  const int p = len - s1 + n, kv = h / a.G;
-  const float ks = E4M3 ? a.k_scale[kv] : 1.0f, vs = E4M3 ? a.v_scale[kv] : 1.0f;
-  float q[3], acc[2] = {0.0f, 0.0f}, m = -INFINITY, l = 0.0f;
-  const int nk = a.Dk / 64, nv = a.Dv / 64;
-  for (int c = 0; c < 3; ++c) q[c] = c < nk ? bf16_to_f32(a.q[n * a.q_stride + h * a.Dk + 64 * c + lane]) : 0.0f;
-  auto load = [&](const void* base, size_t at) {
-    if constexpr (E4M3) return e4m3_unpack2(static_cast<const uint8_t*>(base)[at]).x;
-    else return bf16_to_f32(static_cast<const uint16_t*>(base)[at]);
-  };
-  for (int j = wave; j <= p; j += 4) {
-    if (a.window && p - j >= a.window && j >= a.sinks) continue;
-    int id = a.table[(size_t)b * a.max_pages + (j >> a.page_shift)];
-    if (id < 0 || id >= a.n_pages) {
-      if (a.status && lane == 0) a.status[0] = MIMO_ERR_SLOT;
-      id = 0;
+  const AtRange rg = at_range(base_pos, base_pos + toks - 1, a.window, a.sinks, C::UNIT);
+  const int ns = item.slot0 < 0 ? 1 : (rg.I + item.chunk - 1) / item.chunk;
+  if (item.split >= ns) return;
+  const int it0 = item.slot0 < 0 ? 0 : item.split * item.chunk, it1 = item.slot0 < 0 ? rg.I : min(rg.I, it0 + item.chunk);
+  if (a.meta && item.split == 0 && t < toks)
+    a.meta[(size_t)(item.s0 + tok0 + t) * a.Hh + item.hh] = make_int2(item.slot0, ns | (t << 16));
+
+  // queries as the B operand: row r32, dimensions 16 s + 8 h ..; c = |scale| k_scale log2 e, a negative scale turns q round
+  float c = a.scale * kLog2e * (C::F8 ? a.k_scale[kv] : 1.0f);
+  const uint32_t flip = c < 0.0f ? 0x80008000u : 0u;
+  const bool zero = c == 0.0f;
+  c = zero ? 1.0f : fabsf(c);
+  bf16x8 Q[C::DK / 16];
+  {
+    const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + qt) * a.q_stride + head * C::DK + 8 * h;
+#pragma unroll
+    for (int s = 0; s < C::DK / 16; ++s) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (valid && !zero) x = *reinterpret_cast<const uint4*>(qp + 16 * s);
+      Q[s] = __builtin_bit_cast(bf16x8, make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
     }
-    const size_t row = ((((size_t)id * a.Hkv + kv) << a.page_shift)) + (j & ((1 << a.page_shift) - 1));
-    float s = 0.0f;
-    for (int c = 0; c < nk; ++c) s += q[c] * load(a.k, row * a.Dk + 64 * c + lane);
-    s = dpp_sum_f32(s) * ks * a.scale;
-    const float top = fmaxf(m, s), was = m == top ? 1.0f : __expf(m - top), w = s == top && s != -INFINITY ? 1.0f : (s == -INFINITY ? 0.0f : __expf(s - top));
-    l = l * was + w;
-    for (int c = 0; c < nv; ++c) acc[c] = acc[c] * was + w * load(a.v, row * a.Dv + 64 * c + lane);
-    m = top;
   }
-  __shared__ float sm[4], sl[4], sa[4][128];
-  if (lane == 0) sm[wave] = m, sl[wave] = l;
-  sa[wave][lane] = acc[0];
-  sa[wave][64 + lane] = acc[1];
-  __syncthreads();
-  const float sink = a.sink_logits ? a.sink_logits[h] : -INFINITY;
-  const float top = fmaxf(fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3])), sink);
-  float tot = sink == -INFINITY ? 0.0f : __expf(sink - top);
-  for (int w = 0; w < 4; ++w) tot += sm[w] == -INFINITY ? 0.0f : sl[w] * __expf(sm[w] - top);
-  for (int d = threadIdx.x; d < a.Dv; d += 256) {
-    float x = 0.0f;
-    for (int w = 0; w < 4; ++w) x += sm[w] == -INFINITY ? 0.0f : sa[w][d] * __expf(sm[w] - top);
-    o[d] = tot == 0.0f ? 0 : f32_to_bf16(x * vs / tot);
+  const int pos = base_pos + qt;                           // this lane's position
+  const int w_first = C::WIDE ? 32 * wave / a.HT : 0, w_last = min(toks - 1, ((C::WIDE ? 32 * wave : 0) + 31) / a.HT);
+  const bool busy = w_first <= w_last;                     // the wave has rows
+  const int wp_min = base_pos + w_first, wp_max = base_pos + w_last;
+
+  // copies: lane's row inside a row group and its 16-byte cell (the cell stored at place p of row x is p ^ swizzle(x))
+  const int cr = lane / (C::CBB / 16);
+  const int cell = (lane & (C::CBB / 16 - 1)) ^ (C::F8 ? (lane >> 4) & 3 : (lane >> 3) & 7);
+  const uint32_t lds0 = lds_addr(lds) + (C::WIDE ? 0 : wave * C::STAGE);
+  auto start_of = [&](int it) { return (it < rg.st ? it : rg.ws + it - rg.st) * C::UNIT; };
+  constexpr int NG = C::WIDE ? 1 : 2;                      // 16-key groups that the wave copies
+  AtKeys kg[NG];
+  auto look = [&](int it) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) kg[g] = at_keys(a, rg, b, start_of(it) + (C::WIDE ? 16 : 32) * wave + 16 * g);
+  };
+  size_t crow[C::LR];
+  auto rows_of = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < C::LR; ++x) {
+      const int g = x * C::GR / 16;
+      crow[x] = at_row(a, rg, kg[g], at_page(a, kg[g].id), kv, x * C::GR % 16 + cr);
+    }
+  };
+  constexpr int ES = C::F8 ? 1 : 2;
+  auto issue_k = [&](uint32_t stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < C::LR; ++x) {
+      const uint8_t* p = a.k + crow[x] * (C::DK * ES) + 16 * cell;
+#pragma unroll
+      for (int cb = 0; cb < C::KCB; ++cb)
+        at_copy16(p + cb * C::CBB, stage + cb * (C::KEYS * C::CBB) + ((C::WIDE ? wave * C::LR : 0) + x) * 1024);
+    }
+  };
+  auto issue_v = [&](uint32_t stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < C::LR; ++x) {
+      const uint8_t* p = a.v + crow[x] * (C::DV * ES) + 16 * cell;
+#pragma unroll
+      for (int cb = 0; cb < C::VCB; ++cb)
+        at_copy16(p + cb * C::CBB, stage + C::KBYTES + cb * (C::KEYS * C::CBB) + ((C::WIDE ? wave * C::LR : 0) + x) * 1024);
+    }
+  };
+
+  // operand addresses in a tile: K row r32, cell 2 s + h (E4M3: cell s, half h); V as the transposing reads want them
+  const int i16 = lane & 15, d16 = (lane >> 4) & 1;
+  const int k_at = C::F8 ? r32 * 64 + 16 * ((r32 >> 2) & 3) + 8 * h : r32 * 128 + 16 * (h ^ (r32 & 7));
+  const int v_row = C::F8 ? 4 * h + ((i16 >> 1) & 3) + 8 * (i16 >> 3) : 4 * h + (i16 >> 2);
+  const int v_at = C::F8 ? v_row * 64 + 16 * (d16 ^ ((v_row >> 2) & 3)) + 8 * (i16 & 1)
+                         : v_row * 128 + 16 * ((2 * d16 + ((i16 >> 1) & 1)) ^ (v_row & 7)) + 8 * (i16 & 1);
+  auto k_frag = [&](const uint8_t* st, int kb, int s) __attribute__((always_inline)) {
+    if constexpr (C::F8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(st + (k_at ^ (16 * (s & 3))) + (s >> 2) * (C::KEYS * 64) + kb * 32 * 64);
+      return at_f8_bf16x8(w.x, w.y);
+    } else {
+      return *reinterpret_cast<const bf16x8*>(st + (k_at ^ (32 * (s & 3))) + (s >> 2) * (C::KEYS * 128) + kb * 32 * 128);
+    }
+  };
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"   // LDS pointers are 32 bits on the device
+  auto v_frag = [&](const uint8_t* st, int kb, int s, int d) __attribute__((always_inline)) {
+    typedef __attribute__((address_space(3))) v4s* lds4;
+    typedef __attribute__((address_space(3))) v2i* lds2;
+    if constexpr (C::F8) {
+      const uint8_t* p = st + C::KBYTES + (v_at ^ (32 * (d & 1))) + (d >> 1) * (C::KEYS * 64) + (32 * kb + 16 * s) * 64;
+      const v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)(uint32_t)(uintptr_t)p);
+      return at_f8_bf16x8(w[0], w[1]);
+    } else {
+      const uint8_t* p = st + C::KBYTES + (v_at ^ (64 * (d & 1))) + (d >> 1) * (C::KEYS * 128) + (32 * kb + 16 * s) * 128;
+      const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uint32_t)(uintptr_t)p);
+      const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uint32_t)((uintptr_t)p + 8 * 128));
+      return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  };
+#pragma clang diagnostic pop
+
+  v16f O[C::DV / 32];
+#pragma unroll
+  for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) O[d][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;                           // l: this lane half's keys
+  bool suspect = false;
+
+  v16f S[C::NB];
+  bf16x8 P[C::NB][2];
+  // operands are read PX products ahead; the barriers keep the compiler from reading them all at once (spilled registers)
+  constexpr int PX = 4;
+  auto scores = [&](const uint8_t* st) __attribute__((always_inline)) {
+    constexpr int NS = C::DK / 16, F = C::NB * NS;
+    bf16x8 X[PX];
+#pragma unroll
+    for (int f = 0; f < PX; ++f) X[f] = k_frag(st, f % C::NB, f / C::NB);
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const int kb = f % C::NB, s = f / C::NB;
+      __builtin_amdgcn_sched_barrier(0);
+      if (s == 0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[kb][i] = 0.0f;
+      }
+      S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(X[f % PX], Q[s], S[kb], 0, 0, 0);
+      if (f + PX < F) X[f % PX] = k_frag(st, (f + PX) % C::NB, (f + PX) / C::NB);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto softmax = [&](int j0, bool masked) __attribute__((always_inline)) {
+    if (masked) {
+#pragma unroll
+      for (int kb = 0; kb < C::NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = j0 + 32 * kb + 8 * (i / 4) + 4 * h + i % 4;
+          const bool seen = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
+          S[kb][i] = seen ? S[kb][i] : -INFINITY;
+        }
+    }
+    float top = S[0][0];
+#pragma unroll
+    for (int kb = 0; kb < C::NB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, S[kb][i]);
+    top = at_swap_max(top) * c;
+    // m may lag behind the maximum by 8 (weights of up to 2^8, exact as any others); past that O and l are rescaled
+    if (__ballot(top > m + 8.0f || (m == -INFINITY && top > m))) {
+      const float next = fmaxf(m, top), was = at_exp2(m - (next == -INFINITY ? 0.0f : next));
+      m = next;
+      l *= was;
+#pragma unroll
+      for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) O[d][i] *= was;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int kb = 0; kb < C::NB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = at_exp2(__builtin_fmaf(S[kb][i], c, -ref));
+        l += p;
+        P[kb][i / 8][i % 8] = (__bf16)p;
+      }
+  };
+  auto values = [&](const uint8_t* st, bool watch) __attribute__((always_inline)) {
+    constexpr int ND = C::DV / 32, F = C::NB * 2 * ND;
+    uint32_t odd = 0;
+    bf16x8 X[PX];
+#pragma unroll
+    for (int f = 0; f < PX; ++f) X[f] = v_frag(st, f / (2 * ND), f / ND % 2, f % ND);
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const int kb = f / (2 * ND), s = f / ND % 2, d = f % ND;
+      __builtin_amdgcn_sched_barrier(0);
+      if (watch) {                                         // an exponent of all ones carries into bit 15
+        const uint4 w = __builtin_bit_cast(uint4, X[f % PX]);
+        odd |= ((w.x & 0x7F807F80u) + 0x00800080u) | ((w.y & 0x7F807F80u) + 0x00800080u) | ((w.z & 0x7F807F80u) + 0x00800080u) |
+               ((w.w & 0x7F807F80u) + 0x00800080u);
+      }
+      O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(X[f % PX], P[kb][s], O[d], 0, 0, 0);
+      if (f + PX < F) X[f % PX] = v_frag(st, (f + PX) / (2 * ND), (f + PX) / ND % 2, (f + PX) % ND);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (watch && __ballot((odd & 0x80008000u) != 0)) suspect = true;
+  };
+  // every row of the wave sees all keys j0 .. j0 + n - 1
+  auto open = [&](int j0, int n) {
+    return j0 + n - 1 <= wp_min && (!a.window || j0 > wp_max - a.window || j0 + n <= a.sinks);
+  };
+
+  look(it0);
+  rows_of();
+  if constexpr (C::WIDE) {
+    issue_k(lds0);
+    issue_v(lds0);
+    for (int it = it0; it < it1; ++it) {
+      const int cur = (it - it0) & 1, j0 = start_of(it);
+      if (it + 1 < it1) look(it + 1);
+      at_wait_vm(0);
+      __syncthreads();                                     // the tile has landed everywhere; the other one is free
+      if (it + 1 < it1) {
+        rows_of();
+        issue_k(lds0 + (cur ^ 1) * C::STAGE);
+        issue_v(lds0 + (cur ^ 1) * C::STAGE);
+      }
+      if (!busy || j0 > wp_max) continue;
+      const uint8_t* st = lds + cur * C::STAGE;
+      scores(st);
+      if (open(j0, C::UNIT)) {
+        softmax(j0, false);
+        values(st, false);
+      } else {
+        softmax(j0, true);
+        values(st, true);
+      }
+    }
+  } else {
+    const uint8_t* st = lds + wave * C::STAGE;
+    constexpr int NK = C::LR * C::KCB, NV = C::LR * C::VCB;
+    issue_k(lds0);
+    issue_v(lds0);
+    for (int it = it0; it < it1; ++it) {
+      const int j0 = start_of(it) + 32 * wave;
+      const bool more = it + 1 < it1;
+      if (more) look(it + 1);
+      at_wait_vm(NV);
+      scores(st);
+      at_wait_lds();                                       // K has been read: its room takes the next keys
+      if (more) {
+        rows_of();
+        issue_k(lds0);
+      }
+      const bool op = open(j0, 32);
+      if (op) softmax(j0, false);
+      else softmax(j0, true);
+      if (more) at_wait_vm(NK);
+      else at_wait_vm(0);
+      if (op || wp_min == wp_max) values(st, false);       // one position: what a row does not see, no row sees
+      else values(st, true);
+      at_wait_lds();
+      if (more) issue_v(lds0);
+    }
+  }
+  const float vs = C::F8 ? a.v_scale[kv] : 1.0f;
+  // both kinds of sums go their own way to the end: joined before it, they would not fit the registers
+  auto slow = [&](v16f (&O)[C::DV / 32], float& m, float& l) __attribute__((always_inline)) {
+    at_slow<C>(a, rg, b, kv, it0, it1, C::WIDE ? 0 : 32 * wave, C::WIDE ? C::UNIT : 32, Q, pos, valid, c, O, m, l);
+  };
+
+  if constexpr (C::WIDE) {
+    auto finish = [&](const v16f (&O)[C::DV / 32], float m, float l) __attribute__((always_inline)) {
+    l = at_swap_sum(l);
+    if (!valid) return;
+    if (ns > 1) {
+      const size_t slot = (size_t)item.slot0 + (size_t)item.split * a.Hh, row = slot * (a.TQ * a.HT) + qt * a.HT + qh;
+      if (h == 0) a.part_ml[2 * row] = m, a.part_ml[2 * row + 1] = l;
+#pragma unroll
+      for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(a.part_o + row * C::DV + 32 * d + 2 * i + 4 * h) =
+              make_float4(O[d][i] * vs, O[d][i + 1] * vs, O[d][i + 2] * vs, O[d][i + 3] * vs);
+      return;
+    }
+    const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
+    const float top = fmaxf(m, sink), ref = top == -INFINITY ? 0.0f : top;
+    const float f = at_exp2(m - ref), tot = l * f + at_exp2(sink - ref);
+    const float w = tot == 0.0f ? 0.0f : vs * f / tot;
+#pragma unroll
+    for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        uint2 x;
+        x.x = (uint32_t)f32_to_bf16(O[d][i] * w) | ((uint32_t)f32_to_bf16(O[d][i + 1] * w) << 16);
+        x.y = (uint32_t)f32_to_bf16(O[d][i + 2] * w) | ((uint32_t)f32_to_bf16(O[d][i + 3] * w) << 16);
+        if (tot == 0.0f) x = make_uint2(0, 0);
+        *reinterpret_cast<uint2*>(a.out + out_at + 32 * d + 2 * i + 4 * h) = x;
+      }
+    };
+    if (suspect) {
+      v16f O2[C::DV / 32];
+      float m2, l2;
+      slow(O2, m2, l2);
+      finish(O2, m2, l2);
+    } else {
+      finish(O, m, l);
+    }
+  } else {
+    // the waves' parts, joined over LDS in wave order: row r at [wave][r][DV], 16-byte pieces turned by the row
+    float* po = reinterpret_cast<float*>(lds);
+    float* pm = po + 4 * 32 * C::DV;
+    at_wait_vm(0);
+    __syncthreads();                                       // every wave is done with its tiles
+    constexpr int NP = C::DV / 4;
+    auto put = [&](const v16f (&O)[C::DV / 32], float m, float l) __attribute__((always_inline)) {
+    l = at_swap_sum(l);
+#pragma unroll
+    for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int piece = 8 * d + i / 2 + h;
+        *reinterpret_cast<float4*>(po + (wave * 32 + r32) * C::DV + 4 * ((piece + r32) & (NP - 1))) =
+            make_float4(O[d][i], O[d][i + 1], O[d][i + 2], O[d][i + 3]);
+      }
+    if (h == 0) pm[2 * (32 * wave + r32)] = m, pm[2 * (32 * wave + r32) + 1] = l;
+    };
+    if (suspect) {
+      v16f O2[C::DV / 32];
+      float m2, l2;
+      slow(O2, m2, l2);
+      put(O2, m2, l2);
+    } else {
+      put(O, m, l);
+    }
+    __syncthreads();
+    for (int e = t; e < 32 * NP; e += AT_THREADS) {
+      const int row = e / NP, piece = e & (NP - 1), rt = row / a.HT, rh = row - rt * a.HT;
+      if (rt >= toks || rh >= heads) continue;
+      float mw[4], top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mw[w] = pm[2 * (32 * w + row)], top = fmaxf(top, mw[w]);
+      const int hd = kv * a.G + hg * a.HT + rh;
+      const float sink = ns == 1 && a.sink_logits ? a.sink_logits[hd] * kLog2e : -INFINITY;
+      const float all = fmaxf(top, sink), ref = all == -INFINITY ? 0.0f : all;
+      float tot = ns == 1 ? at_exp2(sink - ref) : 0.0f;
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = at_exp2(mw[w] - ref);
+        const float4 o = *reinterpret_cast<const float4*>(po + (w * 32 + row) * C::DV + 4 * ((piece + row) & (NP - 1)));
+        tot += pm[2 * (32 * w + row) + 1] * f;
+        x[0] += o.x * f, x[1] += o.y * f, x[2] += o.z * f, x[3] += o.w * f;
+      }
+      if (ns > 1) {
+        const size_t slot = (size_t)item.slot0 + (size_t)item.split * a.Hh, pr = slot * (a.TQ * a.HT) + row;
+        *reinterpret_cast<float4*>(a.part_o + pr * C::DV + 4 * piece) = make_float4(x[0] * vs, x[1] * vs, x[2] * vs, x[3] * vs);
+        if (piece == 0) a.part_ml[2 * pr] = all, a.part_ml[2 * pr + 1] = tot;
+      } else {
+        const float w = tot == 0.0f ? 0.0f : vs / tot;
+        uint2 y;
+        y.x = (uint32_t)f32_to_bf16(x[0] * w) | ((uint32_t)f32_to_bf16(x[1] * w) << 16);
+        y.y = (uint32_t)f32_to_bf16(x[2] * w) | ((uint32_t)f32_to_bf16(x[3] * w) << 16);
+        if (tot == 0.0f) y = make_uint2(0, 0);
+        *reinterpret_cast<uint2*>(a.out + ((size_t)(item.s0 + tok0 + rt) * a.Hq + hd) * C::DV + 4 * piece) = y;
+      }
+    }
+  }
+}
+
+// The parts of split row tiles, joined in order: out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j.  A block takes one token
+// and head group, hpb of its heads; its four waves share the parts of a head.
+template <int DV>
+__global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a, int hpb) {
+  __shared__ float sl[4], so[4][DV];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = (a.HT + hpb - 1) / hpb;
+  const int n = blockIdx.x / (a.Hh * per), rest = blockIdx.x - n * a.Hh * per, hh = rest / per, q0 = (rest - hh * per) * hpb;
+  const int first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N);
+  if (n < first || n >= last) return;
+  const int2 mt = a.meta[(size_t)n * a.Hh + hh];
+  const int ns = mt.y & 0xFFFF;
+  if (ns <= 1 || mt.x < 0) return;
+  const int hg = hh % a.HG, kv = hh / a.HG, heads = min(a.HT, a.G - hg * a.HT);
+  constexpr int E = DV / 64;
+  for (int qh = q0; qh < min(heads, q0 + hpb); ++qh) {
+    const size_t rows = (size_t)a.TQ * a.HT, row0 = (size_t)mt.x * rows + (size_t)(mt.y >> 16) * a.HT + qh, step = rows * a.Hh;
+    float top = -INFINITY;
+    for (int j = lane; j < ns; j += 64) top = fmaxf(top, a.part_ml[2 * (row0 + j * step)]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float tot = 0.0f, x[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = 0.0f;
+#pragma unroll 4
+    for (int j = wave; j < ns; j += 4) {
+      const size_t row = row0 + j * step;
+      const float f = at_exp2(a.part_ml[2 * row] - ref);
+      tot += f * a.part_ml[2 * row + 1];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] += f * a.part_o[row * DV + E * lane + e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) so[wave][E * lane + e] = x[e];
+    if (lane == 0) sl[wave] = tot;
+    __syncthreads();
+    const int head = kv * a.G + hg * a.HT + qh;
+    const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
+    const float all = fmaxf(top, sink), r2 = all == -INFINITY ? 0.0f : all, g = at_exp2(top - r2);
+    const float sum = (sl[0] + sl[1] + sl[2] + sl[3]) * g + at_exp2(sink - r2);
+    for (int d = threadIdx.x; d < DV; d += 256) {
+      const float y = (so[0][d] + so[1][d] + so[2][d] + so[3][d]) * g;
+      a.out[((size_t)n * a.Hq + head) * DV + d] = sum == 0.0f ? 0 : f32_to_bf16(y / sum);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ host
+static void at_tiles(int rows, int N, int heads, int kv_heads, AttendArgs& a) {
+  a.G = heads / kv_heads;
+  a.HT = std::min(a.G, rows);
+  a.HG = (a.G + a.HT - 1) / a.HT;
+  a.Hh = kv_heads * a.HG;
+  a.TQ = std::max(1, std::min(rows / a.HT, N));
+}
+
+struct AtRoom {
+  size_t o, ml, meta;
+};
+static AtRoom at_room(int rows, int target, int N, int heads, int kv_heads, int v_dim) {
+  AttendArgs a{};
+  at_tiles(rows, N, heads, kv_heads, a);
+  // a request is split when its tiles walk more than chunk units, so its blocks are at most twice its share of the target
+  const size_t pr = (size_t)2 * target * a.TQ * a.HT;
+  return {align256(pr * v_dim * 4), align256(pr * 8), align256((size_t)N * a.Hh * sizeof(int2))};
+}
+
+template <class C>
+static int at_launch(AttendArgs a, bool join, hipStream_t st) {
+  static std::atomic<uint64_t> allowed{0};                 // devices on which the kernel may use its LDS
+  int dev = 0;
+  MIMO_HIP(hipGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(allowed.load(std::memory_order_acquire) & bit)) {
+    MIMO_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
+    allowed.fetch_or(bit, std::memory_order_release);
+  }
+  // row tiles: at most sum ceil(n_b / TQ) over at most min(B, N) requests with rows; blocks: tiles plus splits
+  const int64_t tiles = ((int64_t)a.N + (int64_t)std::min(a.B, a.N) * (a.TQ - 1)) / a.TQ;
+  const int64_t grid = tiles * a.Hh + (join ? a.target : 0);
+  MIMO_REQUIRE(grid < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many tiles");
+  {
+    ProfScope p(st, C::WIDE ? "attend_wide" : "attend_narrow");
+    attend_kernel<C><<<(unsigned)grid, AT_THREADS, C::LDS, st>>>(a);
+  }
+  if (int e = check_launch("attend")) return e;
+  if (!join) return MIMO_OK;
+  const int hpb = (int64_t)a.N * a.Hh >= 1024 ? a.HT : 1;
+  const int64_t blocks = (int64_t)a.N * a.Hh * ((a.HT + hpb - 1) / hpb);
+  MIMO_REQUIRE(blocks < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many rows");
+  {
+    ProfScope p(st, "attend_join");
+    attend_join_kernel<C::DV><<<(unsigned)blocks, 256, 0, st>>>(a, hpb);
+  }
+  return check_launch("attend_join");
+}
+
+template <bool F8, bool WIDE>
+static int at_dims(const AttendArgs& a, int dk, bool join, hipStream_t st) {
+  switch (dk) {
+    case 64: return at_launch<AtCfg<64, 64, F8, WIDE>>(a, join, st);
+    case 128: return at_launch<AtCfg<128, 128, F8, WIDE>>(a, join, st);
+    default: return at_launch<AtCfg<192, 128, F8, WIDE>>(a, join, st);
   }
 }
 
@@ -82,8 +798,9 @@ using namespace mimo;
 extern "C" {
 
 size_t mimo_cache_attend_workspace_size(int N, int heads, int kv_heads, int v_dim) {
-  if (N < 0 || heads < 1 || kv_heads < 1 || v_dim < 1) return 0;
-  return 256;
+  if (N < 1 || heads < 1 || kv_heads < 1 || v_dim < 1 || heads % kv_heads) return 256;
+  const AtRoom w = at_room(128, AT_WIDE_TARGET, N, heads, kv_heads, v_dim), n = at_room(32, AT_NARROW_TARGET, N, heads, kv_heads, v_dim);
+  return std::max(w.o + w.ml + w.meta, n.o + n.ml + n.meta);
 }
 
 int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, const mimo_kv_cache* cache, int B,
@@ -96,8 +813,10 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   MIMO_REQUIRE(q && starts && lens && table && out, MIMO_ERR_ARG, "cache_attend: null pointer");
   MIMO_REQUIRE(heads >= 1 && heads % cache->kv_heads == 0 && heads <= 1024, MIMO_ERR_SHAPE,
                "cache_attend: %d heads on %d K/V heads (a multiple, at most 1024)", heads, cache->kv_heads);
-  MIMO_REQUIRE(B >= 1 && B <= (1 << 20) && max_pages >= 1 && max_new >= 0 && (int64_t)max_pages * cache->page_size <= 0x7fffffff,
-               MIMO_ERR_SHAPE, "cache_attend: need 1 <= B <= 2^20, max_pages >= 1, max_new >= 0 (got %d, %d, %d)", B, max_pages, max_new);
+  MIMO_REQUIRE(B >= 1 && max_pages >= 1 && max_new >= 0 && (int64_t)max_pages * cache->page_size <= 0x7fffffff &&
+                   (int64_t)max_pages * B <= 0x7fffffff, MIMO_ERR_SHAPE,
+               "cache_attend: need B, max_pages >= 1, max_new >= 0, at most 2^31 - 1 table entries and tokens of a request (got %d, %d, %d)",
+               B, max_pages, max_new);
   MIMO_REQUIRE(window >= 0 && sink_tokens >= 0, MIMO_ERR_SHAPE, "cache_attend: window and sink_tokens must be >= 0");
   MIMO_REQUIRE(scale == scale && scale - scale == 0.0f, MIMO_ERR_ARG, "cache_attend: scale must be finite");
   MIMO_REQUIRE(q_stride >= (int64_t)heads * cache->k_dim, MIMO_ERR_SHAPE, "cache_attend: rows closer than their length");
@@ -106,16 +825,31 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   const size_t need = mimo_cache_attend_workspace_size(N, heads, cache->kv_heads, cache->v_dim);
   MIMO_REQUIRE(ws && ws_bytes >= need, MIMO_ERR_WORKSPACE, "cache_attend: workspace %zu < %zu", ws_bytes, need);
   MIMO_REQUIRE(aligned16(ws), MIMO_ERR_ALIGN, "cache_attend: 16-byte alignment of the workspace");
-  AttendArgs a{q, q_stride, N, heads, cache->kv_heads, heads / cache->kv_heads, cache->k_dim, cache->v_dim, B, max_pages,
-               cache->n_pages, __builtin_ctz(cache->page_size), window, sink_tokens, starts, lens, table, cache->k, cache->v,
-               cache->k_scale, cache->v_scale, sink_logits, scale, out, status};
+  AttendArgs a{};
+  a.q = q, a.q_stride = q_stride, a.N = N, a.Hq = heads, a.Hkv = cache->kv_heads, a.B = B, a.max_pages = max_pages;
+  a.n_pages = cache->n_pages, a.page_shift = __builtin_ctz(cache->page_size), a.window = window, a.sinks = window ? sink_tokens : 0;
+  a.starts = starts, a.lens = lens, a.table = table;
+  a.k = static_cast<const uint8_t*>(cache->k), a.v = static_cast<const uint8_t*>(cache->v);
+  a.k_scale = cache->k_scale, a.v_scale = cache->v_scale, a.sink_logits = sink_logits;
+  a.scale = scale, a.out = out, a.status = status;
+  const bool wide = (int64_t)std::min(max_new, N) * (heads / cache->kv_heads) > 32;
+  at_tiles(wide ? 128 : 32, N, heads, cache->kv_heads, a);
+  a.chunk_min = wide ? AT_WIDE_MIN : AT_NARROW_MIN;
+  a.target = wide ? AT_WIDE_TARGET : AT_NARROW_TARGET;
+  // no tile can walk more units than the table or the window holds; if that is within chunk_min nothing is ever split
+  const int64_t unit = wide ? 64 : 128;
+  int64_t most = ((int64_t)max_pages * cache->page_size - 1) / unit + 1;
+  if (window) most = std::min(most, ((int64_t)window + a.TQ - 2) / unit + 2 + ((int64_t)a.sinks + unit - 1) / unit);
+  const bool join = most > a.chunk_min;
+  const AtRoom room = at_room(wide ? 128 : 32, a.target, N, heads, cache->kv_heads, cache->v_dim);
+  char* w = static_cast<char*>(ws);
+  a.part_o = reinterpret_cast<float*>(w);
+  a.part_ml = reinterpret_cast<float*>(w + room.o);
+  a.meta = join ? reinterpret_cast<int2*>(w + room.o + room.ml) : nullptr;
   hipStream_t st = as_stream(stream);
-  {
-    ProfScope p(st, "cache_attend");
-    if (cache->dtype == MIMO_KV_E4M3) attend_simple_kernel<true><<<dim3(N, heads), 256, 0, st>>>(a);
-    else attend_simple_kernel<false><<<dim3(N, heads), 256, 0, st>>>(a);
-  }
-  return check_launch("cache_attend");
+  const bool f8 = cache->dtype == MIMO_KV_E4M3;
+  if (wide) return f8 ? at_dims<true, true>(a, cache->k_dim, join, st) : at_dims<false, true>(a, cache->k_dim, join, st);
+  return f8 ? at_dims<true, false>(a, cache->k_dim, join, st) : at_dims<false, false>(a, cache->k_dim, join, st);
 }
 
 }  // extern "C"
