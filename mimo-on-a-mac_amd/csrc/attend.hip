@@ -248,56 +248,40 @@ __device__ __forceinline__ size_t at_row(const AttendArgs& a, const AtRange& r, 
   return (((size_t)page * a.Hkv + kv) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
 }
 
-// One wave's 32 query rows against its keys, one after another in plain 32-bit arithmetic, a hidden key never touched: the
-// sums of a wave that met a NaN or an infinity in a value that not all of its rows see.
+// One query row (at q, position p) against the keys of units it0 .. it1 - 1, `count` keys from `first` on in each, in plain
+// 32-bit arithmetic with the wave's lanes along the head: a hidden key is never touched.  For waves that met a NaN or an
+// infinity in a value that not all of their rows see.  O: dimensions 64 e + lane.
 template <class C>
 __device__ __forceinline__ void at_slow(const AttendArgs& a, const AtRange& r, int b, int kv, int it0, int it1, int first, int count,
-                                        const bf16x8 (&Q)[C::DK / 16], int p, bool valid, float c, v16f (&O)[C::DV / 32], float& m,
-                                        float& l) {
-  const int h = (threadIdx.x >> 5) & 1;
+                                        const uint16_t* q, int p, float c, float (&O)[C::VCB], float& m, float& l) {
+  const int lane = threadIdx.x & 63;
+  float x[C::KCB];
 #pragma unroll
-  for (int d = 0; d < C::DV / 32; ++d)
+  for (int e = 0; e < C::KCB; ++e) x[e] = bf16_to_f32(q[64 * e + lane]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) O[d][i] = 0.0f;
+  for (int e = 0; e < C::VCB; ++e) O[e] = 0.0f;
   m = -INFINITY, l = 0.0f;
+  auto load = [&](const uint8_t* base, size_t at) {
+    return C::F8 ? e4m3_unpack2(base[at]).x : bf16_to_f32(reinterpret_cast<const uint16_t*>(base)[at]);
+  };
 #pragma unroll 1
   for (int it = it0; it < it1; ++it) {
     const int base = (it < r.st ? it : r.ws + it - r.st) * C::UNIT + first;
 #pragma unroll 1
-    for (int j = base; j < base + count; ++j) {
-      if (j > r.p_max || (j < r.lo && j >= r.sinks)) continue;
-      const bool seen = valid && j <= p && (!a.window || j > p - a.window || j < a.sinks);
+    for (int j = base; j < base + count && j <= p; ++j) {
+      if (a.window && j <= p - a.window && j >= a.sinks) continue;
       const int page = at_page(a, a.table[(size_t)b * a.max_pages + (j >> a.page_shift)]);
       const size_t row = (((size_t)page * a.Hkv + kv) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
       float s = 0.0f;
 #pragma unroll
-      for (int e = 0; e < C::DK / 16; ++e) {
-        bf16x8 x;
-        if constexpr (C::F8) {
-          const uint2 w = *reinterpret_cast<const uint2*>(a.k + row * C::DK + 16 * e + 8 * h);
-          x = at_f8_bf16x8(w.x, w.y);
-        } else {
-          x = *reinterpret_cast<const bf16x8*>(a.k + (row * C::DK + 16 * e + 8 * h) * 2);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s += (float)x[i] * (float)Q[e][i];
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      s = at_swap_sum(s) * c;
-      if (!seen) s = -INFINITY;
+      for (int e = 0; e < C::KCB; ++e) s += x[e] * load(a.k, row * C::DK + 64 * e + lane);
+      s = dpp_sum_f32(s) * c;
       const float top = fmaxf(m, s), ref = top == -INFINITY ? 0.0f : top;
-      const float was = at_exp2(m - ref), w = seen ? at_exp2(s - ref) : 0.0f;
+      const float was = at_exp2(m - ref), w = at_exp2(s - ref);
       m = top;
-      l = l * was + (h ? 0.0f : w);                        // the halves' sums are added at the end
+      l = l * was + w;
 #pragma unroll
-      for (int d = 0; d < C::DV / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const size_t at = row * C::DV + 32 * d + 8 * (i / 4) + 4 * h + i % 4;
-          const float x = C::F8 ? e4m3_unpack2(a.v[at]).x : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.v)[at]);
-          O[d][i] = O[d][i] * was + (w > 0.0f || w != w ? w * x : 0.0f);
-          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
+      for (int e = 0; e < C::VCB; ++e) O[e] = O[e] * was + (w == 0.0f ? 0.0f : w * load(a.v, row * C::DV + 64 * e + lane));
     }
   }
 }
@@ -340,18 +324,19 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   if (a.meta && item.split == 0 && t < toks)
     a.meta[(size_t)(item.s0 + tok0 + t) * a.Hh + item.hh] = make_int2(item.slot0, ns | (t << 16));
 
-  // queries as the B operand: row r32, dimensions 16 s + 8 h ..; c = |scale| k_scale log2 e, a negative scale turns q round
+  // queries as the B operand: row r32, dimensions 16 s + 8 h .. (E4M3: 32 (s / 2) + 16 h + 8 (s % 2) .., since a lane's 16
+  // bytes of K are 16 dimensions, two products' worth); c = |scale| k_scale log2 e, a negative scale turns q round
   float c = a.scale * kLog2e * (C::F8 ? a.k_scale[kv] : 1.0f);
   const uint32_t flip = c < 0.0f ? 0x80008000u : 0u;
   const bool zero = c == 0.0f;
   c = zero ? 1.0f : fabsf(c);
   bf16x8 Q[C::DK / 16];
   {
-    const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + qt) * a.q_stride + head * C::DK + 8 * h;
+    const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + qt) * a.q_stride + head * C::DK + (C::F8 ? 16 : 8) * h;
 #pragma unroll
     for (int s = 0; s < C::DK / 16; ++s) {
       uint4 x = make_uint4(0, 0, 0, 0);
-      if (valid && !zero) x = *reinterpret_cast<const uint4*>(qp + 16 * s);
+      if (valid && !zero) x = *reinterpret_cast<const uint4*>(qp + (C::F8 ? 32 * (s >> 1) + 8 * (s & 1) : 16 * s));
       Q[s] = __builtin_bit_cast(bf16x8, make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
     }
   }
@@ -360,9 +345,12 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   const bool busy = w_first <= w_last;                     // the wave has rows
   const int wp_min = base_pos + w_first, wp_max = base_pos + w_last;
 
-  // copies: lane's row inside a row group and its 16-byte cell (the cell stored at place p of row x is p ^ swizzle(x))
+  // copies: lane's row inside a row group and its 16-byte cell; the cell at place p of row x is p ^ swizzle(x).  bf16 K:
+  // (x / 2) % 8, so that 16 rows' cells of one column differ in their banks; V: 4 ((x / 2) % 2), so that the 4 rows of 64 bytes
+  // of a transposing read do; E4M3: (x / 4) % 4 for both.
   const int cr = lane / (C::CBB / 16);
-  const int cell = (lane & (C::CBB / 16 - 1)) ^ (C::F8 ? (lane >> 4) & 3 : (lane >> 3) & 7);
+  const int cell_k = C::F8 ? (lane & 3) ^ ((lane >> 4) & 3) : (lane & 7) ^ (lane >> 4);
+  const int cell_v = C::F8 ? cell_k : (lane & 7) ^ (4 * ((lane >> 4) & 1));
   const uint32_t lds0 = lds_addr(lds) + (C::WIDE ? 0 : wave * C::STAGE);
   auto start_of = [&](int it) { return (it < rg.st ? it : rg.ws + it - rg.st) * C::UNIT; };
   constexpr int NG = C::WIDE ? 1 : 2;                      // 16-key groups that the wave copies
@@ -383,7 +371,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   auto issue_k = [&](uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < C::LR; ++x) {
-      const uint8_t* p = a.k + crow[x] * (C::DK * ES) + 16 * cell;
+      const uint8_t* p = a.k + crow[x] * (C::DK * ES) + 16 * (C::F8 ? cell_k : cell_k ^ (4 * (x & 1)));
 #pragma unroll
       for (int cb = 0; cb < C::KCB; ++cb)
         at_copy16(p + cb * C::CBB, stage + cb * (C::KEYS * C::CBB) + ((C::WIDE ? wave * C::LR : 0) + x) * 1024);
@@ -392,26 +380,22 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   auto issue_v = [&](uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < C::LR; ++x) {
-      const uint8_t* p = a.v + crow[x] * (C::DV * ES) + 16 * cell;
+      const uint8_t* p = a.v + crow[x] * (C::DV * ES) + 16 * cell_v;
 #pragma unroll
       for (int cb = 0; cb < C::VCB; ++cb)
         at_copy16(p + cb * C::CBB, stage + C::KBYTES + cb * (C::KEYS * C::CBB) + ((C::WIDE ? wave * C::LR : 0) + x) * 1024);
     }
   };
 
-  // operand addresses in a tile: K row r32, cell 2 s + h (E4M3: cell s, half h); V as the transposing reads want them
+  // operand addresses in a tile: K row r32, cell 2 s + h; V as the transposing reads want them
   const int i16 = lane & 15, d16 = (lane >> 4) & 1;
-  const int k_at = C::F8 ? r32 * 64 + 16 * ((r32 >> 2) & 3) + 8 * h : r32 * 128 + 16 * (h ^ (r32 & 7));
+  const int k_at = C::F8 ? r32 * 64 + 16 * (h ^ ((r32 >> 2) & 3)) : r32 * 128 + 16 * (h ^ ((r32 >> 1) & 7));
   const int v_row = C::F8 ? 4 * h + ((i16 >> 1) & 3) + 8 * (i16 >> 3) : 4 * h + (i16 >> 2);
   const int v_at = C::F8 ? v_row * 64 + 16 * (d16 ^ ((v_row >> 2) & 3)) + 8 * (i16 & 1)
-                         : v_row * 128 + 16 * ((2 * d16 + ((i16 >> 1) & 1)) ^ (v_row & 7)) + 8 * (i16 & 1);
-  auto k_frag = [&](const uint8_t* st, int kb, int s) __attribute__((always_inline)) {
-    if constexpr (C::F8) {
-      const uint2 w = *reinterpret_cast<const uint2*>(st + (k_at ^ (16 * (s & 3))) + (s >> 2) * (C::KEYS * 64) + kb * 32 * 64);
-      return at_f8_bf16x8(w.x, w.y);
-    } else {
-      return *reinterpret_cast<const bf16x8*>(st + (k_at ^ (32 * (s & 3))) + (s >> 2) * (C::KEYS * 128) + kb * 32 * 128);
-    }
+                         : v_row * 128 + 16 * ((2 * d16 + ((i16 >> 1) & 1)) ^ (4 * ((v_row >> 1) & 1))) + 8 * (i16 & 1);
+  auto k_read = [&](const uint8_t* st, int kb, int s) __attribute__((always_inline)) {   // cell 2 s + h of key 32 kb + r32
+    if constexpr (C::F8) return *reinterpret_cast<const uint4*>(st + (k_at ^ (32 * (s & 1))) + (s >> 1) * (C::KEYS * 64) + kb * 32 * 64);
+    else return *reinterpret_cast<const uint4*>(st + (k_at ^ (32 * (s & 3))) + (s >> 2) * (C::KEYS * 128) + kb * 32 * 128);
   };
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Wint-to-pointer-cast"   // LDS pointers are 32 bits on the device
@@ -444,10 +428,10 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   // operands are read PX products ahead; the barriers keep the compiler from reading them all at once (spilled registers)
   constexpr int PX = 4;
   auto scores = [&](const uint8_t* st) __attribute__((always_inline)) {
-    constexpr int NS = C::DK / 16, F = C::NB * NS;
-    bf16x8 X[PX];
+    constexpr int PER = C::F8 ? 2 : 1, F = C::NB * C::DK / (16 * PER);   // products per read
+    uint4 X[PX];
 #pragma unroll
-    for (int f = 0; f < PX; ++f) X[f] = k_frag(st, f % C::NB, f / C::NB);
+    for (int f = 0; f < PX && f < F; ++f) X[f] = k_read(st, f % C::NB, f / C::NB);
 #pragma unroll
     for (int f = 0; f < F; ++f) {
       const int kb = f % C::NB, s = f / C::NB;
@@ -456,22 +440,38 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
 #pragma unroll
         for (int i = 0; i < 16; ++i) S[kb][i] = 0.0f;
       }
-      S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(X[f % PX], Q[s], S[kb], 0, 0, 0);
-      if (f + PX < F) X[f % PX] = k_frag(st, (f + PX) % C::NB, (f + PX) / C::NB);
+      const uint4 x = X[f % PX];
+      if constexpr (C::F8) {
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.x, x.y), Q[2 * s], S[kb], 0, 0, 0);
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.z, x.w), Q[2 * s + 1], S[kb], 0, 0, 0);
+      } else {
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), Q[s], S[kb], 0, 0, 0);
+      }
+      if (f + PX < F) X[f % PX] = k_read(st, (f + PX) % C::NB, (f + PX) / C::NB);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto softmax = [&](int j0, bool masked) __attribute__((always_inline)) {
-    if (masked) {
+  // keys that a row does not see: unsigned(pos - j) < span for the causal order and the window together
+  const uint32_t span = a.window ? (uint32_t)a.window : 0x80000000u;
+  auto mask = [&](int j0) __attribute__((always_inline)) {
+    const uint32_t back = (uint32_t)(pos - j0 - 4 * h);
+    if (j0 >= a.sinks) {
+#pragma unroll
+      for (int kb = 0; kb < C::NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[kb][i] = back - (uint32_t)(32 * kb + 8 * (i / 4) + i % 4) < span ? S[kb][i] : -INFINITY;
+    } else {
+      const int first = min(a.sinks, pos + 1) - j0 - 4 * h;  // first tokens that the row sees, from the lane's first key on
 #pragma unroll
       for (int kb = 0; kb < C::NB; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int j = j0 + 32 * kb + 8 * (i / 4) + 4 * h + i % 4;
-          const bool seen = j <= pos && (!a.window || j > pos - a.window || j < a.sinks);
-          S[kb][i] = seen ? S[kb][i] : -INFINITY;
+          const int o = 32 * kb + 8 * (i / 4) + i % 4;
+          S[kb][i] = back - (uint32_t)o < span || o < first ? S[kb][i] : -INFINITY;
         }
     }
+  };
+  auto softmax = [&]() __attribute__((always_inline)) {
     float top = S[0][0];
 #pragma unroll
     for (int kb = 0; kb < C::NB; ++kb)
@@ -498,9 +498,8 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
         P[kb][i / 8][i % 8] = (__bf16)p;
       }
   };
-  auto values = [&](const uint8_t* st, bool watch) __attribute__((always_inline)) {
+  auto values = [&](const uint8_t* st) __attribute__((always_inline)) {
     constexpr int ND = C::DV / 32, F = C::NB * 2 * ND;
-    uint32_t odd = 0;
     bf16x8 X[PX];
 #pragma unroll
     for (int f = 0; f < PX; ++f) X[f] = v_frag(st, f / (2 * ND), f / ND % 2, f % ND);
@@ -508,16 +507,27 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
     for (int f = 0; f < F; ++f) {
       const int kb = f / (2 * ND), s = f / ND % 2, d = f % ND;
       __builtin_amdgcn_sched_barrier(0);
-      if (watch) {                                         // an exponent of all ones carries into bit 15
-        const uint4 w = __builtin_bit_cast(uint4, X[f % PX]);
-        odd |= ((w.x & 0x7F807F80u) + 0x00800080u) | ((w.y & 0x7F807F80u) + 0x00800080u) | ((w.z & 0x7F807F80u) + 0x00800080u) |
-               ((w.w & 0x7F807F80u) + 0x00800080u);
-      }
       O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(X[f % PX], P[kb][s], O[d], 0, 0, 0);
       if (f + PX < F) X[f % PX] = v_frag(st, (f + PX) / (2 * ND), (f + PX) / ND % 2, (f + PX) % ND);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if (watch && __ballot((odd & 0x80008000u) != 0)) suspect = true;
+  };
+  // a non-finite value in the tile (an exponent of all ones carries into bit 15; E4M3's NaN is one in bf16 too)
+  auto watch = [&](const uint8_t* st) __attribute__((always_inline)) {
+    uint32_t odd = 0;
+#pragma unroll
+    for (int x = 0; x < C::VBYTES / 1024; ++x) {
+      const uint4 w = *reinterpret_cast<const uint4*>(st + C::KBYTES + 1024 * x + 16 * lane);
+      if constexpr (C::F8) {                               // 0x7F or 0xFF
+        odd |= ((w.x & 0x7F7F7F7Fu) + 0x01010101u) | ((w.y & 0x7F7F7F7Fu) + 0x01010101u) | ((w.z & 0x7F7F7F7Fu) + 0x01010101u) |
+               ((w.w & 0x7F7F7F7Fu) + 0x01010101u);
+      } else {
+        odd |= ((w.x & 0x7F807F80u) + 0x00800080u) | ((w.y & 0x7F807F80u) + 0x00800080u) | ((w.z & 0x7F807F80u) + 0x00800080u) |
+               ((w.w & 0x7F807F80u) + 0x00800080u);
+      }
+      if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (__ballot((odd & 0x80808080u & (C::F8 ? 0x80808080u : 0x80008000u)) != 0)) suspect = true;
   };
   // every row of the wave sees all keys j0 .. j0 + n - 1
   auto open = [&](int j0, int n) {
@@ -542,13 +552,12 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
       if (!busy || j0 > wp_max) continue;
       const uint8_t* st = lds + cur * C::STAGE;
       scores(st);
-      if (open(j0, C::UNIT)) {
-        softmax(j0, false);
-        values(st, false);
-      } else {
-        softmax(j0, true);
-        values(st, true);
+      if (!open(j0, C::UNIT)) {
+        mask(j0);
+        watch(st);
       }
+      softmax();
+      values(st);
     }
   } else {
     const uint8_t* st = lds + wave * C::STAGE;
@@ -567,26 +576,50 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
         issue_k(lds0);
       }
       const bool op = open(j0, 32);
-      if (op) softmax(j0, false);
-      else softmax(j0, true);
+      if (!op) mask(j0);
+      softmax();
       if (more) at_wait_vm(NK);
       else at_wait_vm(0);
-      if (op || wp_min == wp_max) values(st, false);       // one position: what a row does not see, no row sees
-      else values(st, true);
+      if (!op && wp_min != wp_max) watch(st);              // one position: what a row does not see, no row sees
+      values(st);
       at_wait_lds();
       if (more) issue_v(lds0);
     }
   }
   const float vs = C::F8 ? a.v_scale[kv] : 1.0f;
-  // both kinds of sums go their own way to the end: joined before it, they would not fit the registers
-  auto slow = [&](v16f (&O)[C::DV / 32], float& m, float& l) __attribute__((always_inline)) {
-    at_slow<C>(a, rg, b, kv, it0, it1, C::WIDE ? 0 : 32 * wave, C::WIDE ? C::UNIT : 32, Q, pos, valid, c, O, m, l);
+  // the wave's rows once more, one by one; done(row, place of the row, its head, O, m, l)
+  auto slow = [&](auto done) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int r = 0; r < 32; ++r) {
+      const int row = __builtin_amdgcn_readfirstlane((C::WIDE ? 32 * wave : 0) + r), rt = row / a.HT, rh = row - rt * a.HT;
+      if (rt >= toks || rh >= heads) continue;
+      const int hd = kv * a.G + hg * a.HT + rh;
+      float O[C::VCB], m, l;
+      at_slow<C>(a, rg, b, kv, it0, it1, C::WIDE ? 0 : 32 * wave, C::WIDE ? C::UNIT : 32,
+                 a.q + (int64_t)(item.s0 + tok0 + rt) * a.q_stride + hd * C::DK, base_pos + rt,
+                 a.scale * kLog2e * (C::F8 ? a.k_scale[kv] : 1.0f), O, m, l);
+      done(r, rt, hd, O, m, l);
+    }
   };
 
   if constexpr (C::WIDE) {
-    auto finish = [&](const v16f (&O)[C::DV / 32], float m, float l) __attribute__((always_inline)) {
-    l = at_swap_sum(l);
+    if (suspect) {
+      slow([&](int r, int rt, int hd, const float (&O)[C::VCB], float m, float l) __attribute__((always_inline)) {
+        const size_t row = ((size_t)item.slot0 + (size_t)item.split * a.Hh) * (a.TQ * a.HT) + 32 * wave + r;
+        if (ns > 1 && lane == 0) a.part_ml[2 * row] = m, a.part_ml[2 * row + 1] = l;
+        const float sink = a.sink_logits ? a.sink_logits[hd] * kLog2e : -INFINITY;
+        const float top = fmaxf(m, sink), ref = top == -INFINITY ? 0.0f : top;
+        const float f = at_exp2(m - ref), tot = l * f + at_exp2(sink - ref);
+#pragma unroll
+        for (int e = 0; e < C::VCB; ++e) {
+          if (ns > 1) a.part_o[row * C::DV + 64 * e + lane] = O[e] * vs;
+          else a.out[((size_t)(item.s0 + tok0 + rt) * a.Hq + hd) * C::DV + 64 * e + lane] = tot == 0.0f ? 0 : f32_to_bf16(O[e] * (vs * f / tot));
+        }
+      });
+      return;
+    }
     if (!valid) return;
+    l = at_swap_sum(l);
     if (ns > 1) {
       const size_t slot = (size_t)item.slot0 + (size_t)item.split * a.Hh, row = slot * (a.TQ * a.HT) + qt * a.HT + qh;
       if (h == 0) a.part_ml[2 * row] = m, a.part_ml[2 * row + 1] = l;
@@ -612,15 +645,6 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
         if (tot == 0.0f) x = make_uint2(0, 0);
         *reinterpret_cast<uint2*>(a.out + out_at + 32 * d + 2 * i + 4 * h) = x;
       }
-    };
-    if (suspect) {
-      v16f O2[C::DV / 32];
-      float m2, l2;
-      slow(O2, m2, l2);
-      finish(O2, m2, l2);
-    } else {
-      finish(O, m, l);
-    }
   } else {
     // the waves' parts, joined over LDS in wave order: row r at [wave][r][DV], 16-byte pieces turned by the row
     float* po = reinterpret_cast<float*>(lds);
@@ -628,25 +652,26 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
     at_wait_vm(0);
     __syncthreads();                                       // every wave is done with its tiles
     constexpr int NP = C::DV / 4;
-    auto put = [&](const v16f (&O)[C::DV / 32], float m, float l) __attribute__((always_inline)) {
-    l = at_swap_sum(l);
-#pragma unroll
-    for (int d = 0; d < C::DV / 32; ++d)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int piece = 8 * d + i / 2 + h;
-        *reinterpret_cast<float4*>(po + (wave * 32 + r32) * C::DV + 4 * ((piece + r32) & (NP - 1))) =
-            make_float4(O[d][i], O[d][i + 1], O[d][i + 2], O[d][i + 3]);
-      }
-    if (h == 0) pm[2 * (32 * wave + r32)] = m, pm[2 * (32 * wave + r32) + 1] = l;
-    };
     if (suspect) {
-      v16f O2[C::DV / 32];
-      float m2, l2;
-      slow(O2, m2, l2);
-      put(O2, m2, l2);
+      slow([&](int r, int, int, const float (&O)[C::VCB], float m, float l) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < C::VCB; ++e) {
+          const int piece = 16 * e + lane / 4;
+          po[(wave * 32 + r) * C::DV + 4 * ((piece + r) & (NP - 1)) + (lane & 3)] = O[e];
+        }
+        if (lane == 0) pm[2 * (32 * wave + r)] = m, pm[2 * (32 * wave + r) + 1] = l;
+      });
     } else {
-      put(O, m, l);
+      l = at_swap_sum(l);
+#pragma unroll
+      for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int piece = 8 * d + i / 2 + h;
+          *reinterpret_cast<float4*>(po + (wave * 32 + r32) * C::DV + 4 * ((piece + r32) & (NP - 1))) =
+              make_float4(O[d][i], O[d][i + 1], O[d][i + 2], O[d][i + 3]);
+        }
+      if (h == 0) pm[2 * (32 * wave + r32)] = m, pm[2 * (32 * wave + r32) + 1] = l;
     }
     __syncthreads();
     for (int e = t; e < 32 * NP; e += AT_THREADS) {
