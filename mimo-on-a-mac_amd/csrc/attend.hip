@@ -118,29 +118,33 @@ __device__ __forceinline__ bf16x8 at_f8_bf16x8(uint32_t a, uint32_t b) {
 }
 
 // ------------------------------------------------------------------ the work of a block
-// The keys a row tile sees: positions p_min .. p_max, keys lo .. p_max and the first `sinks`; it walks the 64- or 128-key
-// units 0 .. st - 1 (first tokens) and ws .. (window), I in all.
+// The keys a row tile sees: positions p_min .. p_max, keys lo .. p_max and the first `sinks`.  It walks them in groups of 16
+// keys (which lie in one page): groups 0 .. sg - 1 hold the first tokens, group sg starts at org, gt groups in all; a unit is
+// 4 (wide) or 8 groups, I units.
 struct AtRange {
-  int p_min, p_max, lo, sinks, st, ws, I;
+  int p_min, p_max, lo, sinks, sg, org, gt, I;
+  __device__ __forceinline__ int key(int g) const { return g < sg ? 16 * g : org + 16 * (g - sg); }
 };
 __device__ __forceinline__ AtRange at_range(int p_min, int p_max, int window, int sinks, int unit) {
   AtRange r;
   r.p_min = p_min, r.p_max = p_max;
   r.lo = window && p_min >= window ? p_min - window + 1 : 0;
   r.sinks = r.lo ? min(sinks, r.lo) : 0;
-  r.ws = r.lo / unit;
-  r.st = (r.sinks + unit - 1) / unit;
-  if (r.st >= r.ws) r.st = r.ws = 0;
-  r.I = r.st + p_max / unit - r.ws + 1;
+  r.sg = (r.sinks + 15) >> 4;
+  r.org = r.lo & ~15;
+  if (16 * r.sg >= r.org) r.sg = r.org = 0;
+  r.gt = r.sg + ((p_max - r.org) >> 4) + 1;
+  r.I = (16 * r.gt + unit - 1) / unit;
   return r;
 }
 // the most units any row tile of a request of `len` tokens walks
-__device__ __forceinline__ int at_most(int len, int window, int sinks, int TQ, int unit) {
+__host__ __device__ __forceinline__ int at_most(int64_t len, int window, int sinks, int TQ, int unit) {
   if (len <= 0) return 0;
-  const int all = (len - 1) / unit + 1;
-  if (!window) return all;
-  const long long w = ((long long)window + TQ - 2) / unit + 2 + ((long long)min(sinks, len) + unit - 1) / unit;
-  return (int)min((long long)all, w);
+  const int64_t all = (len - 1) / unit + 1;
+  if (!window) return (int)all;
+  const int64_t groups = ((sinks < len ? sinks : len) + 15) / 16 + ((int64_t)window + TQ + 13) / 16 + 1;
+  const int64_t w = (16 * groups + unit - 1) / unit;
+  return (int)(w < all ? w : all);
 }
 
 struct AtItem {
@@ -248,7 +252,7 @@ __device__ __forceinline__ size_t at_row(const AttendArgs& a, const AtRange& r, 
   return (((size_t)page * a.Hkv + kv) << a.page_shift) + (key & ((1 << a.page_shift) - 1));
 }
 
-// One query row (at q, position p) against the keys of units it0 .. it1 - 1, `count` keys from `first` on in each, in plain
+// One query row (at q, position p) against the keys of units it0 .. it1 - 1, `count` groups from `first` on in each, in plain
 // 32-bit arithmetic with the wave's lanes along the head: a hidden key is never touched.  For waves that met a NaN or an
 // infinity in a value that not all of their rows see.  O: dimensions 64 e + lane.
 template <class C>
@@ -265,10 +269,11 @@ __device__ __forceinline__ void at_slow(const AttendArgs& a, const AtRange& r, i
     return C::F8 ? e4m3_unpack2(base[at]).x : bf16_to_f32(reinterpret_cast<const uint16_t*>(base)[at]);
   };
 #pragma unroll 1
-  for (int it = it0; it < it1; ++it) {
-    const int base = (it < r.st ? it : r.ws + it - r.st) * C::UNIT + first;
+  for (int g = it0 * (C::UNIT / 16); g < min(r.gt, it1 * (C::UNIT / 16)); ++g) {
+    if (g % (C::UNIT / 16) < first || g % (C::UNIT / 16) >= first + count) continue;
+    const int base = r.key(g);
 #pragma unroll 1
-    for (int j = base; j < base + count && j <= p; ++j) {
+    for (int j = base; j < base + 16 && j <= p; ++j) {
       if (a.window && j <= p - a.window && j >= a.sinks) continue;
       const int page = at_page(a, a.table[(size_t)b * a.max_pages + (j >> a.page_shift)]);
       const size_t row = (((size_t)page * a.Hkv + kv) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
@@ -352,12 +357,13 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   const int cell_k = C::F8 ? (lane & 3) ^ ((lane >> 4) & 3) : (lane & 7) ^ (lane >> 4);
   const int cell_v = C::F8 ? cell_k : (lane & 7) ^ (4 * ((lane >> 4) & 1));
   const uint32_t lds0 = lds_addr(lds) + (C::WIDE ? 0 : wave * C::STAGE);
-  auto start_of = [&](int it) { return (it < rg.st ? it : rg.ws + it - rg.st) * C::UNIT; };
+  constexpr int UG = C::UNIT / 16, TG = C::KEYS / 16;      // groups of a unit, of an LDS tile
+  const int wg = C::WIDE ? 0 : 2 * wave;                   // the tile's first group in its unit
   constexpr int NG = C::WIDE ? 1 : 2;                      // 16-key groups that the wave copies
   AtKeys kg[NG];
   auto look = [&](int it) __attribute__((always_inline)) {
 #pragma unroll
-    for (int g = 0; g < NG; ++g) kg[g] = at_keys(a, rg, b, start_of(it) + (C::WIDE ? 16 : 32) * wave + 16 * g);
+    for (int g = 0; g < NG; ++g) kg[g] = at_keys(a, rg, b, rg.key(it * UG + (C::WIDE ? wave : wg) + g));
   };
   size_t crow[C::LR];
   auto rows_of = [&]() __attribute__((always_inline)) {
@@ -453,22 +459,26 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   };
   // keys that a row does not see: unsigned(pos - j) < span for the causal order and the window together
   const uint32_t span = a.window ? (uint32_t)a.window : 0x80000000u;
-  auto mask = [&](int j0) __attribute__((always_inline)) {
-    const uint32_t back = (uint32_t)(pos - j0 - 4 * h);
-    if (j0 >= a.sinks) {
+  auto mask = [&](int g0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int kb = 0; kb < C::NB; ++kb)
+    for (int x = 0; x < TG; ++x) {
+      const int j0 = rg.key(g0 + x);
+      const uint32_t back = (uint32_t)(pos - j0 - 4 * h);
+      if (j0 >= a.sinks) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) S[kb][i] = back - (uint32_t)(32 * kb + 8 * (i / 4) + i % 4) < span ? S[kb][i] : -INFINITY;
-    } else {
-      const int first = min(a.sinks, pos + 1) - j0 - 4 * h;  // first tokens that the row sees, from the lane's first key on
-#pragma unroll
-      for (int kb = 0; kb < C::NB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int o = 32 * kb + 8 * (i / 4) + i % 4;
-          S[kb][i] = back - (uint32_t)o < span || o < first ? S[kb][i] : -INFINITY;
+        for (int i = 0; i < 8; ++i) {
+          const float s = S[x / 2][8 * (x % 2) + i];
+          S[x / 2][8 * (x % 2) + i] = back - (uint32_t)(8 * (i / 4) + i % 4) < span ? s : -INFINITY;
         }
+      } else {
+        const int first = min(a.sinks, pos + 1) - j0 - 4 * h;   // first tokens that the row sees, from the lane's first key on
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int o = 8 * (i / 4) + i % 4;
+          const float s = S[x / 2][8 * (x % 2) + i];
+          S[x / 2][8 * (x % 2) + i] = back - (uint32_t)o < span || o < first ? s : -INFINITY;
+        }
+      }
     }
   };
   auto softmax = [&]() __attribute__((always_inline)) {
@@ -529,18 +539,19 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
     }
     if (__ballot((odd & 0x80808080u & (C::F8 ? 0x80808080u : 0x80008000u)) != 0)) suspect = true;
   };
-  // every row of the wave sees all keys j0 .. j0 + n - 1
-  auto open = [&](int j0, int n) {
-    return j0 + n - 1 <= wp_min && (!a.window || j0 > wp_max - a.window || j0 + n <= a.sinks);
+  // every row of the wave sees all keys of the tile from group g0 on
+  auto open = [&](int g0) {
+    const int j0 = rg.key(g0);
+    return g0 >= rg.sg && j0 + C::KEYS - 1 <= wp_min && (!a.window || j0 > wp_max - a.window);
   };
 
-  look(it0);
-  rows_of();
   if constexpr (C::WIDE) {
+    look(it0);
+    rows_of();
     issue_k(lds0);
     issue_v(lds0);
     for (int it = it0; it < it1; ++it) {
-      const int cur = (it - it0) & 1, j0 = start_of(it);
+      const int cur = (it - it0) & 1, g0 = it * UG;
       if (it + 1 < it1) look(it + 1);
       at_wait_vm(0);
       __syncthreads();                                     // the tile has landed everywhere; the other one is free
@@ -549,11 +560,11 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
         issue_k(lds0 + (cur ^ 1) * C::STAGE);
         issue_v(lds0 + (cur ^ 1) * C::STAGE);
       }
-      if (!busy || j0 > wp_max) continue;
+      if (!busy || rg.key(g0) > wp_max) continue;
       const uint8_t* st = lds + cur * C::STAGE;
       scores(st);
-      if (!open(j0, C::UNIT)) {
-        mask(j0);
+      if (!open(g0)) {
+        mask(g0);
         watch(st);
       }
       softmax();
@@ -562,11 +573,16 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   } else {
     const uint8_t* st = lds + wave * C::STAGE;
     constexpr int NK = C::LR * C::KCB, NV = C::LR * C::VCB;
-    issue_k(lds0);
-    issue_v(lds0);
-    for (int it = it0; it < it1; ++it) {
-      const int j0 = start_of(it) + 32 * wave;
-      const bool more = it + 1 < it1;
+    const int end = min(it1, (rg.gt - wg + UG - 1) / UG);  // of the units that hold groups of this wave
+    if (it0 < end) {
+      look(it0);
+      rows_of();
+      issue_k(lds0);
+      issue_v(lds0);
+    }
+    for (int it = it0; it < end; ++it) {
+      const int g0 = it * UG + wg;
+      const bool more = it + 1 < end;
       if (more) look(it + 1);
       at_wait_vm(NV);
       scores(st);
@@ -575,8 +591,8 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
         rows_of();
         issue_k(lds0);
       }
-      const bool op = open(j0, 32);
-      if (!op) mask(j0);
+      const bool op = open(g0);
+      if (!op) mask(g0);
       softmax();
       if (more) at_wait_vm(NK);
       else at_wait_vm(0);
@@ -595,7 +611,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
       if (rt >= toks || rh >= heads) continue;
       const int hd = kv * a.G + hg * a.HT + rh;
       float O[C::VCB], m, l;
-      at_slow<C>(a, rg, b, kv, it0, it1, C::WIDE ? 0 : 32 * wave, C::WIDE ? C::UNIT : 32,
+      at_slow<C>(a, rg, b, kv, it0, it1, C::WIDE ? 0 : 2 * wave, C::WIDE ? 4 : 2,
                  a.q + (int64_t)(item.s0 + tok0 + rt) * a.q_stride + hd * C::DK, base_pos + rt,
                  a.scale * kLog2e * (C::F8 ? a.k_scale[kv] : 1.0f), O, m, l);
       done(r, rt, hd, O, m, l);
@@ -708,52 +724,75 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   }
 }
 
-// The parts of split row tiles, joined in order: out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j.  A block takes one token
-// and head group, hpb of its heads; its four waves share the parts of a head.
-template <int DV>
-__global__ void __launch_bounds__(256) attend_join_kernel(AttendArgs a, int hpb) {
-  __shared__ float sl[4], so[4][DV];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int per = (a.HT + hpb - 1) / hpb;
-  const int n = blockIdx.x / (a.Hh * per), rest = blockIdx.x - n * a.Hh * per, hh = rest / per, q0 = (rest - hh * per) * hpb;
+// The parts of split row tiles, joined in order: out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j.  A block looks at `per`
+// (token, head group) entries, of each at hpb heads from the block's on; its W waves share the parts of a head, wave w parts
+// w, w + W, ...: few rows with many parts take 16 waves, so that the parts arrive in one or two round trips.
+template <int DV, int W>
+__global__ void __launch_bounds__(64 * W) attend_join_kernel(AttendArgs a, int per, int hpb) {
+  __shared__ float sl[W], so[W][DV];
+  __shared__ int2 s_meta[256];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int cuts = (a.HT + hpb - 1) / hpb, entries = a.N * a.Hh;
+  const int e0 = blockIdx.x / cuts * per, q0 = blockIdx.x % cuts * hpb;
   const int first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N);
-  if (n < first || n >= last) return;
-  const int2 mt = a.meta[(size_t)n * a.Hh + hh];
-  const int ns = mt.y & 0xFFFF;
-  if (ns <= 1 || mt.x < 0) return;
-  const int hg = hh % a.HG, kv = hh / a.HG, heads = min(a.HT, a.G - hg * a.HT);
+  for (int e = t; e < per; e += 64 * W) {
+    const int n = (e0 + e) / a.Hh;
+    s_meta[e] = e0 + e < entries && n >= first && n < last ? a.meta[e0 + e] : make_int2(0, 0);
+  }
+  __syncthreads();
   constexpr int E = DV / 64;
-  for (int qh = q0; qh < min(heads, q0 + hpb); ++qh) {
-    const size_t rows = (size_t)a.TQ * a.HT, row0 = (size_t)mt.x * rows + (size_t)(mt.y >> 16) * a.HT + qh, step = rows * a.Hh;
-    float top = -INFINITY;
-    for (int j = lane; j < ns; j += 64) top = fmaxf(top, a.part_ml[2 * (row0 + j * step)]);
+  for (int e = 0; e < per; ++e) {
+    const int2 mt = s_meta[e];
+    const int ns = mt.y & 0xFFFF;
+    if (ns <= 1) continue;
+    const int n = (e0 + e) / a.Hh, hh = (e0 + e) % a.Hh;
+    const int hg = hh % a.HG, kv = hh / a.HG, heads = min(a.HT, a.G - hg * a.HT);
+    for (int qh = q0; qh < min(heads, q0 + hpb); ++qh) {
+      const size_t rows = (size_t)a.TQ * a.HT, row0 = (size_t)mt.x * rows + (size_t)(mt.y >> 16) * a.HT + qh, step = rows * a.Hh;
+      float top = -INFINITY;
+      for (int j = lane; j < ns; j += 64) top = fmaxf(top, a.part_ml[2 * (row0 + j * step)]);
 #pragma unroll
-    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float tot = 0.0f, x[E];
+      for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float tot = 0.0f, x[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = 0.0f;
-#pragma unroll 4
-    for (int j = wave; j < ns; j += 4) {
-      const size_t row = row0 + j * step;
-      const float f = at_exp2(a.part_ml[2 * row] - ref);
-      tot += f * a.part_ml[2 * row + 1];
+      for (int i = 0; i < E; ++i) x[i] = 0.0f;
+      for (int j0 = wave; j0 < ns; j0 += 64 * W) {         // lane i: part j0 + W i
+        const int mine = j0 + W * lane, count = min(64, (ns - j0 + W - 1) / W);
+        float f = 0.0f;
+        if (mine < ns) {
+          const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (row0 + mine * step));
+          f = at_exp2(ml.x - ref);
+          tot += f * ml.y;
+        }
+#pragma unroll 8
+        for (int i = 0; i < count; ++i) {
+          const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), i));
+          const float* o = a.part_o + (row0 + (size_t)(j0 + W * i) * step) * DV + E * lane;
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] += f * a.part_o[row * DV + E * lane + e];
+          for (int k = 0; k < E; ++k) x[k] += w * o[k];
+        }
+      }
+#pragma unroll
+      for (int d = 32; d; d >>= 1) tot += __shfl_xor(tot, d, 64);
+#pragma unroll
+      for (int k = 0; k < E; ++k) so[wave][E * lane + k] = x[k];
+      if (lane == 0) sl[wave] = tot;
+      __syncthreads();
+      const int head = kv * a.G + hg * a.HT + qh;
+      const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
+      const float all = fmaxf(top, sink), r2 = all == -INFINITY ? 0.0f : all, g = at_exp2(top - r2);
+      float sum = at_exp2(sink - r2);
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum += sl[w] * g;
+      if (t < DV) {
+        float y = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) y += so[w][t];
+        a.out[((size_t)n * a.Hq + head) * DV + t] = sum == 0.0f ? 0 : f32_to_bf16(y * g / sum);
+      }
+      __syncthreads();
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) so[wave][E * lane + e] = x[e];
-    if (lane == 0) sl[wave] = tot;
-    __syncthreads();
-    const int head = kv * a.G + hg * a.HT + qh;
-    const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
-    const float all = fmaxf(top, sink), r2 = all == -INFINITY ? 0.0f : all, g = at_exp2(top - r2);
-    const float sum = (sl[0] + sl[1] + sl[2] + sl[3]) * g + at_exp2(sink - r2);
-    for (int d = threadIdx.x; d < DV; d += 256) {
-      const float y = (so[0][d] + so[1][d] + so[2][d] + so[3][d]) * g;
-      a.out[((size_t)n * a.Hq + head) * DV + d] = sum == 0.0f ? 0 : f32_to_bf16(y / sum);
-    }
-    __syncthreads();
   }
 }
 
@@ -797,12 +836,18 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   }
   if (int e = check_launch("attend")) return e;
   if (!join) return MIMO_OK;
-  const int hpb = (int64_t)a.N * a.Hh >= 1024 ? a.HT : 1;
-  const int64_t blocks = (int64_t)a.N * a.Hh * ((a.HT + hpb - 1) / hpb);
-  MIMO_REQUIRE(blocks < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many rows");
+  const int64_t entries = (int64_t)a.N * a.Hh, rows = entries * a.HT;
+  MIMO_REQUIRE(rows < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many rows");
   {
     ProfScope p(st, "attend_join");
-    attend_join_kernel<C::DV><<<(unsigned)blocks, 256, 0, st>>>(a, hpb);
+    if (rows <= 256) {
+      attend_join_kernel<C::DV, 16><<<(unsigned)rows, 1024, 0, st>>>(a, 1, 1);
+    } else if (rows <= 8192) {
+      attend_join_kernel<C::DV, 4><<<(unsigned)rows, 256, 0, st>>>(a, 1, 1);
+    } else {                                               // mostly rows that were not split: a block looks at many
+      const int per = (int)std::min<int64_t>(256, (entries + 1023) / 1024);
+      attend_join_kernel<C::DV, 4><<<(unsigned)((entries + per - 1) / per), 256, 0, st>>>(a, per, a.HT);
+    }
   }
   return check_launch("attend_join");
 }
@@ -838,9 +883,10 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   MIMO_REQUIRE(q && starts && lens && table && out, MIMO_ERR_ARG, "cache_attend: null pointer");
   MIMO_REQUIRE(heads >= 1 && heads % cache->kv_heads == 0 && heads <= 1024, MIMO_ERR_SHAPE,
                "cache_attend: %d heads on %d K/V heads (a multiple, at most 1024)", heads, cache->kv_heads);
-  MIMO_REQUIRE(B >= 1 && max_pages >= 1 && max_new >= 0 && (int64_t)max_pages * cache->page_size <= 0x7fffffff &&
+  MIMO_REQUIRE(B >= 1 && max_pages >= 1 && max_new >= 0 && (int64_t)max_pages * cache->page_size <= kMaxTokens &&
                    (int64_t)max_pages * B <= 0x7fffffff, MIMO_ERR_SHAPE,
-               "cache_attend: need B, max_pages >= 1, max_new >= 0, at most 2^31 - 1 table entries and tokens of a request (got %d, %d, %d)",
+               "cache_attend: need B, max_pages >= 1, max_new >= 0, at most 2^31 - 1 table entries, 2^31 - 2^16 tokens of a request "
+               "(got %d, %d, %d)",
                B, max_pages, max_new);
   MIMO_REQUIRE(window >= 0 && sink_tokens >= 0, MIMO_ERR_SHAPE, "cache_attend: window and sink_tokens must be >= 0");
   MIMO_REQUIRE(scale == scale && scale - scale == 0.0f, MIMO_ERR_ARG, "cache_attend: scale must be finite");
@@ -862,9 +908,7 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   a.chunk_min = wide ? AT_WIDE_MIN : AT_NARROW_MIN;
   a.target = wide ? AT_WIDE_TARGET : AT_NARROW_TARGET;
   // no tile can walk more units than the table or the window holds; if that is within chunk_min nothing is ever split
-  const int64_t unit = wide ? 64 : 128;
-  int64_t most = ((int64_t)max_pages * cache->page_size - 1) / unit + 1;
-  if (window) most = std::min(most, ((int64_t)window + a.TQ - 2) / unit + 2 + ((int64_t)a.sinks + unit - 1) / unit);
+  const int most = at_most((int64_t)max_pages * cache->page_size, window, a.sinks, a.TQ, wide ? 64 : 128);
   const bool join = most > a.chunk_min;
   const AtRoom room = at_room(wide ? 128 : 32, a.target, N, heads, cache->kv_heads, cache->v_dim);
   char* w = static_cast<char*>(ws);

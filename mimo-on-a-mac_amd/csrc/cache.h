@@ -6,6 +6,9 @@
 
 namespace mimo {
 
+// tokens of one request that a page table may hold: key numbers a tile past the last stay below 2^31
+constexpr int64_t kMaxTokens = 0x7fff0000;
+
 int check_cache(const mimo_kv_cache* c, const char* what);
 
 }  // namespace mimo

@@ -17,8 +17,8 @@ namespace mimo {
 // T[j] = F[j] while j < freed, else free[n_free - 1 - (j - freed)].  So a step that is taken back restores the stack, and
 // places below n_free are only read, places from n_free on only written: no order between blocks matters.
 //
-// Every block scans all requests for itself (a few KB from L2), so that one launch does the whole step; block 0 writes the
-// tables, all blocks share the tokens.  A token in a page taken in this step gets its page from T directly.
+// Every block scans all requests for itself (a few KB from L2), so that one launch does the whole step and the blocks share
+// tokens, table entries and returned pages.  A token in a page taken in this step gets its page from T directly.
 constexpr int ST_THREADS = 1024;
 constexpr int ST_MAX_REQS = 4096;
 constexpr int ST_MAX_TOKENS = 1 << 20;              // the scan's 1024 partial sums of at most this stay below 2^31
@@ -142,12 +142,13 @@ __global__ void __launch_bounds__(ST_THREADS) cache_step_kernel(StepArgs a) {
     a.slots[n] = slot;
     a.positions[n] = pos;
   }
-  if (!first) return;
-  for (int j = t; j < taken; j += ST_THREADS) {
+  const int from = blockIdx.x * ST_THREADS + t, all = gridDim.x * ST_THREADS;
+  for (int j = from; j < taken; j += all) {
     const int b = owner(s_take, j);
     a.table[(size_t)b * a.max_pages + pages(a.lens[b]) + (j - s_take[b])] = fresh(j);
   }
-  for (int i = t; i < freed - taken; i += ST_THREADS) a.free_pages[n_free + i] = released(freed - 1 - i);
+  for (int i = from; i < freed - taken; i += all) a.free_pages[n_free + i] = released(freed - 1 - i);
+  if (!first) return;
   for (int b = t; b <= B; b += ST_THREADS) a.starts[b] = s_new[b];
   if (a.commit_lens) __syncthreads();                // every read of the old lengths is done
   for (int b = t; b < B; b += ST_THREADS) {
@@ -308,9 +309,9 @@ int mimo_cache_step(const int32_t* lens, const int32_t* target, int B, int32_t* 
                "cache_step: need N, max_new >= 0 and max_pages, n_pages >= 1 (got %d, %d, %d, %d)", N, max_new, max_pages, n_pages);
   MIMO_REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0, MIMO_ERR_SHAPE,
                "cache_step: page_size %d (a power of two from 16 to 1024)", page_size);
-  MIMO_REQUIRE((int64_t)n_pages * page_size <= 0x7fffffff && (int64_t)max_pages * page_size <= 0x7fffffff &&
+  MIMO_REQUIRE((int64_t)n_pages * page_size <= 0x7fffffff && (int64_t)max_pages * page_size <= kMaxTokens &&
                    (int64_t)max_pages * B <= 0x7fffffff, MIMO_ERR_SHAPE,
-               "cache_step: at most 2^31 - 1 slots, tokens of a request and table entries");
+               "cache_step: at most 2^31 - 1 slots and table entries, 2^31 - 2^16 tokens of a request");
   MIMO_REQUIRE(lens_out != lens && n_free_out != n_free, MIMO_ERR_ARG, "cache_step: lens_out and n_free_out may not alias the state");
   MIMO_REQUIRE(!commit_lens == !commit_n_free, MIMO_ERR_ARG, "cache_step: commit_lens and commit_n_free go together");
   StepArgs a{lens, target, n_free, table, free_pages, B, max_pages, n_pages, __builtin_ctz(page_size), N, max_new,
