@@ -19,8 +19,8 @@
 //
 // Masks.  A tile's loads touch only keys that some row of the tile sees: others (past the last position, between the first
 // tokens and the window) read a visible row again, and their weights are set to 0.  A key that one row sees and another does
-// not still meets the other's weight 0 in the product, and 0 * NaN is NaN: tiles with such masks look for non-finite V
-// operands, and a wave that found one takes its sums again key by key.
+// not still meets the other's weight 0 in the product, and 0 * NaN is NaN: a wave whose sums are not finite looks for such
+// values in its tiles with masks, and if there are any takes its sums again key by key.
 //
 // Work is cut so that the card is full: a device-side count of all requests' tiles gives the number of key tiles per block
 // (chunk); a row tile with more is split over several blocks, whose (O, m, l) a second kernel joins in a fixed order.
@@ -427,7 +427,6 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
 #pragma unroll
     for (int i = 0; i < 16; ++i) O[d][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;                           // l: this lane half's keys
-  bool suspect = false;
 
   v16f S[C::NB];
   bf16x8 P[C::NB][2];
@@ -442,16 +441,13 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
     for (int f = 0; f < F; ++f) {
       const int kb = f % C::NB, s = f / C::NB;
       __builtin_amdgcn_sched_barrier(0);
-      if (s == 0) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) S[kb][i] = 0.0f;
-      }
+      const v16f none = {0.0f};
       const uint4 x = X[f % PX];
       if constexpr (C::F8) {
-        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.x, x.y), Q[2 * s], S[kb], 0, 0, 0);
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.x, x.y), Q[2 * s], s == 0 ? none : S[kb], 0, 0, 0);
         S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.z, x.w), Q[2 * s + 1], S[kb], 0, 0, 0);
       } else {
-        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), Q[s], S[kb], 0, 0, 0);
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), Q[s], s == 0 ? none : S[kb], 0, 0, 0);
       }
       if (f + PX < F) X[f % PX] = k_read(st, (f + PX) % C::NB, (f + PX) / C::NB);
     }
@@ -522,23 +518,6 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  // a non-finite value in the tile (an exponent of all ones carries into bit 15; E4M3's NaN is one in bf16 too)
-  auto watch = [&](const uint8_t* st) __attribute__((always_inline)) {
-    uint32_t odd = 0;
-#pragma unroll
-    for (int x = 0; x < C::VBYTES / 1024; ++x) {
-      const uint4 w = *reinterpret_cast<const uint4*>(st + C::KBYTES + 1024 * x + 16 * lane);
-      if constexpr (C::F8) {                               // 0x7F or 0xFF
-        odd |= ((w.x & 0x7F7F7F7Fu) + 0x01010101u) | ((w.y & 0x7F7F7F7Fu) + 0x01010101u) | ((w.z & 0x7F7F7F7Fu) + 0x01010101u) |
-               ((w.w & 0x7F7F7F7Fu) + 0x01010101u);
-      } else {
-        odd |= ((w.x & 0x7F807F80u) + 0x00800080u) | ((w.y & 0x7F807F80u) + 0x00800080u) | ((w.z & 0x7F807F80u) + 0x00800080u) |
-               ((w.w & 0x7F807F80u) + 0x00800080u);
-      }
-      if (x % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-    }
-    if (__ballot((odd & 0x80808080u & (C::F8 ? 0x80808080u : 0x80008000u)) != 0)) suspect = true;
-  };
   // every row of the wave sees all keys of the tile from group g0 on
   auto open = [&](int g0) {
     const int j0 = rg.key(g0);
@@ -563,10 +542,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
       if (!busy || rg.key(g0) > wp_max) continue;
       const uint8_t* st = lds + cur * C::STAGE;
       scores(st);
-      if (!open(g0)) {
-        mask(g0);
-        watch(st);
-      }
+      if (!open(g0)) mask(g0);
       softmax();
       values(st);
     }
@@ -591,15 +567,39 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
         rows_of();
         issue_k(lds0);
       }
-      const bool op = open(g0);
-      if (!op) mask(g0);
+      if (!open(g0)) mask(g0);
       softmax();
       if (more) at_wait_vm(NK);
       else at_wait_vm(0);
-      if (!op && wp_min != wp_max) watch(st);              // one position: what a row does not see, no row sees
       values(st);
       at_wait_lds();
       if (more) issue_v(lds0);
+    }
+  }
+  // Sums that are not finite: if a value of a tile with masks is not (one position sees what another does not), it may have
+  // come through a weight of 0
+  bool suspect = false;
+  {
+    float worst = 0.0f;
+#pragma unroll
+    for (int d = 0; d < C::DV / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) worst += O[d][i] - O[d][i];   // 0, or NaN
+    if (wp_min != wp_max && __ballot(busy && worst != 0.0f)) {
+      bool odd = false;
+#pragma unroll 1
+      for (int g = it0 * UG; g < min(rg.gt, it1 * UG); ++g) {
+        if (open(g / TG * TG)) continue;
+        const AtKeys k = at_keys(a, rg, b, rg.key(g));
+        const int page = at_page(a, k.id);
+#pragma unroll 1
+        for (int x = 0; x < 16; ++x) {
+          const size_t row = at_row(a, rg, k, page, kv, x) * C::DV;
+          const uint32_t w = lane < C::DV * ES / 4 ? *reinterpret_cast<const uint32_t*>(a.v + row * ES + 4 * lane) : 0u;
+          odd |= C::F8 ? (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0 : (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) != 0;
+        }
+      }
+      suspect = __ballot(odd) != 0;
     }
   }
   const float vs = C::F8 ? a.v_scale[kv] : 1.0f;

@@ -10,6 +10,7 @@ runs on one request's KVCache / RotatingKVCache (engine/mimo_stream/model.py:169
 batch: requests decoding one token and requests with a chunk of new tokens, in one call each.  Lengths and tables stay on
 the device, nothing synchronises, and every call can be captured into a HIP graph; a step's one plan serves every layer.
 """
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -19,10 +20,16 @@ import torch
 from . import _lib
 
 E4M3 = torch.float8_e4m3fn
+BF16 = torch.bfloat16
+INT32 = torch.int32
 
 STATUS_MESSAGES = {_lib.ERR_PAGES: "fewer free pages than the step needs",
                    _lib.ERR_SHAPE: "request lengths outside the page table, the step's rows or max_new",
                    _lib.ERR_SLOT: "a page or slot outside the cache"}
+
+# A decode step makes one step call and two calls per layer, each of a few microseconds on the GPU: what they do on the host
+# is kept short (one check per tensor, entry points and structs looked up once).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _device(device):
@@ -30,18 +37,32 @@ def _device(device):
     return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
 
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} on {t.device}, expected {dev}")
+@functools.lru_cache(maxsize=None)
+def _entry(name):
+    return getattr(_lib.load(), name)
+
+
+def _call(name, *args):
+    rc = _entry(name)(*args)
+    if rc != _lib.MIMO_OK:
+        _lib.check(rc, name)
+
+
+def _gpu(dev):
+    if dev.type != "cuda":
+        raise ValueError("libmimo_moe works on device tensors; got a CPU tensor")
+    return dev.index
 
 
 def _int32(t, dev, shape, name):
-    """The int32 device tensor that a kernel reads or writes in place: checked, never converted."""
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: need a contiguous int32 tensor of shape {tuple(shape)}")
-    _same_device(dev, **{name: t})
-    return t
+    """Address of the int32 device tensor that a kernel reads or writes in place: checked, never converted."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is INT32 and t.device == dev and t.shape == shape and t.is_contiguous()):
+        raise ValueError(f"{name}: need a contiguous int32 tensor of shape {tuple(shape)} on {dev}")
+    return t.data_ptr()
+
+
+def _status(plan, dev):
+    return None if plan.status is None else _int32(plan.status, dev, (1,), "plan.status")
 
 
 @dataclass
@@ -70,8 +91,8 @@ class StepPlan:
 class PageTable:
     """Lengths, page tables and the free pages of up to max_seqs requests, on the device.
 
-    One PageTable serves every layer whose caches have its pages.  All state is plain tensors: lens int32 [max_seqs], table
-    int32 [max_seqs, max_pages], free int32 [n_pages] (a stack), n_free int32 [1]."""
+    One PageTable serves every layer whose caches have its pages.  The state is int32 tensors, changed in place only: lens
+    [max_seqs], table [max_seqs, max_pages], free [n_pages] (a stack), n_free [1]."""
 
     def __init__(self, max_seqs, max_pages, n_pages, page_size, device="cuda"):
         dev = _device(device)
@@ -81,10 +102,15 @@ class PageTable:
             raise ValueError("page_size must be a power of two from 16 to 1024")
         self.page_size = int(page_size)
         self.n_pages = int(n_pages)
-        self.lens = torch.zeros(max_seqs, dtype=torch.int32, device=dev)
-        self.table = torch.zeros((max_seqs, max_pages), dtype=torch.int32, device=dev)
-        self.free = torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device=dev)     # page 0 is taken first
-        self.n_free = torch.full((1,), n_pages, dtype=torch.int32, device=dev)
+        self._lens = torch.zeros(max_seqs, dtype=INT32, device=dev)
+        self._table = torch.zeros((max_seqs, max_pages), dtype=INT32, device=dev)
+        self._free = torch.arange(n_pages - 1, -1, -1, dtype=INT32, device=dev)     # page 0 is taken first
+        self._n_free = torch.full((1,), n_pages, dtype=INT32, device=dev)
+
+    lens = property(lambda self: self._lens)
+    table = property(lambda self: self._table)
+    free = property(lambda self: self._free)
+    n_free = property(lambda self: self._n_free)
 
     def step(self, target, n_tokens, max_new=None, commit=True):
         """Bring every request to target[b] tokens (int32 [max_seqs]; 0 ends a request, fewer takes tokens back).
@@ -93,24 +119,27 @@ class PageTable:
         this many new tokens on one request (default n_tokens).  With commit=False the page table keeps its lengths and
         free pages, and the step can be dropped or made again.  Returns a StepPlan; a failure (too few free pages, lengths
         out of range) leaves the state as it was and is in plan.status (plan.check() raises)."""
-        dev = self.lens.device
-        B, width = self.table.shape
-        _lib.require_cuda(self.lens)
-        target = _int32(target, dev, (B,), "target")
+        dev = self._lens.device
+        index = _gpu(dev)
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(dev):
+                return self.step(target, n_tokens, max_new, commit)
+        B, width = self._table.shape
+        at_target = _int32(target, dev, (B,), "target")
         n_tokens = int(n_tokens)
         if n_tokens < 0:
             raise ValueError("n_tokens must be >= 0")
         max_new = n_tokens if max_new is None else int(max_new)
-        with torch.cuda.device(dev):
-            out = torch.empty(2 * B + 3 + 2 * n_tokens, dtype=torch.int32, device=dev)
-            lens, n_free, status, starts, slots, positions = out.split([B, 1, 1, B + 1, n_tokens, n_tokens])
-            _lib.call("mimo_cache_step", _lib.ptr(self.lens), _lib.ptr(target), B, _lib.ptr(self.table), width,
-                      _lib.ptr(self.free), _lib.ptr(self.n_free), self.n_pages, self.page_size, n_tokens, max_new,
-                      _lib.ptr(lens), _lib.ptr(n_free), _lib.ptr(starts), _lib.ptr(slots), _lib.ptr(positions),
-                      _lib.ptr(self.lens if commit else None), _lib.ptr(self.n_free if commit else None), _lib.ptr(status),
-                      _lib.stream_ptr(dev))
-        return StepPlan(starts=starts, lens=lens, slots=slots, positions=positions, table=self.table, max_new=max_new,
-                        n_free=n_free, status=status)
+        out = torch.empty(2 * B + 3 + 2 * n_tokens, dtype=INT32, device=dev)
+        lens, n_free, status, starts, slots, positions = out.split_with_sizes((B, 1, 1, B + 1, n_tokens, n_tokens))
+        at = out.data_ptr()
+        at_starts = at + 4 * B + 8
+        at_slots = at_starts + 4 * B + 4
+        state, count = self._lens.data_ptr(), self._n_free.data_ptr()
+        _call("mimo_cache_step", state, at_target, B, self._table.data_ptr(), width, self._free.data_ptr(), count, self.n_pages,
+              self.page_size, n_tokens, max_new, at, at + 4 * B, at_starts, at_slots, at_slots + 4 * n_tokens,
+              state if commit else None, count if commit else None, at + 4 * B + 4, _raw_stream(index))
+        return StepPlan(starts, lens, slots, positions, self._table, max_new, n_free, status)
 
 
 class KVCache:
@@ -136,6 +165,8 @@ class KVCache:
             raise ValueError("a K/V cache holds bfloat16 or float8_e4m3fn")
         if k.dtype == torch.uint8:
             k, v = k.view(dtype), v.view(dtype)
+        if k.device != v.device:
+            raise ValueError(f"k on {k.device}, v on {v.device}")
         if k.dim() != 4 or v.dim() != 4 or k.shape[:3] != v.shape[:3] or v.dtype != dtype:
             raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [pages, kv_heads, page_size, dim] of one type")
         if not k.is_contiguous() or not v.is_contiguous():
@@ -152,13 +183,16 @@ class KVCache:
                                 for s in (k_scale, v_scale))
         elif k_scale is not None or v_scale is not None:
             raise ValueError("scales belong to an E4M3 cache")
-        self.k, self.v, self.k_scale, self.v_scale, self.dtype = k, v, k_scale, v_scale, dtype
+        self._tensors = (k, v, k_scale, v_scale)             # fixed: the struct holds their addresses
+        self.dtype, self.device = dtype, k.device
         self.kv_heads, self.k_dim, self.v_dim, self.page_size, self.n_pages = heads, k_dim, v.shape[3], page, n_pages
+        self._struct = _lib.MimoKvCache(*(_lib.ptr(t) for t in self._tensors), 1 if dtype == E4M3 else 0, n_pages, page,
+                                        heads, k_dim, v.shape[3])
 
-    def struct(self):
-        return _lib.MimoKvCache(_lib.ptr(self.k), _lib.ptr(self.v), _lib.ptr(self.k_scale), _lib.ptr(self.v_scale),
-                                1 if self.dtype == E4M3 else 0, self.n_pages, self.page_size, self.kv_heads, self.k_dim,
-                                self.v_dim)
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
 
 
 class Rotary:
@@ -176,62 +210,76 @@ class Rotary:
 
 
 def _rows(x, dev, heads, dim, name):
-    """x as bf16 rows the kernels can read: [N, heads, dim] with contiguous, 16-byte aligned tokens at any distance."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.shape[2] != dim or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{name}: need [tokens, {'heads' if heads is None else heads}, {dim}]"
-                         + (f", got {tuple(x.shape)}" if isinstance(x, torch.Tensor) else ""))
-    _lib.require_cuda(x)
-    _same_device(dev, **{name: x})
-    x = x.to(torch.bfloat16)
-    if x.stride(2) != 1 or x.stride(1) != dim or x.stride(0) % 8 or x.stride(0) < x.shape[1] * dim or x.data_ptr() % 16:
-        x = x.contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-    return x
+    """(x, address, elements between tokens): x as bf16 rows the kernels can read, [N, heads, dim] with contiguous, 16-byte
+    aligned tokens at any distance; copied when it is not."""
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name}: need [tokens, {'heads' if heads is None else heads}, {dim}], got {tuple(shape)}")
+    if x.device != dev:
+        raise ValueError(f"{name} on {x.device}, expected {dev}")
+    if x.dtype is not BF16:
+        x = x.to(BF16)
+    s0, s1, s2 = x.stride()
+    row = shape[1] * dim
+    at = x.data_ptr()
+    if shape[0] <= 1:
+        s0 = row                                             # one token: any distance will do
+    if s2 != 1 or (s1 != dim and shape[1] != 1) or s0 % 8 or s0 < row or at % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        s0, at = row, x.data_ptr()
+    return x, at, s0
 
 
 def append(cache, plan, k, v, q=None, rotary=None):
     """Write the new tokens' k [N, kv_heads, k_dim] and v [N, kv_heads, v_dim] to plan.slots (rows with slot -1 are left
     out), k rotated to plan.positions; returns q [N, heads, k_dim] rotated likewise (None without q).  q, k and v may be
     views of one projection's rows."""
-    dev = cache.k.device
-    _lib.require_cuda(cache.k)
-    k = _rows(k, dev, cache.kv_heads, cache.k_dim, "k")
-    v = _rows(v, dev, cache.kv_heads, cache.v_dim, "v")
+    dev = cache.device
+    index = _gpu(dev)
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(dev):
+            return append(cache, plan, k, v, q, rotary)
+    k, at_k, k_stride = _rows(k, dev, cache.kv_heads, cache.k_dim, "k")
+    v, at_v, v_stride = _rows(v, dev, cache.kv_heads, cache.v_dim, "v")
     N = k.shape[0]
     if v.shape[0] != N:
         raise ValueError(f"{N} tokens of k, {v.shape[0]} of v")
-    slots = _int32(plan.slots, dev, (N,), "plan.slots")
-    positions = _int32(plan.positions, dev, (N,), "plan.positions")
-    _same_device(dev, status=plan.status)
-    dim = 0
+    at_slots = _int32(plan.slots, dev, (N,), "plan.slots")
+    at_positions = _int32(plan.positions, dev, (N,), "plan.positions")
+    dim, turns = 0, None
     if rotary is not None:
         dim = rotary.dim
         if dim > cache.k_dim:
             raise ValueError(f"rotary dimension {dim} past the head's {cache.k_dim}")
-        _same_device(dev, rotary=rotary.turns)
-    out, heads = None, 0
+        if rotary.turns.device != dev:
+            raise ValueError(f"rotary on {rotary.turns.device}, expected {dev}")
+        turns = rotary.turns.data_ptr()
+    out, at_q, at_out, q_stride, heads = None, None, None, 0, 0
     if q is not None:
-        q = _rows(q, dev, None, cache.k_dim, "q")
+        q, at_q, q_stride = _rows(q, dev, None, cache.k_dim, "q")
         if q.shape[0] != N:
             raise ValueError(f"{N} tokens of k, {q.shape[0]} of q")
         heads = q.shape[1]
-        out = torch.empty((N, heads, cache.k_dim), dtype=torch.bfloat16, device=dev)
-    if N == 0:
-        return out
-    with torch.cuda.device(dev):
-        _lib.call("mimo_cache_append", _lib.ptr(q), 0 if q is None else q.stride(0), heads, _lib.ptr(k), k.stride(0),
-                  _lib.ptr(v), v.stride(0), N, _lib.ptr(positions), _lib.ptr(slots), cache.struct(), dim,
-                  _lib.ptr(None if rotary is None else rotary.turns), _lib.ptr(out), _lib.ptr(plan.status),
-                  _lib.stream_ptr(dev))
+        out = torch.empty((N, heads, cache.k_dim), dtype=BF16, device=dev)
+        at_out = out.data_ptr()
+    status = _status(plan, dev)
+    if N:
+        _call("mimo_cache_append", at_q, q_stride, heads, at_k, k_stride, at_v, v_stride, N, at_positions, at_slots,
+              cache._struct, dim, turns, at_out, status, _raw_stream(index))
     return out
 
 
-def _workspace(nbytes, dev):
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(N, heads, kv_heads, v_dim):
+    return _entry("mimo_cache_attend_workspace_size")(N, heads, kv_heads, v_dim)
+
+
+def _workspace(nbytes, dev, stream):
     """A workspace of this call's own in a captured graph (two graphs never share one), else the stream's cached one."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    return _lib.workspace(nbytes, dev, "attend")
+    ws = _lib._ws.get((dev.index, stream, "attend"))
+    return ws if ws is not None and ws.numel() >= nbytes else _lib.workspace(nbytes, dev, "attend")
 
 
 def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None, out=None):
@@ -240,39 +288,40 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
     A token at position p sees its request's keys j <= p; with window > 0 those with p - j < window, and the first
     sink_tokens.  scale defaults to k_dim ** -0.5.  sink_logits fp32 [heads]: a logit that joins each row's softmax without
     a value.  Returns bf16 [N, heads, v_dim] (out, if given: contiguous bf16); rows of no request are 0."""
-    dev = cache.k.device
-    _lib.require_cuda(cache.k)
-    q = _rows(q, dev, None, cache.k_dim, "q")
-    N, heads = q.shape[:2]
+    dev = cache.device
+    index = _gpu(dev)
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(dev):
+            return attend(q, cache, plan, scale, window, sink_tokens, sink_logits, out)
+    q, at_q, q_stride = _rows(q, dev, None, cache.k_dim, "q")
+    N, heads, _ = q.shape
     if heads < 1 or heads % cache.kv_heads:
         raise ValueError(f"{heads} heads on {cache.kv_heads} K/V heads")
     if plan.table is None or plan.table.dim() != 2:
         raise ValueError("the plan has no page table")
     B, width = plan.table.shape
-    table = _int32(plan.table, dev, (B, width), "plan.table")
-    starts = _int32(plan.starts, dev, (B + 1,), "plan.starts")
-    lens = _int32(plan.lens, dev, (B,), "plan.lens")
-    _same_device(dev, status=plan.status)
+    at_table = _int32(plan.table, dev, (B, width), "plan.table")
+    at_starts = _int32(plan.starts, dev, (B + 1,), "plan.starts")
+    at_lens = _int32(plan.lens, dev, (B,), "plan.lens")
     if window < 0 or sink_tokens < 0:
         raise ValueError("window and sink_tokens must be >= 0")
+    at_logits = None
     if sink_logits is not None:
-        if tuple(sink_logits.shape) != (heads,):
-            raise ValueError(f"sink_logits of shape {tuple(sink_logits.shape)} for {heads} heads")
-        _same_device(dev, sink_logits=sink_logits)
+        if sink_logits.shape != (heads,) or sink_logits.device != dev:
+            raise ValueError(f"sink_logits of shape {tuple(sink_logits.shape)} on {sink_logits.device} for {heads} heads on {dev}")
         sink_logits = sink_logits.to(torch.float32).contiguous()
+        at_logits = sink_logits.data_ptr()
     shape = (N, heads, cache.v_dim)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != shape or not out.is_contiguous() or out.device != dev:
-        raise ValueError(f"out: need a contiguous bf16 tensor of shape {shape} on {dev}")
+        out = torch.empty(shape, dtype=BF16, device=dev)
+    elif out.dtype is not BF16 or out.shape != shape or not out.is_contiguous() or out.device != dev or out.data_ptr() % 16:
+        raise ValueError(f"out: need a contiguous, 16-byte aligned bf16 tensor of shape {shape} on {dev}")
+    status = _status(plan, dev)
     if N == 0:
         return out
-    scale = cache.k_dim ** -0.5 if scale is None else float(scale)
-    max_new = N if plan.max_new is None else min(N, int(plan.max_new))
-    with torch.cuda.device(dev):
-        nbytes = _lib.load().mimo_cache_attend_workspace_size(N, heads, cache.kv_heads, cache.v_dim)
-        ws = _workspace(nbytes, dev)
-        _lib.call("mimo_cache_attend", _lib.ptr(q), q.stride(0), N, heads, cache.struct(), B, _lib.ptr(starts), _lib.ptr(lens),
-                  _lib.ptr(table), width, max_new, scale, int(window), int(sink_tokens), _lib.ptr(sink_logits), _lib.ptr(out),
-                  _lib.ptr(plan.status), _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev))
+    stream = _raw_stream(index)
+    ws = _workspace(_workspace_size(N, heads, cache.kv_heads, cache.v_dim), dev, stream)
+    _call("mimo_cache_attend", at_q, q_stride, N, heads, cache._struct, B, at_starts, at_lens, at_table, width,
+          N if plan.max_new is None else min(N, int(plan.max_new)), cache.k_dim ** -0.5 if scale is None else float(scale),
+          int(window), int(sink_tokens), at_logits, out.data_ptr(), status, ws.data_ptr(), ws.numel(), stream)
     return out
