@@ -48,16 +48,18 @@ struct AttendArgs {
   int32_t* status;
   // rows of a tile: TQ tokens of HT heads (HG groups of HT heads cover G), Hh = Hkv * HG
   int TQ, HT, HG, Hh, chunk_min, target;
-  // split tiles: per block TQ * HT rows of O (fp32 [Dv]) and (m, l); per (token, head group) the first block's slot and
-  // blocks | token's place << 16.  meta is null when no tile can be split.
+  // split tiles: per slot TQ * HT rows of O (fp32 [Dv]) and (m, l); per (token, head group) the first part's slot and
+  // parts | token's place in its tile << 16.  Part i > 0 is in slot (first & ~part_mask) + i part_step.  meta is null when no
+  // tile can be split.
   float *part_o, *part_ml;
   int2* meta;
+  int part_mask, part_step;
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int AT_THREADS = 256;
 constexpr int AT_WIDE_TARGET = 512, AT_WIDE_MIN = 4;      // blocks wanted, least 64-key tiles of a block
-constexpr int AT_NARROW_TARGET = 1024, AT_NARROW_MIN = 2; // the same in 128-key units
+constexpr int AT_NARROW_TARGET = 512, AT_NARROW_MIN = 2;  // blocks (two per CU), least 128-key units of one
 
 template <int DK_, int DV_, bool F8_, bool WIDE_> struct AtCfg {
   static constexpr int DK = DK_, DV = DV_;
@@ -147,71 +149,82 @@ __host__ __device__ __forceinline__ int at_most(int64_t len, int window, int sin
   return (int)(w < all ? w : all);
 }
 
+// One row tile of one request and head group, units it0 .. it1 - 1 of its I: part `split` of ns, kept in `slot` when ns > 1.
 struct AtItem {
-  int b, s0, n, len, tt, hh, split, chunk, slot0;   // slot0: of the tile's first block; -1 when the request is not split
+  int b, s0, n, len, tt, hh, it0, it1, ns, slot;
 };
 
-// Block blockIdx.x's item: every block counts all requests' work for itself (a few KB from L2) and takes its place in the
-// list of (request, row tile from the last to the first, split) x head group, head groups fastest: neighbouring blocks, on
-// different XCDs, work on different heads, and an XCD keeps meeting the same ones.  false: past the end of the list.
-__device__ __forceinline__ bool at_find(const AttendArgs& a, int unit, int* sh, AtItem& it) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+// Request b's rows s0 .. s0 + n - 1 and length, clamped: whatever starts and lens hold, nothing is out of range.
+__device__ __forceinline__ void at_request(const AttendArgs& a, int b, int& s0, int& n, int& len) {
+  s0 = min(max(a.starts[b], 0), a.N);
+  n = min(max(a.starts[b + 1], s0), a.N) - s0;
+  len = a.lens[b];
+  if (n && (len < n || len > ((long long)a.max_pages << a.page_shift))) len = 0;   // refused: its rows are set to 0
+}
+// a block's exclusive prefix sums of two values per thread, and their totals
+__device__ __forceinline__ void at_scan2(long long& x, int& y, long long& tx, int& ty, int* sh) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  long long* shl = reinterpret_cast<long long*>(sh);
+  long long ix = x;
+  int iy = y;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const long long p = __shfl_up(ix, d, 64);
+    const int q = __shfl_up(iy, d, 64);
+    if (lane >= d) ix += p, iy += q;
+  }
+  if (lane == 63) shl[wave] = ix, sh[8 + wave] = iy;
+  __syncthreads();
+  x = ix - x, y = iy - y, tx = 0, ty = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    x += w < wave ? shl[w] : 0, y += w < wave ? sh[8 + w] : 0;
+    tx += shl[w], ty += sh[8 + w];
+  }
+  __syncthreads();
+}
+
+// Wide tiles.  Block blockIdx.x's item: every block counts all requests' work for itself (a few KB from L2) and takes its
+// place in the list of (request, row tile from the last to the first, part) x head group, head groups fastest: neighbouring
+// blocks, on different XCDs, work on different heads, and an XCD keeps meeting the same ones.  A tile is cut into parts of
+// `chunk` units, the fair share of `target` blocks.  false: past the end of the list, or a part that this tile does not have.
+template <class C>
+__device__ __forceinline__ bool at_find(const AttendArgs& a, int* sh, AtItem& it) {
+  const int t = threadIdx.x;
   const int per = (a.B + AT_THREADS - 1) / AT_THREADS;
   const int b0 = min(a.B, t * per), b1 = min(a.B, b0 + per);
-  const long long cap = (long long)a.max_pages << a.page_shift;
-  auto request = [&](int b, int& s0, int& n, int& len) {   // clamped: whatever starts and lens hold, nothing is out of range
-    s0 = min(max(a.starts[b], 0), a.N);
-    n = min(max(a.starts[b + 1], s0), a.N) - s0;
-    len = a.lens[b];
-    if (n && (len < n || len > cap)) len = 0;              // refused: its rows are set to 0
-  };
-  long long work = 0;
-  int s0, n, len;
+  long long work = 0, total;
+  int s0, n, len, parts = 0, all;
   for (int b = b0; b < b1; ++b) {
-    request(b, s0, n, len);
-    if (n) work += (long long)((n + a.TQ - 1) / a.TQ) * at_most(len, a.window, a.sinks, a.TQ, unit);
+    at_request(a, b, s0, n, len);
+    if (n) work += (long long)((n + a.TQ - 1) / a.TQ) * at_most(len, a.window, a.sinks, a.TQ, C::UNIT);
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) work += __shfl_xor(work, d, 64);
-  long long* shl = reinterpret_cast<long long*>(sh);
-  if (lane == 0) shl[wave] = work;
   if (t == 0) sh[20] = -1;
-  __syncthreads();
-  work = min(shl[0] + shl[1] + shl[2] + shl[3], 1ll << 50);   // starts that overlap may ask for anything: then nothing is split
-  const long long fair = (work * a.Hh + a.target - 1) / a.target;
-  const int chunk = (int)min((long long)0x3fffffff, max((long long)a.chunk_min, fair));
+  at_scan2(work, parts, total, all, sh);
+  total = min(total, 1ll << 50);                           // starts that overlap may ask for anything: then nothing is split
+  const int chunk = (int)min((long long)0x3fffffff, max((long long)a.chunk_min, (total * a.Hh + a.target - 1) / a.target));
   long long units = 0;
-  int parts = 0;
+  parts = 0;
   for (int b = b0; b < b1; ++b) {
-    request(b, s0, n, len);
+    at_request(a, b, s0, n, len);
     if (!n) continue;
-    const int nt = (n + a.TQ - 1) / a.TQ, ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, unit) + chunk - 1) / chunk);
+    const int nt = (n + a.TQ - 1) / a.TQ, ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, C::UNIT) + chunk - 1) / chunk);
     units += (long long)nt * ns;
     parts += ns > 1 ? nt * ns : 0;
   }
-  long long iu = units;
-  int ip = parts;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const long long x = __shfl_up(iu, d, 64);
-    const int y = __shfl_up(ip, d, 64);
-    if (lane >= d) iu += x, ip += y;
-  }
-  if (lane == 63) shl[4 + wave] = iu, sh[16 + wave] = ip;
-  __syncthreads();
-  long long ub = iu - units;
-  int pb = ip - parts;
-  for (int w = 0; w < wave; ++w) ub += shl[4 + w], pb += sh[16 + w];
-  const int u = blockIdx.x / a.Hh;
+  long long ub = units;
+  int pb = parts;
+  at_scan2(ub, pb, total, all, sh);
+  const int u = blockIdx.x / a.Hh, hh = blockIdx.x % a.Hh;
   if (u >= ub && u < ub + units) {
     for (int b = b0; b < b1; ++b) {
-      request(b, s0, n, len);
+      at_request(a, b, s0, n, len);
       if (!n) continue;
-      const int nt = (n + a.TQ - 1) / a.TQ, ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, unit) + chunk - 1) / chunk);
+      const int nt = (n + a.TQ - 1) / a.TQ, ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, C::UNIT) + chunk - 1) / chunk);
       if (u < ub + (long long)nt * ns) {
-        const int at = (int)(u - ub) / ns;
-        sh[20] = b, sh[21] = s0, sh[22] = n, sh[23] = len, sh[24] = nt - 1 - at, sh[25] = (int)(u - ub) - at * ns;
-        sh[26] = ns > 1 ? (pb + at * ns) * a.Hh + blockIdx.x % a.Hh : -1;
+        const int at = (int)(u - ub) / ns, split = (int)(u - ub) - at * ns;
+        sh[20] = b, sh[21] = s0, sh[22] = n, sh[23] = len, sh[24] = nt - 1 - at, sh[25] = split;
+        sh[26] = (pb + at * ns + split) * a.Hh + hh, sh[27] = ns;
         break;
       }
       ub += (long long)nt * ns;
@@ -219,11 +232,19 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, int unit, int* sh, 
     }
   }
   __syncthreads();
-  it.b = sh[20], it.s0 = sh[21], it.n = sh[22], it.len = sh[23], it.tt = sh[24], it.split = sh[25], it.slot0 = sh[26];
-  it.hh = blockIdx.x % a.Hh;
-  it.chunk = chunk;
+  it.b = sh[20], it.s0 = sh[21], it.n = sh[22], it.len = sh[23], it.tt = sh[24], it.slot = sh[26], it.hh = hh;
+  const int split = sh[25], ns = sh[27];
   __syncthreads();                                         // the scratch is free
-  return it.b >= 0;
+  if (it.b < 0) return false;
+  it.it0 = 0, it.it1 = 0x7fffffff, it.ns = 1;
+  if (ns > 1) {
+    const int p0 = it.len - it.n + it.tt * a.TQ, p1 = min(p0 + a.TQ, it.len) - 1;
+    const int I = at_range(p0, p1, a.window, a.sinks, C::UNIT).I;
+    it.ns = (I + chunk - 1) / chunk;
+    if (split >= it.ns) return false;
+    it.it0 = split * chunk, it.it1 = it.it0 + chunk;
+  }
+  return true;
 }
 
 // 16 keys from a multiple of 16 on, of which a tile may load: their page and what hidden keys read instead
@@ -291,22 +312,14 @@ __device__ __forceinline__ void at_slow(const AttendArgs& a, const AtRange& r, i
   }
 }
 
+// One item.
 template <class C>
-__global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a) {
-  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  const int t = threadIdx.x, lane = t & 63, r32 = lane & 31, h = lane >> 5;
+__device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const AtItem& item) {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));                              // nothing per lane is kept in registers from one item to the next
+  const int lane = t & 63, r32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  {                                                        // rows of no request
-    const int first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N);
-    const int gap = first + a.N - last, row = a.Hq * C::DV / 8;
-    for (int i = blockIdx.x; i < gap; i += gridDim.x) {
-      uint4* o = reinterpret_cast<uint4*>(a.out) + (size_t)(i < first ? i : last + i - first) * row;
-      for (int d = t; d < row; d += AT_THREADS) o[d] = make_uint4(0, 0, 0, 0);
-    }
-  }
-  AtItem item;
-  if (!at_find(a, C::UNIT, reinterpret_cast<int*>(lds), item)) return;
-  const int b = __builtin_amdgcn_readfirstlane(item.b), hg = item.hh % a.HG, kv = item.hh / a.HG;
+  const int b = __builtin_amdgcn_readfirstlane(item.b), hg = item.hh % a.HG, kv = item.hh / a.HG, ns = item.ns;
   const int tok0 = item.tt * a.TQ, toks = min(a.TQ, item.n - tok0);
   const int heads = min(a.HT, a.G - hg * a.HT);
   const int qrow = (C::WIDE ? 32 * wave : 0) + r32;        // this lane's query row
@@ -315,19 +328,16 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   const int head = kv * a.G + hg * a.HT + qh;
   const size_t out_at = ((size_t)(item.s0 + tok0 + qt) * a.Hq + head) * C::DV;
   const int base_pos = item.len - item.n + tok0;
-  if (item.len == 0) {                                     // a refused request (it is never split)
+  if (a.meta && item.it0 == 0 && t < toks)
+    a.meta[(size_t)(item.s0 + tok0 + t) * a.Hh + item.hh] = make_int2(item.slot, ns | (t << 16));
+  if (item.len == 0) {                                     // a refused request
     if (a.status && t == 0) a.status[0] = MIMO_ERR_SHAPE;
     if (valid && (C::WIDE || wave == 0))
       for (int d = 0; d < C::DV / 2; d += 8) *reinterpret_cast<uint4*>(a.out + out_at + h * (C::DV / 2) + d) = make_uint4(0, 0, 0, 0);
-    if (a.meta && t < toks) a.meta[(size_t)(item.s0 + tok0 + t) * a.Hh + item.hh] = make_int2(0, 1);
     return;
   }
   const AtRange rg = at_range(base_pos, base_pos + toks - 1, a.window, a.sinks, C::UNIT);
-  const int ns = item.slot0 < 0 ? 1 : (rg.I + item.chunk - 1) / item.chunk;
-  if (item.split >= ns) return;
-  const int it0 = item.slot0 < 0 ? 0 : item.split * item.chunk, it1 = item.slot0 < 0 ? rg.I : min(rg.I, it0 + item.chunk);
-  if (a.meta && item.split == 0 && t < toks)
-    a.meta[(size_t)(item.s0 + tok0 + t) * a.Hh + item.hh] = make_int2(item.slot0, ns | (t << 16));
+  const int it0 = item.it0, it1 = min(item.it1, rg.I);
 
   // queries as the B operand: row r32, dimensions 16 s + 8 h .. (E4M3: 32 (s / 2) + 16 h + 8 (s % 2) .., since a lane's 16
   // bytes of K are 16 dimensions, two products' worth); c = |scale| k_scale log2 e, a negative scale turns q round
@@ -335,16 +345,21 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   const uint32_t flip = c < 0.0f ? 0x80008000u : 0u;
   const bool zero = c == 0.0f;
   c = zero ? 1.0f : fabsf(c);
-  bf16x8 Q[C::DK / 16];
+  uint4 qraw[C::DK / 16];
   {
     const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + qt) * a.q_stride + head * C::DK + (C::F8 ? 16 : 8) * h;
 #pragma unroll
     for (int s = 0; s < C::DK / 16; ++s) {
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (valid && !zero) x = *reinterpret_cast<const uint4*>(qp + (C::F8 ? 32 * (s >> 1) + 8 * (s & 1) : 16 * s));
-      Q[s] = __builtin_bit_cast(bf16x8, make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip));
+      qraw[s] = make_uint4(0, 0, 0, 0);
+      if (valid && !zero) qraw[s] = *reinterpret_cast<const uint4*>(qp + (C::F8 ? 32 * (s >> 1) + 8 * (s & 1) : 16 * s));
     }
   }
+  bf16x8 Q[C::DK / 16];
+  auto take_q = [&]() __attribute__((always_inline)) {     // once the first copies are on their way
+#pragma unroll
+    for (int s = 0; s < C::DK / 16; ++s)
+      Q[s] = __builtin_bit_cast(bf16x8, make_uint4(qraw[s].x ^ flip, qraw[s].y ^ flip, qraw[s].z ^ flip, qraw[s].w ^ flip));
+  };
   const int pos = base_pos + qt;                           // this lane's position
   const int w_first = C::WIDE ? 32 * wave / a.HT : 0, w_last = min(toks - 1, ((C::WIDE ? 32 * wave : 0) + 31) / a.HT);
   const bool busy = w_first <= w_last;                     // the wave has rows
@@ -529,6 +544,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
     rows_of();
     issue_k(lds0);
     issue_v(lds0);
+    take_q();
     for (int it = it0; it < it1; ++it) {
       const int cur = (it - it0) & 1, g0 = it * UG;
       if (it + 1 < it1) look(it + 1);
@@ -556,6 +572,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
       issue_k(lds0);
       issue_v(lds0);
     }
+    take_q();
     for (int it = it0; it < end; ++it) {
       const int g0 = it * UG + wg;
       const bool more = it + 1 < end;
@@ -621,7 +638,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
   if constexpr (C::WIDE) {
     if (suspect) {
       slow([&](int r, int rt, int hd, const float (&O)[C::VCB], float m, float l) __attribute__((always_inline)) {
-        const size_t row = ((size_t)item.slot0 + (size_t)item.split * a.Hh) * (a.TQ * a.HT) + 32 * wave + r;
+        const size_t row = (size_t)item.slot * (a.TQ * a.HT) + 32 * wave + r;
         if (ns > 1 && lane == 0) a.part_ml[2 * row] = m, a.part_ml[2 * row + 1] = l;
         const float sink = a.sink_logits ? a.sink_logits[hd] * kLog2e : -INFINITY;
         const float top = fmaxf(m, sink), ref = top == -INFINITY ? 0.0f : top;
@@ -637,7 +654,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
     if (!valid) return;
     l = at_swap_sum(l);
     if (ns > 1) {
-      const size_t slot = (size_t)item.slot0 + (size_t)item.split * a.Hh, row = slot * (a.TQ * a.HT) + qt * a.HT + qh;
+      const size_t row = (size_t)item.slot * (a.TQ * a.HT) + qt * a.HT + qh;
       if (h == 0) a.part_ml[2 * row] = m, a.part_ml[2 * row + 1] = l;
 #pragma unroll
       for (int d = 0; d < C::DV / 32; ++d)
@@ -709,7 +726,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
         x[0] += o.x * f, x[1] += o.y * f, x[2] += o.z * f, x[3] += o.w * f;
       }
       if (ns > 1) {
-        const size_t slot = (size_t)item.slot0 + (size_t)item.split * a.Hh, pr = slot * (a.TQ * a.HT) + row;
+        const size_t pr = (size_t)item.slot * (a.TQ * a.HT) + row;
         *reinterpret_cast<float4*>(a.part_o + pr * C::DV + 4 * piece) = make_float4(x[0] * vs, x[1] * vs, x[2] * vs, x[3] * vs);
         if (piece == 0) a.part_ml[2 * pr] = all, a.part_ml[2 * pr + 1] = tot;
       } else {
@@ -721,7 +738,98 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_kernel(AttendArgs a
         *reinterpret_cast<uint2*>(a.out + ((size_t)(item.s0 + tok0 + rt) * a.Hq + hd) * C::DV + 4 * piece) = y;
       }
     }
+    __syncthreads();                                       // the next item's copies may come
   }
+}
+
+// rows of no request
+__device__ __forceinline__ void at_clear(const AttendArgs& a, int row) {
+  const int first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N), gap = first + a.N - last;
+  for (int i = blockIdx.x; i < gap; i += gridDim.x) {
+    uint4* o = reinterpret_cast<uint4*>(a.out + (size_t)(i < first ? i : last + i - first) * row);
+    for (int d = threadIdx.x; d < row / 8; d += AT_THREADS) o[d] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <class C>
+__global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_wide_kernel(AttendArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  AtItem item;
+  if (at_find<C>(a, reinterpret_cast<int*>(lds), item)) at_tile<C>(a, lds, item);
+  at_clear(a, a.Hq * C::DV);
+}
+
+// Narrow tiles: all units of a head group, request after request, in equal shares for the n blocks of the group.  A block
+// walks its share tile by tile; a tile on the border of two shares is split.  Slot 2 (j Hh + hh) holds block j's part of a
+// tile that began in an earlier share (or with this one), the slot behind it the part of one that goes on in the next.
+template <class C>
+__global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(AttendArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  int* sh = reinterpret_cast<int*>(lds);
+  const int t = threadIdx.x, hh = blockIdx.x % a.Hh, j = blockIdx.x / a.Hh;
+  const int per = (a.B + AT_THREADS - 1) / AT_THREADS;
+  const int b0 = min(a.B, t * per), b1 = min(a.B, b0 + per);
+  long long units = 0, total;
+  int tiles = 0, all;
+  // without room for parts (no tile can have more than chunk_min units) a share is whole tiles, each counted as one
+  auto size = [&](int b, int& s0, int& n, int& len, int& nt, int& I) {
+    at_request(a, b, s0, n, len);
+    nt = (n + a.TQ - 1) / a.TQ;
+    I = a.meta ? max(1, at_most(len, a.window, a.sinks, a.TQ, C::UNIT)) : 1;
+  };
+  auto divide = [](long long x, long long y) -> long long {   // 64-bit division is a long way round
+    return ((unsigned long long)x | (unsigned long long)y) >> 32 ? x / y : (uint32_t)x / (uint32_t)y;
+  };
+  int s0, n, len, nt, I;
+  for (int b = b0; b < b1; ++b) {
+    size(b, s0, n, len, nt, I);
+    units += (long long)nt * I;
+    tiles += nt;
+  }
+  long long before = units;
+  at_scan2(before, tiles, total, all, sh);
+  // blocks that share the work: at least chunk_min units each, and one per CU while that leaves them no more than 8 and the
+  // tiles alone do not fill the card
+  const bool few = total * a.Hh <= 8 * (a.target / 2) && (long long)all * a.Hh < a.target / 2;
+  const long long most = max(1, (few ? a.target / 2 : a.target) / a.Hh);
+  const long long shares = max(1ll, min(most, a.meta ? divide(total + a.chunk_min - 1, a.chunk_min) : total));
+  if (j < shares && total < (1ll << 50)) {                 // more: starts that overlap; nothing is computed
+    const long long u0 = divide(j * total, shares), u1 = divide((j + 1) * total, shares);
+    for (long long u = u0; u < u1;) {
+      if (u >= before && u < before + units) {
+        long long at = before;
+        for (int b = b0; b < b1; ++b) {
+          size(b, s0, n, len, nt, I);
+          if (u < at + (long long)nt * I) {
+            const int tt = (int)divide(u - at, I);
+            sh[0] = b, sh[1] = s0, sh[2] = n, sh[3] = len, sh[4] = tt, sh[5] = I;
+            *reinterpret_cast<long long*>(sh + 6) = at + (long long)tt * I;
+            break;
+          }
+          at += (long long)nt * I;
+        }
+      }
+      __syncthreads();
+      AtItem item;
+      item.b = sh[0], item.s0 = sh[1], item.n = sh[2], item.len = sh[3], item.tt = sh[4], item.hh = hh;
+      const int bound = sh[5];
+      const long long start = *reinterpret_cast<long long*>(sh + 6);
+      __syncthreads();                                     // the scratch is free
+      const int p0 = item.len - item.n + item.tt * a.TQ, p1 = min(p0 + a.TQ, item.len) - 1;
+      const int real = item.len ? at_range(p0, p1, a.window, a.sinks, C::UNIT).I : 1;
+      item.ns = 1, item.slot = 0, item.it0 = 0, item.it1 = real;
+      if (a.meta) {
+        // the share that holds unit x is ((x + 1) shares - 1) / total
+        if (start < u0 || start + real > u1)
+          item.ns = (int)(divide((start + real) * shares - 1, total) - divide((start + 1) * shares - 1, total)) + 1;
+        item.slot = 2 * (j * a.Hh + hh) + (start > u0 ? 1 : 0);
+        item.it0 = (int)(u - start), item.it1 = (int)min((long long)real, u1 - start);
+      }
+      if (item.it0 < item.it1) at_tile<C>(a, lds, item);
+      u = start + bound;
+    }
+  }
+  at_clear(a, a.Hq * C::DV);
 }
 
 // The parts of split row tiles, joined in order: out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j.  A block looks at `per`
@@ -748,33 +856,42 @@ __global__ void __launch_bounds__(64 * W) attend_join_kernel(AttendArgs a, int p
     const int n = (e0 + e) / a.Hh, hh = (e0 + e) % a.Hh;
     const int hg = hh % a.HG, kv = hh / a.HG, heads = min(a.HT, a.G - hg * a.HT);
     for (int qh = q0; qh < min(heads, q0 + hpb); ++qh) {
-      const size_t rows = (size_t)a.TQ * a.HT, row0 = (size_t)mt.x * rows + (size_t)(mt.y >> 16) * a.HT + qh, step = rows * a.Hh;
+      const size_t rows = (size_t)a.TQ * a.HT, in = (size_t)(mt.y >> 16) * a.HT + qh;
+      auto part = [&](int j) { return (size_t)(j ? (mt.x & ~a.part_mask) + j * a.part_step : mt.x) * rows + in; };
+      // the wave's first eight parts are asked for before the weights are known
+      float o[8][E];
+      float2 ml[8];
+      auto fetch = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (j0 + W * i >= ns) break;
+          const size_t row = part(j0 + W * i);
+          const float* p = a.part_o + row * DV + E * lane;
+          ml[i] = *reinterpret_cast<const float2*>(a.part_ml + 2 * row);
+#pragma unroll
+          for (int k = 0; k < E; ++k) o[i][k] = p[k];
+        }
+      };
+      if (wave < ns) fetch(wave);
       float top = -INFINITY;
-      for (int j = lane; j < ns; j += 64) top = fmaxf(top, a.part_ml[2 * (row0 + j * step)]);
+      for (int j = lane; j < ns; j += 64) top = fmaxf(top, a.part_ml[2 * part(j)]);
 #pragma unroll
       for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
       const float ref = top == -INFINITY ? 0.0f : top;
       float tot = 0.0f, x[E];
 #pragma unroll
       for (int i = 0; i < E; ++i) x[i] = 0.0f;
-      for (int j0 = wave; j0 < ns; j0 += 64 * W) {         // lane i: part j0 + W i
-        const int mine = j0 + W * lane, count = min(64, (ns - j0 + W - 1) / W);
-        float f = 0.0f;
-        if (mine < ns) {
-          const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (row0 + mine * step));
-          f = at_exp2(ml.x - ref);
-          tot += f * ml.y;
-        }
-#pragma unroll 8
-        for (int i = 0; i < count; ++i) {
-          const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), i));
-          const float* o = a.part_o + (row0 + (size_t)(j0 + W * i) * step) * DV + E * lane;
+      for (int j0 = wave; j0 < ns; j0 += 8 * W) {
+        if (j0 != wave) fetch(j0);
 #pragma unroll
-          for (int k = 0; k < E; ++k) x[k] += w * o[k];
+        for (int i = 0; i < 8; ++i) {
+          if (j0 + W * i >= ns) break;
+          const float f = at_exp2(ml[i].x - ref);
+          tot += f * ml[i].y;
+#pragma unroll
+          for (int k = 0; k < E; ++k) x[k] += f * o[i][k];
         }
       }
-#pragma unroll
-      for (int d = 32; d; d >>= 1) tot += __shfl_xor(tot, d, 64);
 #pragma unroll
       for (int k = 0; k < E; ++k) so[wave][E * lane + k] = x[k];
       if (lane == 0) sl[wave] = tot;
@@ -785,11 +902,11 @@ __global__ void __launch_bounds__(64 * W) attend_join_kernel(AttendArgs a, int p
       float sum = at_exp2(sink - r2);
 #pragma unroll
       for (int w = 0; w < W; ++w) sum += sl[w] * g;
-      if (t < DV) {
+      for (int d = t; d < DV; d += 64 * W) {
         float y = 0.0f;
 #pragma unroll
-        for (int w = 0; w < W; ++w) y += so[w][t];
-        a.out[((size_t)n * a.Hq + head) * DV + t] = sum == 0.0f ? 0 : f32_to_bf16(y * g / sum);
+        for (int w = 0; w < W; ++w) y += so[w][d];
+        a.out[((size_t)n * a.Hq + head) * DV + d] = sum == 0.0f ? 0 : f32_to_bf16(y * g / sum);
       }
       __syncthreads();
     }
@@ -811,28 +928,35 @@ struct AtRoom {
 static AtRoom at_room(int rows, int target, int N, int heads, int kv_heads, int v_dim) {
   AttendArgs a{};
   at_tiles(rows, N, heads, kv_heads, a);
-  // a request is split when its tiles walk more than chunk units, so its blocks are at most twice its share of the target
-  const size_t pr = (size_t)2 * target * a.TQ * a.HT;
+  // wide: a request is split when its tiles walk more than chunk units, so its parts are at most twice its share of the
+  // target; narrow: two slots a block
+  const size_t pr = (size_t)2 * std::max(target, a.Hh) * a.TQ * a.HT;
   return {align256(pr * v_dim * 4), align256(pr * 8), align256((size_t)N * a.Hh * sizeof(int2))};
 }
 
 template <class C>
 static int at_launch(AttendArgs a, bool join, hipStream_t st) {
+  const auto kernel = [] {
+    if constexpr (C::WIDE) return &attend_wide_kernel<C>;
+    else return &attend_narrow_kernel<C>;
+  }();
   static std::atomic<uint64_t> allowed{0};                 // devices on which the kernel may use its LDS
   int dev = 0;
   MIMO_HIP(hipGetDevice(&dev));
   const uint64_t bit = 1ull << (dev & 63);
   if (!(allowed.load(std::memory_order_acquire) & bit)) {
-    MIMO_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_kernel<C>), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
+    MIMO_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
     allowed.fetch_or(bit, std::memory_order_release);
   }
-  // row tiles: at most sum ceil(n_b / TQ) over at most min(B, N) requests with rows; blocks: tiles plus splits
+  // row tiles: at most sum ceil(n_b / TQ) over at most min(B, N) requests with rows; wide blocks: tiles plus splits
   const int64_t tiles = ((int64_t)a.N + (int64_t)std::min(a.B, a.N) * (a.TQ - 1)) / a.TQ;
-  const int64_t grid = tiles * a.Hh + (join ? a.target : 0);
+  const int64_t grid = C::WIDE ? tiles * a.Hh + (join ? a.target : 0) : (int64_t)std::max(1, a.target / a.Hh) * a.Hh;
   MIMO_REQUIRE(grid < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many tiles");
+  a.part_mask = C::WIDE ? 0 : 1;
+  a.part_step = C::WIDE ? a.Hh : 2 * a.Hh;
   {
     ProfScope p(st, C::WIDE ? "attend_wide" : "attend_narrow");
-    attend_kernel<C><<<(unsigned)grid, AT_THREADS, C::LDS, st>>>(a);
+    kernel<<<(unsigned)grid, AT_THREADS, C::LDS, st>>>(a);
   }
   if (int e = check_launch("attend")) return e;
   if (!join) return MIMO_OK;
@@ -842,8 +966,10 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
     ProfScope p(st, "attend_join");
     if (rows <= 256) {
       attend_join_kernel<C::DV, 16><<<(unsigned)rows, 1024, 0, st>>>(a, 1, 1);
-    } else if (rows <= 8192) {
+    } else if (rows <= 1024) {
       attend_join_kernel<C::DV, 4><<<(unsigned)rows, 256, 0, st>>>(a, 1, 1);
+    } else if (rows <= 16384) {
+      attend_join_kernel<C::DV, 1><<<(unsigned)rows, 64, 0, st>>>(a, 1, 1);
     } else {                                               // mostly rows that were not split: a block looks at many
       const int per = (int)std::min<int64_t>(256, (entries + 1023) / 1024);
       attend_join_kernel<C::DV, 4><<<(unsigned)((entries + per - 1) / per), 256, 0, st>>>(a, per, a.HT);
@@ -907,7 +1033,7 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   at_tiles(wide ? 128 : 32, N, heads, cache->kv_heads, a);
   a.chunk_min = wide ? AT_WIDE_MIN : AT_NARROW_MIN;
   a.target = wide ? AT_WIDE_TARGET : AT_NARROW_TARGET;
-  // no tile can walk more units than the table or the window holds; if that is within chunk_min nothing is ever split
+  // no tile can walk more units than the table or the window holds; within chunk_min it is never split
   const int most = at_most((int64_t)max_pages * cache->page_size, window, a.sinks, a.TQ, wide ? 64 : 128);
   const bool join = most > a.chunk_min;
   const AtRoom room = at_room(wide ? 128 : 32, a.target, N, heads, cache->kv_heads, cache->v_dim);
