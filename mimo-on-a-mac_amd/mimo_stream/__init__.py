@@ -11,4 +11,4 @@ from .model import Router, MoEBlock, select_from_logits, prefill_dispatch  # noq
 from .store import ExpertStore, load_block, load_router, write_expert_layer  # noqa: F401
 from .residency import StagingBanks, StreamedMoEBlock  # noqa: F401
 from .layer import MoELayer, load_layer, load_norm, layernorm_epsilon  # noqa: F401
-from .attention import PageTable, StepPlan, KVCache, Rotary, append, attend  # noqa: F401
+from .attention import PageTable, StepPlan, KVCache, Rotary, append, attend, AttentionLayer  # noqa: F401

@@ -325,3 +325,64 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
           N if plan.max_new is None else min(N, int(plan.max_new)), cache.k_dim ** -0.5 if scale is None else float(scale),
           int(window), int(sink_tokens), at_logits, out.data_ptr(), status, ws.data_ptr(), ws.numel(), stream)
     return out
+
+
+class AttentionLayer:
+    """The attention half of a decoder layer (engine/mimo_stream/model.py:296-298 around mimo_v2.py:110-150):
+
+        r = input_layernorm(x);  q, k, v = r Wq, r Wk, r Wv;  h = x + attend(q, cache) Wo
+
+    norm_weight bf16 [hidden] and eps as in MoELayer; qkv_weight bf16 [heads k_dim + kv_heads (k_dim + v_dim), hidden]
+    (q rows, then k, then v), o_weight bf16 [hidden, heads v_dim]; cache: the layer's KVCache; rotary, window, sink_tokens,
+    sink_logits and scale as in append and attend.  The two projections are library GEMMs, the rest the library's kernels.
+    MoELayer takes its output: h = moe_layer(attention_layer(x, plan)), one plan for all layers of a step."""
+
+    def __init__(self, norm_weight, eps, qkv_weight, o_weight, heads, cache, rotary=None, window=0, sink_tokens=0,
+                 sink_logits=None, scale=None):
+        dev = cache.device
+        self.cache, self.heads, self.rotary, self.scale = cache, int(heads), rotary, scale
+        self.window, self.sink_tokens = int(window), int(sink_tokens)
+        self.norm_weight, self.qkv_weight, self.o_weight = (
+            torch.as_tensor(w).to(device=dev, dtype=BF16).contiguous() for w in (norm_weight, qkv_weight, o_weight))
+        self.sink_logits = None if sink_logits is None else torch.as_tensor(sink_logits).to(device=dev, dtype=torch.float32).contiguous()
+        self.eps = float(eps)
+        if not self.eps >= 0.0:
+            raise ValueError("eps must be a non-negative number")
+        self.hidden = self.norm_weight.numel()
+        self.split = (self.heads * cache.k_dim, cache.kv_heads * cache.k_dim, cache.kv_heads * cache.v_dim)
+        if self.heads < 1 or self.heads % cache.kv_heads:
+            raise ValueError(f"{heads} heads on {cache.kv_heads} K/V heads")
+        for name, w, shape in (("norm_weight", self.norm_weight, (self.hidden,)),
+                               ("qkv_weight", self.qkv_weight, (sum(self.split), self.hidden)),
+                               ("o_weight", self.o_weight, (self.hidden, self.heads * cache.v_dim))):
+            if tuple(w.shape) != shape:
+                raise ValueError(f"{name} of shape {tuple(w.shape)}, expected {shape}")
+        if self.sink_logits is not None and tuple(self.sink_logits.shape) != (self.heads,):
+            raise ValueError(f"sink_logits of shape {tuple(self.sink_logits.shape)} for {heads} heads")
+
+    def __call__(self, x, plan):
+        """h for x bf16 [N, hidden], the rows of the step that made plan."""
+        dev = self.cache.device
+        index = _gpu(dev)
+        if x.device != dev or x.dim() != 2 or x.shape[1] != self.hidden:
+            raise ValueError(f"x: need [tokens, {self.hidden}] on {dev}, got {tuple(x.shape)} on {x.device}")
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(dev):
+                return self(x, plan)
+        x = x.to(BF16).contiguous()
+        if x.data_ptr() % 16:
+            x = x.clone()
+        h = torch.empty_like(x)
+        N = x.shape[0]
+        if N == 0:
+            return h
+        r = torch.empty_like(x)
+        _call("mimo_rmsnorm", x.data_ptr(), N, self.hidden, self.norm_weight.data_ptr(), self.eps, r.data_ptr(), _raw_stream(index))
+        c = self.cache
+        q, k, v = torch.matmul(r, self.qkv_weight.T).split_with_sizes(self.split, 1)
+        q = append(c, plan, k.unflatten(1, (c.kv_heads, c.k_dim)), v.unflatten(1, (c.kv_heads, c.v_dim)),
+                   q=q.unflatten(1, (self.heads, c.k_dim)), rotary=self.rotary)
+        o = attend(q, c, plan, self.scale, self.window, self.sink_tokens, self.sink_logits)
+        y = torch.matmul(o.flatten(1), self.o_weight.T)
+        _call("mimo_residual_add", x.data_ptr(), y.data_ptr(), x.numel(), h.data_ptr(), _raw_stream(index))
+        return h
