@@ -161,81 +161,80 @@ __device__ __forceinline__ void at_request(const AttendArgs& a, int b, int& s0, 
   len = a.lens[b];
   if (n && (len < n || len > ((long long)a.max_pages << a.page_shift))) len = 0;   // refused: its rows are set to 0
 }
-// a block's exclusive prefix sums of two values per thread, and their totals
-__device__ __forceinline__ void at_scan2(long long& x, int& y, long long& tx, int& ty, int* sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  long long* shl = reinterpret_cast<long long*>(sh);
-  long long ix = x;
-  int iy = y;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const long long p = __shfl_up(ix, d, 64);
-    const int q = __shfl_up(iy, d, 64);
-    if (lane >= d) ix += p, iy += q;
-  }
-  if (lane == 63) shl[wave] = ix, sh[8 + wave] = iy;
-  __syncthreads();
-  x = ix - x, y = iy - y, tx = 0, ty = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    x += w < wave ? shl[w] : 0, y += w < wave ? sh[8 + w] : 0;
-    tx += shl[w], ty += sh[8 + w];
-  }
-  __syncthreads();
+// a wave's inclusive prefix sum (row shifts by 1, 2, 4, 8, then the rows' last lanes to the rows behind) and its total
+__device__ __forceinline__ int at_prefix(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+__device__ __forceinline__ int at_last(int v) { return __builtin_amdgcn_readlane(v, 63); }
+// quotient of non-negative numbers; 64-bit division is a long way round
+__device__ __forceinline__ int64_t at_div(int64_t x, int64_t y) {
+  return (uint64_t)(x | y) >> 32 ? x / y : (uint32_t)x / (uint32_t)y;
 }
 
-// Wide tiles.  Block blockIdx.x's item: every block counts all requests' work for itself (a few KB from L2) and takes its
-// place in the list of (request, row tile from the last to the first, part) x head group, head groups fastest: neighbouring
-// blocks, on different XCDs, work on different heads, and an XCD keeps meeting the same ones.  A tile is cut into parts of
-// `chunk` units, the fair share of `target` blocks.  false: past the end of the list, or a part that this tile does not have.
+// The list of work, which every wave makes for itself without a word to the others: lane l looks at requests l per ..,
+// and the prefix sums of what they ask for are the places in the list.  Sizes are kept below 2^31 by refusing what only
+// starts that overlap can ask for (then nothing is computed).
+// Wide tiles.  Block blockIdx.x's item: (request, row tile from the last to the first, part) x head group, head groups
+// fastest: neighbouring blocks, on different XCDs, work on different heads, and an XCD keeps meeting the same ones.  A tile
+// is cut into parts of `chunk` units, the fair share of `target` blocks.  false: past the end of the list, or a part that
+// this tile does not have.
 template <class C>
-__device__ __forceinline__ bool at_find(const AttendArgs& a, int* sh, AtItem& it) {
-  const int t = threadIdx.x;
-  const int per = (a.B + AT_THREADS - 1) / AT_THREADS;
-  const int b0 = min(a.B, t * per), b1 = min(a.B, b0 + per);
-  long long work = 0, total;
-  int s0, n, len, parts = 0, all;
+__device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
+  const int lane = threadIdx.x & 63;
+  const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
+  int s0, n, len, tiles = 0;
+  float load = 0.0f;                                       // units of all tiles; only their share per block is wanted
   for (int b = b0; b < b1; ++b) {
     at_request(a, b, s0, n, len);
-    if (n) work += (long long)((n + a.TQ - 1) / a.TQ) * at_most(len, a.window, a.sinks, a.TQ, C::UNIT);
+    const int nt = (n + a.TQ - 1) / a.TQ;
+    tiles = min(tiles + nt, 1 << 22);
+    load += (float)nt * at_most(len, a.window, a.sinks, a.TQ, C::UNIT);
   }
-  if (t == 0) sh[20] = -1;
-  at_scan2(work, parts, total, all, sh);
-  total = min(total, 1ll << 50);                           // starts that overlap may ask for anything: then nothing is split
-  const int chunk = (int)min((long long)0x3fffffff, max((long long)a.chunk_min, (total * a.Hh + a.target - 1) / a.target));
-  long long units = 0;
-  parts = 0;
-  for (int b = b0; b < b1; ++b) {
+  tiles = at_last(at_prefix(tiles));
+  load = dpp_sum_f32(load);
+  if (tiles > 1 << 21) return false;                       // at most N + 1 a request: starts that overlap
+  // rounded up by more than the sum's error, so that the parts are within twice the target
+  const int chunk = max(a.chunk_min, (int)fminf(load * 1.0001f * a.Hh / a.target + 1.0f, 1.0e9f));
+  auto cut = [&](int b, int& nt, int& ns) {
     at_request(a, b, s0, n, len);
-    if (!n) continue;
-    const int nt = (n + a.TQ - 1) / a.TQ, ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, C::UNIT) + chunk - 1) / chunk);
-    units += (long long)nt * ns;
+    nt = (n + a.TQ - 1) / a.TQ;
+    ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, C::UNIT) + chunk - 1) / chunk);
+  };
+  int units = 0, parts = 0, nt, ns;
+  for (int b = b0; b < b1; ++b) {
+    cut(b, nt, ns);
+    units += nt * ns;
     parts += ns > 1 ? nt * ns : 0;
   }
-  long long ub = units;
-  int pb = parts;
-  at_scan2(ub, pb, total, all, sh);
+  int ub = at_prefix(units) - units, pb = at_prefix(parts) - parts;
   const int u = blockIdx.x / a.Hh, hh = blockIdx.x % a.Hh;
-  if (u >= ub && u < ub + units) {
-    for (int b = b0; b < b1; ++b) {
-      at_request(a, b, s0, n, len);
-      if (!n) continue;
-      const int nt = (n + a.TQ - 1) / a.TQ, ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, C::UNIT) + chunk - 1) / chunk);
-      if (u < ub + (long long)nt * ns) {
-        const int at = (int)(u - ub) / ns, split = (int)(u - ub) - at * ns;
-        sh[20] = b, sh[21] = s0, sh[22] = n, sh[23] = len, sh[24] = nt - 1 - at, sh[25] = split;
-        sh[26] = (pb + at * ns + split) * a.Hh + hh, sh[27] = ns;
-        break;
-      }
-      ub += (long long)nt * ns;
+  int f_b = 0, f_tt = 0, f_split = 0, f_slot = 0, f_ns = 0;
+  const bool here = u >= ub && u < ub + units;
+  if (here) {
+    int b = b0;
+    for (;; ++b) {
+      cut(b, nt, ns);
+      if (u < ub + nt * ns) break;
+      ub += nt * ns;
       pb += ns > 1 ? nt * ns : 0;
     }
+    const int at = (u - ub) / ns;
+    f_b = b, f_tt = nt - 1 - at, f_split = u - ub - at * ns, f_slot = (pb + u - ub) * a.Hh + hh, f_ns = ns;
   }
-  __syncthreads();
-  it.b = sh[20], it.s0 = sh[21], it.n = sh[22], it.len = sh[23], it.tt = sh[24], it.slot = sh[26], it.hh = hh;
-  const int split = sh[25], ns = sh[27];
-  __syncthreads();                                         // the scratch is free
-  if (it.b < 0) return false;
+  const uint64_t who = __ballot(here);
+  if (!who) return false;
+  const int src = __builtin_ctzll(who);
+  auto from = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
+  it.b = from(f_b), it.tt = from(f_tt), it.slot = from(f_slot), it.hh = hh;
+  it.s0 = from(s0), it.n = from(n), it.len = from(len);
+  const int split = from(f_split);
+  ns = from(f_ns);
   it.it0 = 0, it.it1 = 0x7fffffff, it.ns = 1;
   if (ns > 1) {
     const int p0 = it.len - it.n + it.tt * a.TQ, p1 = min(p0 + a.TQ, it.len) - 1;
@@ -651,9 +650,9 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       });
       return;
     }
-    if (!valid) return;
     l = at_swap_sum(l);
     if (ns > 1) {
+      if (!valid) return;
       const size_t row = (size_t)item.slot * (a.TQ * a.HT) + qt * a.HT + qh;
       if (h == 0) a.part_ml[2 * row] = m, a.part_ml[2 * row + 1] = l;
 #pragma unroll
@@ -664,19 +663,23 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
               make_float4(O[d][i] * vs, O[d][i + 1] * vs, O[d][i + 2] * vs, O[d][i + 3] * vs);
       return;
     }
-    const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
+    const float sink = a.sink_logits && valid ? a.sink_logits[head] * kLog2e : -INFINITY;
     const float top = fmaxf(m, sink), ref = top == -INFINITY ? 0.0f : top;
     const float f = at_exp2(m - ref), tot = l * f + at_exp2(sink - ref);
     const float w = tot == 0.0f ? 0.0f : vs * f / tot;
+    // the halves of a row trade quads of values, so that a lane stores 16 bytes
 #pragma unroll
     for (int d = 0; d < C::DV / 32; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        uint2 x;
-        x.x = (uint32_t)f32_to_bf16(O[d][i] * w) | ((uint32_t)f32_to_bf16(O[d][i + 1] * w) << 16);
-        x.y = (uint32_t)f32_to_bf16(O[d][i + 2] * w) | ((uint32_t)f32_to_bf16(O[d][i + 3] * w) << 16);
-        if (tot == 0.0f) x = make_uint2(0, 0);
-        *reinterpret_cast<uint2*>(a.out + out_at + 32 * d + 2 * i + 4 * h) = x;
+      for (int i = 0; i < 16; i += 8) {
+        uint32_t x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int e = i + 2 * k;
+          x[k] = tot == 0.0f ? 0u : (uint32_t)f32_to_bf16(O[d][e] * w) | ((uint32_t)f32_to_bf16(O[d][e + 1] * w) << 16);
+        }
+        const auto p = __builtin_amdgcn_permlane32_swap(x[0], x[2], false, false), q = __builtin_amdgcn_permlane32_swap(x[1], x[3], false, false);
+        if (valid) *reinterpret_cast<uint4*>(a.out + out_at + 32 * d + 2 * i + 8 * h) = make_uint4(p[0], q[0], p[1], q[1]);
       }
   } else {
     // the waves' parts, joined over LDS in wave order: row r at [wave][r][DV], 16-byte pieces turned by the row
@@ -755,7 +758,7 @@ template <class C>
 __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_wide_kernel(AttendArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   AtItem item;
-  if (at_find<C>(a, reinterpret_cast<int*>(lds), item)) at_tile<C>(a, lds, item);
+  if (at_find<C>(a, item)) at_tile<C>(a, lds, item);
   at_clear(a, a.Hq * C::DV);
 }
 
@@ -765,65 +768,66 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_wide_kernel(AttendA
 template <class C>
 __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(AttendArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  int* sh = reinterpret_cast<int*>(lds);
-  const int t = threadIdx.x, hh = blockIdx.x % a.Hh, j = blockIdx.x / a.Hh;
-  const int per = (a.B + AT_THREADS - 1) / AT_THREADS;
-  const int b0 = min(a.B, t * per), b1 = min(a.B, b0 + per);
-  long long units = 0, total;
-  int tiles = 0, all;
+  const int lane = threadIdx.x & 63, hh = blockIdx.x % a.Hh, j = blockIdx.x / a.Hh;
+  const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
   // without room for parts (no tile can have more than chunk_min units) a share is whole tiles, each counted as one
-  auto size = [&](int b, int& s0, int& n, int& len, int& nt, int& I) {
+  int s0, n, len, nt, I;
+  auto size = [&](int b) {
     at_request(a, b, s0, n, len);
     nt = (n + a.TQ - 1) / a.TQ;
     I = a.meta ? max(1, at_most(len, a.window, a.sinks, a.TQ, C::UNIT)) : 1;
   };
-  auto divide = [](long long x, long long y) -> long long {   // 64-bit division is a long way round
-    return ((unsigned long long)x | (unsigned long long)y) >> 32 ? x / y : (uint32_t)x / (uint32_t)y;
-  };
-  int s0, n, len, nt, I;
+  int64_t mine = 0;
+  int tiles = 0;
   for (int b = b0; b < b1; ++b) {
-    size(b, s0, n, len, nt, I);
-    units += (long long)nt * I;
-    tiles += nt;
+    size(b);
+    mine += (int64_t)nt * I;
+    tiles = min(tiles + nt, 1 << 22);
   }
-  long long before = units;
-  at_scan2(before, tiles, total, all, sh);
+  tiles = at_last(at_prefix(tiles));
+  int64_t before = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t p = __shfl_up(before, d, 64);
+    if (lane >= d) before += p;
+  }
+  const int64_t total = __shfl(before, 63, 64);
+  before -= mine;
   // blocks that share the work: at least chunk_min units each, and one per CU while that leaves them no more than 8 and the
   // tiles alone do not fill the card
-  const bool few = total * a.Hh <= 8 * (a.target / 2) && (long long)all * a.Hh < a.target / 2;
-  const long long most = max(1, (few ? a.target / 2 : a.target) / a.Hh);
-  const long long shares = max(1ll, min(most, a.meta ? divide(total + a.chunk_min - 1, a.chunk_min) : total));
-  if (j < shares && total < (1ll << 50)) {                 // more: starts that overlap; nothing is computed
-    const long long u0 = divide(j * total, shares), u1 = divide((j + 1) * total, shares);
-    for (long long u = u0; u < u1;) {
-      if (u >= before && u < before + units) {
-        long long at = before;
-        for (int b = b0; b < b1; ++b) {
-          size(b, s0, n, len, nt, I);
-          if (u < at + (long long)nt * I) {
-            const int tt = (int)divide(u - at, I);
-            sh[0] = b, sh[1] = s0, sh[2] = n, sh[3] = len, sh[4] = tt, sh[5] = I;
-            *reinterpret_cast<long long*>(sh + 6) = at + (long long)tt * I;
-            break;
-          }
-          at += (long long)nt * I;
+  const bool few = total * a.Hh <= 8 * (a.target / 2) && (int64_t)tiles * a.Hh < a.target / 2;
+  const int64_t most = max(1, (few ? a.target / 2 : a.target) / a.Hh);
+  const int64_t shares = max((int64_t)1, min(most, a.meta ? at_div(total + a.chunk_min - 1, a.chunk_min) : total));
+  if (j < shares && tiles <= 1 << 21) {                    // more (at most N + 1 a request): starts that overlap
+    const int64_t u0 = at_div(j * total, shares), u1 = at_div((j + 1) * total, shares);
+    for (int64_t u = u0; u < u1;) {
+      int f_b = 0, f_tt = 0, f_off = 0;
+      const bool here = u >= before && u < before + mine;
+      if (here) {
+        int64_t at = before;
+        int b = b0;
+        for (;; ++b) {
+          size(b);
+          if (u < at + (int64_t)nt * I) break;
+          at += (int64_t)nt * I;
         }
+        f_b = b, f_tt = (int)at_div(u - at, I), f_off = (int)(u - at - (int64_t)f_tt * I);
       }
-      __syncthreads();
+      const int src = __builtin_ctzll(__ballot(here));
+      auto from = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
       AtItem item;
-      item.b = sh[0], item.s0 = sh[1], item.n = sh[2], item.len = sh[3], item.tt = sh[4], item.hh = hh;
-      const int bound = sh[5];
-      const long long start = *reinterpret_cast<long long*>(sh + 6);
-      __syncthreads();                                     // the scratch is free
+      item.b = from(f_b), item.s0 = from(s0), item.n = from(n), item.len = from(len), item.tt = from(f_tt), item.hh = hh;
+      const int bound = from(I), off = from(f_off);
+      const int64_t start = u - off;
       const int p0 = item.len - item.n + item.tt * a.TQ, p1 = min(p0 + a.TQ, item.len) - 1;
       const int real = item.len ? at_range(p0, p1, a.window, a.sinks, C::UNIT).I : 1;
       item.ns = 1, item.slot = 0, item.it0 = 0, item.it1 = real;
       if (a.meta) {
         // the share that holds unit x is ((x + 1) shares - 1) / total
         if (start < u0 || start + real > u1)
-          item.ns = (int)(divide((start + real) * shares - 1, total) - divide((start + 1) * shares - 1, total)) + 1;
+          item.ns = (int)(at_div((start + real) * shares - 1, total) - at_div((start + 1) * shares - 1, total)) + 1;
         item.slot = 2 * (j * a.Hh + hh) + (start > u0 ? 1 : 0);
-        item.it0 = (int)(u - start), item.it1 = (int)min((long long)real, u1 - start);
+        item.it0 = off, item.it1 = (int)min((int64_t)real, u1 - start);
       }
       if (item.it0 < item.it1) at_tile<C>(a, lds, item);
       u = start + bound;

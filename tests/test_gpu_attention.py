@@ -128,7 +128,7 @@ def _scales(rng, heads):
 
 @pytest.mark.parametrize("dims", list(DIMS))
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
-@pytest.mark.parametrize("N,Hq,Hkv,rot,page", [(1, 4, 2, 16, 16), (7, 5, 1, 64, 32), (65, 3, 3, 32, 16), (33, 16, 2, 0, 64)])
+@pytest.mark.parametrize("N,Hq,Hkv,rot,page", [(1, 4, 2, 16, 16), (7, 5, 1, 64, 32), (65, 3, 3, 32, 16), (33, 12, 2, 0, 64)])
 def test_append_matches_oracle(rng, dims, dtype, N, Hq, Hkv, rot, page):
     Dk, Dv = DIMS[dims]
     theta = 10000.0
@@ -266,7 +266,7 @@ RAGGED = ([1, 15, 16, 17, 63, 64, 65, 130, 300], [1] * 9)
 
 @pytest.mark.parametrize("dims", list(DIMS))
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
-@pytest.mark.parametrize("heads", [(1, 1), (4, 4), (6, 2), (16, 1), (10, 2), (33, 1)])
+@pytest.mark.parametrize("heads", [(1, 1), (4, 4), (6, 2), (20, 1), (10, 2), (33, 1)])
 def test_attend_decode(rng, dims, dtype, heads):
     _check(*_attend_case(rng, *RAGGED, *heads, *DIMS[dims], 16, dtype=dtype))
 
@@ -280,7 +280,7 @@ def test_attend_chunks(rng, page, lens, new):
 
 @pytest.mark.parametrize("dims", list(DIMS))
 @pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
-@pytest.mark.parametrize("heads", [(3, 1), (16, 1), (10, 2), (4, 4), (40, 1), (160, 1)])
+@pytest.mark.parametrize("heads", [(3, 1), (20, 1), (10, 2), (4, 4), (40, 1), (160, 1)])
 def test_attend_mixed_batch(rng, dims, dtype, heads):
     _check(*_attend_case(rng, [150, 33, 200, 70, 1], [150, 1, 41, 5, 1], *heads, *DIMS[dims], 32, dtype=dtype, logits=True))
 
@@ -398,7 +398,7 @@ def test_attend_strided_rows_and_zero_tokens(rng):
 
 
 def test_attend_repeats_bit_for_bit(rng):
-    q, cache, plan, kw = _attend_case(rng, [7000, 100, 2500], [1, 70, 1], 16, 2, 192, 128, 64, logits=True)
+    q, cache, plan, kw = _attend_case(rng, [7000, 100, 2500], [1, 70, 1], 20, 2, 192, 128, 64, logits=True)
     first = attend(q, cache, plan, **kw)
     for _ in range(3):
         assert torch.equal(attend(q, cache, plan, **kw), first)
