@@ -239,9 +239,9 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
   if (ns > 1) {
     const int p0 = it.len - it.n + it.tt * a.TQ, p1 = min(p0 + a.TQ, it.len) - 1;
     const int I = at_range(p0, p1, a.window, a.sinks, C::UNIT).I;
-    it.ns = (I + chunk - 1) / chunk;
+    it.ns = (I + chunk - 1) / chunk;                       // in parts of equal size
     if (split >= it.ns) return false;
-    it.it0 = split * chunk, it.it1 = it.it0 + chunk;
+    it.it0 = split * I / it.ns, it.it1 = (split + 1) * I / it.ns;
   }
   return true;
 }
@@ -836,85 +836,97 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
   at_clear(a, a.Hq * C::DV);
 }
 
-// The parts of split row tiles, joined in order: out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j.  A block looks at `per`
-// (token, head group) entries, of each at hpb heads from the block's on; its W waves share the parts of a head, wave w parts
-// w, w + W, ...: few rows with many parts take 16 waves, so that the parts arrive in one or two round trips.
+// The parts of a split row, joined in order by W waves: out = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) l_j, wave w parts w,
+// w + W, ... (eight at once, asked for before the weights are known).  The sums of the other waves come through LDS.
 template <int DV, int W>
-__global__ void __launch_bounds__(64 * W) attend_join_kernel(AttendArgs a, int per, int hpb) {
-  __shared__ float sl[W], so[W][DV];
-  __shared__ int2 s_meta[256];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int cuts = (a.HT + hpb - 1) / hpb, entries = a.N * a.Hh;
-  const int e0 = blockIdx.x / cuts * per, q0 = blockIdx.x % cuts * hpb;
-  const int first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N);
-  for (int e = t; e < per; e += 64 * W) {
-    const int n = (e0 + e) / a.Hh;
-    s_meta[e] = e0 + e < entries && n >= first && n < last ? a.meta[e0 + e] : make_int2(0, 0);
-  }
-  __syncthreads();
+__device__ __forceinline__ void at_join(const AttendArgs& a, int n, int hh, int qh, int2 mt, float (*so)[DV], float* sl) {
+  const int t = threadIdx.x, lane = t & 63, wave = W == 1 ? 0 : t >> 6;
   constexpr int E = DV / 64;
-  for (int e = 0; e < per; ++e) {
-    const int2 mt = s_meta[e];
-    const int ns = mt.y & 0xFFFF;
-    if (ns <= 1) continue;
-    const int n = (e0 + e) / a.Hh, hh = (e0 + e) % a.Hh;
-    const int hg = hh % a.HG, kv = hh / a.HG, heads = min(a.HT, a.G - hg * a.HT);
-    for (int qh = q0; qh < min(heads, q0 + hpb); ++qh) {
-      const size_t rows = (size_t)a.TQ * a.HT, in = (size_t)(mt.y >> 16) * a.HT + qh;
-      auto part = [&](int j) { return (size_t)(j ? (mt.x & ~a.part_mask) + j * a.part_step : mt.x) * rows + in; };
-      // the wave's first eight parts are asked for before the weights are known
-      float o[8][E];
-      float2 ml[8];
-      auto fetch = [&](int j0) __attribute__((always_inline)) {
+  const int ns = mt.y & 0xFFFF, hg = hh % a.HG, kv = hh / a.HG, head = kv * a.G + hg * a.HT + qh;
+  const size_t rows = (size_t)a.TQ * a.HT, in = (size_t)(mt.y >> 16) * a.HT + qh;
+  auto part = [&](int j) { return (size_t)(j ? (mt.x & ~a.part_mask) + j * a.part_step : mt.x) * rows + in; };
+  float o[8][E];
+  float2 ml[8];
+  auto fetch = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (j0 + W * i >= ns) break;
-          const size_t row = part(j0 + W * i);
-          const float* p = a.part_o + row * DV + E * lane;
-          ml[i] = *reinterpret_cast<const float2*>(a.part_ml + 2 * row);
+    for (int i = 0; i < 8; ++i) {
+      if (j0 + W * i >= ns) break;
+      const size_t row = part(j0 + W * i);
+      const float* p = a.part_o + row * DV + E * lane;
+      ml[i] = *reinterpret_cast<const float2*>(a.part_ml + 2 * row);
 #pragma unroll
-          for (int k = 0; k < E; ++k) o[i][k] = p[k];
-        }
-      };
-      if (wave < ns) fetch(wave);
-      float top = -INFINITY;
-      for (int j = lane; j < ns; j += 64) top = fmaxf(top, a.part_ml[2 * part(j)]);
+      for (int k = 0; k < E; ++k) o[i][k] = p[k];
+    }
+  };
+  if (wave < ns) fetch(wave);
+  float top = -INFINITY;
+  for (int j = lane; j < ns; j += 64) top = fmaxf(top, a.part_ml[2 * part(j)]);
 #pragma unroll
-      for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-      const float ref = top == -INFINITY ? 0.0f : top;
-      float tot = 0.0f, x[E];
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float tot = 0.0f, x[E];
 #pragma unroll
-      for (int i = 0; i < E; ++i) x[i] = 0.0f;
-      for (int j0 = wave; j0 < ns; j0 += 8 * W) {
-        if (j0 != wave) fetch(j0);
+  for (int i = 0; i < E; ++i) x[i] = 0.0f;
+  for (int j0 = wave; j0 < ns; j0 += 8 * W) {
+    if (j0 != wave) fetch(j0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (j0 + W * i >= ns) break;
-          const float f = at_exp2(ml[i].x - ref);
-          tot += f * ml[i].y;
+    for (int i = 0; i < 8; ++i) {
+      if (j0 + W * i >= ns) break;
+      const float f = at_exp2(ml[i].x - ref);
+      tot += f * ml[i].y;
 #pragma unroll
-          for (int k = 0; k < E; ++k) x[k] += f * o[i][k];
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < E; ++k) so[wave][E * lane + k] = x[k];
-      if (lane == 0) sl[wave] = tot;
-      __syncthreads();
-      const int head = kv * a.G + hg * a.HT + qh;
-      const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
-      const float all = fmaxf(top, sink), r2 = all == -INFINITY ? 0.0f : all, g = at_exp2(top - r2);
-      float sum = at_exp2(sink - r2);
-#pragma unroll
-      for (int w = 0; w < W; ++w) sum += sl[w] * g;
-      for (int d = t; d < DV; d += 64 * W) {
-        float y = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; ++w) y += so[w][d];
-        a.out[((size_t)n * a.Hq + head) * DV + d] = sum == 0.0f ? 0 : f32_to_bf16(y * g / sum);
-      }
-      __syncthreads();
+      for (int k = 0; k < E; ++k) x[k] += f * o[i][k];
     }
   }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) so[wave][E * lane + k] = x[k];
+    if (lane == 0) sl[wave] = tot;
+    __syncthreads();
+    tot = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) tot += sl[w];
+  }
+  const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
+  const float all = fmaxf(top, sink), r2 = all == -INFINITY ? 0.0f : all, g = at_exp2(top - r2), sum = tot * g + at_exp2(sink - r2);
+  uint16_t* out = a.out + ((size_t)n * a.Hq + head) * DV;
+  if constexpr (W > 1) {
+    for (int d = t; d < DV; d += 64 * W) {
+      float y = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) y += so[w][d];
+      out[d] = sum == 0.0f ? 0 : f32_to_bf16(y * g / sum);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < E; ++k) out[E * lane + k] = sum == 0.0f ? 0 : f32_to_bf16(x[k] * g / sum);
+  }
+}
+// the parts of an entry (a token and head group) that was split, or 0; read whether or not the token belongs to a request
+__device__ __forceinline__ int2 at_meta(const AttendArgs& a, int entry) {
+  const int2 mt = a.meta[entry];
+  const int n = entry / a.Hh, first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N);
+  return n >= first && n < last && (mt.y & 0xFFFF) > 1 ? mt : make_int2(0, 0);
+}
+
+// Few rows: a block for each, of W waves (few rows with many parts take 16, so that the parts arrive in one or two round trips).
+template <int DV, int W>
+__global__ void __launch_bounds__(64 * W) attend_join_kernel(AttendArgs a) {
+  __shared__ float sl[W], so[W][DV];
+  const int entry = blockIdx.x / a.HT, qh = blockIdx.x - entry * a.HT;
+  const int2 mt = at_meta(a, entry);
+  if (!mt.y || entry % a.Hh % a.HG * a.HT + qh >= a.G) return;
+  at_join<DV, W>(a, entry / a.Hh, entry % a.Hh, qh, mt, so, sl);
+}
+// Many rows: a wave for hpw heads of an entry.
+template <int DV>
+__global__ void __launch_bounds__(256) attend_join_many_kernel(AttendArgs a, int hpw) {
+  const int item = blockIdx.x * 4 + (threadIdx.x >> 6), cuts = (a.HT + hpw - 1) / hpw, e = item / cuts;
+  if (e >= a.N * a.Hh) return;
+  const int2 mt = at_meta(a, e);
+  if (!mt.y) return;
+  const int q0 = (item - e * cuts) * hpw, heads = min(min(a.HT, a.G - e % a.Hh % a.HG * a.HT), q0 + hpw);
+  for (int qh = q0; qh < heads; ++qh) at_join<DV, 1>(a, e / a.Hh, e % a.Hh, qh, mt, nullptr, nullptr);
 }
 
 // ------------------------------------------------------------------ host
@@ -969,14 +981,13 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   {
     ProfScope p(st, "attend_join");
     if (rows <= 256) {
-      attend_join_kernel<C::DV, 16><<<(unsigned)rows, 1024, 0, st>>>(a, 1, 1);
+      attend_join_kernel<C::DV, 16><<<(unsigned)rows, 1024, 0, st>>>(a);
     } else if (rows <= 1024) {
-      attend_join_kernel<C::DV, 4><<<(unsigned)rows, 256, 0, st>>>(a, 1, 1);
-    } else if (rows <= 16384) {
-      attend_join_kernel<C::DV, 1><<<(unsigned)rows, 64, 0, st>>>(a, 1, 1);
-    } else {                                               // mostly rows that were not split: a block looks at many
-      const int per = (int)std::min<int64_t>(256, (entries + 1023) / 1024);
-      attend_join_kernel<C::DV, 4><<<(unsigned)((entries + per - 1) / per), 256, 0, st>>>(a, per, a.HT);
+      attend_join_kernel<C::DV, 4><<<(unsigned)rows, 256, 0, st>>>(a);
+    } else {
+      const int hpw = rows <= 65536 ? 1 : a.HT;            // mostly rows that were not split
+      const int64_t waves = entries * ((a.HT + hpw - 1) / hpw);
+      attend_join_many_kernel<C::DV><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a, hpw);
     }
   }
   return check_launch("attend_join");
@@ -1013,9 +1024,9 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   MIMO_REQUIRE(q && starts && lens && table && out, MIMO_ERR_ARG, "cache_attend: null pointer");
   MIMO_REQUIRE(heads >= 1 && heads % cache->kv_heads == 0 && heads <= 1024, MIMO_ERR_SHAPE,
                "cache_attend: %d heads on %d K/V heads (a multiple, at most 1024)", heads, cache->kv_heads);
-  MIMO_REQUIRE(B >= 1 && max_pages >= 1 && max_new >= 0 && (int64_t)max_pages * cache->page_size <= kMaxTokens &&
+  MIMO_REQUIRE(B >= 1 && B <= (1 << 20) && max_pages >= 1 && max_new >= 0 && (int64_t)max_pages * cache->page_size <= kMaxTokens &&
                    (int64_t)max_pages * B <= 0x7fffffff, MIMO_ERR_SHAPE,
-               "cache_attend: need B, max_pages >= 1, max_new >= 0, at most 2^31 - 1 table entries, 2^31 - 2^16 tokens of a request "
+               "cache_attend: need 1 <= B <= 2^20, max_pages >= 1, max_new >= 0, at most 2^31 - 1 table entries, 2^31 - 2^16 tokens of a request "
                "(got %d, %d, %d)",
                B, max_pages, max_new);
   MIMO_REQUIRE(window >= 0 && sink_tokens >= 0, MIMO_ERR_SHAPE, "cache_attend: window and sink_tokens must be >= 0");
