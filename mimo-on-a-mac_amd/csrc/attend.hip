@@ -161,16 +161,6 @@ __device__ __forceinline__ void at_request(const AttendArgs& a, int b, int& s0, 
   len = a.lens[b];
   if (n && (len < n || len > ((long long)a.max_pages << a.page_shift))) len = 0;   // refused: its rows are set to 0
 }
-// a wave's inclusive prefix sum (row shifts by 1, 2, 4, 8, then the rows' last lanes to the rows behind) and its total
-__device__ __forceinline__ int at_prefix(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-  return v;
-}
 __device__ __forceinline__ int at_last(int v) { return __builtin_amdgcn_readlane(v, 63); }
 // quotient of non-negative numbers; 64-bit division is a long way round
 __device__ __forceinline__ int64_t at_div(int64_t x, int64_t y) {
@@ -196,7 +186,7 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
     tiles = min(tiles + nt, 1 << 22);
     load += (float)nt * at_most(len, a.window, a.sinks, a.TQ, C::UNIT);
   }
-  tiles = at_last(at_prefix(tiles));
+  tiles = at_last(dpp_prefix_i32(tiles));
   load = dpp_sum_f32(load);
   if (tiles > 1 << 21) return false;                       // at most N + 1 a request: starts that overlap
   // rounded up by more than the sum's error, so that the parts are within twice the target
@@ -212,7 +202,7 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
     units += nt * ns;
     parts += ns > 1 ? nt * ns : 0;
   }
-  int ub = at_prefix(units) - units, pb = at_prefix(parts) - parts;
+  int ub = dpp_prefix_i32(units) - units, pb = dpp_prefix_i32(parts) - parts;
   const int u = blockIdx.x / a.Hh, hh = blockIdx.x % a.Hh;
   int f_b = 0, f_tt = 0, f_split = 0, f_slot = 0, f_ns = 0;
   const bool here = u >= ub && u < ub + units;
@@ -784,7 +774,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
     mine += (int64_t)nt * I;
     tiles = min(tiles + nt, 1 << 22);
   }
-  tiles = at_last(at_prefix(tiles));
+  tiles = at_last(dpp_prefix_i32(tiles));
   int64_t before = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {

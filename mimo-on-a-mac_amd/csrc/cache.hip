@@ -33,30 +33,19 @@ struct StepArgs {
 
 // Exclusive scan of one value per thread over the block's 1024 threads, for three values at once; totals in tot[3].
 __device__ __forceinline__ void st_scan3(int v[3], int tot[3], int* sh) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int inc[3];
 #pragma unroll
   for (int q = 0; q < 3; ++q) {
-    int x = v[q];
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int y = __shfl_up(x, d, 64);
-      if (lane >= d) x += y;
-    }
-    inc[q] = x;
-    if (lane == 63) sh[16 * q + wave] = x;
+    inc[q] = dpp_prefix_i32(v[q]);
+    if (lane == 63) sh[16 * q + wave] = inc[q];
   }
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < 3; ++q) {
-    int base = 0, all = 0;
-    for (int w = 0; w < ST_THREADS / 64; ++w) {
-      const int t = sh[16 * q + w];
-      base += w < wave ? t : 0;
-      all += t;
-    }
-    v[q] = base + inc[q] - v[q];
-    tot[q] = all;
+    const int before = dpp_prefix_i32(lane < ST_THREADS / 64 ? sh[16 * q + lane] : 0);   // of the waves' sums
+    v[q] = (wave ? __builtin_amdgcn_readlane(before, wave - 1) : 0) + inc[q] - v[q];
+    tot[q] = __builtin_amdgcn_readlane(before, 63);
   }
   __syncthreads();
 }
@@ -189,6 +178,7 @@ struct AppendArgs {
 };
 
 constexpr int AP_MAX_ROT = 256;
+constexpr int AP_BLOCKS = 2048;                          // blocks that the card holds at once
 
 __device__ __forceinline__ void ap_unpack(uint4 x, float* f) {
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -214,12 +204,41 @@ __device__ __forceinline__ uint2 ap_pack_e4m3(const float* f, float scale) {
   return make_uint2(w[0], w[1]);
 }
 
+// A token is gridDim.y blocks of 256 threads, a thread one unit of 8 values (of a pair, two) at a time; the first unit is on
+// its way while the token's angles are worked out.
 template <bool E4M3>
 __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
 #pragma clang fp contract(off)
   __shared__ float s_cos[AP_MAX_ROT / 2], s_sin[AP_MAX_ROT / 2];
   const int n = blockIdx.x, half = a.rot >> 1;
   const int pos = a.positions[n], slot = a.slots[n];
+  const bool keep = slot >= 0 && slot < a.n_slots;
+  if (slot >= a.n_slots && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;
+  // units of 8 values: per q and k head rot / 16 pairs of units and (Dk - rot) / 8 units that stay, then v
+  const int pairs = a.rot >> 4, U = pairs + ((a.Dk - a.rot) >> 3), Uv = a.Dv >> 3;
+  const int nq = a.q ? a.Hq * U : 0, nk = a.Hkv * U, all = keep ? nq + nk + a.Hkv * Uv : nq;
+  struct Unit {
+    int kind, h, d;                                        // 0 q, 1 k, 2 v; head; first dimension
+    bool pair;
+    uint4 x, y;
+  };
+  auto load = [&](int u) __attribute__((always_inline)) {
+    Unit r;
+    r.kind = u < nq ? 0 : (u < nq + nk ? 1 : 2);
+    const int w = r.kind == 0 ? u : (r.kind == 1 ? u - nq : u - nq - nk), per = r.kind == 2 ? Uv : U;
+    r.h = w / per;
+    const int c = w - r.h * per;
+    r.pair = r.kind != 2 && c < pairs;
+    r.d = r.kind == 2 || r.pair ? 8 * c : a.rot + 8 * (c - pairs);
+    const uint16_t* row = r.kind == 0 ? a.q + n * a.q_stride + r.h * a.Dk : (r.kind == 1 ? a.k + n * a.k_stride + r.h * a.Dk : a.v + n * a.v_stride + r.h * a.Dv);
+    r.x = *reinterpret_cast<const uint4*>(row + r.d);
+    r.y = make_uint4(0, 0, 0, 0);
+    if (r.pair) r.y = *reinterpret_cast<const uint4*>(row + r.d + half);
+    return r;
+  };
+  int u = blockIdx.y * 256 + threadIdx.x;
+  Unit first{};
+  if (u < all) first = load(u);
   for (int i = threadIdx.x; i < half; i += 256) {
     const double t = (double)pos * a.turns[i];
     const float f = (float)(t - floor(t));
@@ -228,49 +247,37 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
     s_cos[i] = cs, s_sin[i] = sn;
   }
   __syncthreads();
-  const bool keep = slot >= 0 && slot < a.n_slots;
-  if (slot >= a.n_slots && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;
   const int mask = (1 << a.page_shift) - 1;
   const size_t prow = keep ? ((size_t)(slot >> a.page_shift) * a.Hkv << a.page_shift) + (slot & mask) : 0;
-  // units of 8 values: per q and k head rot / 16 pairs of units and (Dk - rot) / 8 units that stay, then v
-  const int pairs = a.rot >> 4, U = pairs + ((a.Dk - a.rot) >> 3), Uv = a.Dv >> 3;
-  const int nq = a.q ? a.Hq * U : 0, nk = a.Hkv * U, nv = a.Hkv * Uv;
   auto put = [&](void* pages, int h, int D, int d, const float* f, const float* scale) {
     const size_t at = (prow + ((size_t)h << a.page_shift)) * D + d;
     if constexpr (E4M3) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + at) = ap_pack_e4m3(f, scale[h]);
     else *reinterpret_cast<uint4*>(static_cast<uint16_t*>(pages) + at) = ap_pack(f);
   };
-  for (int u = threadIdx.x; u < nq + nk + nv; u += 256) {
-    const bool is_q = u < nq, is_v = u >= nq + nk;
-    if (!is_q && !keep) break;
-    if (is_v) {
-      const int w = u - nq - nk, h = w / Uv, d = (w - h * Uv) * 8;
-      float f[8];
-      ap_unpack(*reinterpret_cast<const uint4*>(a.v + n * a.v_stride + h * a.Dv + d), f);
-      put(a.v_pages, h, a.Dv, d, f, a.v_scale);
+  for (bool again = false; u < all; u += gridDim.y * 256, again = true) {
+    const Unit r = again ? load(u) : first;
+    float x[8], y[8];
+    ap_unpack(r.x, x);
+    if (r.kind == 2) {
+      put(a.v_pages, r.h, a.Dv, r.d, x, a.v_scale);
       continue;
     }
-    const int w = is_q ? u : u - nq, h = w / U, c = w - h * U;
-    const uint16_t* row = (is_q ? a.q + n * a.q_stride : a.k + n * a.k_stride) + h * a.Dk;
-    const int d = c < pairs ? 8 * c : a.rot + 8 * (c - pairs);
-    float x[8], y[8];
-    ap_unpack(*reinterpret_cast<const uint4*>(row + d), x);
-    if (c < pairs) {
-      ap_unpack(*reinterpret_cast<const uint4*>(row + d + half), y);
+    if (r.pair) {
+      ap_unpack(r.y, y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float cs = s_cos[d + i], sn = s_sin[d + i], p = x[i], r = y[i];
-        x[i] = p * cs - r * sn;
-        y[i] = r * cs + p * sn;
+        const float cs = s_cos[r.d + i], sn = s_sin[r.d + i], p = x[i], q = y[i];
+        x[i] = p * cs - q * sn;
+        y[i] = q * cs + p * sn;
       }
     }
-    if (is_q) {
-      uint16_t* o = a.q_out + ((size_t)n * a.Hq + h) * a.Dk;
-      *reinterpret_cast<uint4*>(o + d) = ap_pack(x);
-      if (c < pairs) *reinterpret_cast<uint4*>(o + d + half) = ap_pack(y);
+    if (r.kind == 0) {
+      uint16_t* o = a.q_out + ((size_t)n * a.Hq + r.h) * a.Dk + r.d;
+      *reinterpret_cast<uint4*>(o) = ap_pack(x);
+      if (r.pair) *reinterpret_cast<uint4*>(o + half) = ap_pack(y);
     } else {
-      put(a.k_pages, h, a.Dk, d, x, a.k_scale);
-      if (c < pairs) put(a.k_pages, h, a.Dk, d + half, y, a.k_scale);
+      put(a.k_pages, r.h, a.Dk, r.d, x, a.k_scale);
+      if (r.pair) put(a.k_pages, r.h, a.Dk, r.d + half, y, a.k_scale);
     }
   }
 }
@@ -356,8 +363,11 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
   hipStream_t st = as_stream(stream);
   {
     ProfScope p(st, "cache_append");
-    if (cache->dtype == MIMO_KV_E4M3) cache_append_kernel<true><<<N, 256, 0, st>>>(a);
-    else cache_append_kernel<false><<<N, 256, 0, st>>>(a);
+    // few tokens are spread over several blocks each
+    const int units = ((q ? heads : 0) * (cache->k_dim - rotary_dim / 2) + cache->kv_heads * (cache->k_dim - rotary_dim / 2 + cache->v_dim)) / 8;
+    const dim3 grid(N, std::max(1, std::min((units + 255) / 256, AP_BLOCKS / N)));
+    if (cache->dtype == MIMO_KV_E4M3) cache_append_kernel<true><<<grid, 256, 0, st>>>(a);
+    else cache_append_kernel<false><<<grid, 256, 0, st>>>(a);
   }
   return check_launch("cache_append");
 }

@@ -209,6 +209,17 @@ __device__ __forceinline__ uint32_t dpp_min_u32(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 
+// wave64 inclusive prefix sum: row shifts by 1, 2, 4 and 8, then the last lanes of rows to the rows behind them
+__device__ __forceinline__ int dpp_prefix_i32(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
 // order-preserving map of an fp32 key to uint32 (NaN lowest, -0 treated as +0)
 __device__ __forceinline__ uint32_t key_to_ordered(float k) {
   const uint32_t u = __float_as_uint(k == 0.0f ? 0.0f : k);
