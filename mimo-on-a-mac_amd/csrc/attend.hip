@@ -775,14 +775,20 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
     tiles = min(tiles + nt, 1 << 22);
   }
   tiles = at_last(dpp_prefix_i32(tiles));
-  int64_t before = mine;
+  int64_t before, total;
+  if (!__ballot(mine >> 25)) {                             // 64 of them stay below 2^31
+    const int p = dpp_prefix_i32((int)mine);
+    before = p - mine, total = at_last(p);
+  } else {
+    before = mine;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t p = __shfl_up(before, d, 64);
-    if (lane >= d) before += p;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t p = __shfl_up(before, d, 64);
+      if (lane >= d) before += p;
+    }
+    total = __shfl(before, 63, 64);
+    before -= mine;
   }
-  const int64_t total = __shfl(before, 63, 64);
-  before -= mine;
   // blocks that share the work: at least chunk_min units each, and one per CU while that leaves them no more than 8 and the
   // tiles alone do not fill the card
   const bool few = total * a.Hh <= 8 * (a.target / 2) && (int64_t)tiles * a.Hh < a.target / 2;
