@@ -162,11 +162,6 @@ __device__ __forceinline__ void at_request(const AttendArgs& a, int b, int& s0, 
   if (n && (len < n || len > ((long long)a.max_pages << a.page_shift))) len = 0;   // refused: its rows are set to 0
 }
 __device__ __forceinline__ int at_last(int v) { return __builtin_amdgcn_readlane(v, 63); }
-// quotient of non-negative numbers; 64-bit division is a long way round
-__device__ __forceinline__ int64_t at_div(int64_t x, int64_t y) {
-  return (uint64_t)(x | y) >> 32 ? x / y : (uint32_t)x / (uint32_t)y;
-}
-
 // The list of work, which every wave makes for itself without a word to the others: lane l looks at requests l per ..,
 // and the prefix sums of what they ask for are the places in the list.  Sizes are kept below 2^31 by refusing what only
 // starts that overlap can ask for (then nothing is computed).
@@ -792,10 +787,15 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
   // blocks that share the work: at least chunk_min units each, and one per CU while that leaves them no more than 8 and the
   // tiles alone do not fill the card
   const bool few = total * a.Hh <= 8 * (a.target / 2) && (int64_t)tiles * a.Hh < a.target / 2;
-  const int64_t most = max(1, (few ? a.target / 2 : a.target) / a.Hh);
-  const int64_t shares = max((int64_t)1, min(most, a.meta ? at_div(total + a.chunk_min - 1, a.chunk_min) : total));
-  if (j < shares && tiles <= 1 << 21) {                    // more (at most N + 1 a request): starts that overlap
-    const int64_t u0 = at_div(j * total, shares), u1 = at_div((j + 1) * total, shares);
+  const int most = max(1, (few ? a.target / 2 : a.target) / a.Hh), least = a.meta ? a.chunk_min : 1;
+  const uint32_t shares = total >= (int64_t)most * least ? most : max(1, (int)total / least);
+  // share x begins at unit (x coarse / shares) << sh, sh chosen so that 32 bits hold the products: no 64-bit division
+  const int sh = max(0, 65 - __builtin_clzll(total | 1) - __builtin_clz(shares));
+  const uint32_t coarse = (uint32_t)(total >> sh);
+  auto begin = [&](uint32_t x) { return x == shares ? total : (int64_t)(x * coarse / shares) << sh; };
+  auto holder = [&](int64_t x) { return (int)min(shares - 1, (((uint32_t)(x >> sh) + 1) * shares - 1) / max(1u, coarse)); };
+  if (j < (int)shares && tiles <= 1 << 21) {               // more (at most N + 1 a request): starts that overlap
+    const int64_t u0 = begin(j), u1 = begin(j + 1);
     for (int64_t u = u0; u < u1;) {
       int f_b = 0, f_tt = 0, f_off = 0;
       const bool here = u >= before && u < before + mine;
@@ -807,7 +807,12 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
           if (u < at + (int64_t)nt * I) break;
           at += (int64_t)nt * I;
         }
-        f_b = b, f_tt = (int)at_div(u - at, I), f_off = (int)(u - at - (int64_t)f_tt * I);
+        // tile of the request: the quotient by I, found bit by bit where 32 bits do not hold it
+        int64_t x = u - at;
+        for (int bit = 20; x >> 32; --bit)
+          if (x >= (int64_t)I << bit) x -= (int64_t)I << bit, f_tt += 1 << bit;
+        const uint32_t q = (uint32_t)x / (uint32_t)I;
+        f_b = b, f_tt += q, f_off = (uint32_t)x - q * I;
       }
       const int src = __builtin_ctzll(__ballot(here));
       auto from = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
@@ -819,9 +824,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
       const int real = item.len ? at_range(p0, p1, a.window, a.sinks, C::UNIT).I : 1;
       item.ns = 1, item.slot = 0, item.it0 = 0, item.it1 = real;
       if (a.meta) {
-        // the share that holds unit x is ((x + 1) shares - 1) / total
-        if (start < u0 || start + real > u1)
-          item.ns = (int)(at_div((start + real) * shares - 1, total) - at_div((start + 1) * shares - 1, total)) + 1;
+        if (start < u0 || start + real > u1) item.ns = holder(start + real - 1) - holder(start) + 1;
         item.slot = 2 * (j * a.Hh + hh) + (start > u0 ? 1 : 0);
         item.it0 = off, item.it1 = (int)min((int64_t)real, u1 - start);
       }
