@@ -53,7 +53,7 @@ struct AttendArgs {
   // tile can be split.
   float *part_o, *part_ml;
   int2* meta;
-  int part_mask, part_step;
+  int part_mask, part_step, slots;
 };
 
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -901,11 +901,14 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, int n, int hh, int 
     for (int k = 0; k < E; ++k) out[E * lane + k] = sum == 0.0f ? 0 : f32_to_bf16(x[k] * g / sum);
   }
 }
-// the parts of an entry (a token and head group) that was split, or 0; read whether or not the token belongs to a request
+// The parts of an entry (a token and head group) that was split, or 0.  It is read whether or not the token belongs to a
+// request, and starts that overlap may leave a row without one: what cannot be right is not followed.
 __device__ __forceinline__ int2 at_meta(const AttendArgs& a, int entry) {
   const int2 mt = a.meta[entry];
   const int n = entry / a.Hh, first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N);
-  return n >= first && n < last && (mt.y & 0xFFFF) > 1 ? mt : make_int2(0, 0);
+  const int ns = mt.y & 0xFFFF, place = (uint32_t)mt.y >> 16;
+  const bool ok = n >= first && n < last && ns > 1 && place < a.TQ && mt.x >= 0 && mt.x + (int64_t)(ns - 1) * a.part_step < a.slots;
+  return ok ? mt : make_int2(0, 0);
 }
 
 // Few rows: a block for each, of W waves (few rows with many parts take 16, so that the parts arrive in one or two round trips).
@@ -969,6 +972,7 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   MIMO_REQUIRE(grid < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many tiles");
   a.part_mask = C::WIDE ? 0 : 1;
   a.part_step = C::WIDE ? a.Hh : 2 * a.Hh;
+  a.slots = 2 * std::max(a.target, a.Hh);
   {
     ProfScope p(st, C::WIDE ? "attend_wide" : "attend_narrow");
     kernel<<<(unsigned)grid, AT_THREADS, C::LDS, st>>>(a);
@@ -1033,6 +1037,8 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   MIMO_REQUIRE(q_stride >= (int64_t)heads * cache->k_dim, MIMO_ERR_SHAPE, "cache_attend: rows closer than their length");
   MIMO_REQUIRE(aligned16(q) && aligned16(out) && q_stride % 8 == 0, MIMO_ERR_ALIGN,
                "cache_attend: 16-byte alignment of q, its rows and out");
+  MIMO_REQUIRE(!overlap(q, ((size_t)(N - 1) * q_stride + (size_t)heads * cache->k_dim) * 2, out, (size_t)N * heads * cache->v_dim * 2),
+               MIMO_ERR_ARG, "cache_attend: out may not overlap q");
   const size_t need = mimo_cache_attend_workspace_size(N, heads, cache->kv_heads, cache->v_dim);
   MIMO_REQUIRE(ws && ws_bytes >= need, MIMO_ERR_WORKSPACE, "cache_attend: workspace %zu < %zu", ws_bytes, need);
   MIMO_REQUIRE(aligned16(ws), MIMO_ERR_ALIGN, "cache_attend: 16-byte alignment of the workspace");

@@ -357,6 +357,12 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
   const int64_t kn = (int64_t)cache->kv_heads * cache->k_dim, vn = (int64_t)cache->kv_heads * cache->v_dim;
   MIMO_REQUIRE(k_stride >= kn && v_stride >= vn && (!q || q_stride >= (int64_t)heads * cache->k_dim), MIMO_ERR_SHAPE,
                "cache_append: rows closer than their length");
+  if (q) {
+    const size_t out = (size_t)N * heads * cache->k_dim * 2;
+    MIMO_REQUIRE(!overlap(q, ((size_t)(N - 1) * q_stride + (size_t)heads * cache->k_dim) * 2, q_out, out) &&
+                     !overlap(k, ((size_t)(N - 1) * k_stride + kn) * 2, q_out, out) && !overlap(v, ((size_t)(N - 1) * v_stride + vn) * 2, q_out, out),
+                 MIMO_ERR_ARG, "cache_append: q_out may not overlap q, k or v");
+  }
   AppendArgs a{q, k, v, q_stride, k_stride, v_stride, heads, cache->kv_heads, cache->k_dim, cache->v_dim, N, rotary_dim, turns,
                positions, slots, q_out, cache->k, cache->v, cache->k_scale, cache->v_scale, __builtin_ctz(cache->page_size),
                cache->n_pages * cache->page_size, status};

@@ -68,6 +68,7 @@ def test_cpu_tensors_are_refused():
 # ---- the C entries check on the host before any HIP call
 HOST = ctypes.create_string_buffer(4096)
 ADDR = (ctypes.addressof(HOST) + 255) // 256 * 256
+OUT = ADDR + 1024                                        # outputs that overlap no input
 
 
 def _kv(**kw):
@@ -98,21 +99,22 @@ def test_step_refusals(bad, code):
 
 def _append(cache=None, **kw):
     f = dict(q=ADDR, qs=128, heads=2, k=ADDR, ks=128, v=ADDR, vs=128, N=1, positions=ADDR, slots=ADDR, cache=cache or _kv(), dim=16,
-             turns=ADDR, q_out=ADDR, status=None, stream=None)
+             turns=ADDR, q_out=OUT, status=None, stream=None)
     f.update(kw)
     return _lib.load().mimo_cache_append(*f.values())
 
 
 @pytest.mark.parametrize("bad,code", [(dict(k=None), "ARG"), (dict(q_out=None), "ARG"), (dict(turns=None), "ARG"), (dict(dim=24), "SHAPE"),
                                       (dict(dim=80), "SHAPE"), (dict(N=-1), "SHAPE"), (dict(ks=120), "SHAPE"), (dict(vs=132), "ALIGN"),
-                                      (dict(q=ADDR + 8), "ALIGN"), (dict(heads=0), "SHAPE")])
+                                      (dict(q=ADDR + 8), "ALIGN"), (dict(heads=0), "SHAPE"),
+                                      (dict(q_out=ADDR), "ARG"), (dict(q=OUT, k=OUT + 256, q_out=OUT + 256), "ARG"), (dict(v=OUT + 240), "ARG")])
 def test_append_refusals(bad, code):
     assert _append(**bad) == getattr(_lib, "ERR_" + code)
 
 
 def _attend(cache=None, **kw):
     f = dict(q=ADDR, qs=128, N=1, heads=2, cache=cache or _kv(), B=1, starts=ADDR, lens=ADDR, table=ADDR, max_pages=1, max_new=1, scale=1.0,
-             window=0, sinks=0, logits=None, out=ADDR, status=None, ws=ADDR, bytes=1 << 40, stream=None)
+             window=0, sinks=0, logits=None, out=OUT, status=None, ws=ADDR, bytes=1 << 40, stream=None)
     f.update(kw)
     return _lib.load().mimo_cache_attend(*f.values())
 
@@ -120,8 +122,9 @@ def _attend(cache=None, **kw):
 @pytest.mark.parametrize("bad,code", [(dict(q=None), "ARG"), (dict(table=None), "ARG"), (dict(heads=3), "SHAPE"), (dict(heads=0), "SHAPE"),
                                       (dict(N=-1), "SHAPE"), (dict(B=0), "SHAPE"), (dict(max_pages=0), "SHAPE"), (dict(window=-1), "SHAPE"),
                                       (dict(sinks=-1), "SHAPE"), (dict(scale=float("nan")), "ARG"), (dict(scale=float("inf")), "ARG"),
-                                      (dict(qs=64), "SHAPE"), (dict(out=ADDR + 8), "ALIGN"), (dict(ws=None), "WORKSPACE"),
-                                      (dict(bytes=0), "WORKSPACE")])
+                                      (dict(qs=64), "SHAPE"), (dict(out=OUT + 8), "ALIGN"), (dict(ws=None), "WORKSPACE"),
+                                      (dict(bytes=0), "WORKSPACE"), (dict(out=ADDR), "ARG"), (dict(out=ADDR + 240), "ARG"), (dict(B=(1 << 20) + 1), "SHAPE"),
+                                      (dict(max_pages=1 << 27), "SHAPE"), (dict(N=(1 << 20) + 1), "SHAPE")])
 def test_attend_refusals(bad, code):
     assert _attend(**bad) == getattr(_lib, "ERR_" + code)
 

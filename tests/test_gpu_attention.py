@@ -333,6 +333,98 @@ def test_attend_never_looks_at_masked_values(rng, heads, new, dtype):
         assert (np.abs(x - ref) <= 2.0 ** -8 * np.abs(ref) + (2.0 ** -8 + 2.0 ** -11) * size).all()
 
 
+@pytest.mark.parametrize("lens,new,heads", [([3000], [4], (4, 1)), ([5000, 90], [40, 90], (2, 1)), ([400], [300], (6, 2))])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+def test_attend_keeps_one_rows_nan_from_the_others(rng, lens, new, heads, dtype):
+    """A chunk's last token holds NaN in K or V, over contexts that are split and that are not: only its own row turns NaN."""
+    for what in ("k", "v"):
+        q, cache, plan, kw = _attend_case(rng, lens, new, *heads, 128, 128, 16, dtype=dtype)
+        table = plan.table.cpu().numpy()
+        want, size = _oracle(q, cache, plan, kw)
+        getattr(cache, what)[table[0, (lens[0] - 1) // 16], :, (lens[0] - 1) % 16] = float("nan")
+        out = f64(attend(q, cache, plan, **kw))
+        last = new[0] - 1
+        assert np.isnan(out[last]).all()
+        rest = np.arange(len(out)) != last
+        assert (np.abs(out - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -11) * size)[rest].all()
+
+
+def test_attend_non_finite_values_that_all_rows_see(rng):
+    """An infinity in V reaches every row that weighs it, with its sign; a NaN in one request's q stays in that request."""
+    q, cache, plan, kw = _attend_case(rng, [300, 40], [60, 2], 4, 2, 64, 64, 16)
+    table = plan.table.cpu().numpy()
+    cache.v[table[0, 0], 0, 3, 7] = float("inf")
+    q[61] = float("nan")
+    out = attend(q, cache, plan, **kw).float()
+    assert (out[:60, :2, 7] == float("inf")).all() and torch.isnan(out[61]).all()
+    out[:60, :2, 7] = 0
+    assert torch.isfinite(out[:61]).all()
+
+
+@pytest.mark.parametrize("max_new", [None, 1, 64])
+def test_attend_does_not_depend_on_max_new(rng, max_new):
+    q, cache, plan, kw = _attend_case(rng, [300, 40, 9], [50, 1, 9], 6, 2, 128, 128, 16)
+    plan.max_new = max_new
+    _check(q, cache, plan, kw)
+
+
+@pytest.mark.parametrize("B,most", [(65, 1), (300, 1), (130, 40)])
+def test_attend_many_requests(rng, B, most):
+    """More requests than lanes, some of them idle, in one call."""
+    new = rng.integers(0, most + 1, B)
+    lens = new + rng.integers(0, 200, B)
+    new[lens == 0] = 0
+    _check(*_attend_case(rng, lens.tolist(), new.tolist(), 4, 2, 64, 64, 32, window=70, sinks=3))
+
+
+def test_attend_and_append_past_32_bit_offsets(rng):
+    """Pages whose bytes lie past 2^32 in the cache."""
+    pages, page, heads, dim = 70000, 32, 8, 128            # 4.3 GiB of K and of V
+    cache = KVCache.of(*(torch.empty(pages, heads, page, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    small = KVCache(4, page, heads, dim, dim)
+    high = [69999, 66000, 69998, 65999]
+    N = 100
+    x = torch.from_numpy(rng.standard_normal((N, 16 + 2 * heads, dim)).astype(np.float32)).to(torch.bfloat16).cuda()
+    outs = []
+    for c, ids in ((cache, high), (small, [0, 1, 2, 3])):
+        pos = np.arange(N)
+        plan = StepPlan(starts=i32([0, N]), lens=i32([N]), table=i32([ids]), positions=i32(pos),
+                        slots=i32(np.asarray(ids)[pos // page] * page + pos % page), status=torch.zeros(1, dtype=torch.int32, device="cuda"))
+        q = append(c, plan, x[:, 16:16 + heads], x[:, 16 + heads:], q=x[:, :16], rotary=Rotary(128))
+        outs.append(attend(q, c, plan))
+        plan.check()
+    assert torch.equal(*outs)
+    assert torch.equal(cache.k[high[1]], small.k[1]) and torch.equal(cache.v[high[2]], small.v[2])
+
+
+def test_a_failed_step_writes_nothing(rng):
+    pt, cache = PageTable(2, 4, 3, 16), KVCache(3, 16, 1, 64, 64)
+    x = torch.ones(40, 3, 64, dtype=torch.bfloat16, device="cuda")
+    plan = pt.step(i32([33, 7]), 40)                       # four pages of three
+    q = append(cache, plan, x[:, 1:2], x[:, 2:], q=x[:, :1])
+    out = attend(q, cache, plan)
+    assert (out == 0).all() and (cache.k == 0).all() and (cache.v == 0).all()
+    with pytest.raises(ValueError, match="pages"):
+        plan.check()
+    assert pt.lens.tolist() == [0, 0] and pt.n_free.item() == 3
+
+
+def test_attend_malformed_starts_stay_in_range(rng):
+    """starts that run backwards, past the rows or over one another: no fault, and other calls are as before."""
+    q, cache, plan, kw = _attend_case(rng, [40, 90, 20], [3, 33, 1], 4, 2, 64, 64, 16)
+    want = attend(q, cache, plan)
+    good = plan.starts.clone()
+    for bad in ([5, 3, 40, 2], [0, 37, 0, 37], [-9, 1 << 30, -5, 7], [40, 40, 40, 40], [2 ** 31 - 1] * 4, [-2 ** 31] * 4):
+        plan.starts.copy_(i32(bad))
+        for max_new in (1, 33):
+            plan.max_new = max_new
+            attend(q, cache, plan)
+    torch.cuda.synchronize()
+    plan.starts.copy_(good)
+    plan.max_new = 33
+    assert torch.equal(attend(q, cache, plan), want)
+
+
 def test_attend_scores_of_minus_infinity(rng):
     """Visible keys of score -inf weigh nothing; a row of only such keys, with no sink, is 0."""
     q, cache, plan, kw = _attend_case(rng, [40], [3], 2, 1, 64, 64, 16)
