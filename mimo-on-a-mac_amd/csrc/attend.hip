@@ -10,8 +10,9 @@
 //   P = 2^(c S - m)  in registers; the row maximum needs one exchange between the lane halves
 //   O^T += V^T P^T   the P registers 8 s .. 8 s + 7, rounded to bf16, are the B operand of keys 16 s .. as they stand: the
 //                    order of keys inside a product is free, so V^T is read in the same order, by transposing LDS reads
-// so neither S nor P leaves its lane, and m, l and the rescaling of O are per lane too.  P is rounded to bf16 because V is;
-// l sums the unrounded values.
+// so neither S nor P leaves its lane, and m, l and the rescaling of O are per lane too.  V is bf16, so P has to be: wide tiles
+// round it once (2^-9 of each weight; a second product for the rest would be 40% more matrix work), narrow ones, which wait
+// for memory, multiply the rounded rest as well, and their weights are as good as 32 bits.  l sums the unrounded values.
 //
 // K and V go from HBM to LDS without passing registers, 16 bytes a lane; in LDS a tile is [64-element column block][key][128
 // bytes, E4M3 64] with the 16-byte cells of a row permuted by its number, which keeps the operand reads free of bank conflicts.
@@ -428,7 +429,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   float m = -INFINITY, l = 0.0f;                           // l: this lane half's keys
 
   v16f S[C::NB];
-  bf16x8 P[C::NB][2];
+  bf16x8 P[C::NB][2], rest[C::WIDE ? 1 : C::NB][2];        // narrow: what the rounding of P leaves off, rounded
   // operands are read PX products ahead; the barriers keep the compiler from reading them all at once (spilled registers)
   constexpr int PX = 4;
   auto scores = [&](const uint8_t* st) __attribute__((always_inline)) {
@@ -501,6 +502,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
         const float p = at_exp2(__builtin_fmaf(S[kb][i], c, -ref));
         l += p;
         P[kb][i / 8][i % 8] = (__bf16)p;
+        if constexpr (!C::WIDE) rest[kb][i / 8][i % 8] = (__bf16)(p - (float)P[kb][i / 8][i % 8]);
       }
   };
   auto values = [&](const uint8_t* st) __attribute__((always_inline)) {
@@ -513,6 +515,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       const int kb = f / (2 * ND), s = f / ND % 2, d = f % ND;
       __builtin_amdgcn_sched_barrier(0);
       O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(X[f % PX], P[kb][s], O[d], 0, 0, 0);
+      if constexpr (!C::WIDE) O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(X[f % PX], rest[kb][s], O[d], 0, 0, 0);
       if (f + PX < F) X[f % PX] = v_frag(st, (f + PX) / (2 * ND), (f + PX) / ND % 2, (f + PX) % ND);
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -577,8 +580,9 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       if (more) issue_v(lds0);
     }
   }
-  // Sums that are not finite: if a value of a tile with masks is not (one position sees what another does not), it may have
-  // come through a weight of 0
+  // Sums that are not finite.  What a row sees makes them so rightly; wrongly, a value that it does not see and another does
+  // (through its weight of 0), or an infinity times a weight of 0 (a hidden key's copy, the rest of a weight) that makes it
+  // a NaN.
   bool suspect = false;
   {
     float worst = 0.0f;
@@ -586,18 +590,22 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
     for (int d = 0; d < C::DV / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) worst += O[d][i] - O[d][i];   // 0, or NaN
-    if (wp_min != wp_max && __ballot(busy && worst != 0.0f)) {
+    const bool apart = wp_min != wp_max;                   // rows that see different keys
+    if ((apart || !C::F8) && __ballot(busy && worst != 0.0f)) {
       bool odd = false;
 #pragma unroll 1
       for (int g = it0 * UG; g < min(rg.gt, it1 * UG); ++g) {
-        if (open(g / TG * TG)) continue;
+        const bool op = open(g / TG * TG);
+        if (op && (C::WIDE || C::F8)) continue;
         const AtKeys k = at_keys(a, rg, b, rg.key(g));
         const int page = at_page(a, k.id);
 #pragma unroll 1
         for (int x = 0; x < 16; ++x) {
           const size_t row = at_row(a, rg, k, page, kv, x) * C::DV;
           const uint32_t w = lane < C::DV * ES / 4 ? *reinterpret_cast<const uint32_t*>(a.v + row * ES + 4 * lane) : 0u;
-          odd |= C::F8 ? (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0 : (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) != 0;
+          if (C::F8) odd |= (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
+          else if (apart && !op) odd |= (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) != 0;
+          else odd |= (w & 0x7FFFu) == 0x7F80u || (w >> 16 & 0x7FFFu) == 0x7F80u;
         }
       }
       suspect = __ballot(odd) != 0;

@@ -349,16 +349,24 @@ def test_attend_keeps_one_rows_nan_from_the_others(rng, lens, new, heads, dtype)
         assert (np.abs(out - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -11) * size)[rest].all()
 
 
-def test_attend_non_finite_values_that_all_rows_see(rng):
-    """An infinity in V reaches every row that weighs it, with its sign; a NaN in one request's q stays in that request."""
-    q, cache, plan, kw = _attend_case(rng, [300, 40], [60, 2], 4, 2, 64, 64, 16)
+@pytest.mark.parametrize("new,heads", [([60, 2], (4, 2)), ([1, 1], (4, 2)), ([4, 2], (8, 2)), ([1, 1], (130, 1))])
+@pytest.mark.parametrize("key", [3, 295])
+def test_attend_non_finite_values_that_rows_see(rng, new, heads, key):
+    """An infinity in V reaches every row that weighs it, with its sign, wherever it lies; a NaN in one request's q stays in
+    that request."""
+    q, cache, plan, kw = _attend_case(rng, [300, 40], new, *heads, 64, 64, 16)
     table = plan.table.cpu().numpy()
-    cache.v[table[0, 0], 0, 3, 7] = float("inf")
-    q[61] = float("nan")
+    G, n = heads[0] // heads[1], new[0]
+    cache.v[table[0, key // 16], 0, key % 16, 7] = float("inf")
+    cache.v[table[0, key // 16], 0, key % 16, 9] = -float("inf")
+    q[n] = float("nan")
     out = attend(q, cache, plan, **kw).float()
-    assert (out[:60, :2, 7] == float("inf")).all() and torch.isnan(out[61]).all()
-    out[:60, :2, 7] = 0
-    assert torch.isfinite(out[:61]).all()
+    sees = torch.arange(300 - n, 300, device="cuda") >= key
+    assert (out[:n][sees][:, :G, 7] == float("inf")).all() and (out[:n][sees][:, :G, 9] == -float("inf")).all()
+    assert torch.isnan(out[n]).all()
+    out[:n, :G, 7] = torch.where(sees[:, None], 0.0, out[:n, :G, 7])
+    out[:n, :G, 9] = torch.where(sees[:, None], 0.0, out[:n, :G, 9])
+    assert torch.isfinite(out[:n]).all() and torch.isfinite(out[n + 1:]).all()
 
 
 @pytest.mark.parametrize("max_new", [None, 1, 64])
