@@ -30,6 +30,7 @@ STATUS_MESSAGES = {_lib.ERR_PAGES: "fewer free pages than the step needs",
 # A decode step makes one step call and two calls per layer, each of a few microseconds on the GPU: what they do on the host
 # is kept short (one check per tensor, entry points and structs looked up once).
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _device(device):
@@ -40,12 +41,6 @@ def _device(device):
 @functools.lru_cache(maxsize=None)
 def _entry(name):
     return getattr(_lib.load(), name)
-
-
-def _call(name, *args):
-    rc = _entry(name)(*args)
-    if rc != _lib.MIMO_OK:
-        _lib.check(rc, name)
 
 
 def _gpu(dev):
@@ -121,7 +116,7 @@ class PageTable:
         out of range) leaves the state as it was and is in plan.status (plan.check() raises)."""
         dev = self._lens.device
         index = _gpu(dev)
-        if torch.cuda.current_device() != index:
+        if _current_device() != index:
             with torch.cuda.device(dev):
                 return self.step(target, n_tokens, max_new, commit)
         B, width = self._table.shape
@@ -136,9 +131,12 @@ class PageTable:
         at_starts = at + 4 * B + 8
         at_slots = at_starts + 4 * B + 4
         state, count = self._lens.data_ptr(), self._n_free.data_ptr()
-        _call("mimo_cache_step", state, at_target, B, self._table.data_ptr(), width, self._free.data_ptr(), count, self.n_pages,
-              self.page_size, n_tokens, max_new, at, at + 4 * B, at_starts, at_slots, at_slots + 4 * n_tokens,
-              state if commit else None, count if commit else None, at + 4 * B + 4, _raw_stream(index))
+        rc = _entry("mimo_cache_step")(
+            state, at_target, B, self._table.data_ptr(), width, self._free.data_ptr(), count, self.n_pages, self.page_size,
+            n_tokens, max_new, at, at + 4 * B, at_starts, at_slots, at_slots + 4 * n_tokens, state if commit else None,
+            count if commit else None, at + 4 * B + 4, _raw_stream(index))
+        if rc:
+            _lib.check(rc, "mimo_cache_step")
         return StepPlan(starts, lens, slots, positions, self._table, max_new, n_free, status)
 
 
@@ -236,7 +234,7 @@ def append(cache, plan, k, v, q=None, rotary=None):
     views of one projection's rows."""
     dev = cache.device
     index = _gpu(dev)
-    if torch.cuda.current_device() != index:
+    if _current_device() != index:
         with torch.cuda.device(dev):
             return append(cache, plan, k, v, q, rotary)
     k, at_k, k_stride = _rows(k, dev, cache.kv_heads, cache.k_dim, "k")
@@ -264,8 +262,11 @@ def append(cache, plan, k, v, q=None, rotary=None):
         at_out = out.data_ptr()
     status = _status(plan, dev)
     if N:
-        _call("mimo_cache_append", at_q, q_stride, heads, at_k, k_stride, at_v, v_stride, N, at_positions, at_slots,
-              cache._struct, dim, turns, at_out, status, _raw_stream(index))
+        rc = _entry("mimo_cache_append")(
+            at_q, q_stride, heads, at_k, k_stride, at_v, v_stride, N, at_positions, at_slots, cache._struct, dim, turns, at_out,
+            status, _raw_stream(index))
+        if rc:
+            _lib.check(rc, "mimo_cache_append")
     return out
 
 
@@ -290,7 +291,7 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
     a value.  Returns bf16 [N, heads, v_dim] (out, if given: contiguous bf16); rows of no request are 0."""
     dev = cache.device
     index = _gpu(dev)
-    if torch.cuda.current_device() != index:
+    if _current_device() != index:
         with torch.cuda.device(dev):
             return attend(q, cache, plan, scale, window, sink_tokens, sink_logits, out)
     q, at_q, q_stride = _rows(q, dev, None, cache.k_dim, "q")
@@ -321,9 +322,12 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
         return out
     stream = _raw_stream(index)
     ws = _workspace(_workspace_size(N, heads, cache.kv_heads, cache.v_dim), dev, stream)
-    _call("mimo_cache_attend", at_q, q_stride, N, heads, cache._struct, B, at_starts, at_lens, at_table, width,
-          N if plan.max_new is None else min(N, int(plan.max_new)), cache.k_dim ** -0.5 if scale is None else float(scale),
-          int(window), int(sink_tokens), at_logits, out.data_ptr(), status, ws.data_ptr(), ws.numel(), stream)
+    rc = _entry("mimo_cache_attend")(
+        at_q, q_stride, N, heads, cache._struct, B, at_starts, at_lens, at_table, width,
+        N if plan.max_new is None else min(N, int(plan.max_new)), cache.k_dim ** -0.5 if scale is None else float(scale),
+        int(window), int(sink_tokens), at_logits, out.data_ptr(), status, ws.data_ptr(), ws.numel(), stream)
+    if rc:
+        _lib.check(rc, "mimo_cache_attend")
     return out
 
 
@@ -366,7 +370,7 @@ class AttentionLayer:
         index = _gpu(dev)
         if x.device != dev or x.dim() != 2 or x.shape[1] != self.hidden:
             raise ValueError(f"x: need [tokens, {self.hidden}] on {dev}, got {tuple(x.shape)} on {x.device}")
-        if torch.cuda.current_device() != index:
+        if _current_device() != index:
             with torch.cuda.device(dev):
                 return self(x, plan)
         x = x.to(BF16).contiguous()
@@ -377,12 +381,12 @@ class AttentionLayer:
         if N == 0:
             return h
         r = torch.empty_like(x)
-        _call("mimo_rmsnorm", x.data_ptr(), N, self.hidden, self.norm_weight.data_ptr(), self.eps, r.data_ptr(), _raw_stream(index))
+        _lib.call("mimo_rmsnorm", _lib.ptr(x), N, self.hidden, _lib.ptr(self.norm_weight), self.eps, _lib.ptr(r), _lib.stream_ptr(dev))
         c = self.cache
         q, k, v = torch.matmul(r, self.qkv_weight.T).split_with_sizes(self.split, 1)
         q = append(c, plan, k.unflatten(1, (c.kv_heads, c.k_dim)), v.unflatten(1, (c.kv_heads, c.v_dim)),
                    q=q.unflatten(1, (self.heads, c.k_dim)), rotary=self.rotary)
         o = attend(q, c, plan, self.scale, self.window, self.sink_tokens, self.sink_logits)
         y = torch.matmul(o.flatten(1), self.o_weight.T)
-        _call("mimo_residual_add", x.data_ptr(), y.data_ptr(), x.numel(), h.data_ptr(), _raw_stream(index))
+        _lib.call("mimo_residual_add", _lib.ptr(x), _lib.ptr(y), x.numel(), _lib.ptr(h), _lib.stream_ptr(dev))
         return h
