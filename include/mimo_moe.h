@@ -251,19 +251,19 @@ typedef struct mimo_kv_cache {
  * requests and stack entries at and above n_free are written in place; they mean nothing under the old lengths, so a step
  * whose outputs are dropped leaves the state as it was.  commit_lens / commit_n_free (both or neither; lens and n_free
  * themselves, as a rule) receive the new lengths and count after everything else.  status [1] is overwritten: MIMO_OK,
- * MIMO_ERR_PAGES when too few pages are free, MIMO_ERR_SHAPE when a length is outside [0, max_pages * page_size] (at most 2^31 - 2^16), a request
- * grows by more than max_new, the new tokens are more than N (at most 2^20) or n_free and the table disagree; then starts
- * are 0, slots -1, and lens_out / n_free_out the old state. */
+ * MIMO_ERR_PAGES when too few pages are free, MIMO_ERR_SHAPE when a length is outside [0, max_pages * page_size] (at most
+ * 2^31 - 2^16), a request grows by more than max_new, the new tokens are more than N (at most 2^20) or n_free and the lengths
+ * disagree; then starts are 0, slots -1, and lens_out / n_free_out the old state. */
 int mimo_cache_step(const int32_t* lens, const int32_t* target, int B, int32_t* table, int max_pages,
                     int32_t* free_pages, const int32_t* n_free, int n_pages, int page_size, int N, int max_new,
                     int32_t* lens_out, int32_t* n_free_out, int32_t* starts, int32_t* slots, int32_t* positions,
                     int32_t* commit_lens, int32_t* commit_n_free, int32_t* status, void* stream);
 
 /* Rotary positions on q and k (the first rotary_dim dimensions of a head, pairs (i, i + rotary_dim / 2); the reference's
- * partial RoPE, engine/mimo_stream/mimo_v2.py:66-150) and the write of k and v to their slots.  q bf16 [N, heads, k_dim] (NULL:
- * none), k [N, kv_heads, k_dim], v [N, kv_heads, v_dim], tokens *_stride elements apart (multiples of 8); turns fp64
- * [rotary_dim / 2]: turns per position of each pair (frequency / 2 pi).  q_out bf16 [N, heads, k_dim] may not overlap q, k or v.  A slot
- * below 0 writes no k and v; slots are distinct otherwise.  Rotated values are rounded once, to bf16 or (divided by their
+ * partial RoPE, engine/mimo_stream/mimo_v2.py:66-150) and the write of k and v to their slots.  q bf16 [N, heads, k_dim]
+ * (NULL: none), k [N, kv_heads, k_dim], v [N, kv_heads, v_dim], tokens *_stride elements apart (multiples of 8); turns fp64
+ * [rotary_dim / 2]: turns per position of each pair (frequency / 2 pi).  q_out bf16 [N, heads, k_dim] may not overlap q, k
+ * or v.  A slot below 0 writes no k and v; slots are distinct otherwise.  Rotated values are rounded once, to bf16 or (divided by their
  * head's scale, clamped to +-448) to E4M3.  status (optional) receives MIMO_ERR_SLOT for a slot past the cache, which is
  * skipped; it is not cleared. */
 int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k, int64_t k_stride,
@@ -277,10 +277,10 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
  * window > 0 those with p - j < window, and the first sink_tokens.  out[n, h] = sum_j w_j v_j / (sum_j w_j + w_sink), w_j =
  * exp(scale q.k_j - m), w_sink = exp(sink_logits[h] - m) (NULL: none); a row whose weights sum to 0 gives 0.  Masked keys and
  * values are not looked at: they may be NaN.  heads is a multiple of kv_heads, q bf16 [N, heads, k_dim] with tokens q_stride
- * elements apart, out bf16 [N, heads, v_dim] (not overlapping q); rows that belong to no request are set to 0.  max_new: no request has more new
- * tokens (it picks the kernel; results do not depend on it).  status (optional, not cleared) receives MIMO_ERR_SLOT for a
- * page id outside the cache (page 0 is read) and MIMO_ERR_SHAPE for a request whose lens is below its rows or past max_pages
- * (its rows are 0). */
+ * elements apart, out bf16 [N, heads, v_dim] (not overlapping q); rows that belong to no request are set to 0.  max_new: no
+ * request has more new tokens (it picks the kernel: a wrong one costs time, and results differ by their roundings only).
+ * status (optional, not cleared) receives MIMO_ERR_SLOT for a page id outside the cache (page 0 is read) and MIMO_ERR_SHAPE
+ * for a request whose lens is below its rows or past max_pages (its rows are 0). */
 int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, const mimo_kv_cache* cache, int B,
                       const int32_t* starts, const int32_t* lens, const int32_t* table, int max_pages, int max_new,
                       float scale, int window, int sink_tokens, const float* sink_logits, uint16_t* out,

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(ST_THREADS) cache_step_kernel(StepArgs a) {
   int status = s_bad;
   if (!status && tot[0] > a.N) status = MIMO_ERR_SHAPE;
   if (!status && (long long)taken - freed > n_free) status = MIMO_ERR_PAGES;
-  if (!status && n_free + freed - taken > a.n_pages) status = MIMO_ERR_SHAPE;
+  if (!status && (long long)n_free + freed - taken > a.n_pages) status = MIMO_ERR_SHAPE;
   const bool first = blockIdx.x == 0;
   if (status) {                                      // nothing moves: no new tokens, lengths and the stack as they were
     if (first) {

@@ -121,6 +121,18 @@ def test_step_failures_leave_the_state(what):
     assert plan.starts.abs().sum().item() == 0 and (plan.slots == -1).all() and torch.equal(plan.lens, pt.lens)
 
 
+def test_step_refuses_more_returned_pages_than_32_bits_hold():
+    # lengths that were never written, at the largest table: the pages that ending all requests gives back are 2^31 - 4096
+    width, page, n_pages = (1 << 19) - 1, 16, 1 << 20
+    pt = PageTable(4096, width, n_pages, page)
+    pt.lens.fill_(width * page)
+    plan = pt.step(torch.zeros_like(pt.lens), 4)
+    with pytest.raises(ValueError, match="lengths"):
+        plan.check()
+    assert int(pt.n_free.item()) == n_pages and bool((pt.lens == width * page).all()) and (plan.slots == -1).all()
+    assert torch.equal(pt.free, torch.arange(n_pages - 1, -1, -1, dtype=torch.int32, device="cuda"))
+
+
 # ------------------------------------------------------------------ append
 def _scales(rng, heads):
     return torch.from_numpy((2.0 ** rng.uniform(-6, -3, heads)).astype(np.float32)).cuda()
