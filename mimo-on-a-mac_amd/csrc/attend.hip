@@ -847,7 +847,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
 // w + W, ... (eight at once, asked for before the weights are known).  The sums of the other waves come through LDS.
 template <int DV, int W>
 __device__ __forceinline__ void at_join(const AttendArgs& a, int n, int hh, int qh, int2 mt, float (*so)[DV], float* sl) {
-  const int t = threadIdx.x, lane = t & 63, wave = W == 1 ? 0 : t >> 6;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   constexpr int E = DV / 64;
   const int ns = mt.y & 0xFFFF, hg = hh % a.HG, kv = hh / a.HG, head = kv * a.G + hg * a.HT + qh;
   const size_t rows = (size_t)a.TQ * a.HT, in = (size_t)(mt.y >> 16) * a.HT + qh;
@@ -885,28 +885,21 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, int n, int hh, int 
       for (int k = 0; k < E; ++k) x[k] += f * o[i][k];
     }
   }
-  if constexpr (W > 1) {
 #pragma unroll
-    for (int k = 0; k < E; ++k) so[wave][E * lane + k] = x[k];
-    if (lane == 0) sl[wave] = tot;
-    __syncthreads();
-    tot = 0.0f;
+  for (int k = 0; k < E; ++k) so[wave][E * lane + k] = x[k];
+  if (lane == 0) sl[wave] = tot;
+  __syncthreads();
+  tot = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) tot += sl[w];
-  }
+  for (int w = 0; w < W; ++w) tot += sl[w];
   const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
   const float all = fmaxf(top, sink), r2 = all == -INFINITY ? 0.0f : all, g = at_exp2(top - r2), sum = tot * g + at_exp2(sink - r2);
   uint16_t* out = a.out + ((size_t)n * a.Hq + head) * DV;
-  if constexpr (W > 1) {
-    for (int d = t; d < DV; d += 64 * W) {
-      float y = 0.0f;
+  for (int d = t; d < DV; d += 64 * W) {
+    float y = 0.0f;
 #pragma unroll
-      for (int w = 0; w < W; ++w) y += so[w][d];
-      out[d] = sum == 0.0f ? 0 : f32_to_bf16(y * g / sum);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < E; ++k) out[E * lane + k] = sum == 0.0f ? 0 : f32_to_bf16(x[k] * g / sum);
+    for (int w = 0; w < W; ++w) y += so[w][d];
+    out[d] = sum == 0.0f ? 0 : f32_to_bf16(y * g / sum);
   }
 }
 // The parts of an entry (a token and head group) that was split, or 0.  It is read whether or not the token belongs to a
@@ -928,15 +921,59 @@ __global__ void __launch_bounds__(64 * W) attend_join_kernel(AttendArgs a) {
   if (!mt.y || entry % a.Hh % a.HG * a.HT + qh >= a.G) return;
   at_join<DV, W>(a, entry / a.Hh, entry % a.Hh, qh, mt, so, sl);
 }
-// Many rows: a wave for hpw heads of an entry.
+// Many rows: DV / 4 lanes for `per` heads of an entry, one after another; a row's parts come PB at a time, under a running
+// maximum.
 template <int DV>
-__global__ void __launch_bounds__(256) attend_join_many_kernel(AttendArgs a, int hpw) {
-  const int item = blockIdx.x * 4 + (threadIdx.x >> 6), cuts = (a.HT + hpw - 1) / hpw, e = item / cuts;
-  if (e >= a.N * a.Hh) return;
-  const int2 mt = at_meta(a, e);
-  if (!mt.y) return;
-  const int q0 = (item - e * cuts) * hpw, heads = min(min(a.HT, a.G - e % a.Hh % a.HG * a.HT), q0 + hpw);
-  for (int qh = q0; qh < heads; ++qh) at_join<DV, 1>(a, e / a.Hh, e % a.Hh, qh, mt, nullptr, nullptr);
+__global__ void __launch_bounds__(256, 8) attend_join_many_kernel(AttendArgs a, int per) {
+  constexpr int LANES = DV / 4, PB = 4;
+  const int d = 4 * (threadIdx.x & (LANES - 1)), cuts = (a.HT + per - 1) / per;
+  const int item = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, entry = item / cuts;
+  if (entry >= a.N * a.Hh) return;
+  const int2 mt = at_meta(a, entry);
+  const int ns = mt.y & 0xFFFF, n = entry / a.Hh, hh = entry - n * a.Hh, kv = hh / a.HG, hg = hh - kv * a.HG;
+  const int q0 = (item - entry * cuts) * per, q1 = ns ? min(min(a.HT, a.G - hg * a.HT), q0 + per) : 0;
+#pragma unroll 1
+  for (int qh = q0; qh < q1; ++qh) {
+    const int head = kv * a.G + hg * a.HT + qh;
+    const size_t tile = (size_t)a.TQ * a.HT, in = (size_t)((uint32_t)mt.y >> 16) * a.HT + qh;
+    float top = -INFINITY, tot = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j0 = 0; j0 < ns; j0 += PB) {
+      float2 ml[PB];
+      float4 o[PB];
+#pragma unroll
+      for (int i = 0; i < PB; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.0f);
+        o[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (j0 + i < ns) {
+          const size_t at = (size_t)(j0 + i ? (mt.x & ~a.part_mask) + (j0 + i) * a.part_step : mt.x) * tile + in;
+          ml[i] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+          o[i] = *reinterpret_cast<const float4*>(a.part_o + at * DV + d);
+        }
+      }
+      float next = top;
+#pragma unroll
+      for (int i = 0; i < PB; ++i) next = fmaxf(next, ml[i].x);
+      const float ref = next == -INFINITY ? 0.0f : next, was = at_exp2(top - ref);
+      top = next;
+      tot *= was;
+      x.x *= was, x.y *= was, x.z *= was, x.w *= was;
+#pragma unroll
+      for (int i = 0; i < PB; ++i) {
+        const float f = at_exp2(ml[i].x - ref);
+        tot += f * ml[i].y;
+        x.x += f * o[i].x, x.y += f * o[i].y, x.z += f * o[i].z, x.w += f * o[i].w;
+      }
+    }
+    const float sink = a.sink_logits ? a.sink_logits[head] * kLog2e : -INFINITY;
+    const float all = fmaxf(top, sink), ref = all == -INFINITY ? 0.0f : all, g = at_exp2(top - ref), sum = tot * g + at_exp2(sink - ref);
+    const float w = sum == 0.0f ? 0.0f : g / sum;
+    uint2 y;
+    y.x = (uint32_t)f32_to_bf16(x.x * w) | ((uint32_t)f32_to_bf16(x.y * w) << 16);
+    y.y = (uint32_t)f32_to_bf16(x.z * w) | ((uint32_t)f32_to_bf16(x.w * w) << 16);
+    if (sum == 0.0f) y = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(a.out + ((size_t)n * a.Hq + head) * DV + d) = y;
+  }
 }
 
 // ------------------------------------------------------------------ host
@@ -996,9 +1033,10 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
     } else if (rows <= 1024) {
       attend_join_kernel<C::DV, 4><<<(unsigned)rows, 256, 0, st>>>(a);
     } else {
-      const int hpw = rows <= 65536 ? 1 : a.HT;            // mostly rows that were not split
-      const int64_t waves = entries * ((a.HT + hpw - 1) / hpw);
-      attend_join_many_kernel<C::DV><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a, hpw);
+      const int per = rows <= 65536 ? 1 : std::min(a.HT, 8);   // mostly rows that were not split
+      const int64_t items = entries * ((a.HT + per - 1) / per);
+      constexpr int IPB = 1024 / C::DV;
+      attend_join_many_kernel<C::DV><<<(unsigned)((items + IPB - 1) / IPB), 256, 0, st>>>(a, per);
     }
   }
   return check_launch("attend_join");
