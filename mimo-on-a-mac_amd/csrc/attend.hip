@@ -60,6 +60,7 @@ struct AttendArgs {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int AT_THREADS = 256;
 constexpr int AT_WIDE_TARGET = 512, AT_WIDE_MIN = 4;      // blocks wanted, least 64-key tiles of a block
+constexpr int AT_START = 8;                               // 64-key tiles that a wide block's start and a part's join cost
 constexpr int AT_NARROW_TARGET = 512, AT_NARROW_MIN = 2;  // blocks (two per CU), least 128-key units of one
 
 template <int DK_, int DV_, bool F8_, bool WIDE_> struct AtCfg {
@@ -166,38 +167,73 @@ __device__ __forceinline__ int at_last(int v) { return __builtin_amdgcn_readlane
 // The list of work, which every wave makes for itself without a word to the others: lane l looks at requests l per ..,
 // and the prefix sums of what they ask for are the places in the list.  Sizes are kept below 2^31 by refusing what only
 // starts that overlap can ask for (then nothing is computed).
-// Wide tiles.  Block blockIdx.x's item: (request, row tile from the last to the first, part) x head group, head groups
-// fastest: neighbouring blocks, on different XCDs, work on different heads, and an XCD keeps meeting the same ones.  A tile
-// is cut into parts of `chunk` units, the fair share of `target` blocks.  false: past the end of the list, or a part that
-// this tile does not have.
+// Wide tiles.  Block blockIdx.x's item: (request, part, row tile from the last to the first) x head group, head groups
+// fastest: neighbouring blocks, on different XCDs, work on different heads, and an XCD keeps meeting the same ones.  Parts
+// that a request's shorter tiles do not have stand together at its end (were a tile's parts neighbours, these blocks without
+// work would all fall on the same XCDs: 320 tiles, half of them split, took 333 us instead of 185).  A tile is cut into parts
+// of `chunk` units.  false: past the end of the list, or a part that this tile does not have.
 template <class C>
 __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
   const int lane = threadIdx.x & 63;
   const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
-  int s0, n, len, tiles = 0;
+  int s0, n, len, tiles = 0, nt, ns, I, first_nt = 0, first_I = 0, longest = 0;
   float load = 0.0f;                                       // units of all tiles; only their share per block is wanted
-  for (int b = b0; b < b1; ++b) {
-    at_request(a, b, s0, n, len);
-    const int nt = (n + a.TQ - 1) / a.TQ;
-    tiles = min(tiles + nt, 1 << 22);
-    load += (float)nt * at_most(len, a.window, a.sinks, a.TQ, C::UNIT);
-  }
-  tiles = at_last(dpp_prefix_i32(tiles));
-  load = dpp_sum_f32(load);
-  if (tiles > 1 << 21) return false;                       // at most N + 1 a request: starts that overlap
-  // rounded up by more than the sum's error, so that the parts are within twice the target
-  const int chunk = max(a.chunk_min, (int)fminf(load * 1.0001f * a.Hh / a.target + 1.0f, 1.0e9f));
-  auto cut = [&](int b, int& nt, int& ns) {
+  auto size = [&](int b) {
     at_request(a, b, s0, n, len);
     nt = (n + a.TQ - 1) / a.TQ;
-    ns = max(1, (at_most(len, a.window, a.sinks, a.TQ, C::UNIT) + chunk - 1) / chunk);
+    I = at_most(len, a.window, a.sinks, a.TQ, C::UNIT);
   };
-  int units = 0, parts = 0, nt, ns;
   for (int b = b0; b < b1; ++b) {
-    cut(b, nt, ns);
-    units += nt * ns;
-    parts += ns > 1 ? nt * ns : 0;
+    size(b);
+    if (b == b0) first_nt = nt, first_I = I;
+    tiles = min(tiles + nt, 1 << 22);
+    load += (float)nt * I;
+    if (nt) longest = max(longest, I);
   }
+  tiles = at_last(dpp_prefix_i32(tiles));
+  load = dpp_sum_f32(load) * a.Hh;
+  longest = (int)dpp_max_u32((uint32_t)longest);
+  if (tiles > 1 << 21) return false;                       // at most N + 1 a request: starts that overlap
+  int chunk = 0, units = 0, parts = 0;
+  auto count = [&](int c) {                                // this lane's blocks and those of split tiles; their units
+    float cut = 0.0f;
+    units = 0, parts = 0;
+    for (int b = b0; b < b1; ++b) {
+      if (b == b0) nt = first_nt, I = first_I;
+      else size(b);
+      ns = max(1, (I + c - 1) / c);
+      units += nt * ns;
+      if (ns > 1) parts += nt * ns, cut += (float)nt * I;
+    }
+    return cut;
+  };
+  // Parts that fit k rounds of `target` blocks: the fair share, rounded up by more than the sum's error (which leaves fewer
+  // than target blocks more than tiles, and parts within twice the target), then larger while the split tiles' parts are more
+  // than their share of the blocks.  One round, unless the card would stay half empty and two of smaller parts are sooner
+  // done, a block's start and its part's join counted as 8 units.
+  float best = 0.0f;
+#pragma unroll 1
+  for (int k = 1; k <= 2; ++k) {
+    const float blocks = (float)(k * a.target);
+    int c = max(a.chunk_min, (int)fminf(load * 1.0001f / blocks + 1.0f, 1.0e9f));
+    bool more = false;
+#pragma unroll 1
+    for (int trial = 0; trial < 3; ++trial) {
+      const float cut = dpp_sum_f32(count(c)) * a.Hh, over = dpp_sum_f32((float)parts) * a.Hh * load / (cut * blocks);
+      if (!(over > 1.0f)) break;                           // also where nothing is split
+      more = true;
+      c = (int)fminf(c * over + 1.0f, 1.0e9f);
+    }
+    if (k == 1) {
+      chunk = c, best = (float)(min(c, longest) + AT_START);
+      if (!more) break;
+    } else if (2.0f * (c + AT_START) < best) {
+      count(c);
+      const int64_t all = at_last(dpp_prefix_i32(min(parts, 1 << 22))), blk = at_last(dpp_prefix_i32(min(units, 1 << 22)));
+      if (all * a.Hh <= a.slots && (blk - tiles) * a.Hh <= 2 * a.target) chunk = c;
+    }
+  }
+  count(chunk);
   int ub = dpp_prefix_i32(units) - units, pb = dpp_prefix_i32(parts) - parts;
   const int u = blockIdx.x / a.Hh, hh = blockIdx.x % a.Hh;
   int f_b = 0, f_tt = 0, f_split = 0, f_slot = 0, f_ns = 0;
@@ -205,13 +241,15 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
   if (here) {
     int b = b0;
     for (;; ++b) {
-      cut(b, nt, ns);
+      size(b);
+      ns = max(1, (I + chunk - 1) / chunk);
       if (u < ub + nt * ns) break;
       ub += nt * ns;
       pb += ns > 1 ? nt * ns : 0;
     }
-    const int at = (u - ub) / ns;
-    f_b = b, f_tt = nt - 1 - at, f_split = u - ub - at * ns, f_slot = (pb + u - ub) * a.Hh + hh, f_ns = ns;
+    f_split = (u - ub) / nt;
+    const int at = u - ub - f_split * nt;
+    f_b = b, f_tt = nt - 1 - at, f_slot = (pb + at * ns + f_split) * a.Hh + hh, f_ns = ns;
   }
   const uint64_t who = __ballot(here);
   if (!who) return false;
@@ -1013,7 +1051,7 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   }
   // row tiles: at most sum ceil(n_b / TQ) over at most min(B, N) requests with rows; wide blocks: tiles plus splits
   const int64_t tiles = ((int64_t)a.N + (int64_t)std::min(a.B, a.N) * (a.TQ - 1)) / a.TQ;
-  const int64_t grid = C::WIDE ? tiles * a.Hh + (join ? a.target : 0) : (int64_t)std::max(1, a.target / a.Hh) * a.Hh;
+  const int64_t grid = C::WIDE ? tiles * a.Hh + (join ? 2 * a.target : 0) : (int64_t)std::max(1, a.target / a.Hh) * a.Hh;
   MIMO_REQUIRE(grid < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many tiles");
   a.part_mask = C::WIDE ? 0 : 1;
   a.part_step = C::WIDE ? a.Hh : 2 * a.Hh;

@@ -312,6 +312,12 @@ def test_attend_long_contexts(rng, lens, new, heads, dtype):
     _check(*_attend_case(rng, lens, new, *heads, 128, 128, 64, dtype=dtype, gain=2.0))
 
 
+@pytest.mark.parametrize("new", [[150], [200], [304], [420], [130, 60], [7, 150, 1]])
+def test_attend_tiles_that_fill_the_card_in_part(rng, new):
+    # a tile a token: these counts are split into one or two rounds of blocks, some requests' shorter tiles into fewer parts
+    _check(*_attend_case(rng, [2600 + 13 * i for i in range(len(new))], new, 128, 1, 64, 64, 64))
+
+
 def test_attend_large_scores(rng):
     """Scores far apart (one key takes all the weight) and far from 0, and a scale of the caller's."""
     q, cache, plan, kw = _attend_case(rng, [100, 400], [3, 100], 4, 2, 64, 64, 16)
