@@ -25,6 +25,17 @@
 //
 // Work is cut so that the card is full: a device-side count of all requests' tiles gives the number of key tiles per block
 // (chunk); a row tile with more is split over several blocks, whose (O, m, l) a second kernel joins in a fixed order.
+//
+// What bounds it.  Wide: the matrix pipes next to the softmax, under a clock that the power limits.  4096 tokens at 8192, 64/4
+// heads of 192/128 (1.72 TFLOP): 1540-1740 us on different cards, 1.0-1.1 PFLOP/s at 1.70-1.77 GHz, where a large bf16 product
+// reaches 1.39; matrix pipes busy 55-59%, VALU 54-62%, no bank conflicts; 1.24 PFLOP/s without the softmax, and as much
+// without the copies.  Two blocks of 4 waves on a CU fill each other's pauses: one block 0.86; 64 rows a wave, one wave a SIMD
+// 0.97 (sums moved between the register files); the next tile's products woven into the softmax by hand 0.58 (spills; heads
+// of 64, which have the room, 0.59 against 0.70); row sums by a matrix product, operands read further ahead, wave priorities:
+// no change.  Heads of 64: the exponentials (16 cycles for 64 of them) and what is around them, 0.66-0.70 PFLOP/s.
+// Narrow: HBM.  48 requests of 500 to 16384 keys (1.03 GB) 187 us, 5.5 TB/s; 32 of 1000 to 32768 in E4M3 (1.13 GB) 208 us, 5.4
+// TB/s, above a large copy's 4.9 (read and written); a call of few keys 9 us, a chain of round trips (starts and lengths,
+// the table, K and V, the waves' parts through LDS).
 #include <algorithm>
 #include <atomic>
 
@@ -48,7 +59,7 @@ struct AttendArgs {
   uint16_t* out;
   int32_t* status;
   // rows of a tile: TQ tokens of HT heads (HG groups of HT heads cover G), Hh = Hkv * HG
-  int TQ, HT, HG, Hh, chunk_min, target;
+  int TQ, HT, HG, Hh, target;
   // split tiles: per slot TQ * HT rows of O (fp32 [Dv]) and (m, l); per (token, head group) the first part's slot and
   // parts | token's place in its tile << 16.  Part i > 0 is in slot (first & ~part_mask) + i part_step.  meta is null when no
   // tile can be split.
@@ -59,9 +70,13 @@ struct AttendArgs {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int AT_THREADS = 256;
-constexpr int AT_WIDE_TARGET = 512, AT_WIDE_MIN = 4;      // blocks wanted, least 64-key tiles of a block
-constexpr int AT_START = 8;                               // 64-key tiles that a wide block's start and a part's join cost
-constexpr int AT_NARROW_TARGET = 512, AT_NARROW_MIN = 2;  // blocks (two per CU), least 128-key units of one
+// Blocks wanted: two per CU.  Wide: 512 tokens at 8192, 64/4 heads, 185 us; wanting 640 or 768 makes three parts of tiles that
+// two fit: 215.  Narrow: 1024 makes one request of 32768 keys 27.7 us (25.6), 256 makes 128 windowed decodes 39.6 (27.9).
+constexpr int AT_WIDE_TARGET = 512, AT_NARROW_TARGET = 512;
+// Parts of wide tiles have at least 4 units of 64 keys: 40 tokens of 32/8 heads at 3000 21.7 us; 27.3 with 2, 24.9 with 8.
+// Narrow tiles of up to 2 units of 128 keys (a window of 128) are not split, which saves the join's launch.
+constexpr int AT_WIDE_MIN = 4, AT_NARROW_MIN = 2;
+constexpr int AT_START = 8;                               // units that a wide block's start and a part's join cost
 
 template <int DK_, int DV_, bool F8_, bool WIDE_> struct AtCfg {
   static constexpr int DK = DK_, DV = DV_;
@@ -210,12 +225,14 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
   // Parts that fit k rounds of `target` blocks: the fair share, rounded up by more than the sum's error (which leaves fewer
   // than target blocks more than tiles, and parts within twice the target), then larger while the split tiles' parts are more
   // than their share of the blocks.  One round, unless the card would stay half empty and two of smaller parts are sooner
-  // done, a block's start and its part's join counted as 8 units.
+  // done, a block's start and its part's join counted as AT_START units (32/8 heads at 8192: 640 tokens 150 us with the fair
+  // share, 113 with one round; 1200 tokens 237 with one round, 209 with two.  AT_START 16 gains 5% on 800 tokens and makes a
+  // chunk beside 32 long decodes 214 us instead of 160).
   float best = 0.0f;
 #pragma unroll 1
   for (int k = 1; k <= 2; ++k) {
     const float blocks = (float)(k * a.target);
-    int c = max(a.chunk_min, (int)fminf(load * 1.0001f / blocks + 1.0f, 1.0e9f));
+    int c = max(AT_WIDE_MIN, (int)fminf(load * 1.0001f / blocks + 1.0f, 1.0e9f));
     bool more = false;
 #pragma unroll 1
     for (int trial = 0; trial < 3; ++trial) {
@@ -793,7 +810,9 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_wide_kernel(AttendA
   at_clear(a, a.Hq * C::DV);
 }
 
-// Narrow tiles: all units of a head group, request after request, in equal shares for the n blocks of the group.  A block
+// Narrow tiles: all units of a head group, request after request, in equal shares for the blocks of the group, so that none
+// ends late whatever the lengths (48 requests of 500 to 16384 keys 191 us; a list of parts as for wide tiles 209; wide tiles
+// lose by it, 24 mixed requests 91 us instead of 52, for each cut costs them a start and 128 rows of a join).  A block
 // walks its share tile by tile; a tile on the border of two shares is split.  Slot 2 (j Hh + hh) holds block j's part of a
 // tile that began in an earlier share (or with this one), the slot behind it the part of one that goes on in the next.
 template <class C>
@@ -801,7 +820,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, hh = blockIdx.x % a.Hh, j = blockIdx.x / a.Hh;
   const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
-  // without room for parts (no tile can have more than chunk_min units) a share is whole tiles, each counted as one
+  // without room for parts (no tile can have more than AT_NARROW_MIN units) a share is whole tiles, each counted as one
   int s0, n, len, nt, I;
   auto size = [&](int b) {
     at_request(a, b, s0, n, len);
@@ -830,11 +849,12 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
     total = __shfl(before, 63, 64);
     before -= mine;
   }
-  // blocks that share the work: at least chunk_min units each, and one per CU while that leaves them no more than 8 and the
-  // tiles alone do not fill the card
+  // blocks that share the work: a unit each at least, and one per CU while that leaves them no more than 8 units and the tiles
+  // alone do not fill the card (one request of 32768 keys, 64/4 heads: 25.6 us with 256 blocks, 27.8 with 512; 8 of 4000: 24.1
+  // and 25.5; a limit of 32 units changes neither)
   const bool few = total * a.Hh <= 8 * (a.target / 2) && (int64_t)tiles * a.Hh < a.target / 2;
-  const int most = max(1, (few ? a.target / 2 : a.target) / a.Hh), least = a.meta ? a.chunk_min : 1;
-  const uint32_t shares = total >= (int64_t)most * least ? most : max(1, (int)total / least);
+  const int most = max(1, (few ? a.target / 2 : a.target) / a.Hh);
+  const uint32_t shares = total >= most ? most : max(1, (int)total);
   // share x begins at unit (x coarse / shares) << sh, sh chosen so that 32 bits hold the products: no 64-bit division
   const int sh = max(0, 65 - __builtin_clzll(total | 1) - __builtin_clz(shares));
   const uint32_t coarse = (uint32_t)(total >> sh);
@@ -950,7 +970,8 @@ __device__ __forceinline__ int2 at_meta(const AttendArgs& a, int entry) {
   return ok ? mt : make_int2(0, 0);
 }
 
-// Few rows: a block for each, of W waves (few rows with many parts take 16, so that the parts arrive in one or two round trips).
+// Few rows: a block for each, of W waves (few rows with many parts take 16, so that the parts arrive in one or two round
+// trips).  Bound by the round trips: a launch, the entry, the parts; 4.3 us for 64 rows of 64 parts, 5.3 for 1024 of a few.
 template <int DV, int W>
 __global__ void __launch_bounds__(64 * W) attend_join_kernel(AttendArgs a) {
   __shared__ float sl[W], so[W][DV];
@@ -960,7 +981,8 @@ __global__ void __launch_bounds__(64 * W) attend_join_kernel(AttendArgs a) {
   at_join<DV, W>(a, entry / a.Hh, entry % a.Hh, qh, mt, so, sl);
 }
 // Many rows: DV / 4 lanes for `per` heads of an entry, one after another; a row's parts come PB at a time, under a running
-// maximum.
+// maximum.  Round trips again, so many rows have to be on their way at once: 32768 rows of two parts, DV 128 (34 MB) 9.9 us,
+// 21.3 with a wave a row; 20000 rows of four parts, DV 64 6.0 us (13.3).
 template <int DV>
 __global__ void __launch_bounds__(256, 8) attend_join_many_kernel(AttendArgs a, int per) {
   constexpr int LANES = DV / 4, PB = 4;
@@ -1066,12 +1088,16 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   MIMO_REQUIRE(rows < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many rows");
   {
     ProfScope p(st, "attend_join");
+    // rows of few tokens have many parts: at 64 rows of 64 parts 16 waves a row 4.3 us; at 512 rows (8 decodes of 4000 keys)
+    // 4 waves 24.0 us in all, 16 25.1, a part of a wave 24.5
     if (rows <= 256) {
       attend_join_kernel<C::DV, 16><<<(unsigned)rows, 1024, 0, st>>>(a);
     } else if (rows <= 1024) {
       attend_join_kernel<C::DV, 4><<<(unsigned)rows, 256, 0, st>>>(a);
     } else {
-      const int per = rows <= 65536 ? 1 : std::min(a.HT, 8);   // mostly rows that were not split
+      // very many rows are mostly rows that were not split: 262144 of them 4.8 us in eights, 15 more one by one; fewer may
+      // all be split, and then have to be on their way together (48 decodes 192 us in all, 202 in eights)
+      const int per = rows <= 65536 ? 1 : std::min(a.HT, 8);
       const int64_t items = entries * ((a.HT + per - 1) / per);
       constexpr int IPB = 1024 / C::DV;
       attend_join_many_kernel<C::DV><<<(unsigned)((items + IPB - 1) / IPB), 256, 0, st>>>(a, per);
@@ -1133,13 +1159,14 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   a.k = static_cast<const uint8_t*>(cache->k), a.v = static_cast<const uint8_t*>(cache->v);
   a.k_scale = cache->k_scale, a.v_scale = cache->v_scale, a.sink_logits = sink_logits;
   a.scale = scale, a.out = out, a.status = status;
+  // narrow tiles hold the rows of a request in 32, wide ones are up to a quarter filled: at 5 to 8 rows of 8 heads the wide
+  // ones take 132-136 us for 32 requests of 4000 keys, two and more narrow tiles 136-139, and at 12 143 against 356
   const bool wide = (int64_t)std::min(max_new, N) * (heads / cache->kv_heads) > 32;
   at_tiles(wide ? 128 : 32, N, heads, cache->kv_heads, a);
-  a.chunk_min = wide ? AT_WIDE_MIN : AT_NARROW_MIN;
   a.target = wide ? AT_WIDE_TARGET : AT_NARROW_TARGET;
-  // no tile can walk more units than the table or the window holds; within chunk_min it is never split
+  // no tile can walk more units than the table or the window holds; where none has to be split there is no second launch
   const int most = at_most((int64_t)max_pages * cache->page_size, window, a.sinks, a.TQ, wide ? 64 : 128);
-  const bool join = most > a.chunk_min;
+  const bool join = most > (wide ? AT_WIDE_MIN : AT_NARROW_MIN);
   const AtRoom room = at_room(wide ? 128 : 32, a.target, N, heads, cache->kv_heads, cache->v_dim);
   char* w = static_cast<char*>(ws);
   a.part_o = reinterpret_cast<float*>(w);
