@@ -191,16 +191,22 @@ template <class C>
 __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
   const int lane = threadIdx.x & 63;
   const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
-  int s0, n, len, tiles = 0, nt, ns, I, first_nt = 0, first_I = 0, longest = 0;
+  int s0, n, len, tiles = 0, nt, ns, I, longest = 0;
   float load = 0.0f;                                       // units of all tiles; only their share per block is wanted
-  auto size = [&](int b) {
+  auto read = [&](int b) {
     at_request(a, b, s0, n, len);
     nt = (n + a.TQ - 1) / a.TQ;
     I = at_most(len, a.window, a.sinks, a.TQ, C::UNIT);
   };
+  // the lane's first request, as a rule its only one, is kept
+  int first[5] = {0, 0, 0, 0, 0};
+  auto size = [&](int b) {
+    if (b == b0) s0 = first[0], n = first[1], len = first[2], nt = first[3], I = first[4];
+    else read(b);
+  };
   for (int b = b0; b < b1; ++b) {
-    size(b);
-    if (b == b0) first_nt = nt, first_I = I;
+    read(b);
+    if (b == b0) first[0] = s0, first[1] = n, first[2] = len, first[3] = nt, first[4] = I;
     tiles = min(tiles + nt, 1 << 22);
     load += (float)nt * I;
     if (nt) longest = max(longest, I);
@@ -209,13 +215,12 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
   load = dpp_sum_f32(load) * a.Hh;
   longest = (int)dpp_max_u32((uint32_t)longest);
   if (tiles > 1 << 21) return false;                       // at most N + 1 a request: starts that overlap
-  int chunk = 0, units = 0, parts = 0;
+  int chunk = 1 << 30, units = 0, parts = 0;
   auto count = [&](int c) {                                // this lane's blocks and those of split tiles; their units
     float cut = 0.0f;
     units = 0, parts = 0;
     for (int b = b0; b < b1; ++b) {
-      if (b == b0) nt = first_nt, I = first_I;
-      else size(b);
+      size(b);
       ns = max(1, (I + c - 1) / c);
       units += nt * ns;
       if (ns > 1) parts += nt * ns, cut += (float)nt * I;
@@ -230,7 +235,7 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
   // chunk beside 32 long decodes 214 us instead of 160).
   float best = 0.0f;
 #pragma unroll 1
-  for (int k = 1; k <= 2; ++k) {
+  for (int k = 1; a.meta && k <= 2; ++k) {
     const float blocks = (float)(k * a.target);
     int c = max(AT_WIDE_MIN, (int)fminf(load * 1.0001f / blocks + 1.0f, 1.0e9f));
     bool more = false;
@@ -379,6 +384,16 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   const AtRange rg = at_range(base_pos, base_pos + toks - 1, a.window, a.sinks, C::UNIT);
   const int it0 = item.it0, it1 = min(item.it1, rg.I);
 
+  constexpr int UG = C::UNIT / 16, TG = C::KEYS / 16;      // groups of a unit, of an LDS tile
+  const int wg = C::WIDE ? 0 : 2 * wave;                   // the tile's first group in its unit
+  constexpr int NG = C::WIDE ? 1 : 2;                      // 16-key groups that the wave copies
+  AtKeys kg[NG];
+  auto look = [&](int it) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) kg[g] = at_keys(a, rg, b, rg.key(it * UG + (C::WIDE ? wave : wg) + g));
+  };
+  look(it0);                                               // the table is read while the queries are asked for
+
   // queries as the B operand: row r32, dimensions 16 s + 8 h .. (E4M3: 32 (s / 2) + 16 h + 8 (s % 2) .., since a lane's 16
   // bytes of K are 16 dimensions, two products' worth); c = |scale| k_scale log2 e, a negative scale turns q round
   float c = a.scale * kLog2e * (C::F8 ? a.k_scale[kv] : 1.0f);
@@ -412,14 +427,6 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   const int cell_k = C::F8 ? (lane & 3) ^ ((lane >> 4) & 3) : (lane & 7) ^ (lane >> 4);
   const int cell_v = C::F8 ? cell_k : (lane & 7) ^ (4 * ((lane >> 4) & 1));
   const uint32_t lds0 = lds_addr(lds) + (C::WIDE ? 0 : wave * C::STAGE);
-  constexpr int UG = C::UNIT / 16, TG = C::KEYS / 16;      // groups of a unit, of an LDS tile
-  const int wg = C::WIDE ? 0 : 2 * wave;                   // the tile's first group in its unit
-  constexpr int NG = C::WIDE ? 1 : 2;                      // 16-key groups that the wave copies
-  AtKeys kg[NG];
-  auto look = [&](int it) __attribute__((always_inline)) {
-#pragma unroll
-    for (int g = 0; g < NG; ++g) kg[g] = at_keys(a, rg, b, rg.key(it * UG + (C::WIDE ? wave : wg) + g));
-  };
   size_t crow[C::LR];
   auto rows_of = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -582,7 +589,6 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   };
 
   if constexpr (C::WIDE) {
-    look(it0);
     rows_of();
     issue_k(lds0);
     issue_v(lds0);
@@ -609,7 +615,6 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
     constexpr int NK = C::LR * C::KCB, NV = C::LR * C::VCB;
     const int end = min(it1, (rg.gt - wg + UG - 1) / UG);  // of the units that hold groups of this wave
     if (it0 < end) {
-      look(it0);
       rows_of();
       issue_k(lds0);
       issue_v(lds0);
