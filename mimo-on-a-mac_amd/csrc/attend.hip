@@ -20,8 +20,9 @@
 //
 // Masks.  A tile's loads touch only keys that some row of the tile sees: others (past the last position, between the first
 // tokens and the window) read a visible row again, and their weights are set to 0.  A key that one row sees and another does
-// not still meets the other's weight 0 in the product, and 0 * NaN is NaN: a wave whose sums are not finite looks for such
-// values in its tiles with masks, and if there are any takes its sums again key by key.
+// not (of another wave's, too: all waves of a wide tile share its keys) still meets the other's weight 0 in the product, and
+// 0 * NaN is NaN: a wave whose sums are not finite looks for such values in its tiles with masks, and if there are any takes
+// its sums again key by key.
 //
 // Work is cut so that the card is full: a device-side count of all requests' tiles gives the number of key tiles per block
 // (chunk); a row tile with more is split over several blocks, whose (O, m, l) a second kernel joins in a fixed order.
@@ -650,7 +651,8 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
     for (int d = 0; d < C::DV / 32; ++d)
 #pragma unroll
       for (int i = 0; i < 16; ++i) worst += O[d][i] - O[d][i];   // 0, or NaN
-    const bool apart = wp_min != wp_max;                   // rows that see different keys
+    // The tile's rows see different keys, the wave's own or another wave's: the keys in LDS are those that any of them sees.
+    const bool apart = rg.p_min != rg.p_max;
     if ((apart || !C::F8) && __ballot(busy && worst != 0.0f)) {
       bool odd = false;
 #pragma unroll 1

@@ -367,6 +367,25 @@ def test_attend_keeps_one_rows_nan_from_the_others(rng, lens, new, heads, dtype)
         assert (np.abs(out - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -11) * size)[rest].all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("heads,new,window", [((32, 1), 4, 0), ((64, 2), 7, 0), ((40, 1), 3, 0), ((130, 1), 2, 0), ((32, 1), 4, 20),
+                                              ((16, 1), 3, 20), ((8, 1), 5, 20), ((16, 1), 3, 64), ((48, 3), 11, 33)])
+@pytest.mark.parametrize("length", [50, 301, 3000])
+def test_attend_nan_beside_a_wave_of_one_token(rng, heads, new, window, length, dtype):
+    """Waves whose rows are one token's, in a tile of several tokens: a NaN that another token of the tile sees (the last
+    one's own value; with a window the oldest key of the first one too) stays with the tokens that see it."""
+    last = np.arange(new) == new - 1
+    places = [(length - 1, last)] + ([(length - new - window + 1, np.arange(new) == 0)] if window and length - new >= window else [])
+    for key, sees in places:
+        q, cache, plan, kw = _attend_case(rng, [length], [new], *heads, 64, 64, 16, dtype=dtype, window=window)
+        want, size = _oracle(q, cache, plan, kw)
+        table = plan.table.cpu().numpy()
+        cache.v[table[0, key // 16], :, key % 16] = float("nan")
+        out = f64(attend(q, cache, plan, **kw))
+        assert np.isnan(out[sees]).all()
+        assert (np.abs(out - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -11) * size)[~sees].all()
+
+
 @pytest.mark.parametrize("new,heads", [([60, 2], (4, 2)), ([1, 1], (4, 2)), ([4, 2], (8, 2)), ([1, 1], (130, 1))])
 @pytest.mark.parametrize("key", [3, 295])
 def test_attend_non_finite_values_that_rows_see(rng, new, heads, key):
