@@ -42,6 +42,7 @@
 
 #include "cache.h"
 #include "device.h"
+#include "parts.h"
 
 namespace mimo {
 
@@ -288,7 +289,7 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
     const int I = at_range(p0, p1, a.window, a.sinks, C::UNIT).I;
     it.ns = (I + chunk - 1) / chunk;                       // in parts of equal size
     if (split >= it.ns) return false;
-    it.it0 = split * I / it.ns, it.it1 = (split + 1) * I / it.ns;
+    it.it0 = part_begin(split, I, it.ns), it.it1 = part_begin(split + 1, I, it.ns);
   }
   return true;
 }

@@ -442,6 +442,33 @@ def test_attend_and_append_past_32_bit_offsets(rng):
     assert torch.equal(cache.k[high[1]], small.k[1]) and torch.equal(cache.v[high[2]], small.v[2])
 
 
+@pytest.mark.parametrize("N", [33, 1])
+@pytest.mark.parametrize("length", [300_000_000, (1 << 31) - (1 << 16)])
+def test_attend_longest_requests(rng, length, N):
+    """Contexts past 2^28 keys, whose table names the same 16 pages again and again: 33 rows (wide tiles) and one (narrow).
+    With scale 0 every visible key weighs 1, and V is a whole number from -2 to 2 that changes from one sixteenth of the
+    context to the next, so a part's sums (2^22 keys, below 2^24) are exact.  What is left is the join's 512 products and
+    sums (2 x 512 x 2^-24 of the mean of |v|), its division, and the output's rounding (2^-8 |ref|)."""
+    page, dim = 1024, 64
+    width = (length + page - 1) // page
+    ids = (np.arange(width, dtype=np.int64) * 16 // width).astype(np.int32)
+    values = rng.integers(-2, 3, (16, dim))
+    v = torch.from_numpy(values.astype(np.float32)).to(torch.bfloat16).cuda()[:, None, None, :].expand(16, 1, page, dim).contiguous()
+    cache = KVCache.of(torch.ones_like(v), v)
+    q = torch.ones(N, 1, dim, dtype=torch.bfloat16, device="cuda")
+    plan = StepPlan(starts=i32([0, N]), lens=i32([length]), table=torch.from_numpy(ids).cuda()[None], max_new=N,
+                    status=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    out = f64(attend(q, cache, plan, scale=0.0))[:, 0]
+    plan.check()
+    for i in range(N):
+        keys = length - N + i + 1                        # keys that row i sees
+        count = np.bincount(ids[:keys // page], minlength=16) * page
+        count[ids[min(keys // page, width - 1)]] += keys % page
+        assert count.sum() == keys
+        ref, size = count @ values / keys, count @ np.abs(values) / keys
+        assert (np.abs(out[i] - ref) <= 2.0 ** -8 * np.abs(ref) + 2.0 ** -13 * size).all()
+
+
 def test_a_failed_step_writes_nothing(rng):
     pt, cache = PageTable(2, 4, 3, 16), KVCache(3, 16, 1, 64, 64)
     x = torch.ones(40, 3, 64, dtype=torch.bfloat16, device="cuda")
