@@ -173,32 +173,37 @@ struct AtItem {
   int b, s0, n, len, tt, hh, it0, it1, ns, slot;
 };
 
-// Request b's rows s0 .. s0 + n - 1 and length, clamped: whatever starts and lens hold, nothing is out of range.
-__device__ __forceinline__ void at_request(const AttendArgs& a, int b, int& s0, int& n, int& len) {
-  s0 = min(max(a.starts[b], 0), a.N);
-  n = min(max(a.starts[b + 1], s0), a.N) - s0;
+// Request b's rows s0 .. s0 + n - 1 and length, clamped: whatever starts and lens hold, nothing is out of range.  false: its
+// starts run backwards or are not among the rows.
+__device__ __forceinline__ bool at_request(const AttendArgs& a, int b, int& s0, int& n, int& len) {
+  const int from = a.starts[b], to = a.starts[b + 1];
+  s0 = min(max(from, 0), a.N);
+  n = min(max(to, s0), a.N) - s0;
   len = a.lens[b];
   if (n && (len < n || len > ((long long)a.max_pages << a.page_shift))) len = 0;   // refused: its rows are set to 0
+  return s0 == from && s0 + n == to;
 }
+constexpr int AT_REFUSED = 1 << 22;                         // 64 lanes of this stay below 2^31
 __device__ __forceinline__ int at_last(int v) { return __builtin_amdgcn_readlane(v, 63); }
 // The list of work, which every wave makes for itself without a word to the others: lane l looks at requests l per ..,
-// and the prefix sums of what they ask for are the places in the list.  Sizes are kept below 2^31 by refusing what only
-// starts that overlap can ask for (then nothing is computed).
+// and the prefix sums of what they ask for are the places in the list.  Starts in order ask for at most N <= 2^20 tiles; a
+// request whose starts are not counts as AT_REFUSED of them, which refuses the call.
 // Wide tiles.  Block blockIdx.x's item: (request, part, row tile from the last to the first) x head group, head groups
 // fastest: neighbouring blocks, on different XCDs, work on different heads, and an XCD keeps meeting the same ones.  Parts
 // that a request's shorter tiles do not have stand together at its end (were a tile's parts neighbours, these blocks without
 // work would all fall on the same XCDs: 320 tiles, half of them split, took 333 us instead of 185).  A tile is cut into parts
-// of `chunk` units.  false: past the end of the list, or a part that this tile does not have.
+// of `chunk` units.  0: past the end of the list, or a part that this tile does not have; -1: the call is refused.
 template <class C>
-__device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
+__device__ __forceinline__ int at_find(const AttendArgs& a, AtItem& it) {
   const int lane = threadIdx.x & 63;
   const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
   int s0, n, len, tiles = 0, nt, ns, I, longest = 0;
   float load = 0.0f;                                       // units of all tiles; only their share per block is wanted
   auto read = [&](int b) {
-    at_request(a, b, s0, n, len);
+    const bool sound = at_request(a, b, s0, n, len);
     nt = (n + a.TQ - 1) / a.TQ;
     I = at_most(len, a.window, a.sinks, a.TQ, C::UNIT);
+    return sound;
   };
   // the lane's first request, as a rule its only one, is kept
   int first[5] = {0, 0, 0, 0, 0};
@@ -207,16 +212,16 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
     else read(b);
   };
   for (int b = b0; b < b1; ++b) {
-    read(b);
+    const bool sound = read(b);
     if (b == b0) first[0] = s0, first[1] = n, first[2] = len, first[3] = nt, first[4] = I;
-    tiles = min(tiles + nt, 1 << 22);
+    tiles = sound ? min(tiles + nt, AT_REFUSED) : AT_REFUSED;
     load += (float)nt * I;
     if (nt) longest = max(longest, I);
   }
   tiles = at_last(dpp_prefix_i32(tiles));
   load = dpp_sum_f32(load) * a.Hh;
   longest = (int)dpp_max_u32((uint32_t)longest);
-  if (tiles > 1 << 21) return false;                       // at most N + 1 a request: starts that overlap
+  if (tiles >= AT_REFUSED) return -1;
   int chunk = 1 << 30, units = 0, parts = 0;
   auto count = [&](int c) {                                // this lane's blocks and those of split tiles; their units
     float cut = 0.0f;
@@ -276,7 +281,7 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
     f_b = b, f_tt = nt - 1 - at, f_slot = (pb + at * ns + f_split) * a.Hh + hh, f_ns = ns;
   }
   const uint64_t who = __ballot(here);
-  if (!who) return false;
+  if (!who) return 0;
   const int src = __builtin_ctzll(who);
   auto from = [&](int v) { return __builtin_amdgcn_readlane(v, src); };
   it.b = from(f_b), it.tt = from(f_tt), it.slot = from(f_slot), it.hh = hh;
@@ -288,10 +293,10 @@ __device__ __forceinline__ bool at_find(const AttendArgs& a, AtItem& it) {
     const int p0 = it.len - it.n + it.tt * a.TQ, p1 = min(p0 + a.TQ, it.len) - 1;
     const int I = at_range(p0, p1, a.window, a.sinks, C::UNIT).I;
     it.ns = (I + chunk - 1) / chunk;                       // in parts of equal size
-    if (split >= it.ns) return false;
+    if (split >= it.ns) return 0;
     it.it0 = part_begin(split, I, it.ns), it.it1 = part_begin(split + 1, I, it.ns);
   }
-  return true;
+  return 1;
 }
 
 // 16 keys from a multiple of 16 on, of which a tile may load: their page and what hidden keys read instead
@@ -803,18 +808,28 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
 
 // rows of no request
 __device__ __forceinline__ void at_clear(const AttendArgs& a, int row) {
-  const int first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N), gap = first + a.N - last;
+  const int first = a.starts[0], last = a.starts[a.B], gap = first + a.N - last;
   for (int i = blockIdx.x; i < gap; i += gridDim.x) {
     uint4* o = reinterpret_cast<uint4*>(a.out + (size_t)(i < first ? i : last + i - first) * row);
     for (int d = threadIdx.x; d < row / 8; d += AT_THREADS) o[d] = make_uint4(0, 0, 0, 0);
   }
+}
+// a refused call: all rows, and nothing is left for the join
+__device__ __forceinline__ void at_refuse(const AttendArgs& a, int row) {
+  const int64_t from = (int64_t)blockIdx.x * AT_THREADS + threadIdx.x, step = (int64_t)gridDim.x * AT_THREADS;
+  for (int64_t i = from; i < (int64_t)a.N * row / 8; i += step) reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+  if (a.meta)
+    for (int64_t i = from; i < (int64_t)a.N * a.Hh; i += step) a.meta[i] = make_int2(0, 0);
+  if (from == 0 && a.status) a.status[0] = MIMO_ERR_SHAPE;
 }
 
 template <class C>
 __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_wide_kernel(AttendArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   AtItem item;
-  if (at_find<C>(a, item)) at_tile<C>(a, lds, item);
+  const int found = at_find<C>(a, item);
+  if (found < 0) return at_refuse(a, a.Hq * C::DV);
+  if (found) at_tile<C>(a, lds, item);
   at_clear(a, a.Hq * C::DV);
 }
 
@@ -831,18 +846,20 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
   // without room for parts (no tile can have more than AT_NARROW_MIN units) a share is whole tiles, each counted as one
   int s0, n, len, nt, I;
   auto size = [&](int b) {
-    at_request(a, b, s0, n, len);
+    const bool sound = at_request(a, b, s0, n, len);
     nt = (n + a.TQ - 1) / a.TQ;
     I = a.meta ? max(1, at_most(len, a.window, a.sinks, a.TQ, C::UNIT)) : 1;
+    return sound;
   };
   int64_t mine = 0;
   int tiles = 0;
   for (int b = b0; b < b1; ++b) {
-    size(b);
+    const bool sound = size(b);
     mine += (int64_t)nt * I;
-    tiles = min(tiles + nt, 1 << 22);
+    tiles = sound ? min(tiles + nt, AT_REFUSED) : AT_REFUSED;
   }
   tiles = at_last(dpp_prefix_i32(tiles));
+  if (tiles >= AT_REFUSED) return at_refuse(a, a.Hq * C::DV);
   int64_t before, total;
   if (!__ballot(mine >> 25)) {                             // 64 of them stay below 2^31
     const int p = dpp_prefix_i32((int)mine);
@@ -868,7 +885,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
   const uint32_t coarse = (uint32_t)(total >> sh);
   auto begin = [&](uint32_t x) { return x == shares ? total : (int64_t)(x * coarse / shares) << sh; };
   auto holder = [&](int64_t x) { return (int)min(shares - 1, (((uint32_t)(x >> sh) + 1) * shares - 1) / max(1u, coarse)); };
-  if (j < (int)shares && tiles <= 1 << 21) {               // more (at most N + 1 a request): starts that overlap
+  if (j < (int)shares) {
     const int64_t u0 = begin(j), u1 = begin(j + 1);
     for (int64_t u = u0; u < u1;) {
       int f_b = 0, f_tt = 0, f_off = 0;
@@ -969,7 +986,7 @@ __device__ __forceinline__ void at_join(const AttendArgs& a, int n, int hh, int 
   }
 }
 // The parts of an entry (a token and head group) that was split, or 0.  It is read whether or not the token belongs to a
-// request, and starts that overlap may leave a row without one: what cannot be right is not followed.
+// request (then nobody wrote it): what cannot be right is not followed.
 __device__ __forceinline__ int2 at_meta(const AttendArgs& a, int entry) {
   const int2 mt = a.meta[entry];
   const int n = entry / a.Hh, first = min(max(a.starts[0], 0), a.N), last = min(max(a.starts[a.B], first), a.N);

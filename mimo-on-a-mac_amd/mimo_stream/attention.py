@@ -24,7 +24,7 @@ BF16 = torch.bfloat16
 INT32 = torch.int32
 
 STATUS_MESSAGES = {_lib.ERR_PAGES: "fewer free pages than the step needs",
-                   _lib.ERR_SHAPE: "request lengths outside the page table, the step's rows or max_new",
+                   _lib.ERR_SHAPE: "request lengths or starts outside the page table, the rows or max_new",
                    _lib.ERR_SLOT: "a page or slot outside the cache"}
 
 # A decode step makes one step call and two calls per layer, each of a few microseconds on the GPU: what they do on the host

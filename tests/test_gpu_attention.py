@@ -497,6 +497,49 @@ def test_attend_malformed_starts_stay_in_range(rng):
     assert torch.equal(attend(q, cache, plan), want)
 
 
+@pytest.mark.parametrize("heads", [(4, 2), (64, 2)])
+@pytest.mark.parametrize("long", [90, 5000])
+def test_attend_refuses_malformed_starts(rng, heads, long):
+    """starts that run backwards, before the rows or past them (a plan of more rows than q has): every row is 0, the status
+    says so, and a request in order beside the bad one is not answered in part; also where rows were split a call before."""
+    q, cache, plan, kw = _attend_case(rng, [40, long, 20], [3, 33, 1], *heads, 64, 64, 16)
+    good = plan.starts.clone()
+    for max_new in (1, 33):
+        plan.max_new = max_new
+        want = attend(q, cache, plan)
+        plan.check()
+        for bad in ([5, 3, 40, 2], [0, 37, 0, 37], [-9, 1 << 30, -5, 7], [40, 40, 40, 40], [2 ** 31 - 1] * 4, [-2 ** 31] * 4,
+                    [0, 3, 36, 38], [-1, 3, 36, 37], [0, 3, 2, 37], [3, 2, 36, 37]):
+            plan.starts.copy_(i32(bad))
+            out = torch.full_like(want, float("nan"))
+            attend(q, cache, plan, out=out)
+            with pytest.raises(ValueError, match="starts"):
+                plan.check()
+            assert (out == 0).all(), bad
+            plan.status.zero_()
+        plan.starts.copy_(good)
+        assert torch.equal(attend(q, cache, plan), want)
+        plan.check()
+    out = torch.full_like(want[:-1], float("nan"))         # q without the plan's last row
+    attend(q[:-1], cache, plan, out=out)
+    with pytest.raises(ValueError, match="starts"):
+        plan.check()
+    assert (out == 0).all()
+
+
+@pytest.mark.parametrize("max_new", [1, 1 << 20])
+def test_attend_refuses_starts_that_ask_for_millions_of_tiles(max_new):
+    N, B = 1 << 20, 256
+    cache = KVCache(2, 16, 1, 64, 64)
+    plan = StepPlan(starts=i32([0, N] * (B // 2) + [0]), lens=i32([N] * B), table=torch.zeros(B, N // 16, dtype=torch.int32, device="cuda"),
+                    max_new=max_new, status=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    out = torch.full((N, 1, 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+    attend(torch.zeros_like(out), cache, plan, out=out)
+    with pytest.raises(ValueError, match="starts"):
+        plan.check()
+    assert (out == 0).all()
+
+
 def test_attend_scores_of_minus_infinity(rng):
     """Visible keys of score -inf weigh nothing; a row of only such keys, with no sink, is 0."""
     q, cache, plan, kw = _attend_case(rng, [40], [3], 2, 1, 64, 64, 16)
