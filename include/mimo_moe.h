@@ -281,7 +281,7 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
  * request has more new tokens (it picks the kernel: a wrong one costs time, and results differ by their roundings only).
  * status (optional, not cleared) receives MIMO_ERR_SLOT for a page id outside the cache (page 0 is read) and MIMO_ERR_SHAPE
  * for a request whose lens is below its rows or past max_pages (its rows are 0), or for starts that run backwards or are not
- * in 0 .. N (all rows are 0). */
+ * in 0 .. N (all rows are 0).  Threads may call it at once on one stream with one workspace. */
 int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, const mimo_kv_cache* cache, int B,
                       const int32_t* starts, const int32_t* lens, const int32_t* table, int max_pages, int max_new,
                       float scale, int window, int sink_tokens, const float* sink_logits, uint16_t* out,

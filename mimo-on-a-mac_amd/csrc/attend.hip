@@ -39,6 +39,7 @@
 // the table, K and V, the waves' parts through LDS).
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 #include "cache.h"
 #include "device.h"
@@ -1082,6 +1083,10 @@ static AtRoom at_room(int rows, int target, int N, int heads, int kv_heads, int 
   return {align256(pr * v_dim * 4), align256(pr * 8), align256((size_t)N * a.Hh * sizeof(int2))};
 }
 
+// Held while a call's kernel and its join are queued: threads that share a stream share its workspace, and a kernel of one
+// between the two of another would write over the parts that are to be joined.
+static std::mutex at_queue;
+
 template <class C>
 static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   const auto kernel = [] {
@@ -1103,6 +1108,8 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   a.part_mask = C::WIDE ? 0 : 1;
   a.part_step = C::WIDE ? a.Hh : 2 * a.Hh;
   a.slots = 2 * std::max(a.target, a.Hh);
+  std::unique_lock<std::mutex> queue(at_queue, std::defer_lock);
+  if (join) queue.lock();
   {
     ProfScope p(st, C::WIDE ? "attend_wide" : "attend_narrow");
     kernel<<<(unsigned)grid, AT_THREADS, C::LDS, st>>>(a);

@@ -6,6 +6,8 @@ of the stored type (bf16 2^-8 |ref|; E4M3 2^-4 |ref|, or 2^-10 of the scale belo
 rounded to bf16 for the product with V (2^-8 of the weighted mean of |v|), the output is rounded to bf16 (2^-8 |ref|), and
 scores, exponentials and sums in 32 bits add less than 2^-11 of the weighted mean of |v|: a score of |q||k| scale <= 32 is
 off by at most (192 + 4) 2^-24 32 < 2^-11, as much relative to its weight, and only differences of scores count."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -731,3 +733,24 @@ def test_on_another_stream(rng):
         got = attend(q, cache, plan, **kw)
     s.synchronize()
     assert torch.equal(got, want)
+
+
+def test_threads_on_one_stream(rng):
+    """Calls of two threads on one stream, whose rows are split and joined over the stream's one workspace."""
+    cases = [_attend_case(rng, [5000, 900], [1, 1], 8, 2, 64, 64, 16), _attend_case(rng, [4000], [90], 4, 2, 128, 128, 64),
+             _attend_case(rng, [3000, 7, 2000], [1, 1, 1], 8, 2, 64, 64, 32)]
+    want = [attend(q, cache, plan, **kw) for q, cache, plan, kw in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(first):
+        for i in range(20):
+            order = [(first + i + k) % len(cases) for k in range(12)]
+            got = [attend(q, cache, plan, **kw) for q, cache, plan, kw in (cases[k] for k in order)]
+            bad.extend((first, i, k) for g, k in zip(got, order) if not torch.equal(g, want[k]))
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad[:5]
