@@ -56,6 +56,11 @@ def _int32(t, dev, shape, name):
     return t.data_ptr()
 
 
+def _same_pages(plan, cache):
+    if plan.page_size is not None and plan.page_size != cache.page_size:
+        raise ValueError(f"a plan of pages of {plan.page_size} tokens for a cache whose pages hold {cache.page_size}")
+
+
 def _status(plan, dev):
     return None if plan.status is None else _int32(plan.status, dev, (1,), "plan.status")
 
@@ -66,7 +71,7 @@ class StepPlan:
 
     starts [B + 1]: request b's new tokens are rows starts[b] .. starts[b + 1] - 1; lens [B]: lengths with them; slots,
     positions [N] of the rows (-1 and 0 behind the last); table [B, max_pages]; n_free [1]; status [1]: the step's device
-    status, to which append and attend add theirs."""
+    status, to which append and attend add theirs; page_size: of the slots and the table (None: not compared with the cache's)."""
     starts: Optional[torch.Tensor] = None
     lens: Optional[torch.Tensor] = None
     slots: Optional[torch.Tensor] = None
@@ -75,6 +80,7 @@ class StepPlan:
     max_new: Optional[int] = None
     n_free: Optional[torch.Tensor] = None
     status: Optional[torch.Tensor] = None
+    page_size: Optional[int] = None
 
     def check(self, what="step"):
         """Raise ValueError if the step, or an append or attend of its plan, found a failure (synchronises)."""
@@ -137,7 +143,7 @@ class PageTable:
             count if commit else None, at + 4 * B + 4, _raw_stream(index))
         if rc:
             _lib.check(rc, "mimo_cache_step")
-        return StepPlan(starts, lens, slots, positions, self._table, max_new, n_free, status)
+        return StepPlan(starts, lens, slots, positions, self._table, max_new, n_free, status, self.page_size)
 
 
 class KVCache:
@@ -232,6 +238,7 @@ def append(cache, plan, k, v, q=None, rotary=None):
     """Write the new tokens' k [N, kv_heads, k_dim] and v [N, kv_heads, v_dim] to plan.slots (rows with slot -1 are left
     out), k rotated to plan.positions; returns q [N, heads, k_dim] rotated likewise (None without q).  q, k and v may be
     views of one projection's rows."""
+    _same_pages(plan, cache)
     dev = cache.device
     index = _gpu(dev)
     if _current_device() != index:
@@ -289,6 +296,7 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
     A token at position p sees its request's keys j <= p; with window > 0 those with p - j < window, and the first
     sink_tokens.  scale defaults to k_dim ** -0.5.  sink_logits fp32 [heads]: a logit that joins each row's softmax without
     a value.  Returns bf16 [N, heads, v_dim] (out, if given: contiguous bf16); rows of no request are 0."""
+    _same_pages(plan, cache)
     dev = cache.device
     index = _gpu(dev)
     if _current_device() != index:

@@ -65,6 +65,20 @@ def test_cpu_tensors_are_refused():
         attend(torch.zeros(1, 2, 64, dtype=BF), c, plan)
 
 
+def test_a_plan_of_other_pages_is_refused():
+    c = _cache()
+    plan = StepPlan(starts=torch.zeros(2, dtype=torch.int32), lens=torch.zeros(1, dtype=torch.int32),
+                    table=torch.zeros(1, 1, dtype=torch.int32), slots=torch.zeros(1, dtype=torch.int32),
+                    positions=torch.zeros(1, dtype=torch.int32), page_size=32)
+    x = torch.zeros(1, 2, 64, dtype=BF)
+    for call in (lambda: append(c, plan, x, x), lambda: attend(x, c, plan)):
+        with pytest.raises(ValueError, match="pages of 32 tokens"):
+            call()
+    plan.page_size = 16                                  # the cache's: the next refusal is the CPU tensor's
+    with pytest.raises(ValueError, match="device tensors"):
+        attend(x, c, plan)
+
+
 # ---- the C entries check on the host before any HIP call
 HOST = ctypes.create_string_buffer(4096)
 ADDR = (ctypes.addressof(HOST) + 255) // 256 * 256

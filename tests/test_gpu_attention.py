@@ -661,6 +661,16 @@ def test_step_append_attend_like_one_sequence(rng, window, sinks):
         assert (np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + (2.0 ** -7 + 2.0 ** -8 + 2.0 ** -11) * size).all()
 
 
+def test_a_step_of_other_pages_is_refused():
+    pt, cache = PageTable(1, 4, 8, 64), KVCache(8, 16, 1, 64, 64)
+    plan = pt.step(i32([20]), 20)
+    x = torch.ones(20, 1, 64, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: append(cache, plan, x, x), lambda: attend(x, cache, plan)):
+        with pytest.raises(ValueError, match="pages of 64 tokens"):
+            call()
+    assert (cache.k == 0).all() and plan.page_size == 64
+
+
 def test_rollback_gives_the_same_step_again(rng):
     """Tokens taken back (a rejected speculation) leave no trace: the same step again gives the same bits."""
     pt, cache, rotary = PageTable(2, 8, 9, 16), KVCache(9, 16, 1, 128, 128), Rotary(128)
