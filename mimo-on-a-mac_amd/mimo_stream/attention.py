@@ -33,6 +33,9 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
 
+INT32_MAX = 0x7FFFFFFF                                   # ctypes takes the low bits of larger numbers without a word
+
+
 def _device(device):
     device = torch.device(device)
     return torch.device("cuda", torch.cuda.current_device()) if device.type == "cuda" and device.index is None else device
@@ -101,6 +104,8 @@ class PageTable:
             raise ValueError("need at least one request, one page per request and one page")
         if page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
             raise ValueError("page_size must be a power of two from 16 to 1024")
+        if n_pages * page_size > INT32_MAX:
+            raise ValueError(f"{n_pages} pages of {page_size} (at most 2^31 - 1 slots)")
         self.page_size = int(page_size)
         self.n_pages = int(n_pages)
         self._lens = torch.zeros(max_seqs, dtype=INT32, device=dev)
@@ -120,6 +125,8 @@ class PageTable:
         this many new tokens on one request (default n_tokens).  With commit=False the page table keeps its lengths and
         free pages, and the step can be dropped or made again.  Returns a StepPlan; a failure (too few free pages, lengths
         out of range) leaves the state as it was and is in plan.status (plan.check() raises)."""
+        if not 0 <= n_tokens <= 1 << 20 or (max_new is not None and not 0 <= max_new <= INT32_MAX):
+            raise ValueError(f"n_tokens must be from 0 to 2^20 and max_new from 0 to 2^31 - 1 (got {n_tokens}, {max_new})")
         dev = self._lens.device
         index = _gpu(dev)
         if _current_device() != index:
@@ -128,8 +135,6 @@ class PageTable:
         B, width = self._table.shape
         at_target = _int32(target, dev, (B,), "target")
         n_tokens = int(n_tokens)
-        if n_tokens < 0:
-            raise ValueError("n_tokens must be >= 0")
         max_new = n_tokens if max_new is None else int(max_new)
         out = torch.empty(2 * B + 3 + 2 * n_tokens, dtype=INT32, device=dev)
         lens, n_free, status, starts, slots, positions = out.split_with_sizes((B, 1, 1, B + 1, n_tokens, n_tokens))
@@ -296,6 +301,8 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
     A token at position p sees its request's keys j <= p; with window > 0 those with p - j < window, and the first
     sink_tokens.  scale defaults to k_dim ** -0.5.  sink_logits fp32 [heads]: a logit that joins each row's softmax without
     a value.  Returns bf16 [N, heads, v_dim] (out, if given: contiguous bf16); rows of no request are 0."""
+    if not (0 <= window <= INT32_MAX and 0 <= sink_tokens <= INT32_MAX):
+        raise ValueError(f"window and sink_tokens must be from 0 to 2^31 - 1 (got {window}, {sink_tokens})")
     _same_pages(plan, cache)
     dev = cache.device
     index = _gpu(dev)
@@ -312,8 +319,6 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
     at_table = _int32(plan.table, dev, (B, width), "plan.table")
     at_starts = _int32(plan.starts, dev, (B + 1,), "plan.starts")
     at_lens = _int32(plan.lens, dev, (B,), "plan.lens")
-    if window < 0 or sink_tokens < 0:
-        raise ValueError("window and sink_tokens must be >= 0")
     at_logits = None
     if sink_logits is not None:
         if sink_logits.shape != (heads,) or sink_logits.device != dev:
@@ -332,7 +337,7 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
     ws = _workspace(_workspace_size(N, heads, cache.kv_heads, cache.v_dim), dev, stream)
     rc = _entry("mimo_cache_attend")(
         at_q, q_stride, N, heads, cache._struct, B, at_starts, at_lens, at_table, width,
-        N if plan.max_new is None else min(N, int(plan.max_new)), cache.k_dim ** -0.5 if scale is None else float(scale),
+        N if plan.max_new is None else max(-1, min(N, int(plan.max_new))), cache.k_dim ** -0.5 if scale is None else float(scale),
         int(window), int(sink_tokens), at_logits, out.data_ptr(), status, ws.data_ptr(), ws.numel(), stream)
     if rc:
         _lib.check(rc, "mimo_cache_attend")

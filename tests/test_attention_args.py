@@ -79,6 +79,28 @@ def test_a_plan_of_other_pages_is_refused():
         attend(x, c, plan)
 
 
+def test_numbers_past_32_bits_are_refused():
+    """2^32 + 5 would reach the library as 5."""
+    c = _cache()
+    plan = StepPlan()
+    x = torch.zeros(1, 2, 64, dtype=BF)
+    for bad in (-1, 1 << 31, (1 << 32) + 5, -(1 << 32)):
+        with pytest.raises(ValueError, match="window"):
+            attend(x, c, plan, window=bad)
+        with pytest.raises(ValueError, match="sink_tokens"):
+            attend(x, c, plan, window=3, sink_tokens=bad)
+    pt = PageTable(1, 4, 8, 16, device="cpu")
+    target = torch.zeros(1, dtype=torch.int32)
+    for bad in (-1, (1 << 20) + 1, (1 << 32) + 5):
+        with pytest.raises(ValueError, match="n_tokens"):
+            pt.step(target, bad)
+    for bad in (-1, 1 << 31, 1 << 32, -(1 << 32)):
+        with pytest.raises(ValueError, match="max_new"):
+            pt.step(target, 4, max_new=bad)
+    with pytest.raises(ValueError, match="slots"):
+        PageTable(1, 4, (1 << 32) + 8, 16, device="cpu")
+
+
 # ---- the C entries check on the host before any HIP call
 HOST = ctypes.create_string_buffer(4096)
 ADDR = (ctypes.addressof(HOST) + 255) // 256 * 256
