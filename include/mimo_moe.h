@@ -260,7 +260,7 @@ int mimo_cache_step(const int32_t* lens, const int32_t* target, int B, int32_t* 
                     int32_t* commit_lens, int32_t* commit_n_free, int32_t* status, void* stream);
 
 /* Rotary positions on q and k (the first rotary_dim dimensions of a head, pairs (i, i + rotary_dim / 2); the reference's
- * partial RoPE, engine/mimo_stream/mimo_v2.py:66-150) and the write of k and v to their slots.  q bf16 [N, heads, k_dim]
+ * partial RoPE, engine/mimo_stream/mimo_v2.py:66-150) and the write of k and v to their slots.  N is below 2^24.  q bf16 [N, heads, k_dim]
  * (NULL: none), k [N, kv_heads, k_dim], v [N, kv_heads, v_dim], tokens *_stride elements apart (multiples of 8); turns fp64
  * [rotary_dim / 2]: turns per position of each pair (frequency / 2 pi).  q_out bf16 [N, heads, k_dim] may not overlap q, k
  * or v.  A slot below 0 writes no k and v; slots are distinct otherwise.  Rotated values are rounded once, to bf16 or (divided by their
@@ -281,7 +281,9 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
  * request has more new tokens (it picks the kernel: a wrong one costs time, and results differ by their roundings only).
  * status (optional, not cleared) receives MIMO_ERR_SLOT for a page id outside the cache (page 0 is read) and MIMO_ERR_SHAPE
  * for a request whose lens is below its rows or past max_pages (its rows are 0), or for starts that run backwards or are not
- * in 0 .. N (all rows are 0).  Threads may call it at once on one stream with one workspace. */
+ * in 0 .. N (all rows are 0).  Threads may call it at once on one stream with one workspace.
+ * MIMO_ERR_SHAPE, before anything is queued, for a call of more row tiles times head groups, or rows to join, than one launch
+ * has blocks (2^24 - 1 of them; at 2^20 tokens that takes more than a hundred K/V heads, or hundreds of thousands of requests). */
 int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, const mimo_kv_cache* cache, int B,
                       const int32_t* starts, const int32_t* lens, const int32_t* table, int max_pages, int max_new,
                       float scale, int window, int sink_tokens, const float* sink_logits, uint16_t* out,

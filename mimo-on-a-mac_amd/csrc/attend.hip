@@ -1093,6 +1093,17 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
     if constexpr (C::WIDE) return &attend_wide_kernel<C>;
     else return &attend_narrow_kernel<C>;
   }();
+  // row tiles: at most sum ceil(n_b / TQ) over at most min(B, N) requests with rows; wide blocks: tiles plus splits
+  const int64_t tiles = ((int64_t)a.N + (int64_t)std::min(a.B, a.N) * (a.TQ - 1)) / a.TQ;
+  const int64_t grid = C::WIDE ? tiles * a.Hh + (join ? 2 * a.target : 0) : (int64_t)std::max(1, a.target / a.Hh) * a.Hh;
+  MIMO_REQUIRE(grid <= kMaxBlocks, MIMO_ERR_SHAPE, "cache_attend: %lld row tiles of head groups", (long long)grid);
+  // the join: a block for each of few rows; many (mostly rows that were not split: 262144 of them 4.8 us in eights, 15 more one
+  // by one; fewer may all be split, and then have to be on their way together: 48 decodes 192 us in all, 202 in eights)
+  const int64_t entries = (int64_t)a.N * a.Hh, rows = entries * a.HT;
+  const int per = rows <= 65536 ? 1 : std::min(a.HT, 8);
+  constexpr int IPB = 1024 / C::DV;
+  const int64_t joins = (entries * ((a.HT + per - 1) / per) + IPB - 1) / IPB;
+  MIMO_REQUIRE(!join || joins <= kMaxBlocks, MIMO_ERR_SHAPE, "cache_attend: %lld rows to join", (long long)rows);
   static std::atomic<uint64_t> allowed{0};                 // devices on which the kernel may use its LDS
   int dev = 0;
   MIMO_HIP(hipGetDevice(&dev));
@@ -1101,10 +1112,6 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
     MIMO_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDS));
     allowed.fetch_or(bit, std::memory_order_release);
   }
-  // row tiles: at most sum ceil(n_b / TQ) over at most min(B, N) requests with rows; wide blocks: tiles plus splits
-  const int64_t tiles = ((int64_t)a.N + (int64_t)std::min(a.B, a.N) * (a.TQ - 1)) / a.TQ;
-  const int64_t grid = C::WIDE ? tiles * a.Hh + (join ? 2 * a.target : 0) : (int64_t)std::max(1, a.target / a.Hh) * a.Hh;
-  MIMO_REQUIRE(grid < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many tiles");
   a.part_mask = C::WIDE ? 0 : 1;
   a.part_step = C::WIDE ? a.Hh : 2 * a.Hh;
   a.slots = 2 * std::max(a.target, a.Hh);
@@ -1116,8 +1123,6 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   }
   if (int e = check_launch("attend")) return e;
   if (!join) return MIMO_OK;
-  const int64_t entries = (int64_t)a.N * a.Hh, rows = entries * a.HT;
-  MIMO_REQUIRE(rows < (1ll << 31), MIMO_ERR_SHAPE, "cache_attend: too many rows");
   {
     ProfScope p(st, "attend_join");
     // rows of few tokens have many parts: at 64 rows of 64 parts 16 waves a row 4.3 us; at 512 rows (8 decodes of 4000 keys)
@@ -1127,12 +1132,7 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
     } else if (rows <= 1024) {
       attend_join_kernel<C::DV, 4><<<(unsigned)rows, 256, 0, st>>>(a);
     } else {
-      // very many rows are mostly rows that were not split: 262144 of them 4.8 us in eights, 15 more one by one; fewer may
-      // all be split, and then have to be on their way together (48 decodes 192 us in all, 202 in eights)
-      const int per = rows <= 65536 ? 1 : std::min(a.HT, 8);
-      const int64_t items = entries * ((a.HT + per - 1) / per);
-      constexpr int IPB = 1024 / C::DV;
-      attend_join_many_kernel<C::DV><<<(unsigned)((items + IPB - 1) / IPB), 256, 0, st>>>(a, per);
+      attend_join_many_kernel<C::DV><<<(unsigned)joins, 256, 0, st>>>(a, per);
     }
   }
   return check_launch("attend_join");

@@ -353,7 +353,7 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
                       int64_t v_stride, int N, const int32_t* positions, const int32_t* slots, const mimo_kv_cache* cache,
                       int rotary_dim, const double* turns, uint16_t* q_out, int32_t* status, void* stream) {
   if (int e = check_cache(cache, "cache_append")) return e;
-  MIMO_REQUIRE(N >= 0, MIMO_ERR_SHAPE, "cache_append: N must be >= 0");
+  MIMO_REQUIRE(N >= 0 && N <= kMaxBlocks, MIMO_ERR_SHAPE, "cache_append: %d tokens (0 to 2^24 - 1)", N);
   if (N == 0) return MIMO_OK;
   MIMO_REQUIRE(k && v && positions && slots, MIMO_ERR_ARG, "cache_append: null pointer");
   MIMO_REQUIRE(!q == !q_out, MIMO_ERR_ARG, "cache_append: q and q_out go together");

@@ -165,6 +165,22 @@ def test_attend_refusals(bad, code):
     assert _attend(**bad) == getattr(_lib, "ERR_" + code)
 
 
+FAR = 1 << 44                                            # far from every input
+
+
+@pytest.mark.parametrize("kv,dims,B,max_pages", [(128, (128, 128), 1, 64), (1024, (64, 64), 1, 64), (64, (64, 64), 1 << 20, 1)])
+def test_attend_refuses_more_blocks_than_a_launch_has(kv, dims, B, max_pages):
+    """Rows to join, or row tiles over requests, past 2^24 blocks of 256 threads: refused before anything is queued."""
+    N, cache = 1 << 20, _kv(kv_heads=kv, k_dim=dims[0], v_dim=dims[1], page_size=1024)
+    heads = min(1024, 16 * kv) if B > 1 else kv
+    rc = _attend(cache, N=N, heads=heads, qs=heads * dims[0], B=B, max_pages=max_pages, max_new=N, out=FAR)
+    assert rc == _lib.ERR_SHAPE and b"row" in _lib.load().mimo_last_error()
+
+
+def test_append_refuses_more_tokens_than_a_launch_has_blocks():
+    assert _append(N=1 << 24, q_out=FAR) == _lib.ERR_SHAPE and b"2^24" in _lib.load().mimo_last_error()
+
+
 @pytest.mark.parametrize("bad,code", BAD_CACHES)
 def test_cache_refusals(bad, code):
     assert _append(_kv(**bad)) == getattr(_lib, "ERR_" + code)
