@@ -352,7 +352,8 @@ class AttentionLayer:
     norm_weight bf16 [hidden] and eps as in MoELayer; qkv_weight bf16 [heads k_dim + kv_heads (k_dim + v_dim), hidden]
     (q rows, then k, then v), o_weight bf16 [hidden, heads v_dim]; cache: the layer's KVCache; rotary, window, sink_tokens,
     sink_logits and scale as in append and attend.  The two projections are library GEMMs, the rest the library's kernels.
-    MoELayer takes its output: h = moe_layer(attention_layer(x, plan)), one plan for all layers of a step."""
+    MoELayer takes its output: h = moe_layer(attention_layer(x, plan)), one plan for all layers of a step.  For inference: the
+    weights are taken without their gradients' graph."""
 
     def __init__(self, norm_weight, eps, qkv_weight, o_weight, heads, cache, rotary=None, window=0, sink_tokens=0,
                  sink_logits=None, scale=None):
@@ -360,8 +361,8 @@ class AttentionLayer:
         self.cache, self.heads, self.rotary, self.scale = cache, int(heads), rotary, scale
         self.window, self.sink_tokens = int(window), int(sink_tokens)
         self.norm_weight, self.qkv_weight, self.o_weight = (
-            torch.as_tensor(w).to(device=dev, dtype=BF16).contiguous() for w in (norm_weight, qkv_weight, o_weight))
-        self.sink_logits = None if sink_logits is None else torch.as_tensor(sink_logits).to(device=dev, dtype=torch.float32).contiguous()
+            torch.as_tensor(w).detach().to(device=dev, dtype=BF16).contiguous() for w in (norm_weight, qkv_weight, o_weight))
+        self.sink_logits = None if sink_logits is None else torch.as_tensor(sink_logits).detach().to(device=dev, dtype=torch.float32).contiguous()
         self.eps = float(eps)
         if not self.eps >= 0.0:
             raise ValueError("eps must be a non-negative number")

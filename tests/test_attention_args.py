@@ -5,7 +5,7 @@ import os
 import pytest
 import torch
 
-from mimo_stream import KVCache, PageTable, Rotary, StepPlan, _lib, append, attend
+from mimo_stream import AttentionLayer, KVCache, PageTable, Rotary, StepPlan, _lib, append, attend
 
 pytestmark = pytest.mark.skipif(not os.path.exists(_lib.LIB_PATH), reason="libmimo_moe.so not built")
 
@@ -99,6 +99,16 @@ def test_numbers_past_32_bits_are_refused():
             pt.step(target, 4, max_new=bad)
     with pytest.raises(ValueError, match="slots"):
         PageTable(1, 4, (1 << 32) + 8, 16, device="cpu")
+
+
+def test_layer_weights_leave_their_graph():
+    """Parameters of a module may be given as they are: the layer shares their memory and builds no graph over them."""
+    c = _cache()
+    norm, qkv, o = (torch.nn.Parameter(torch.ones(shape, dtype=BF)) for shape in ((32,), (2 * 64 * 3, 32), (32, 128)))
+    sinks = torch.nn.Parameter(torch.zeros(2))
+    layer = AttentionLayer(norm, 1e-5, qkv, o, 2, c, sink_logits=sinks)
+    for kept, given in ((layer.norm_weight, norm), (layer.qkv_weight, qkv), (layer.o_weight, o), (layer.sink_logits, sinks)):
+        assert not kept.requires_grad and kept.data_ptr() == given.data_ptr()
 
 
 # ---- the C entries check on the host before any HIP call
