@@ -11,8 +11,8 @@
 //   O^T += V^T P^T   the P registers 8 s .. 8 s + 7, rounded to bf16, are the B operand of keys 16 s .. as they stand: the
 //                    order of keys inside a product is free, so V^T is read in the same order, by transposing LDS reads
 // so neither S nor P leaves its lane, and m, l and the rescaling of O are per lane too.  V is bf16, so P has to be: wide tiles
-// round it once (2^-9 of each weight; a second product for the rest would be 40% more matrix work), narrow ones, which wait
-// for memory, multiply the rounded rest as well, and their weights are as good as 32 bits.  l sums the unrounded values.
+// round it once (by up to 2^-8 of a weight; a second product for the rest would be 40% more matrix work), narrow ones, which
+// wait for memory, multiply the rounded rest as well, which leaves 2^-17 of a weight.  l sums the unrounded values.
 //
 // K and V go from HBM to LDS without passing registers, 16 bytes a lane; in LDS a tile is [64-element column block][key][128
 // bytes, E4M3 64] with the 16-byte cells of a row permuted by its number, which keeps the operand reads free of bank conflicts.

@@ -275,6 +275,18 @@ def _check(q, cache, plan, kw, scale=None):
     return out
 
 
+def _tight(q, cache, plan, kw, scale=None):
+    """As _check, for calls of few rows, whose weights keep 16 bits of their own (rounded rests included, off by 2^-17): no
+    term for weights rounded to bf16, their rest is within what 2^-11 leaves over."""
+    out = attend(q, cache, plan, scale=scale, **kw)
+    plan.check()
+    ref, size = _oracle(q, cache, plan, kw, scale)
+    tol = 2.0 ** -8 * np.abs(ref) + 2.0 ** -11 * size
+    off = np.abs(f64(out) - ref) - tol
+    assert not (off > 0).any(), f"worst {off.max():.3e} at {np.unravel_index(off.argmax(), off.shape)}"
+    return ref, tol
+
+
 RAGGED = ([1, 15, 16, 17, 63, 64, 65, 130, 300], [1] * 9)
 
 
@@ -283,6 +295,47 @@ RAGGED = ([1, 15, 16, 17, 63, 64, 65, 130, 300], [1] * 9)
 @pytest.mark.parametrize("heads", [(1, 1), (4, 4), (6, 2), (20, 1), (10, 2), (33, 1)])
 def test_attend_decode(rng, dims, dtype, heads):
     _check(*_attend_case(rng, *RAGGED, *heads, *DIMS[dims], 16, dtype=dtype))
+
+
+@pytest.mark.parametrize("dims", list(DIMS))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("lens,new,heads", [(*RAGGED, (6, 2)), (*RAGGED, (32, 1)), ([3000, 7, 20000], [1, 1, 1], (8, 2)), ([900, 77], [4, 2], (8, 1))])
+def test_attend_few_rows_keep_their_weights(rng, dims, dtype, lens, new, heads):
+    _tight(*_attend_case(rng, lens, new, *heads, *DIMS[dims], 16, dtype=dtype, logits=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, E4M3])
+@pytest.mark.parametrize("length", [33, 300, 5000])
+@pytest.mark.parametrize("window", [0, 200])
+def test_attend_few_rows_at_the_worst_rounding(rng, dtype, length, window):
+    """Weights of 1 and, for two of three keys, just below 0.5 + 2^-9, which bf16 rounds to 0.5, on values that cancel: weights
+    rounded once (worked out here) miss the tolerance."""
+    q, cache, plan, kw = _attend_case(rng, [length], [1], 4, 2, 64, 64, 16, dtype=dtype, window=window)
+    down = np.arange(length) % 3 != 0
+    want = np.log(0.5 + 2.0 ** -9 * 0.97)                # the score of those keys, in 8 dimensions of what the cache can hold
+    k = np.zeros((length, 64), np.float64)
+    scale = 1.0 if dtype == torch.bfloat16 else 2.0 ** -8
+    rest = want / scale
+    for d in range(8):
+        piece = torch.tensor(rest, dtype=torch.float32).to(dtype).float().item()
+        k[down, d] = piece
+        rest -= piece
+    v = rng.choice([0.5, 0.75, 1.0, 1.5, -0.5, -1.25], (1, 64)) * np.where(down, -1.0, 1.0)[:, None]
+    table = plan.table.cpu().numpy()[0]
+    for j in range(length):
+        cache.k[table[j // 16], :, j % 16] = torch.from_numpy(k[j]).to(dtype).cuda()
+        cache.v[table[j // 16], :, j % 16] = torch.from_numpy(v[j]).to(dtype).cuda()
+    if dtype == E4M3:
+        cache.k_scale.fill_(scale)
+        cache.v_scale.fill_(1.0)
+    q.zero_()
+    q[:, :, :8] = 1.0
+    ref, tol = _tight(q, cache, plan, kw, scale=1.0)
+    seen = np.arange(length) >= (length - window if window else 0)
+    w = np.exp(scale * k.sum(1)) * seen
+    once = torch.from_numpy(w).to(torch.bfloat16).double().numpy()
+    assert np.allclose((w @ v) / w.sum(), ref[0])
+    assert (np.abs((once @ v) / w.sum() - ref[0, 0]) > tol[0, 0]).all()
 
 
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 1024])
