@@ -249,7 +249,8 @@ typedef struct mimo_kv_cache {
  * Outputs: lens_out [B], n_free_out [1], starts [B + 1] (the new tokens of request b are rows starts[b] .. starts[b + 1] - 1
  * of the step), slots [N] and positions [N] of the new tokens, rows behind the last one -1 and 0.  table entries of grown
  * requests and stack entries at and above n_free are written in place; they mean nothing under the old lengths, so a step
- * whose outputs are dropped leaves the state as it was.  commit_lens / commit_n_free (both or neither; lens and n_free
+ * whose outputs are dropped leaves the state as it was (not what the cache holds, if new tokens were written: pages that one
+ * request gives back are the first that others take in the same step).  commit_lens / commit_n_free (both or neither; lens and n_free
  * themselves, as a rule) receive the new lengths and count after everything else.  status [1] is overwritten: MIMO_OK,
  * MIMO_ERR_PAGES when too few pages are free, MIMO_ERR_SHAPE when a length is outside [0, max_pages * page_size] (at most
  * 2^31 - 2^16), a request grows by more than max_new, the new tokens are more than N (at most 2^20) or n_free and the lengths

@@ -741,6 +741,29 @@ def test_rollback_gives_the_same_step_again(rng):
     assert torch.equal(go([22, 32], 14), first)
 
 
+def test_a_growing_step_can_be_dropped_after_its_append(rng):
+    """New tokens written in a step that is not committed and gives no pages back change nothing for the requests as they
+    were; the step made again, with other tokens, is as if the first had not been."""
+    x = torch.from_numpy(rng.standard_normal((60, 3, 128)).astype(np.float32)).to(torch.bfloat16).cuda()
+    y = torch.from_numpy(rng.standard_normal((60, 3, 128)).astype(np.float32)).to(torch.bfloat16).cuda()
+
+    def go(pt, cache, target, rows, x, commit=True):
+        plan = pt.step(i32(target), rows, commit=commit)
+        q = append(cache, plan, x[:rows, 2:], x[:rows, 1:2], q=x[:rows, :1], rotary=Rotary(128))
+        out = attend(q, cache, plan)
+        plan.check()
+        return out
+    outs = []
+    for drop in (False, True):
+        pt, cache = PageTable(3, 8, 9, 16), KVCache(9, 16, 1, 128, 128)
+        go(pt, cache, [14, 26, 0], 40, x)
+        if drop:
+            go(pt, cache, [34, 27, 5], 26, y, commit=False)
+        outs.append([go(pt, cache, [15, 27, 1], 3, x, commit=False), go(pt, cache, [14, 50, 3], 27, x), pt.n_free.clone()])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
 def test_graph_replays_follow_the_state(rng):
     """A captured decode step (step, append, attend) replayed as the lengths grow equals the eager steps; two captured graphs
     and eager work in between do not disturb each other."""
