@@ -250,8 +250,8 @@ typedef struct mimo_kv_cache {
  * of the step), slots [N] and positions [N] of the new tokens, rows behind the last one -1 and 0.  table entries of grown
  * requests and stack entries at and above n_free are written in place; they mean nothing under the old lengths, so a step
  * whose outputs are dropped leaves the state as it was (not what the cache holds, if new tokens were written: pages that one
- * request gives back are the first that others take in the same step).  commit_lens / commit_n_free (both or neither; lens and n_free
- * themselves, as a rule) receive the new lengths and count after everything else.  status [1] is overwritten: MIMO_OK,
+ * request gives back are the first that others take in the same step).  commit_lens / commit_n_free (both or neither; lens
+ * and n_free themselves, as a rule) receive the new lengths and count after everything else.  status [1] is overwritten: MIMO_OK,
  * MIMO_ERR_PAGES when too few pages are free, MIMO_ERR_SHAPE when a length is outside [0, max_pages * page_size] (at most
  * 2^31 - 2^16), a request grows by more than max_new, the new tokens are more than N (at most 2^20) or n_free and the lengths
  * disagree; then starts are 0, slots -1, and lens_out / n_free_out the old state. */
@@ -261,8 +261,8 @@ int mimo_cache_step(const int32_t* lens, const int32_t* target, int B, int32_t* 
                     int32_t* commit_lens, int32_t* commit_n_free, int32_t* status, void* stream);
 
 /* Rotary positions on q and k (the first rotary_dim dimensions of a head, pairs (i, i + rotary_dim / 2); the reference's
- * partial RoPE, engine/mimo_stream/mimo_v2.py:66-150) and the write of k and v to their slots.  N is below 2^24.  q bf16 [N, heads, k_dim]
- * (NULL: none), k [N, kv_heads, k_dim], v [N, kv_heads, v_dim], tokens *_stride elements apart (multiples of 8); turns fp64
+ * partial RoPE, engine/mimo_stream/mimo_v2.py:66-150) and the write of k and v to their slots.  N is below 2^24.  q bf16
+ * [N, heads, k_dim] (NULL: none), k [N, kv_heads, k_dim], v [N, kv_heads, v_dim], tokens *_stride elements apart (multiples of 8); turns fp64
  * [rotary_dim / 2]: turns per position of each pair (frequency / 2 pi).  q_out bf16 [N, heads, k_dim] may not overlap q, k
  * or v.  A slot below 0 writes no k and v; slots are distinct otherwise.  Rotated values are rounded once, to bf16 or (divided by their
  * head's scale, clamped to +-448) to E4M3.  status (optional) receives MIMO_ERR_SLOT for a slot past the cache, which is

@@ -125,8 +125,9 @@ class PageTable:
         n_tokens: rows of the step, at least the sum of new tokens (more: the rows behind are padding); max_new: at most
         this many new tokens on one request (default n_tokens).  With commit=False the page table keeps its lengths and
         free pages, and the step can be dropped or made again; after an append only if it gave no pages back (a request's
-        pages that end in a step are the first that others take in it, and then hold their tokens).  Returns a StepPlan; a failure (too few free pages, lengths
-        out of range) leaves the state as it was and is in plan.status (plan.check() raises)."""
+        pages that end in a step are the first that others take in it, and then hold their tokens).  Returns a StepPlan; a
+        failure (too few free pages, lengths out of range) leaves the state as it was and is in plan.status (plan.check()
+        raises)."""
         if not 0 <= n_tokens <= 1 << 20 or (max_new is not None and not 0 <= max_new <= INT32_MAX):
             raise ValueError(f"n_tokens must be from 0 to 2^20 and max_new from 0 to 2^31 - 1 (got {n_tokens}, {max_new})")
         dev = self._lens.device
@@ -303,8 +304,9 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
     A token at position p sees its request's keys j <= p; with window > 0 those with p - j < window, and the first
     sink_tokens.  scale defaults to k_dim ** -0.5.  q of another type than bf16 is rounded to it first.  In a call whose
     requests have up to 32 rows each (new tokens x heads / kv_heads, by plan.max_new) the softmax weights keep 17 bits in the
-    product with v, else 8: a decoding request beside a chunk differs by that rounding.  sink_logits fp32 [heads]: a logit that joins each row's softmax without
-    a value.  Returns bf16 [N, heads, v_dim] (out, if given: contiguous bf16); rows of no request are 0."""
+    product with v, else 8: a decoding request beside a chunk differs by that rounding.  sink_logits fp32 [heads]: a logit
+    that joins each row's softmax without a value.  Returns bf16 [N, heads, v_dim] (out, if given: contiguous bf16); rows of
+    no request are 0."""
     if not (0 <= window <= INT32_MAX and 0 <= sink_tokens <= INT32_MAX):
         raise ValueError(f"window and sink_tokens must be from 0 to 2^31 - 1 (got {window}, {sink_tokens})")
     _same_pages(plan, cache)
