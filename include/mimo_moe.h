@@ -231,14 +231,16 @@ int mimo_moe_layer_decode_noalloc(const uint16_t* x, int M, const uint16_t* norm
 
 /* One layer's K/V cache: n_pages pages of page_size tokens (a power of two, 16 to 1024), each page with one contiguous
  * [page_size, dim] block per K/V head.  A slot is page * page_size + row, at most 2^31 - 1 of them.  Head dimensions
- * (k_dim / v_dim): 64/64, 128/128, 192/128.  An E4M3 cache holds value / scale, scales fp32 [kv_heads].  (The reference's
+ * (k_dim / v_dim): 64/64, 128/128, 192/128.  An E4M3 cache holds value / scale, scales fp32 [kv_heads].  A cache with block
+ * scales holds E4M3 codes and a byte s for each 16 slots and head (K and V apart): a code stands for code * 2^(s - 127).
+ * append sets the bytes (1 to 246) as it writes, so that nothing has to be known of the values beforehand.  (The reference's
  * KVCache and RotatingKVCache, engine/mimo_stream/model.py:169-170, hold one request each.) */
-enum { MIMO_KV_BF16 = 0, MIMO_KV_E4M3 = 1 };
+enum { MIMO_KV_BF16 = 0, MIMO_KV_E4M3 = 1, MIMO_KV_E4M3_BLOCKS = 2 };
 typedef struct mimo_kv_cache {
   void* k;                 /* [n_pages, kv_heads, page_size, k_dim] bf16 or E4M3 */
   void* v;                 /* [n_pages, kv_heads, page_size, v_dim] */
-  const float* k_scale;    /* fp32 [kv_heads], E4M3 only */
-  const float* v_scale;
+  const void* k_scale;     /* E4M3: fp32 [kv_heads]; E4M3_BLOCKS: bytes [n_pages, kv_heads, page_size / 16], 16-byte aligned, */
+  const void* v_scale;     /*   readable up to the next multiple of 4 bytes, written by append */
   int32_t dtype, n_pages, page_size, kv_heads, k_dim, v_dim;
 } mimo_kv_cache;
 
@@ -271,6 +273,30 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
                       const uint16_t* v, int64_t v_stride, int N, const int32_t* positions, const int32_t* slots,
                       const mimo_kv_cache* cache, int rotary_dim, const double* turns, uint16_t* q_out,
                       int32_t* status, void* stream);
+
+/* mimo_cache_append with the rotation in full (NULL: none): pairs (i, i + dim / 2), or (2 i, 2 i + 1) where interleaved is 1;
+ * turns fp64 [dim / 2] as above (a host may stretch them for long contexts); rotated values times magnitude (finite; 1: as
+ * they are).  Into a cache with block scales (either entry; N up to 2^23 - 17): the rows of one block of 16 slots have to
+ * follow one another, as a step lays a request's tokens.  A call that writes a block's first slot begins the block anew,
+ * whatever it held; else its byte grows if the new values need it, and what the block held is kept, in the new scale.  Values
+ * past 448 * 2^119 saturate.  status also receives MIMO_ERR_SLOT for a slot that follows itself; if a block's rows do not stand
+ * together that block's contents are undefined, and nothing else is touched. */
+typedef struct mimo_rotary {
+  const double* turns;
+  int32_t dim, interleaved;
+  float magnitude;
+} mimo_rotary;
+int mimo_cache_append_rotary(const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k, int64_t k_stride,
+                             const uint16_t* v, int64_t v_stride, int N, const int32_t* positions, const int32_t* slots,
+                             const mimo_kv_cache* cache, const mimo_rotary* rotary, uint16_t* q_out, int32_t* status,
+                             void* stream);
+
+/* Cached tokens back as rows: k_out bf16 [N, kv_heads, k_dim] and v_out [N, kv_heads, v_dim], row n from slots[n] (in any order,
+ * any slot any number of times), code times scale rounded once; a slot below 0 gives a row of 0.  The outputs may not overlap
+ * the cache, the slots or one another.  N is below 2^24.  status (optional, not cleared) receives MIMO_ERR_SLOT for a slot past
+ * the cache, whose row is 0.  (The reference slices its cache arrays, engine/mimo_stream/mimo_v2.py:110-150.) */
+int mimo_cache_read(const mimo_kv_cache* cache, const int32_t* slots, int N, uint16_t* k_out, uint16_t* v_out,
+                    int32_t* status, void* stream);
 
 /* Attention of a step's new tokens over the paged cache that already holds their keys and values (the reference's
  * Attention with its causal and sliding-window masks and sinks, engine/mimo_stream/mimo_v2.py:110-150).  Row n of request b

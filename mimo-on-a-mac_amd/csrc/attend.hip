@@ -58,7 +58,8 @@ struct AttendArgs {
   int N, Hq, Hkv, G, B, max_pages, n_pages, page_shift, window, sinks;
   const int32_t *starts, *lens, *table;
   const uint8_t *k, *v;
-  const float *k_scale, *v_scale, *sink_logits;
+  const void *k_scale, *v_scale;                           // fp32 [Hkv], or bytes for each 16 slots and head
+  const float* sink_logits;
   float scale;
   uint16_t* out;
   int32_t* status;
@@ -82,9 +83,9 @@ constexpr int AT_WIDE_TARGET = 512, AT_NARROW_TARGET = 512;
 constexpr int AT_WIDE_MIN = 4, AT_NARROW_MIN = 2;
 constexpr int AT_START = 8;                               // units that a wide block's start and a part's join cost
 
-template <int DK_, int DV_, bool F8_, bool WIDE_> struct AtCfg {
+template <int DK_, int DV_, int DTYPE, bool WIDE_> struct AtCfg {
   static constexpr int DK = DK_, DV = DV_;
-  static constexpr bool F8 = F8_, WIDE = WIDE_;
+  static constexpr bool F8 = DTYPE != MIMO_KV_BF16, BS = DTYPE == MIMO_KV_E4M3_BLOCKS, HS = F8 && !BS, WIDE = WIDE_;
   static constexpr int CBB = F8 ? 64 : 128;                // bytes of a row in one 64-element column block
   static constexpr int KCB = DK / 64, VCB = DV / 64;
   static constexpr int KEYS = WIDE ? 64 : 32;              // keys of one LDS tile (narrow: one wave's)
@@ -96,7 +97,9 @@ template <int DK_, int DV_, bool F8_, bool WIDE_> struct AtCfg {
   static constexpr int GR = 1024 / CBB;                    // rows of one copy instruction (64 lanes of 16 bytes)
   static constexpr int LR = (WIDE ? 16 : 32) / GR;         // row groups that a wave copies per tile
   static constexpr int MERGE = WIDE ? 0 : 4 * 32 * DV * 4 + 4 * 32 * 8;   // narrow: the waves' O, m, l joined at the end
-  static constexpr int LDS = (WIDE ? 2 * STAGE : 4 * STAGE) > MERGE ? (WIDE ? 2 * STAGE : 4 * STAGE) : MERGE;
+  static constexpr int SCALES = (WIDE ? 2 : 4) * STAGE;    // wide: the two tiles' block scales stand behind them
+  static constexpr int ROOM = SCALES + (BS && WIDE ? 2 * 8 * 4 : 0);
+  static constexpr int LDS = ROOM > MERGE ? ROOM : MERGE;
   static constexpr int WGS = 2;                            // blocks per CU
   static_assert(WGS * LDS <= 163840, "LDS of the blocks of a CU");
 };
@@ -133,10 +136,10 @@ __device__ __forceinline__ float at_swap_sum(float x) {
 }
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// four / two E4M3 codes of a dword to bf16, exact
-__device__ __forceinline__ bf16x8 at_f8_bf16x8(uint32_t a, uint32_t b) {
-  const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true);
-  const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true);
+// eight E4M3 codes times a power of two to bf16, exact
+__device__ __forceinline__ bf16x8 at_f8_bf16x8(uint32_t a, uint32_t b, float by) {
+  const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, true);
+  const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, true);
   return bf16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
 }
 
@@ -320,6 +323,17 @@ __device__ __forceinline__ int at_page(const AttendArgs& a, int id) {
   if (a.status && (threadIdx.x & 63) == 0) a.status[0] = MIMO_ERR_SLOT;
   return 0;
 }
+// the bytes of K and V of a group's block scale, by scalar loads of the dwords around them
+__device__ __forceinline__ uint2 at_scales(const AttendArgs& a, const AtKeys& g, int page, int kv) {
+  typedef const __attribute__((address_space(4))) uint32_t* words;
+  const int part = (g.g0 & ((1 << a.page_shift) - 1)) >> 4;
+  const uint64_t at = (((uint64_t)(uint32_t)page * a.Hkv + kv) << (a.page_shift - 4)) + part;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
+  const uint64_t word = (((uint64_t)hi << 32) | lo) >> 2;
+  const int shift = 8 * (lo & 3);
+  return make_uint2(reinterpret_cast<words>(reinterpret_cast<uintptr_t>(a.k_scale))[word] >> shift & 0xFFu,
+                    reinterpret_cast<words>(reinterpret_cast<uintptr_t>(a.v_scale))[word] >> shift & 0xFFu);
+}
 // cache row (of [page, head, row in page]) of key g0 + r
 __device__ __forceinline__ size_t at_row(const AttendArgs& a, const AtRange& r, const AtKeys& g, int page, int kv, int row) {
   const int j = g.g0 + row;
@@ -340,8 +354,9 @@ __device__ __forceinline__ void at_slow(const AttendArgs& a, const AtRange& r, i
 #pragma unroll
   for (int e = 0; e < C::VCB; ++e) O[e] = 0.0f;
   m = -INFINITY, l = 0.0f;
-  auto load = [&](const uint8_t* base, size_t at) {
-    return C::F8 ? e4m3_unpack2(base[at]).x : bf16_to_f32(reinterpret_cast<const uint16_t*>(base)[at]);
+  float ks = 1.0f, vs = 1.0f;
+  auto load = [&](const uint8_t* base, size_t at, float by) {
+    return C::F8 ? e4m3_unpack2(base[at]).x * by : bf16_to_f32(reinterpret_cast<const uint16_t*>(base)[at]);
   };
 #pragma unroll 1
   for (int g = it0 * (C::UNIT / 16); g < min(r.gt, it1 * (C::UNIT / 16)); ++g) {
@@ -352,16 +367,20 @@ __device__ __forceinline__ void at_slow(const AttendArgs& a, const AtRange& r, i
       if (a.window && j <= p - a.window && j >= a.sinks) continue;
       const int page = at_page(a, a.table[(size_t)b * a.max_pages + (j >> a.page_shift)]);
       const size_t row = (((size_t)page * a.Hkv + kv) << a.page_shift) + (j & ((1 << a.page_shift) - 1));
+      if constexpr (C::BS) {
+        ks = e8m0_f32(static_cast<const uint8_t*>(a.k_scale)[row >> 4]);
+        vs = e8m0_f32(static_cast<const uint8_t*>(a.v_scale)[row >> 4]);
+      }
       float s = 0.0f;
 #pragma unroll
-      for (int e = 0; e < C::KCB; ++e) s += x[e] * load(a.k, row * C::DK + 64 * e + lane);
+      for (int e = 0; e < C::KCB; ++e) s += x[e] * load(a.k, row * C::DK + 64 * e + lane, ks);
       s = dpp_sum_f32(s) * c;
       const float top = fmaxf(m, s), ref = top == -INFINITY ? 0.0f : top;
       const float was = at_exp2(m - ref), w = at_exp2(s - ref);
       m = top;
       l = l * was + w;
 #pragma unroll
-      for (int e = 0; e < C::VCB; ++e) O[e] = O[e] * was + (w == 0.0f ? 0.0f : w * load(a.v, row * C::DV + 64 * e + lane));
+      for (int e = 0; e < C::VCB; ++e) O[e] = O[e] * was + (w == 0.0f ? 0.0f : w * load(a.v, row * C::DV + 64 * e + lane, vs));
     }
   }
 }
@@ -405,7 +424,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
 
   // queries as the B operand: row r32, dimensions 16 s + 8 h .. (E4M3: 32 (s / 2) + 16 h + 8 (s % 2) .., since a lane's 16
   // bytes of K are 16 dimensions, two products' worth); c = |scale| k_scale log2 e, a negative scale turns q round
-  float c = a.scale * kLog2e * (C::F8 ? a.k_scale[kv] : 1.0f);
+  float c = a.scale * kLog2e * (C::HS ? static_cast<const float*>(a.k_scale)[kv] : 1.0f);
   const uint32_t flip = c < 0.0f ? 0x80008000u : 0u;
   const bool zero = c == 0.0f;
   c = zero ? 1.0f : fabsf(c);
@@ -437,13 +456,23 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   const int cell_v = C::F8 ? cell_k : (lane & 7) ^ (4 * ((lane >> 4) & 1));
   const uint32_t lds0 = lds_addr(lds) + (C::WIDE ? 0 : wave * C::STAGE);
   size_t crow[C::LR];
+  uint2 next_scales[C::BS ? NG : 1];                       // the bytes of the tile that is being copied
   auto rows_of = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < C::LR; ++x) {
       const int g = x * C::GR / 16;
       crow[x] = at_row(a, rg, kg[g], at_page(a, kg[g].id), kv, x * C::GR % 16 + cr);
     }
+    if constexpr (C::BS) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) next_scales[g] = at_scales(a, kg[g], at_page(a, kg[g].id), kv);
+    }
   };
+  // Block scales of the tile in hand: of this lane's key in each block of 32, and of each group of 16 keys.  Narrow tiles'
+  // groups are the wave's own; of a wide tile each wave has loaded one group's bytes, and passes them on through LDS.
+  float k_by[C::NB], v_by[2 * C::NB];
+#pragma unroll
+  for (int i = 0; i < C::NB; ++i) k_by[i] = v_by[2 * i] = v_by[2 * i + 1] = 1.0f;
   constexpr int ES = C::F8 ? 1 : 2;
   auto issue_k = [&](uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
@@ -482,7 +511,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
     if constexpr (C::F8) {
       const uint8_t* p = st + C::KBYTES + (v_at ^ (32 * (d & 1))) + (d >> 1) * (C::KEYS * 64) + (32 * kb + 16 * s) * 64;
       const v2i w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)(uint32_t)(uintptr_t)p);
-      return at_f8_bf16x8(w[0], w[1]);
+      return at_f8_bf16x8(w[0], w[1], v_by[2 * kb + s]);
     } else {
       const uint8_t* p = st + C::KBYTES + (v_at ^ (64 * (d & 1))) + (d >> 1) * (C::KEYS * 128) + (32 * kb + 16 * s) * 128;
       const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uint32_t)(uintptr_t)p);
@@ -515,8 +544,8 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       const v16f none = {0.0f};
       const uint4 x = X[f % PX];
       if constexpr (C::F8) {
-        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.x, x.y), Q[2 * s], s == 0 ? none : S[kb], 0, 0, 0);
-        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.z, x.w), Q[2 * s + 1], S[kb], 0, 0, 0);
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.x, x.y, k_by[kb]), Q[2 * s], s == 0 ? none : S[kb], 0, 0, 0);
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.z, x.w, k_by[kb]), Q[2 * s + 1], S[kb], 0, 0, 0);
       } else {
         S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), Q[s], s == 0 ? none : S[kb], 0, 0, 0);
       }
@@ -605,6 +634,8 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
     for (int it = it0; it < it1; ++it) {
       const int cur = (it - it0) & 1, g0 = it * UG;
       if (it + 1 < it1) look(it + 1);
+      uint32_t* sc = reinterpret_cast<uint32_t*>(lds + C::SCALES) + 8 * cur;
+      if (C::BS && lane == 0) sc[wave] = next_scales[0].x << 23, sc[4 + wave] = next_scales[0].y << 23;
       at_wait_vm(0);
       __syncthreads();                                     // the tile has landed everywhere; the other one is free
       if (it + 1 < it1) {
@@ -614,6 +645,12 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       }
       if (!busy || rg.key(g0) > wp_max) continue;
       const uint8_t* st = lds + cur * C::STAGE;
+      if constexpr (C::BS) {
+        const float* by = reinterpret_cast<const float*>(sc);
+        k_by[0] = by[r32 >> 4], k_by[1] = by[2 + (r32 >> 4)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v_by[i] = by[4 + i];
+      }
       scores(st);
       if (!open(g0)) mask(g0);
       softmax();
@@ -632,6 +669,10 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
     for (int it = it0; it < end; ++it) {
       const int g0 = it * UG + wg;
       const bool more = it + 1 < end;
+      if constexpr (C::BS) {
+        k_by[0] = e8m0_f32(r32 < 16 ? next_scales[0].x : next_scales[1].x);
+        v_by[0] = e8m0_f32(next_scales[0].y), v_by[1] = e8m0_f32(next_scales[1].y);
+      }
       if (more) look(it + 1);
       at_wait_vm(NV);
       scores(st);
@@ -681,7 +722,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       suspect = __ballot(odd) != 0;
     }
   }
-  const float vs = C::F8 ? a.v_scale[kv] : 1.0f;
+  const float vs = C::HS ? static_cast<const float*>(a.v_scale)[kv] : 1.0f;
   // the wave's rows once more, one by one; done(row, place of the row, its head, O, m, l)
   auto slow = [&](auto done) __attribute__((always_inline)) {
 #pragma unroll 1
@@ -692,7 +733,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       float O[C::VCB], m, l;
       at_slow<C>(a, rg, b, kv, it0, it1, C::WIDE ? 0 : 2 * wave, C::WIDE ? 4 : 2,
                  a.q + (int64_t)(item.s0 + tok0 + rt) * a.q_stride + hd * C::DK, base_pos + rt,
-                 a.scale * kLog2e * (C::F8 ? a.k_scale[kv] : 1.0f), O, m, l);
+                 a.scale * kLog2e * (C::HS ? static_cast<const float*>(a.k_scale)[kv] : 1.0f), O, m, l);
       done(r, rt, hd, O, m, l);
     }
   };
@@ -1139,13 +1180,17 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   return check_launch("attend_join");
 }
 
-template <bool F8, bool WIDE>
+template <int DTYPE, bool WIDE>
 static int at_dims(const AttendArgs& a, int dk, bool join, hipStream_t st) {
   switch (dk) {
-    case 64: return at_launch<AtCfg<64, 64, F8, WIDE>>(a, join, st);
-    case 128: return at_launch<AtCfg<128, 128, F8, WIDE>>(a, join, st);
-    default: return at_launch<AtCfg<192, 128, F8, WIDE>>(a, join, st);
+    case 64: return at_launch<AtCfg<64, 64, DTYPE, WIDE>>(a, join, st);
+    case 128: return at_launch<AtCfg<128, 128, DTYPE, WIDE>>(a, join, st);
+    default: return at_launch<AtCfg<192, 128, DTYPE, WIDE>>(a, join, st);
   }
+}
+template <int DTYPE>
+static int at_width(const AttendArgs& a, int dk, bool wide, bool join, hipStream_t st) {
+  return wide ? at_dims<DTYPE, true>(a, dk, join, st) : at_dims<DTYPE, false>(a, dk, join, st);
 }
 
 }  // namespace mimo
@@ -1206,9 +1251,11 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   a.part_ml = reinterpret_cast<float*>(w + room.o);
   a.meta = join ? reinterpret_cast<int2*>(w + room.o + room.ml) : nullptr;
   hipStream_t st = as_stream(stream);
-  const bool f8 = cache->dtype == MIMO_KV_E4M3;
-  if (wide) return f8 ? at_dims<true, true>(a, cache->k_dim, join, st) : at_dims<false, true>(a, cache->k_dim, join, st);
-  return f8 ? at_dims<true, false>(a, cache->k_dim, join, st) : at_dims<false, false>(a, cache->k_dim, join, st);
+  switch (cache->dtype) {
+    case MIMO_KV_BF16: return at_width<MIMO_KV_BF16>(a, cache->k_dim, wide, join, st);
+    case MIMO_KV_E4M3: return at_width<MIMO_KV_E4M3>(a, cache->k_dim, wide, join, st);
+    default: return at_width<MIMO_KV_E4M3_BLOCKS>(a, cache->k_dim, wide, join, st);
+  }
 }
 
 }  // extern "C"

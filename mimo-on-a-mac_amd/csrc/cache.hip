@@ -177,10 +177,11 @@ struct AppendArgs {
   int64_t q_stride, k_stride, v_stride;             // elements between two tokens
   int Hq, Hkv, Dk, Dv, N, rot;
   const double* turns;
+  float magnitude;
   const int32_t *positions, *slots;
   uint16_t* q_out;
   void *k_pages, *v_pages;
-  const float *k_scale, *v_scale;
+  const void *k_scale, *v_scale;                    // fp32 [Hkv], or the bytes of a cache with block scales
   int page_shift, n_slots;
   int32_t* status;
 };
@@ -214,18 +215,39 @@ __device__ __forceinline__ uint2 ap_pack_e4m3(const float* f, float scale) {
   return make_uint2(w[0], w[1]);
 }
 
-// A token is gridDim.y blocks of 256 threads, a thread one unit of 8 values (of a pair, two) at a time; the first unit is on
-// its way while the token's angles are worked out.
-template <bool E4M3>
-__global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
+// one rotation of eight pairs (x_i, y_i), of four pairs (x_2i, x_2i+1)
+__device__ __forceinline__ void ap_turn(float* x, float* y, const float* cs, const float* sn) {
 #pragma clang fp contract(off)
-  __shared__ float s_cos[AP_MAX_ROT / 2], s_sin[AP_MAX_ROT / 2];
-  const int n = blockIdx.x, half = a.rot >> 1;
-  const int pos = a.positions[n], slot = a.slots[n];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float p = x[i], q = y[i];
+    x[i] = p * cs[i] - q * sn[i];
+    y[i] = q * cs[i] + p * sn[i];
+  }
+}
+__device__ __forceinline__ void ap_turn_side(float* x, const float* cs, const float* sn) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float p = x[2 * i], q = x[2 * i + 1];
+    x[2 * i] = p * cs[i] - q * sn[i];
+    x[2 * i + 1] = q * cs[i] + p * sn[i];
+  }
+}
+
+// Part `part` of `parts` of token n (its q alone where KIND is AP_Q): 256 threads, a thread one unit of 8 values (of a pair of
+// units, two) at a time; the first unit is on its way while the token's angles are worked out.  SIDE: the rotated pairs lie
+// side by side (2 i, 2 i + 1), so that a unit holds four of them; else unit d is turned with unit d + rot / 2.
+enum { AP_BF16, AP_E4M3, AP_Q };
+template <int KIND, bool SIDE>
+__device__ __forceinline__ void ap_token(const AppendArgs& a, int n, int part, int parts, float* s_cos, float* s_sin) {
+#pragma clang fp contract(off)
+  const int half = a.rot >> 1;
+  const int pos = a.positions[n], slot = KIND == AP_Q ? -1 : a.slots[n];
   const bool keep = slot >= 0 && slot < a.n_slots;
   if (slot >= a.n_slots && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;
   // units of 8 values: per q and k head rot / 16 pairs of units and (Dk - rot) / 8 units that stay, then v
-  const int pairs = a.rot >> 4, U = pairs + ((a.Dk - a.rot) >> 3), Uv = a.Dv >> 3;
+  const int pairs = SIDE ? 0 : a.rot >> 4, U = SIDE ? a.Dk >> 3 : pairs + ((a.Dk - a.rot) >> 3), Uv = a.Dv >> 3;
   const int nq = a.q ? a.Hq * U : 0, nk = a.Hkv * U, all = keep ? nq + nk + a.Hkv * Uv : nq;
   struct Unit {
     int kind, h, d;                                        // 0 q, 1 k, 2 v; head; first dimension
@@ -239,14 +261,14 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
     r.h = w / per;
     const int c = w - r.h * per;
     r.pair = r.kind != 2 && c < pairs;
-    r.d = r.kind == 2 || r.pair ? 8 * c : a.rot + 8 * (c - pairs);
+    r.d = SIDE || r.kind == 2 || r.pair ? 8 * c : a.rot + 8 * (c - pairs);
     const uint16_t* row = r.kind == 0 ? a.q + n * a.q_stride + r.h * a.Dk : (r.kind == 1 ? a.k + n * a.k_stride + r.h * a.Dk : a.v + n * a.v_stride + r.h * a.Dv);
     r.x = *reinterpret_cast<const uint4*>(row + r.d);
     r.y = make_uint4(0, 0, 0, 0);
     if (r.pair) r.y = *reinterpret_cast<const uint4*>(row + r.d + half);
     return r;
   };
-  int u = blockIdx.y * 256 + threadIdx.x;
+  int u = part * 256 + threadIdx.x;
   Unit first{};
   if (u < all) first = load(u);
   for (int i = threadIdx.x; i < half; i += 256) {
@@ -254,17 +276,17 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
     const float f = (float)(t - floor(t));
     float sn, cs;
     sincospif(2.0f * f, &sn, &cs);
-    s_cos[i] = cs, s_sin[i] = sn;
+    s_cos[i] = cs * a.magnitude, s_sin[i] = sn * a.magnitude;
   }
   __syncthreads();
   const int mask = (1 << a.page_shift) - 1;
   const size_t prow = keep ? ((size_t)(slot >> a.page_shift) * a.Hkv << a.page_shift) + (slot & mask) : 0;
-  auto put = [&](void* pages, int h, int D, int d, const float* f, const float* scale) {
+  auto put = [&](void* pages, int h, int D, int d, const float* f, const void* scale) {
     const size_t at = (prow + ((size_t)h << a.page_shift)) * D + d;
-    if constexpr (E4M3) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + at) = ap_pack_e4m3(f, scale[h]);
+    if constexpr (KIND == AP_E4M3) *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + at) = ap_pack_e4m3(f, static_cast<const float*>(scale)[h]);
     else *reinterpret_cast<uint4*>(static_cast<uint16_t*>(pages) + at) = ap_pack(f);
   };
-  for (bool again = false; u < all; u += gridDim.y * 256, again = true) {
+  for (bool again = false; u < all; u += parts * 256, again = true) {
     const Unit r = again ? load(u) : first;
     float x[8], y[8];
     ap_unpack(r.x, x);
@@ -272,14 +294,10 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
       put(a.v_pages, r.h, a.Dv, r.d, x, a.v_scale);
       continue;
     }
+    if (SIDE && r.d < a.rot) ap_turn_side(x, s_cos + r.d / 2, s_sin + r.d / 2);
     if (r.pair) {
       ap_unpack(r.y, y);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float cs = s_cos[r.d + i], sn = s_sin[r.d + i], p = x[i], q = y[i];
-        x[i] = p * cs - q * sn;
-        y[i] = q * cs + p * sn;
-      }
+      ap_turn(x, y, s_cos + r.d, s_sin + r.d);
     }
     if (r.kind == 0) {
       uint16_t* o = a.q_out + ((size_t)n * a.Hq + r.h) * a.Dk + r.d;
@@ -292,9 +310,221 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
   }
 }
 
+template <int KIND, bool SIDE>
+__global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
+  __shared__ float s_cos[AP_MAX_ROT / 2], s_sin[AP_MAX_ROT / 2];
+  ap_token<KIND, SIDE>(a, blockIdx.x, blockIdx.y, gridDim.y, s_cos, s_sin);
+}
+
+// ------------------------------------------------------------------ append with block scales
+// A cache with block scales holds code * 2^(s - 127), with one byte s for K and one for V of each 16 slots (a block) and head.
+// With the largest magnitude M that a call writes to a block, need = the smallest s with M <= 448 * 2^(s - 127), from 1 to
+// 246 (448 * 2^119 is the largest value; past it values saturate, and an infinity does, while a NaN stays one).  A block whose
+// first slot is among the written begins anew with s = need; in any other s = max(s, need), and where it grows the codes of
+// the rows that the call does not write are taken times 2^(old - new).  Powers of two make that exact but for codes that
+// leave E4M3's normal range (2^-9 of the new scale at the coarsest), so a block holds the same whether it was written token by
+// token or at once, and the reader's conversion to bf16 takes the scale for nothing.
+//
+// The rows of a call that belong to one block stand together (a request's tokens do): the first of them, found by looking at
+// the row before, has the block in its care, wave by wave for each head's K and V: rotate and find M, then rotate again
+// (the rows come from the caches by then) and write.  One launch with the q rows.
+constexpr int SB_SHIFT = 4, SB_ROWS = 1 << SB_SHIFT;       // slots that share a scale
+constexpr int SB_TOP = 246;
+
+// the byte that holds magnitudes up to M (an fp32's bits, finite)
+__device__ __forceinline__ int sb_need(uint32_t M) {
+  return min(max((int)(M >> 23) - ((M & 0x7FFFFFu) > 0x600000u ? 7 : 8), 1), SB_TOP);
+}
+__device__ __forceinline__ uint32_t sb_size(const float* f, int count, uint32_t most) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = __float_as_uint(f[i]) & 0x7FFFFFFFu;
+    if (i < count && u < 0x7F800000u) most = max(most, u);
+  }
+  return most;
+}
+__device__ __forceinline__ float sb_power(int e) {         // 2^e, 2^-127 for less
+  return exp2i(max(e, -127));
+}
+__device__ __forceinline__ uint2 sb_pack(const float* f, float inverse) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(ap_clamp(f[4 * i] * inverse), ap_clamp(f[4 * i + 1] * inverse), 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(ap_clamp(f[4 * i + 2] * inverse), ap_clamp(f[4 * i + 3] * inverse), r, true);
+    w[i] = (uint32_t)r;
+  }
+  return make_uint2(w[0], w[1]);
+}
+__device__ __forceinline__ uint32_t sb_rescale(uint32_t w, float by) {
+  const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  const int r = __builtin_amdgcn_cvt_pk_fp8_f32(lo.x * by, lo.y * by, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi.x * by, hi.y * by, r, true);
+}
+
+// The block that row n is the first of, if it is: part `part` of `parts` of its 2 Hkv units (a head's K or V).
+template <bool SIDE>
+__device__ __forceinline__ void ap_run(const AppendArgs& a, int n, int part, int parts, float* s_cos, float* s_sin) {
+#pragma clang fp contract(off)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = a.rot >> 1;
+  const int slot = a.slots[n];
+  if (slot >= a.n_slots && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;
+  if (slot < 0 || slot >= a.n_slots) return;
+  const int block = slot >> SB_SHIFT;
+  if (n > 0 && a.slots[n - 1] >> SB_SHIFT == block) return;
+  // rows n .. n + R - 1 are the block's; lane l < R holds row n + l's place in it
+  const int mine = lane <= SB_ROWS && n + lane < a.N ? a.slots[n + lane] : -1;
+  const uint64_t other = ~__ballot(mine >> SB_SHIFT == block);
+  const int run = __builtin_ctzll(other), R = min(run, SB_ROWS);
+  const int place = mine & (SB_ROWS - 1);
+  uint32_t used = lane < R ? 1u << place : 0u;
+#pragma unroll
+  for (int d = 1; d < SB_ROWS; d <<= 1) used |= __shfl_xor(used, d, 64);
+  used = __builtin_amdgcn_readfirstlane(used);
+  if ((run > SB_ROWS || __builtin_popcount(used) != R) && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;   // a slot twice
+  const bool anew = used & 1u;
+
+  for (int i = threadIdx.x; i < R * half; i += 256) {
+    const int r = i / half, j = i - r * half;
+    const double t = (double)a.positions[n + r] * a.turns[j], f = t - rint(t);   // -1/2 .. 1/2 turns
+    // sine and cosine of what 32 bits hold of the angle, and a first-order step for the rest
+    const float hi = (float)f, lo = (float)((f - (double)hi) * 6.283185307179586);
+    float sn, cs;
+    sincospif(2.0f * hi, &sn, &cs);
+    s_cos[i] = (cs - sn * lo) * a.magnitude, s_sin[i] = (sn + cs * lo) * a.magnitude;
+  }
+  __syncthreads();
+
+  const int mask = (1 << a.page_shift) - 1;
+  const size_t page = (size_t)(slot >> a.page_shift);
+  for (int u = part * 4 + wave; u < 2 * a.Hkv; u += 4 * parts) {
+    const bool is_v = u >= a.Hkv;
+    const int h = is_v ? u - a.Hkv : u, D = is_v ? a.Dv : a.Dk, rot = is_v ? 0 : a.rot;
+    const int pairs = SIDE ? 0 : rot >> 4, P = (D >> 3) - pairs;          // units of a row
+    const size_t head = page * a.Hkv + h;
+    uint8_t* codes = static_cast<uint8_t*>(is_v ? a.v_pages : a.k_pages) + ((head << a.page_shift) + (slot & mask & ~(SB_ROWS - 1))) * D;
+    uint8_t* scale = static_cast<uint8_t*>(const_cast<void*>(is_v ? a.v_scale : a.k_scale)) + (head << (a.page_shift - SB_SHIFT)) + ((slot & mask) >> SB_SHIFT);
+    const uint16_t* rows = is_v ? a.v + n * a.v_stride + h * D : a.k + n * a.k_stride + h * D;
+    const int64_t stride = is_v ? a.v_stride : a.k_stride;
+    const int had = anew ? 0 : *scale;
+    float x[8], y[8];
+    // unit i of the run: row r, first dimension d; true: a pair of units
+    auto take = [&](int i, int& r, int& d) __attribute__((always_inline)) {
+      r = i / P;
+      const int c = i - r * P;
+      const bool pair = c < pairs;
+      d = SIDE || pair ? 8 * c : rot + 8 * (c - pairs);
+      const uint16_t* p = rows + r * stride + d;
+      ap_unpack(*reinterpret_cast<const uint4*>(p), x);
+      if (pair) {
+        ap_unpack(*reinterpret_cast<const uint4*>(p + (rot >> 1)), y);
+        ap_turn(x, y, s_cos + r * half + d, s_sin + r * half + d);
+      } else if (SIDE && d < rot) {
+        ap_turn_side(x, s_cos + r * half + d / 2, s_sin + r * half + d / 2);
+      }
+      return pair;
+    };
+    uint32_t most = 0;
+    for (int i = lane; i < R * P; i += 64) {
+      int r, d;
+      const bool pair = take(i, r, d);
+      most = sb_size(x, 8, most);
+      if (pair) most = sb_size(y, 8, most);
+    }
+    const int need = sb_need(dpp_max_u32(most)), now = anew ? need : max(had, need);
+    if (!anew && now > had) {
+      const float by = sb_power(had - now);
+      const int cells = D >> 4;
+      for (int i = lane; i < SB_ROWS * cells; i += 64) {
+        const int r = i / cells;
+        if (used >> r & 1u) continue;
+        uint4* p = reinterpret_cast<uint4*>(codes + 16 * i);
+        const uint4 w = *p;
+        *p = make_uint4(sb_rescale(w.x, by), sb_rescale(w.y, by), sb_rescale(w.z, by), sb_rescale(w.w, by));
+      }
+    }
+    if (lane == 0 && (anew || now > had)) *scale = (uint8_t)now;
+    const float inverse = sb_power(127 - now);
+    for (int i0 = 0; i0 < R * P; i0 += 64) {
+      const int i = i0 + lane;
+      int r = 0, d = 0;
+      const bool there = i < R * P;
+      const bool pair = there && take(i, r, d);
+      const int to = __shfl(place, r, 64);
+      if (!there) continue;
+      *reinterpret_cast<uint2*>(codes + to * D + d) = sb_pack(x, inverse);
+      if (pair) *reinterpret_cast<uint2*>(codes + to * D + d + (rot >> 1)) = sb_pack(y, inverse);
+    }
+  }
+}
+
+// Blocks 0 .. kv - 1 look at rows for blocks to write, consecutive ones at rows 16 apart (a long chunk's blocks begin every
+// 16 rows: in the order of the rows they would all fall on one XCD); the rest are the q rows'.
+template <bool SIDE>
+__global__ void __launch_bounds__(256) cache_append_scaled_kernel(AppendArgs a, int parts, int q_parts) {
+  __shared__ float s_cos[SB_ROWS * AP_MAX_ROT / 2], s_sin[SB_ROWS * AP_MAX_ROT / 2];
+  const int C = (a.N + SB_ROWS - 1) / SB_ROWS, kv = SB_ROWS * C * parts, b = blockIdx.x;
+  if (b < kv) {
+    const int w = b / parts, n = w % C * SB_ROWS + w / C;
+    if (n < a.N) ap_run<SIDE>(a, n, b - w * parts, parts, s_cos, s_sin);
+  } else {
+    const int n = (b - kv) / q_parts;
+    ap_token<AP_Q, SIDE>(a, n, b - kv - n * q_parts, q_parts, s_cos, s_sin);
+  }
+}
+
+// ------------------------------------------------------------------ read
+// Cached tokens as bf16 rows: code times scale, rounded once (with block scales exact).  A thread turns 8 values; a block of
+// 256 a few tokens one after another, whose rows of a head share cache lines.
+struct ReadArgs {
+  const uint8_t *k, *v;
+  const void *k_scale, *v_scale;
+  const int32_t* slots;
+  uint16_t *k_out, *v_out;
+  int32_t* status;
+  int N, Hkv, Dk, Dv, page_shift, n_slots, tokens;
+};
+
+template <int DTYPE>
+__global__ void __launch_bounds__(256) cache_read_kernel(ReadArgs a) {
+#pragma clang fp contract(off)
+  const int Uk = a.Hkv * (a.Dk >> 3), U = Uk + a.Hkv * (a.Dv >> 3), mask = (1 << a.page_shift) - 1;
+  const int first = blockIdx.x * a.tokens, count = min(a.tokens, a.N - first);
+  for (int e = threadIdx.x; e < count * U; e += 256) {
+    const int t = e / U, w = e - t * U, n = first + t;
+    const bool is_v = w >= Uk;
+    const int D = is_v ? a.Dv : a.Dk, c = is_v ? w - Uk : w, h = c / (D >> 3), d = 8 * (c - h * (D >> 3));
+    const int slot = a.slots[n];
+    if (slot >= a.n_slots && w == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;
+    uint4 out = make_uint4(0, 0, 0, 0);
+    if (slot >= 0 && slot < a.n_slots) {
+      const size_t head = (size_t)(slot >> a.page_shift) * a.Hkv + h, at = ((head << a.page_shift) + (slot & mask)) * D + d;
+      const uint8_t* pages = is_v ? a.v : a.k;
+      const void* scale = is_v ? a.v_scale : a.k_scale;
+      if constexpr (DTYPE == MIMO_KV_BF16) {
+        out = *reinterpret_cast<const uint4*>(pages + 2 * at);
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(pages + at);
+        const float s = DTYPE == MIMO_KV_E4M3 ? static_cast<const float*>(scale)[h]
+                                              : e8m0_f32(static_cast<const uint8_t*>(scale)[(head << (a.page_shift - SB_SHIFT)) + ((slot & mask) >> SB_SHIFT)]);
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t word = i ? x.y : x.x;
+          const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)word, true);
+          f[4 * i] = lo.x * s, f[4 * i + 1] = lo.y * s, f[4 * i + 2] = hi.x * s, f[4 * i + 3] = hi.y * s;
+        }
+        out = ap_pack(f);
+      }
+    }
+    uint16_t* to = is_v ? a.v_out + (size_t)n * a.Hkv * a.Dv : a.k_out + (size_t)n * a.Hkv * a.Dk;
+    *reinterpret_cast<uint4*>(to + h * D + d) = out;
+  }
+}
+
 int check_cache(const mimo_kv_cache* c, const char* what) {
   MIMO_REQUIRE(c && c->k && c->v, MIMO_ERR_ARG, "%s: null pointer", what);
-  MIMO_REQUIRE(c->dtype == MIMO_KV_BF16 || c->dtype == MIMO_KV_E4M3, MIMO_ERR_ARG, "%s: cache dtype %d", what, c->dtype);
+  MIMO_REQUIRE(c->dtype == MIMO_KV_BF16 || c->dtype == MIMO_KV_E4M3 || c->dtype == MIMO_KV_E4M3_BLOCKS, MIMO_ERR_ARG, "%s: cache dtype %d", what, c->dtype);
   MIMO_REQUIRE(c->dtype == MIMO_KV_BF16 || (c->k_scale && c->v_scale), MIMO_ERR_ARG, "%s: an E4M3 cache needs k_scale and v_scale", what);
   MIMO_REQUIRE((c->k_dim == 64 && c->v_dim == 64) || (c->k_dim == 128 && c->v_dim == 128) || (c->k_dim == 192 && c->v_dim == 128),
                MIMO_ERR_SHAPE, "%s: head dimensions %d / %d (64/64, 128/128 and 192/128 are supported)", what, c->k_dim, c->v_dim);
@@ -304,6 +534,8 @@ int check_cache(const mimo_kv_cache* c, const char* what) {
   MIMO_REQUIRE(c->n_pages >= 1 && (int64_t)c->n_pages * c->page_size <= 0x7fffffff, MIMO_ERR_SHAPE,
                "%s: %d pages of %d (at most 2^31 - 1 slots)", what, c->n_pages, c->page_size);
   MIMO_REQUIRE(aligned16(c->k) && aligned16(c->v), MIMO_ERR_ALIGN, "%s: 16-byte alignment", what);
+  MIMO_REQUIRE(c->dtype != MIMO_KV_E4M3_BLOCKS || (aligned16(c->k_scale) && aligned16(c->v_scale)), MIMO_ERR_ALIGN,
+               "%s: 16-byte alignment of the block scales", what);
   return MIMO_OK;
 }
 
@@ -352,15 +584,28 @@ int mimo_cache_step(const int32_t* lens, const int32_t* target, int B, int32_t* 
 int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k, int64_t k_stride, const uint16_t* v,
                       int64_t v_stride, int N, const int32_t* positions, const int32_t* slots, const mimo_kv_cache* cache,
                       int rotary_dim, const double* turns, uint16_t* q_out, int32_t* status, void* stream) {
+  const mimo_rotary rotary{turns, rotary_dim, 0, 1.0f};
+  return mimo_cache_append_rotary(q, q_stride, heads, k, k_stride, v, v_stride, N, positions, slots, cache, &rotary, q_out, status, stream);
+}
+
+int mimo_cache_append_rotary(const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                             int64_t v_stride, int N, const int32_t* positions, const int32_t* slots, const mimo_kv_cache* cache,
+                             const mimo_rotary* rotary, uint16_t* q_out, int32_t* status, void* stream) {
   if (int e = check_cache(cache, "cache_append")) return e;
-  MIMO_REQUIRE(N >= 0 && N <= kMaxBlocks, MIMO_ERR_SHAPE, "cache_append: %d tokens (0 to 2^24 - 1)", N);
+  const bool scaled = cache->dtype == MIMO_KV_E4M3_BLOCKS;
+  const int64_t most = scaled ? kMaxBlocks / 2 - SB_ROWS : kMaxBlocks;
+  MIMO_REQUIRE(N >= 0 && N <= most, MIMO_ERR_SHAPE, "cache_append: %d tokens (0 to %s)", N, scaled ? "2^23 - 17" : "2^24 - 1");
   if (N == 0) return MIMO_OK;
+  const mimo_rotary none{nullptr, 0, 0, 1.0f};
+  const mimo_rotary& ro = rotary ? *rotary : none;
   MIMO_REQUIRE(k && v && positions && slots, MIMO_ERR_ARG, "cache_append: null pointer");
   MIMO_REQUIRE(!q == !q_out, MIMO_ERR_ARG, "cache_append: q and q_out go together");
   MIMO_REQUIRE(!q || (heads >= 1 && heads <= 65536), MIMO_ERR_SHAPE, "cache_append: %d heads", heads);
-  MIMO_REQUIRE(rotary_dim >= 0 && rotary_dim % 16 == 0 && rotary_dim <= cache->k_dim, MIMO_ERR_SHAPE,
-               "cache_append: rotary_dim %d (a multiple of 16 up to k_dim)", rotary_dim);
-  MIMO_REQUIRE(rotary_dim == 0 || turns, MIMO_ERR_ARG, "cache_append: null pointer");
+  MIMO_REQUIRE(ro.dim >= 0 && ro.dim % 16 == 0 && ro.dim <= cache->k_dim, MIMO_ERR_SHAPE,
+               "cache_append: rotary_dim %d (a multiple of 16 up to k_dim)", ro.dim);
+  MIMO_REQUIRE(ro.dim == 0 || ro.turns, MIMO_ERR_ARG, "cache_append: null pointer");
+  MIMO_REQUIRE(ro.interleaved == 0 || ro.interleaved == 1, MIMO_ERR_ARG, "cache_append: interleaved must be 0 or 1");
+  MIMO_REQUIRE(ro.magnitude - ro.magnitude == 0.0f, MIMO_ERR_ARG, "cache_append: magnitude must be finite");
   MIMO_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(q_out) &&
                    (q_stride | k_stride | v_stride) % 8 == 0, MIMO_ERR_ALIGN,
                "cache_append: 16-byte alignment of q, k, v and of their rows");
@@ -373,19 +618,63 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
                      !overlap(k, ((size_t)(N - 1) * k_stride + kn) * 2, q_out, out) && !overlap(v, ((size_t)(N - 1) * v_stride + vn) * 2, q_out, out),
                  MIMO_ERR_ARG, "cache_append: q_out may not overlap q, k or v");
   }
-  AppendArgs a{q, k, v, q_stride, k_stride, v_stride, heads, cache->kv_heads, cache->k_dim, cache->v_dim, N, rotary_dim, turns,
-               positions, slots, q_out, cache->k, cache->v, cache->k_scale, cache->v_scale, __builtin_ctz(cache->page_size),
+  AppendArgs a{q, k, v, q_stride, k_stride, v_stride, heads, cache->kv_heads, cache->k_dim, cache->v_dim, N, ro.dim, ro.turns,
+               ro.magnitude, positions, slots, q_out, cache->k, cache->v, cache->k_scale, cache->v_scale, __builtin_ctz(cache->page_size),
                cache->n_pages * cache->page_size, status};
+  const bool side = ro.dim && ro.interleaved;
   hipStream_t st = as_stream(stream);
+  // few tokens are spread over several blocks each
+  const int per = cache->k_dim - (side ? 0 : ro.dim / 2);
+  auto spread = [&](int units) { return std::max(1, std::min((units + 255) / 256, AP_BLOCKS / N)); };
   {
     ProfScope p(st, "cache_append");
-    // few tokens are spread over several blocks each
-    const int units = ((q ? heads : 0) * (cache->k_dim - rotary_dim / 2) + cache->kv_heads * (cache->k_dim - rotary_dim / 2 + cache->v_dim)) / 8;
-    const dim3 grid(N, std::max(1, std::min((units + 255) / 256, AP_BLOCKS / N)));
-    if (cache->dtype == MIMO_KV_E4M3) cache_append_kernel<true><<<grid, 256, 0, st>>>(a);
-    else cache_append_kernel<false><<<grid, 256, 0, st>>>(a);
+    if (scaled) {
+      const int parts = std::max(1, std::min((cache->kv_heads + 1) / 2, AP_BLOCKS / N)), q_parts = spread(heads * per / 8);
+      const int64_t grid = (int64_t)(N + SB_ROWS - 1) / SB_ROWS * SB_ROWS * parts + (q ? (int64_t)N * q_parts : 0);
+      if (side) cache_append_scaled_kernel<true><<<(unsigned)grid, 256, 0, st>>>(a, parts, q_parts);
+      else cache_append_scaled_kernel<false><<<(unsigned)grid, 256, 0, st>>>(a, parts, q_parts);
+    } else {
+      const int units = ((q ? heads : 0) * per + cache->kv_heads * (per + cache->v_dim)) / 8;
+      const dim3 grid(N, spread(units));
+      const bool f8 = cache->dtype == MIMO_KV_E4M3;
+      if (side && f8) cache_append_kernel<AP_E4M3, true><<<grid, 256, 0, st>>>(a);
+      else if (side) cache_append_kernel<AP_BF16, true><<<grid, 256, 0, st>>>(a);
+      else if (f8) cache_append_kernel<AP_E4M3, false><<<grid, 256, 0, st>>>(a);
+      else cache_append_kernel<AP_BF16, false><<<grid, 256, 0, st>>>(a);
+    }
   }
   return check_launch("cache_append");
+}
+
+int mimo_cache_read(const mimo_kv_cache* cache, const int32_t* slots, int N, uint16_t* k_out, uint16_t* v_out, int32_t* status,
+                    void* stream) {
+  if (int e = check_cache(cache, "cache_read")) return e;
+  MIMO_REQUIRE(N >= 0 && N <= kMaxBlocks, MIMO_ERR_SHAPE, "cache_read: %d tokens (0 to 2^24 - 1)", N);
+  if (N == 0) return MIMO_OK;
+  MIMO_REQUIRE(slots && k_out && v_out, MIMO_ERR_ARG, "cache_read: null pointer");
+  MIMO_REQUIRE(aligned16(k_out) && aligned16(v_out), MIMO_ERR_ALIGN, "cache_read: 16-byte alignment of k_out and v_out");
+  const size_t kn = (size_t)cache->kv_heads * cache->k_dim, vn = (size_t)cache->kv_heads * cache->v_dim;
+  const size_t rows = (size_t)cache->n_pages * cache->page_size * (cache->dtype == MIMO_KV_BF16 ? 2 : 1);
+  const void* outs[2] = {k_out, v_out};
+  const size_t sizes[2] = {N * kn * 2, N * vn * 2};
+  for (int i = 0; i < 2; ++i)
+    MIMO_REQUIRE(!overlap(outs[i], sizes[i], cache->k, rows * kn) && !overlap(outs[i], sizes[i], cache->v, rows * vn) &&
+                     !overlap(outs[i], sizes[i], slots, (size_t)N * 4),
+                 MIMO_ERR_ARG, "cache_read: outputs may not overlap the cache or the slots");
+  MIMO_REQUIRE(!overlap(k_out, sizes[0], v_out, sizes[1]), MIMO_ERR_ARG, "cache_read: k_out may not overlap v_out");
+  ReadArgs a{static_cast<const uint8_t*>(cache->k), static_cast<const uint8_t*>(cache->v), cache->k_scale, cache->v_scale, slots,
+             k_out, v_out, status, N, cache->kv_heads, cache->k_dim, cache->v_dim, __builtin_ctz(cache->page_size),
+             cache->n_pages * cache->page_size, 0};
+  a.tokens = std::max(1, std::min(16, N / 2048));
+  const unsigned grid = (N + a.tokens - 1) / a.tokens;
+  hipStream_t st = as_stream(stream);
+  {
+    ProfScope p(st, "cache_read");
+    if (cache->dtype == MIMO_KV_BF16) cache_read_kernel<MIMO_KV_BF16><<<grid, 256, 0, st>>>(a);
+    else if (cache->dtype == MIMO_KV_E4M3) cache_read_kernel<MIMO_KV_E4M3><<<grid, 256, 0, st>>>(a);
+    else cache_read_kernel<MIMO_KV_E4M3_BLOCKS><<<grid, 256, 0, st>>>(a);
+  }
+  return check_launch("cache_read");
 }
 
 }  // extern "C"

@@ -14,6 +14,7 @@ ABI_VERSION = 2
 MIMO_OK = 0
 ERR_SHAPE, ERR_ALIGN, ERR_ROWS_PER_EXPERT, ERR_SLOT, ERR_WORKSPACE, ERR_HIP, ERR_ARG = -1, -2, -3, -4, -5, -6, -7
 ERR_PAGES = -8
+KV_BF16, KV_E4M3, KV_E4M3_BLOCKS = 0, 1, 2
 _VALUE_ERRORS = {ERR_SHAPE, ERR_ALIGN, ERR_ROWS_PER_EXPERT, ERR_SLOT, ERR_WORKSPACE, ERR_ARG}
 
 
@@ -33,6 +34,12 @@ class MimoKvCache(ctypes.Structure):
                 ("kv_heads", ctypes.c_int32), ("k_dim", ctypes.c_int32), ("v_dim", ctypes.c_int32)]
 
 
+class MimoRotary(ctypes.Structure):
+    """struct mimo_rotary (include/mimo_moe.h)."""
+    _fields_ = [("turns", ctypes.c_void_p), ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("magnitude", ctypes.c_float)]
+
+
 P = ctypes.c_void_p
 I32 = ctypes.c_int32
 I64 = ctypes.c_int64
@@ -41,6 +48,7 @@ F32 = ctypes.c_float
 SZ = ctypes.c_size_t
 BANKP = ctypes.POINTER(MimoBank)
 CACHEP = ctypes.POINTER(MimoKvCache)
+ROTARYP = ctypes.POINTER(MimoRotary)
 
 SIGNATURES = {
     "mimo_abi_version": (I32, []),
@@ -75,6 +83,8 @@ SIGNATURES = {
     "mimo_moe_layer_decode_noalloc": (I32, [P, I32, P, F32, P, P, P, I32, I32, BANKP, P, P, P, P, P, P]),
     "mimo_cache_step": (I32, [P, P, I32, P, I32, P, P, I32, I32, I32, I32, P, P, P, P, P, P, P, P, P]),
     "mimo_cache_append": (I32, [P, I64, I32, P, I64, P, I64, I32, P, P, CACHEP, I32, P, P, P, P]),
+    "mimo_cache_append_rotary": (I32, [P, I64, I32, P, I64, P, I64, I32, P, P, CACHEP, ROTARYP, P, P, P]),
+    "mimo_cache_read": (I32, [CACHEP, P, I32, P, P, P, P]),
     "mimo_cache_attend": (I32, [P, I64, I32, I32, CACHEP, I32, P, P, P, I32, I32, F32, I32, I32, P, P, P, P, SZ, P]),
     "mimo_cache_attend_workspace_size": (SZ, [I32, I32, I32, I32]),
     "mimo_profile_enable": (I32, [I32]),

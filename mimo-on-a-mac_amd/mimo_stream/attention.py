@@ -2,6 +2,7 @@
 
   PageTable.step(target)       request lengths -> page tables, slots and positions of the new tokens, on the device
   append(cache, plan, k, v, q) rotary positions on q and k, K and V written to their slots (bf16 or E4M3)
+  read(cache, slots)           cached tokens back as bf16 rows
   attend(q, cache, plan)       attention of the new tokens over the cache: causal, grouped heads, sliding window, first
                                tokens that stay visible, sink logits
 
@@ -21,6 +22,7 @@ import torch
 from . import _lib
 
 E4M3 = torch.float8_e4m3fn
+E8M0 = torch.float8_e8m0fnu
 BF16 = torch.bfloat16
 INT32 = torch.int32
 
@@ -153,21 +155,52 @@ class PageTable:
             _lib.check(rc, "mimo_cache_step")
         return StepPlan(starts, lens, slots, positions, self._table, max_new, n_free, status, self.page_size)
 
+    def slots(self, request, stop, start=0):
+        """int32 slots of a request's tokens start .. stop - 1, as its page table has them now (read takes them).  The request's
+        length is on the device and is not looked at: tokens past it have slots of no meaning."""
+        B, width = self._table.shape
+        if not (0 <= request < B and 0 <= start <= stop <= width * self.page_size):
+            raise ValueError(f"tokens {start} to {stop} of request {request}: {B} requests of up to {width * self.page_size} tokens")
+        at = torch.arange(start, stop, dtype=INT32, device=self._table.device)
+        return self._table[request][at // self.page_size] * self.page_size + at % self.page_size
+
+
+def _block_scales(s, dev, shape):
+    """Block scales as the bytes that append writes in place: checked, never converted."""
+    if s.dtype == E8M0:
+        s = s.view(torch.uint8)
+    if s.dtype != torch.uint8 or s.device != dev or s.shape != shape or not s.is_contiguous() or s.data_ptr() % 16:
+        raise ValueError(f"block scales: need contiguous, 16-byte aligned bytes of shape {shape} on {dev}, got {s.dtype} "
+                         f"{tuple(s.shape)} on {s.device}")
+    return s
+
 
 class KVCache:
-    """One layer's K/V pages: k [n_pages, kv_heads, page_size, k_dim] and v [..., v_dim], bf16 or float8_e4m3fn with one
-    fp32 scale per K/V head (a stored value stands for value * scale).  Head dimensions 64/64, 128/128 or 192/128."""
+    """One layer's K/V pages: k [n_pages, kv_heads, page_size, k_dim] and v [..., v_dim].  Head dimensions 64/64, 128/128 or
+    192/128.  Of three kinds:
+
+    bf16;
+    float8_e4m3fn with one fp32 scale per K/V head, k_scale and v_scale (a stored value stands for value * scale), which a
+    user has to know beforehand: what is past 448 scales saturates;
+    float8_e4m3fn with block_scales: k_scale and v_scale are bytes [n_pages, kv_heads, page_size / 16], and a value of a slot
+    stands for value * 2 ** (byte - 127).  append sets a block's byte by the values that it writes (mimo_stream.append)."""
 
     def __init__(self, n_pages, page_size, kv_heads, k_dim, v_dim, dtype=torch.bfloat16, k_scale=None, v_scale=None,
-                 device="cuda"):
+                 device="cuda", block_scales=False):
         dev = _device(device)
+        if block_scales:
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("a cache with block scales makes its own (KVCache.of takes existing ones)")
+            k_scale, v_scale = (torch.full((n_pages, kv_heads, max(page_size, 0) // 16), 127, dtype=torch.uint8, device=dev)
+                                for _ in range(2))
         self._bind(torch.zeros((n_pages, kv_heads, page_size, k_dim), dtype=torch.uint8 if dtype == E4M3 else dtype, device=dev),
                    torch.zeros((n_pages, kv_heads, page_size, v_dim), dtype=torch.uint8 if dtype == E4M3 else dtype, device=dev),
                    k_scale, v_scale, dtype)
 
     @classmethod
     def of(cls, k, v, k_scale=None, v_scale=None):
-        """A cache over existing page tensors (not copied)."""
+        """A cache over existing page tensors (not copied).  Scales of three dimensions, uint8 or float8_e8m0fnu, are block
+        scales: bytes 1 to 246, and not copied either."""
         self = cls.__new__(cls)
         self._bind(k, v, k_scale, v_scale, k.dtype)
         return self
@@ -188,18 +221,27 @@ class KVCache:
             raise ValueError("page_size must be a power of two from 16 to 1024")
         if (k_dim, v.shape[3]) not in ((64, 64), (128, 128), (192, 128)):
             raise ValueError(f"head dimensions {k_dim} / {v.shape[3]}: 64/64, 128/128 and 192/128 are supported")
+        kind = _lib.KV_BF16
         if dtype == E4M3:
             if k_scale is None or v_scale is None:
                 raise ValueError("an E4M3 cache needs k_scale and v_scale")
-            k_scale, v_scale = (torch.as_tensor(s, dtype=torch.float32, device=k.device).expand(heads).contiguous()
-                                for s in (k_scale, v_scale))
+            blocks = [isinstance(s, torch.Tensor) and s.dim() == 3 for s in (k_scale, v_scale)]
+            if blocks[0] != blocks[1]:
+                raise ValueError("k_scale and v_scale of two kinds")
+            if blocks[0]:
+                k_scale, v_scale = (_block_scales(s, k.device, (n_pages, heads, page // 16)) for s in (k_scale, v_scale))
+                kind = _lib.KV_E4M3_BLOCKS
+            else:
+                k_scale, v_scale = (torch.as_tensor(s, dtype=torch.float32, device=k.device).expand(heads).contiguous()
+                                    for s in (k_scale, v_scale))
+                kind = _lib.KV_E4M3
         elif k_scale is not None or v_scale is not None:
             raise ValueError("scales belong to an E4M3 cache")
         self._tensors = (k, v, k_scale, v_scale)             # fixed: the struct holds their addresses
         self.dtype, self.device = dtype, k.device
         self.kv_heads, self.k_dim, self.v_dim, self.page_size, self.n_pages = heads, k_dim, v.shape[3], page, n_pages
-        self._struct = _lib.MimoKvCache(*(_lib.ptr(t) for t in self._tensors), 1 if dtype == E4M3 else 0, n_pages, page,
-                                        heads, k_dim, v.shape[3])
+        self.block_scales = kind == _lib.KV_E4M3_BLOCKS
+        self._struct = _lib.MimoKvCache(*(_lib.ptr(t) for t in self._tensors), kind, n_pages, page, heads, k_dim, v.shape[3])
 
     k = property(lambda self: self._tensors[0])
     v = property(lambda self: self._tensors[1])
@@ -207,18 +249,46 @@ class KVCache:
     v_scale = property(lambda self: self._tensors[3])
 
 
-class Rotary:
-    """Rotary positions on the first `dim` dimensions of a head (a multiple of 16), pairs (i, i + dim / 2), frequencies
-    theta ** (-2 i / dim); kept as fp64 turns per position, so that far positions keep their fraction."""
+def stretched(dim, theta, factor, original, few=1.0, many=32.0):
+    """Frequencies fp64 [dim / 2] for contexts `factor` times as long as the `original` length that theta ** (-2 i / dim) was
+    trained at: a pair that turns at least `many` times over the original length keeps its frequency, one of at most `few`
+    turns has it divided by factor, and those between are blended in proportion to i, from the last whole pair number of
+    `many` turns to the first of `few`."""
+    if dim < 2 or dim % 2 or not theta > 1.0 or not factor > 0.0 or not original > 0 or not 0.0 < few < many:
+        raise ValueError(f"need an even dim, theta > 1, factor > 0, original > 0 and 0 < few < many (got {dim}, {theta}, {factor}, "
+                         f"{original}, {few}, {many})")
+    i = torch.arange(dim // 2, dtype=torch.float64)
+    freq = float(theta) ** (-2.0 * i / dim)
+    # pair i turns original theta ** (-2 i / dim) / 2 pi times
+    first, last = (0.5 * dim * math.log(original / (2.0 * math.pi * turns)) / math.log(theta) for turns in (many, few))
+    first, last = max(math.floor(first), 0), min(math.ceil(last), dim // 2 - 1)
+    slow = ((i - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
+    return freq * (1.0 - slow * (1.0 - 1.0 / factor))
 
-    def __init__(self, dim, theta=10000.0, device="cuda"):
+
+class Rotary:
+    """Rotary positions on the first `dim` dimensions of a head (a multiple of 16): pairs (i, i + dim / 2), or (2 i, 2 i + 1) if
+    interleaved; frequencies theta ** (-2 i / dim), or the dim / 2 given ones (stretched makes them for long contexts), kept
+    as fp64 turns per position, so that far positions keep their fraction.  Rotated values are taken times magnitude."""
+
+    def __init__(self, dim, theta=10000.0, device="cuda", interleaved=False, frequencies=None, magnitude=1.0):
         if dim < 16 or dim % 16 or dim > 256:
             raise ValueError("the rotary dimension must be a multiple of 16 up to 256")
         if not theta > 0.0:
             raise ValueError("theta must be positive")
-        self.dim = int(dim)
-        i = torch.arange(0, dim, 2, dtype=torch.float64)
-        self.turns = (float(theta) ** (-i / dim) / (2.0 * math.pi)).to(_device(device))
+        self.dim, self.interleaved, self.magnitude = int(dim), bool(interleaved), float(magnitude)
+        if not math.isfinite(self.magnitude) or abs(self.magnitude) > 3.4e38:
+            raise ValueError("magnitude must be a finite fp32")
+        if frequencies is None:
+            frequencies = float(theta) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+        else:
+            frequencies = torch.as_tensor(frequencies).detach().to(device="cpu", dtype=torch.float64)
+            if frequencies.shape != (dim // 2,) or not bool(torch.isfinite(frequencies).all()):
+                raise ValueError(f"frequencies: need {dim // 2} finite numbers, got shape {tuple(frequencies.shape)}")
+        self._turns = (frequencies / (2.0 * math.pi)).to(_device(device))
+        self._struct = _lib.MimoRotary(self._turns.data_ptr(), self.dim, self.interleaved, self.magnitude)
+
+    turns = property(lambda self: self._turns)               # fixed: the struct holds its address
 
 
 def _rows(x, dev, heads, dim, name):
@@ -245,7 +315,13 @@ def _rows(x, dev, heads, dim, name):
 def append(cache, plan, k, v, q=None, rotary=None):
     """Write the new tokens' k [N, kv_heads, k_dim] and v [N, kv_heads, v_dim] to plan.slots (rows with slot -1 are left
     out), k rotated to plan.positions; returns q [N, heads, k_dim] rotated likewise (None without q).  q, k and v may be
-    views of one projection's rows; other types than bf16 are rounded to it first."""
+    views of one projection's rows; other types than bf16 are rounded to it first.  Slots are distinct.
+
+    Into a cache with block scales, the rows of one block of 16 slots follow one another, as in the plan of a step (a block
+    whose rows do not has undefined contents).  A call that writes a block's first slot begins the block anew; in another the
+    scale of each head grows where the new values need it, and what the block holds is kept: exactly, but for values below
+    2 ** -6 of the new scale, which are rounded to 2 ** -9 of it.  Values past 448 * 2 ** 119 saturate, infinities among
+    them."""
     _same_pages(plan, cache)
     dev = cache.device
     index = _gpu(dev)
@@ -259,14 +335,13 @@ def append(cache, plan, k, v, q=None, rotary=None):
         raise ValueError(f"{N} tokens of k, {v.shape[0]} of v")
     at_slots = _int32(plan.slots, dev, (N,), "plan.slots")
     at_positions = _int32(plan.positions, dev, (N,), "plan.positions")
-    dim, turns = 0, None
+    turn = None
     if rotary is not None:
-        dim = rotary.dim
-        if dim > cache.k_dim:
-            raise ValueError(f"rotary dimension {dim} past the head's {cache.k_dim}")
-        if rotary.turns.device != dev:
-            raise ValueError(f"rotary on {rotary.turns.device}, expected {dev}")
-        turns = rotary.turns.data_ptr()
+        if rotary.dim > cache.k_dim:
+            raise ValueError(f"rotary dimension {rotary.dim} past the head's {cache.k_dim}")
+        if rotary._turns.device != dev:
+            raise ValueError(f"rotary on {rotary._turns.device}, expected {dev}")
+        turn = rotary._struct
     out, at_q, at_out, q_stride, heads = None, None, None, 0, 0
     if q is not None:
         q, at_q, q_stride = _rows(q, dev, None, cache.k_dim, "q")
@@ -277,12 +352,40 @@ def append(cache, plan, k, v, q=None, rotary=None):
         at_out = out.data_ptr()
     status = _status(plan, dev)
     if N:
-        rc = _entry("mimo_cache_append")(
-            at_q, q_stride, heads, at_k, k_stride, at_v, v_stride, N, at_positions, at_slots, cache._struct, dim, turns, at_out,
-            status, _raw_stream(index))
+        rc = _entry("mimo_cache_append_rotary")(
+            at_q, q_stride, heads, at_k, k_stride, at_v, v_stride, N, at_positions, at_slots, cache._struct, turn, at_out, status,
+            _raw_stream(index))
         if rc:
             _lib.check(rc, "mimo_cache_append")
     return out
+
+
+def read(cache, slots, out=None, status=None):
+    """Cached tokens as rows: (k [N, kv_heads, k_dim], v [N, kv_heads, v_dim]) in bf16 of int32 slots [N] (a plan's, or
+    PageTable.slots; in any order, any slot any number of times), stored values times their scales, rounded once; rows of
+    slot -1 are 0.  Keys are as append left them, rotated.  out: two contiguous bf16 tensors to write; status: int32 [1] that
+    receives a failure (a slot past the cache, whose row is 0) as plan.status does."""
+    dev = cache.device
+    index = _gpu(dev)
+    if _current_device() != index:
+        with torch.cuda.device(dev):
+            return read(cache, slots, out, status)
+    N = slots.numel() if isinstance(slots, torch.Tensor) else 0
+    at_slots = _int32(slots, dev, (N,), "slots")
+    shapes = (N, cache.kv_heads, cache.k_dim), (N, cache.kv_heads, cache.v_dim)
+    if out is None:
+        k, v = (torch.empty(shape, dtype=BF16, device=dev) for shape in shapes)
+    else:
+        k, v = out
+        for x, shape in zip((k, v), shapes):
+            if x.dtype is not BF16 or x.shape != shape or not x.is_contiguous() or x.device != dev or x.data_ptr() % 16:
+                raise ValueError(f"out: need a contiguous, 16-byte aligned bf16 tensor of shape {shape} on {dev}")
+    at_status = None if status is None else _int32(status, dev, (1,), "status")
+    if N:
+        rc = _entry("mimo_cache_read")(cache._struct, at_slots, N, k.data_ptr(), v.data_ptr(), at_status, _raw_stream(index))
+        if rc:
+            _lib.check(rc, "mimo_cache_read")
+    return k, v
 
 
 @functools.lru_cache(maxsize=1024)

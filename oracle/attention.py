@@ -87,3 +87,77 @@ def attend(q, k_pages, v_pages, starts, lens, table, scale, window=0, sinks=0, s
             out[rows, g * G:(g + 1) * G] = np.where(total == 0.0, 0.0, o / np.where(total == 0.0, 1.0, total))
             size[rows, g * G:(g + 1) * G] = np.where(total == 0.0, 0.0, z / np.where(total == 0.0, 1.0, total))
     return out, size
+
+
+def turn(x, positions, frequencies, interleaved=False, magnitude=1.0):
+    """x [N, heads, D] float64 with its first 2 len(frequencies) dimensions rotated in pairs (i, i + len) or (2 i, 2 i + 1)."""
+    x = np.array(x, dtype=np.float64)
+    half = len(frequencies)
+    angle = np.asarray(positions, dtype=np.float64)[:, None, None] * np.asarray(frequencies, dtype=np.float64)
+    c, s = magnitude * np.cos(angle), magnitude * np.sin(angle)
+    at = (slice(0, 2 * half, 2), slice(1, 2 * half, 2)) if interleaved else (slice(0, half), slice(half, 2 * half))
+    a, b = x[..., at[0]].copy(), x[..., at[1]].copy()
+    x[..., at[0]], x[..., at[1]] = a * c - b * s, b * c + a * s
+    return x
+
+
+def stretched(dim, theta, factor, original, few, many):
+    """Frequencies of a context stretched by factor, pair by pair: those that turn `many` times over the original length or
+    more are kept, those of up to `few` divided by factor, and pair numbers between are blended in proportion."""
+    freq = [theta ** (-2.0 * i / dim) for i in range(dim // 2)]
+
+    def pair_of(turns):                                    # the real pair number whose frequency makes that many turns
+        return dim * np.log(original / (2 * np.pi * turns)) / (2 * np.log(theta))
+    lo, hi = max(int(np.floor(pair_of(many))), 0), min(int(np.ceil(pair_of(few))), dim // 2 - 1)
+    out = []
+    for i, f in enumerate(freq):
+        share = min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0)
+        out.append((1 - share) * f + share * f / factor)
+    return np.array(out)
+
+
+SCALE_ROWS = 16
+SCALE_TOP = 246
+
+
+def block_byte(most):
+    """The smallest byte s of 1 .. 246 with most <= 448 * 2 ** (s - 127) (246 if none is large enough)."""
+    for s in range(1, SCALE_TOP):
+        if most <= 448.0 * 2.0 ** (s - 127):
+            return s
+    return SCALE_TOP
+
+
+def block_write(held, byte, x, slots, page):
+    """What a cache with block scales holds after x [N, heads, D] (float64; NaN and infinities among it) went to its slots: its
+    values divided by their block's scale, before any rounding, and the bytes.  held [pages, heads, page, D] are the codes'
+    values before, byte [pages, heads, page / 16]."""
+    held, byte = np.array(held, dtype=np.float64), np.array(byte, dtype=np.int64)
+    n = 0
+    while n < len(slots):
+        if slots[n] < 0:
+            n += 1
+            continue
+        rows = [n]
+        while n + 1 < len(slots) and slots[n + 1] >= 0 and slots[n + 1] // SCALE_ROWS == slots[n] // SCALE_ROWS:
+            n += 1
+            rows.append(n)
+        n += 1
+        p, block = slots[rows[0]] // page, slots[rows[0]] % page // SCALE_ROWS
+        span = slice(SCALE_ROWS * block, SCALE_ROWS * (block + 1))
+        for h in range(held.shape[1]):
+            values = np.abs(x[rows, h])
+            need = block_byte(values[np.isfinite(values)].max(initial=0.0))
+            if not any(slots[r] % SCALE_ROWS == 0 for r in rows):
+                old = int(byte[p, h, block])
+                need = max(need, old)
+                held[p, h, span] *= 2.0 ** (old - need)
+            byte[p, h, block] = need
+            for r in rows:
+                held[p, h, slots[r] % page] = np.clip(x[r, h] * 2.0 ** (127 - need), -448.0, 448.0)
+    return held, byte
+
+
+def block_values(codes, byte):
+    """Values [pages, heads, page, D] that codes (as float64) and bytes stand for."""
+    return codes * np.repeat(2.0 ** (np.asarray(byte, dtype=np.float64) - 127.0), SCALE_ROWS, axis=2)[..., None]
