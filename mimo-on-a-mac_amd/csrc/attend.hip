@@ -638,6 +638,12 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       if (C::BS && lane == 0) sc[wave] = next_scales[0].x << 23, sc[4 + wave] = next_scales[0].y << 23;
       at_wait_vm(0);
       __syncthreads();                                     // the tile has landed everywhere; the other one is free
+      if constexpr (C::BS) {                               // on their way while the copies are asked for
+        const float* by = reinterpret_cast<const float*>(sc);
+        k_by[0] = by[r32 >> 4], k_by[1] = by[2 + (r32 >> 4)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v_by[i] = by[4 + i];
+      }
       if (it + 1 < it1) {
         rows_of();
         issue_k(lds0 + (cur ^ 1) * C::STAGE);
@@ -645,12 +651,6 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       }
       if (!busy || rg.key(g0) > wp_max) continue;
       const uint8_t* st = lds + cur * C::STAGE;
-      if constexpr (C::BS) {
-        const float* by = reinterpret_cast<const float*>(sc);
-        k_by[0] = by[r32 >> 4], k_by[1] = by[2 + (r32 >> 4)];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v_by[i] = by[4 + i];
-      }
       scores(st);
       if (!open(g0)) mask(g0);
       softmax();
@@ -669,11 +669,11 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
     for (int it = it0; it < end; ++it) {
       const int g0 = it * UG + wg;
       const bool more = it + 1 < end;
+      if (more) look(it + 1);
       if constexpr (C::BS) {
         k_by[0] = e8m0_f32(r32 < 16 ? next_scales[0].x : next_scales[1].x);
         v_by[0] = e8m0_f32(next_scales[0].y), v_by[1] = e8m0_f32(next_scales[1].y);
       }
-      if (more) look(it + 1);
       at_wait_vm(NV);
       scores(st);
       at_wait_lds();                                       // K has been read: its room takes the next keys

@@ -325,33 +325,52 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
 // leave E4M3's normal range (2^-9 of the new scale at the coarsest), so a block holds the same whether it was written token by
 // token or at once, and the reader's conversion to bf16 takes the scale for nothing.
 //
-// The rows of a call that belong to one block stand together (a request's tokens do): the first of them, found by looking at
-// the row before, has the block in its care, wave by wave for each head's K and V: rotate and find M, then rotate again
-// (the rows come from the caches by then) and write.  One launch with the q rows.
+// The rows of a call that belong to one block stand together (a request's tokens do): the first of them is found by looking at
+// the row before, and the waves that look at it write the whole block: each head's K or V rotated in registers, M, the codes.
+// One launch with the q rows, whose HBM time covers it: 4096 tokens of 64/8 heads (233 MB) 43.8 us, 5.3 TB/s, 37 without K and
+// V and 12 without q.  1687 tokens in pieces of 24 prompts, 32/8 heads 14.1 us (8.2 and 12.6): 130 blocks of slots for each of
+// 8 heads are a chain of round trips (slots, rows, stores), angles in 64 bits and the starts of 3400 blocks.  64 decoded tokens
+// 4.5 us.
 constexpr int SB_SHIFT = 4, SB_ROWS = 1 << SB_SHIFT;       // slots that share a scale
 constexpr int SB_TOP = 246;
+// Blocks that look for work: each is given as few rows as that leaves (1687 tokens in pieces of 24 prompts 14.1 us; 1024
+// blocks 17.5, 4096 14.9; one of 4096 tokens 43.8, 42.6, 48.0: a block without work still costs its start).
+constexpr int SB_BLOCKS = 2048;
 
 // the byte that holds magnitudes up to M (an fp32's bits, finite)
 __device__ __forceinline__ int sb_need(uint32_t M) {
   return min(max((int)(M >> 23) - ((M & 0x7FFFFFu) > 0x600000u ? 7 : 8), 1), SB_TOP);
 }
-__device__ __forceinline__ uint32_t sb_size(const float* f, int count, uint32_t most) {
+// the largest magnitude of eight values and `most`: NaN left out; by bits, and only finite values
+__device__ __forceinline__ float sb_size(const float* f, float most) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) most = fmaxf(most, fabsf(f[i]));
+  return most;
+}
+__device__ __forceinline__ uint32_t sb_finite_size(const float* f, uint32_t most) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t u = __float_as_uint(f[i]) & 0x7FFFFFFFu;
-    if (i < count && u < 0x7F800000u) most = max(most, u);
+    most = max(most, u < 0x7F800000u ? u : 0u);
   }
   return most;
 }
 __device__ __forceinline__ float sb_power(int e) {         // 2^e, 2^-127 for less
   return exp2i(max(e, -127));
 }
-__device__ __forceinline__ uint2 sb_pack(const float* f, float inverse) {
+// E4M3 of f * inverse; `over`: some values may be past 448 and are clamped (the scale keeps the others below it)
+__device__ __forceinline__ uint2 sb_pack(const float* f, float inverse, bool over) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = f[i] * inverse;
+  if (over)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = ap_clamp(x[i]);
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    int r = __builtin_amdgcn_cvt_pk_fp8_f32(ap_clamp(f[4 * i] * inverse), ap_clamp(f[4 * i + 1] * inverse), 0, false);
-    r = __builtin_amdgcn_cvt_pk_fp8_f32(ap_clamp(f[4 * i + 2] * inverse), ap_clamp(f[4 * i + 3] * inverse), r, true);
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], r, true);
     w[i] = (uint32_t)r;
   }
   return make_uint2(w[0], w[1]);
@@ -362,114 +381,175 @@ __device__ __forceinline__ uint32_t sb_rescale(uint32_t w, float by) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi.x * by, hi.y * by, r, true);
 }
 
-// The block that row n is the first of, if it is: part `part` of `parts` of its 2 Hkv units (a head's K or V).
+// The block that row n is the first of: part `part` of `parts` of its 2 Hkv units (a head's K or V).  Up to 4 rows are a wave's
+// work, so that four units are in hand at once; more are shared by the four waves.  slots: lane l holds that of row n + l, 17
+// of them.
+constexpr int SB_HALF = 96;                                // pairs of a head of 192
+struct RunRoom {
+  float cos[SB_ROWS * SB_HALF], sin[SB_ROWS * SB_HALF];
+  uint32_t most[2][4];
+};
+// A barrier for what is in LDS alone: loads and stores on their way to memory are not waited for.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 template <bool SIDE>
-__device__ __forceinline__ void ap_run(const AppendArgs& a, int n, int part, int parts, float* s_cos, float* s_sin) {
+__device__ __forceinline__ void ap_run(const AppendArgs& a, int n, int slots, int part, int parts, RunRoom& room) {
 #pragma clang fp contract(off)
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = a.rot >> 1;
-  const int slot = a.slots[n];
-  if (slot >= a.n_slots && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;
-  if (slot < 0 || slot >= a.n_slots) return;
-  const int block = slot >> SB_SHIFT;
-  if (n > 0 && a.slots[n - 1] >> SB_SHIFT == block) return;
-  // rows n .. n + R - 1 are the block's; lane l < R holds row n + l's place in it
-  const int mine = lane <= SB_ROWS && n + lane < a.N ? a.slots[n + lane] : -1;
-  const uint64_t other = ~__ballot(mine >> SB_SHIFT == block);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = a.rot >> 1;
+  const int slot = __builtin_amdgcn_readfirstlane(slots);
+  const uint64_t other = __ballot(lane > SB_ROWS || slots >> SB_SHIFT != slot >> SB_SHIFT);
   const int run = __builtin_ctzll(other), R = min(run, SB_ROWS);
-  const int place = mine & (SB_ROWS - 1);
-  uint32_t used = lane < R ? 1u << place : 0u;
+  uint32_t used = lane < R ? 1u << (slots & (SB_ROWS - 1)) : 0u;
 #pragma unroll
   for (int d = 1; d < SB_ROWS; d <<= 1) used |= __shfl_xor(used, d, 64);
   used = __builtin_amdgcn_readfirstlane(used);
   if ((run > SB_ROWS || __builtin_popcount(used) != R) && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;   // a slot twice
-  const bool anew = used & 1u;
-
-  for (int i = threadIdx.x; i < R * half; i += 256) {
-    const int r = i / half, j = i - r * half;
-    const double t = (double)a.positions[n + r] * a.turns[j], f = t - rint(t);   // -1/2 .. 1/2 turns
-    // sine and cosine of what 32 bits hold of the angle, and a first-order step for the rest
-    const float hi = (float)f, lo = (float)((f - (double)hi) * 6.283185307179586);
-    float sn, cs;
-    sincospif(2.0f * hi, &sn, &cs);
-    s_cos[i] = (cs - sn * lo) * a.magnitude, s_sin[i] = (sn + cs * lo) * a.magnitude;
-  }
-  __syncthreads();
-
+  const bool anew = used & 1u, shared = R > 4;
   const int mask = (1 << a.page_shift) - 1;
   const size_t page = (size_t)(slot >> a.page_shift);
-  for (int u = part * 4 + wave; u < 2 * a.Hkv; u += 4 * parts) {
-    const bool is_v = u >= a.Hkv;
-    const int h = is_v ? u - a.Hkv : u, D = is_v ? a.Dv : a.Dk, rot = is_v ? 0 : a.rot;
-    const int pairs = SIDE ? 0 : rot >> 4, P = (D >> 3) - pairs;          // units of a row
+  const int me = shared ? threadIdx.x : lane, T = shared ? 256 : 64, per = shared ? 1 : 4;
+
+  // The unit in hand: a head's K or V, and this thread's share of its rows, items of 8 values (of a pair of units, twice 8);
+  // r, d: row of the run and first dimension of an item (-1: none), the same for all K and for all V.
+  constexpr int ITEMS = 2;                                 // 16 rows of 192 over 256 threads, 4 over 64
+  int kind = -1, D = 0, rot = 0, had = 0, r[ITEMS], d[ITEMS];
+  uint8_t *codes, *scale;
+  uint4 x[ITEMS], y[ITEMS];
+  auto load = [&](int unit) __attribute__((always_inline)) {
+    const bool is_v = unit >= a.Hkv;
+    if (kind != (int)is_v) {
+      kind = is_v;
+      D = is_v ? a.Dv : a.Dk, rot = is_v ? 0 : a.rot;
+      const int pairs = SIDE ? 0 : rot >> 4, P = (D >> 3) - pairs;   // P: items of a row
+#pragma unroll
+      for (int e = 0; e < ITEMS; ++e) {
+        const int i = me + T * e, row = i / P, c = i - row * P;
+        r[e] = i < R * P ? row : -1;
+        d[e] = SIDE || c < pairs ? 8 * c : rot + 8 * (c - pairs);
+      }
+    }
+    const int h = is_v ? unit - a.Hkv : unit;
     const size_t head = page * a.Hkv + h;
-    uint8_t* codes = static_cast<uint8_t*>(is_v ? a.v_pages : a.k_pages) + ((head << a.page_shift) + (slot & mask & ~(SB_ROWS - 1))) * D;
-    uint8_t* scale = static_cast<uint8_t*>(const_cast<void*>(is_v ? a.v_scale : a.k_scale)) + (head << (a.page_shift - SB_SHIFT)) + ((slot & mask) >> SB_SHIFT);
+    codes = static_cast<uint8_t*>(is_v ? a.v_pages : a.k_pages) + ((head << a.page_shift) + (slot & mask & ~(SB_ROWS - 1))) * D;
+    scale = static_cast<uint8_t*>(const_cast<void*>(is_v ? a.v_scale : a.k_scale)) + (head << (a.page_shift - SB_SHIFT)) + ((slot & mask) >> SB_SHIFT);
     const uint16_t* rows = is_v ? a.v + n * a.v_stride + h * D : a.k + n * a.k_stride + h * D;
     const int64_t stride = is_v ? a.v_stride : a.k_stride;
-    const int had = anew ? 0 : *scale;
-    float x[8], y[8];
-    // unit i of the run: row r, first dimension d; true: a pair of units
-    auto take = [&](int i, int& r, int& d) __attribute__((always_inline)) {
-      r = i / P;
-      const int c = i - r * P;
-      const bool pair = c < pairs;
-      d = SIDE || pair ? 8 * c : rot + 8 * (c - pairs);
-      const uint16_t* p = rows + r * stride + d;
-      ap_unpack(*reinterpret_cast<const uint4*>(p), x);
-      if (pair) {
-        ap_unpack(*reinterpret_cast<const uint4*>(p + (rot >> 1)), y);
-        ap_turn(x, y, s_cos + r * half + d, s_sin + r * half + d);
-      } else if (SIDE && d < rot) {
-        ap_turn_side(x, s_cos + r * half + d / 2, s_sin + r * half + d / 2);
-      }
-      return pair;
-    };
-    uint32_t most = 0;
-    for (int i = lane; i < R * P; i += 64) {
-      int r, d;
-      const bool pair = take(i, r, d);
-      most = sb_size(x, 8, most);
-      if (pair) most = sb_size(y, 8, most);
+    had = anew ? 0 : *scale;
+#pragma unroll
+    for (int e = 0; e < ITEMS; ++e) {
+      if (r[e] < 0) continue;
+      const uint16_t* p = rows + r[e] * stride + d[e];
+      x[e] = *reinterpret_cast<const uint4*>(p);
+      if (!SIDE && 2 * d[e] < rot) y[e] = *reinterpret_cast<const uint4*>(p + (rot >> 1));
     }
-    const int need = sb_need(dpp_max_u32(most)), now = anew ? need : max(had, need);
+  };
+  int unit = part * per + (shared ? 0 : wave);
+  if (unit < 2 * a.Hkv) load(unit);
+  if (part * per < a.Hkv) {                                // a K is among the units
+    for (int i = threadIdx.x; i < R * half; i += 256) {
+      const int r = i / half, j = i - r * half;
+      const double t = (double)a.positions[n + r] * a.turns[j], f = t - rint(t);   // -1/2 .. 1/2 turns
+      // sine and cosine of what 32 bits hold of the angle, and a first-order step for the rest
+      const float hi = (float)f, lo = (float)((f - (double)hi) * 6.283185307179586);
+      float sn, cs;
+      sincospif(2.0f * hi, &sn, &cs);
+      room.cos[i] = (cs - sn * lo) * a.magnitude, room.sin[i] = (sn + cs * lo) * a.magnitude;
+    }
+    lds_barrier();
+  }
+
+  int turn = 0;
+  // the largest of a value over the unit's threads
+  auto over_unit = [&](uint32_t most) __attribute__((always_inline)) {
+    most = dpp_max_u32(most);
+    if (shared) {
+      if (lane == 0) room.most[turn][wave] = most;
+      lds_barrier();
+      most = max(max(room.most[turn][0], room.most[turn][1]), max(room.most[turn][2], room.most[turn][3]));
+      turn ^= 1;                                           // what it is written to next has been read by then
+    }
+    return (uint32_t)__builtin_amdgcn_readfirstlane(most);
+  };
+#pragma unroll 1
+  for (; unit < 2 * a.Hkv; unit += per * parts) {          // all waves of the block alike where units are shared
+    float f[ITEMS][8], g[ITEMS][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < ITEMS; ++e) {
+      if (r[e] < 0) continue;
+      ap_unpack(x[e], f[e]);
+      if (!SIDE && 2 * d[e] < rot) {
+        ap_unpack(y[e], g[e]);
+        ap_turn(f[e], g[e], room.cos + r[e] * half + d[e], room.sin + r[e] * half + d[e]);
+        top = sb_size(g[e], top);
+      } else if (SIDE && d[e] < rot) {
+        ap_turn_side(f[e], room.cos + r[e] * half + d[e] / 2, room.sin + r[e] * half + d[e] / 2);
+      }
+      top = sb_size(f[e], top);
+    }
+    asm volatile("" : "+v"(had));                          // the byte has come to every thread before one may write it
+    uint32_t most = over_unit(__float_as_uint(top) & 0x7FFFFFFFu);
+    bool over = most > 0x7F600000u;                        // past 448 * 2^119
+    if (most >= 0x7F800000u) {
+      most = 0;
+#pragma unroll
+      for (int e = 0; e < ITEMS; ++e) {
+        if (r[e] < 0) continue;
+        most = sb_finite_size(f[e], most);
+        if (!SIDE && 2 * d[e] < rot) most = sb_finite_size(g[e], most);
+      }
+      most = over_unit(most);
+    }
+    const int need = sb_need(most), now = anew ? need : max(had, need);
     if (!anew && now > had) {
       const float by = sb_power(had - now);
       const int cells = D >> 4;
-      for (int i = lane; i < SB_ROWS * cells; i += 64) {
-        const int r = i / cells;
-        if (used >> r & 1u) continue;
+      for (int i = me; i < SB_ROWS * cells; i += T) {
+        if (used >> (i / cells) & 1u) continue;
         uint4* p = reinterpret_cast<uint4*>(codes + 16 * i);
         const uint4 w = *p;
         *p = make_uint4(sb_rescale(w.x, by), sb_rescale(w.y, by), sb_rescale(w.z, by), sb_rescale(w.w, by));
       }
     }
-    if (lane == 0 && (anew || now > had)) *scale = (uint8_t)now;
+    if (me == 0 && (anew || now > had)) *scale = (uint8_t)now;
     const float inverse = sb_power(127 - now);
-    for (int i0 = 0; i0 < R * P; i0 += 64) {
-      const int i = i0 + lane;
-      int r = 0, d = 0;
-      const bool there = i < R * P;
-      const bool pair = there && take(i, r, d);
-      const int to = __shfl(place, r, 64);
-      if (!there) continue;
-      *reinterpret_cast<uint2*>(codes + to * D + d) = sb_pack(x, inverse);
-      if (pair) *reinterpret_cast<uint2*>(codes + to * D + d + (rot >> 1)) = sb_pack(y, inverse);
+#pragma unroll
+    for (int e = 0; e < ITEMS; ++e) {
+      const int to = __shfl(slots, max(r[e], 0), 64) & (SB_ROWS - 1);
+      if (r[e] < 0) continue;
+      *reinterpret_cast<uint2*>(codes + to * D + d[e]) = sb_pack(f[e], inverse, over);
+      if (!SIDE && 2 * d[e] < rot) *reinterpret_cast<uint2*>(codes + to * D + d[e] + (rot >> 1)) = sb_pack(g[e], inverse, over);
     }
+    if (unit + per * parts < 2 * a.Hkv) load(unit + per * parts);
   }
 }
 
-// Blocks 0 .. kv - 1 look at rows for blocks to write, consecutive ones at rows 16 apart (a long chunk's blocks begin every
-// 16 rows: in the order of the rows they would all fall on one XCD); the rest are the q rows'.
+// Blocks 0 .. kv - 1 look at W rows each (a power of two up to 16) for those that a block of slots begins at, consecutive
+// blocks at rows 16 apart: a long chunk's begin every 16 rows, and in the order of the rows would fall on few XCDs.  The rest
+// are the q rows'.
 template <bool SIDE>
-__global__ void __launch_bounds__(256) cache_append_scaled_kernel(AppendArgs a, int parts, int q_parts) {
-  __shared__ float s_cos[SB_ROWS * AP_MAX_ROT / 2], s_sin[SB_ROWS * AP_MAX_ROT / 2];
-  const int C = (a.N + SB_ROWS - 1) / SB_ROWS, kv = SB_ROWS * C * parts, b = blockIdx.x;
-  if (b < kv) {
-    const int w = b / parts, n = w % C * SB_ROWS + w / C;
-    if (n < a.N) ap_run<SIDE>(a, n, b - w * parts, parts, s_cos, s_sin);
-  } else {
+__global__ void __launch_bounds__(256, 4) cache_append_scaled_kernel(AppendArgs a, int W, int parts, int q_parts) {
+  __shared__ RunRoom room;
+  const int C = (a.N + SB_ROWS - 1) / SB_ROWS, kv = SB_ROWS / W * C * parts, b = blockIdx.x;
+  if (b >= kv) {
     const int n = (b - kv) / q_parts;
-    ap_token<AP_Q, SIDE>(a, n, b - kv - n * q_parts, q_parts, s_cos, s_sin);
+    return ap_token<AP_Q, SIDE>(a, n, b - kv - n * q_parts, q_parts, room.cos, room.sin);
+  }
+  const int x = b / parts, n0 = x % C * SB_ROWS + x / C * W, lane = threadIdx.x & 63;
+  if (n0 >= a.N) return;
+  // lane l: row n0 - 1 + l, up to the 16 rows behind the last
+  const int at = n0 - 1 + lane;
+  const int slot = lane <= W + SB_ROWS && at >= 0 && at < a.N ? a.slots[at] : -1, before = __shfl_up(slot, 1, 64);
+  const bool mine = lane >= 1 && lane <= W;
+  if (mine && slot >= a.n_slots && threadIdx.x < 64 && a.status) a.status[0] = MIMO_ERR_SLOT;
+  uint64_t first = __ballot(mine && slot >= 0 && slot < a.n_slots && slot >> SB_SHIFT != before >> SB_SHIFT);
+  for (bool again = false; first; first &= first - 1, again = true) {
+    const int l = __builtin_ctzll(first);
+    if (again) lds_barrier();                            // the last block's angles have been read
+    ap_run<SIDE>(a, n0 - 1 + l, __shfl(slot, min(lane + l, 63), 64), b - x * parts, parts, room);
   }
 }
 
@@ -629,10 +709,14 @@ int mimo_cache_append_rotary(const uint16_t* q, int64_t q_stride, int heads, con
   {
     ProfScope p(st, "cache_append");
     if (scaled) {
-      const int parts = std::max(1, std::min((cache->kv_heads + 1) / 2, AP_BLOCKS / N)), q_parts = spread(heads * per / 8);
-      const int64_t grid = (int64_t)(N + SB_ROWS - 1) / SB_ROWS * SB_ROWS * parts + (q ? (int64_t)N * q_parts : 0);
-      if (side) cache_append_scaled_kernel<true><<<(unsigned)grid, 256, 0, st>>>(a, parts, q_parts);
-      else cache_append_scaled_kernel<false><<<(unsigned)grid, 256, 0, st>>>(a, parts, q_parts);
+      // four units of a block of slots to a block (two: 15.3 us for the pieces, one 18.8); W rows to look at
+      const int q_parts = spread(heads * per / 8);
+      int parts = (cache->kv_heads + 1) / 2, W = 1;
+      while (W < SB_ROWS && (int64_t)N * parts > (int64_t)W * SB_BLOCKS) W *= 2;
+      parts = std::max(1, std::min(parts, SB_BLOCKS * SB_ROWS / N));
+      const int64_t grid = (int64_t)((N + SB_ROWS - 1) / SB_ROWS) * (SB_ROWS / W) * parts + (q ? (int64_t)N * q_parts : 0);
+      if (side) cache_append_scaled_kernel<true><<<(unsigned)grid, 256, 0, st>>>(a, W, parts, q_parts);
+      else cache_append_scaled_kernel<false><<<(unsigned)grid, 256, 0, st>>>(a, W, parts, q_parts);
     } else {
       const int units = ((q ? heads : 0) * per + cache->kv_heads * (per + cache->v_dim)) / 8;
       const dim3 grid(N, spread(units));
