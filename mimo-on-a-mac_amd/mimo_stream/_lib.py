@@ -114,6 +114,24 @@ def load():
     return _lib
 
 
+_calls = None
+
+
+def calls():
+    """The module of the short host paths (csrc/calls.cpp), bound to the library's entry points; raises if it has not been built."""
+    global _calls
+    if _calls is None:
+        lib = load()
+        try:
+            from . import _calls as module
+        except ImportError as e:
+            raise RuntimeError(f"mimo_stream/_calls.so is not built or not loadable ({e}); run __graft_entry__.build()") from e
+        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "mimo_cache_append_rotary", "mimo_cache_read", "mimo_cache_attend", "mimo_cache_attend_workspace_size")))
+        _calls = module
+    return _calls
+
+
 def check(rc, what=""):
     if rc == MIMO_OK:
         return

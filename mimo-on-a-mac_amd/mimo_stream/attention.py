@@ -12,6 +12,7 @@ batch: requests decoding one token and requests with a chunk of new tokens, in o
 the device, nothing synchronises, and every call can be captured into a HIP graph; a step's one plan serves every layer.
 For inference: no output carries a gradient.
 """
+import ctypes
 import functools
 import math
 from dataclasses import dataclass
@@ -31,12 +32,21 @@ STATUS_MESSAGES = {_lib.ERR_PAGES: "fewer free pages than the step needs",
                    _lib.ERR_SLOT: "a page or slot outside the cache"}
 
 # A decode step makes one step call and two calls per layer, each of a few microseconds on the GPU: what they do on the host
-# is kept short (one check per tensor, entry points and structs looked up once).
+# is kept short.  append, read and attend hand a call to _lib.calls() first, which takes it in its ordinary form (csrc/calls.cpp)
+# and answers NotImplemented for any other: then what stands here checks and converts the arguments one by one.
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 INT32_MAX = 0x7FFFFFFF                                   # ctypes takes the low bits of larger numbers without a word
+
+
+def _taken(code, name):
+    """What a short path answered, if it made the call; a code of the library's raises."""
+    if type(code) is int:
+        _lib.check(code, name)
+    return code
 
 
 def _device(device):
@@ -242,6 +252,10 @@ class KVCache:
         self.kv_heads, self.k_dim, self.v_dim, self.page_size, self.n_pages = heads, k_dim, v.shape[3], page, n_pages
         self.block_scales = kind == _lib.KV_E4M3_BLOCKS
         self._struct = _lib.MimoKvCache(*(_lib.ptr(t) for t in self._tensors), kind, n_pages, page, heads, k_dim, v.shape[3])
+        self._calls = self._call = None
+        if k.device.type == "cuda":
+            self._calls = _lib.calls()
+            self._call = self._calls.cache(ctypes.addressof(self._struct), k.device.index)
 
     k = property(lambda self: self._tensors[0])
     v = property(lambda self: self._tensors[1])
@@ -287,6 +301,8 @@ class Rotary:
                 raise ValueError(f"frequencies: need {dim // 2} finite numbers, got shape {tuple(frequencies.shape)}")
         self._turns = (frequencies / (2.0 * math.pi)).to(_device(device))
         self._struct = _lib.MimoRotary(self._turns.data_ptr(), self.dim, self.interleaved, self.magnitude)
+        self._at = ctypes.addressof(self._struct)
+        self._index = self._turns.device.index if self._turns.is_cuda else -1
 
     turns = property(lambda self: self._turns)               # fixed: the struct holds its address
 
@@ -322,6 +338,11 @@ def append(cache, plan, k, v, q=None, rotary=None):
     scale of each head grows where the new values need it, and what the block holds is kept: exactly, but for values below
     2 ** -6 of the new scale, which are rounded to 2 ** -9 of it.  Values past 448 * 2 ** 119 saturate, infinities among
     them."""
+    if cache._call is not None and (rotary is None or rotary.dim <= cache.k_dim):
+        done = cache._calls.append(cache._call, _current_device(), _raw_stream(cache.device.index), plan.slots, plan.positions, plan.status,
+                                   plan.page_size, k, v, q, 0 if rotary is None else rotary._at, -1 if rotary is None else rotary._index)
+        if done is not NotImplemented:
+            return _taken(done, "mimo_cache_append")
     _same_pages(plan, cache)
     dev = cache.device
     index = _gpu(dev)
@@ -365,6 +386,10 @@ def read(cache, slots, out=None, status=None):
     PageTable.slots; in any order, any slot any number of times), stored values times their scales, rounded once; rows of
     slot -1 are 0.  Keys are as append left them, rotated.  out: two contiguous bf16 tensors to write; status: int32 [1] that
     receives a failure (a slot past the cache, whose row is 0) as plan.status does."""
+    if cache._call is not None and out is None:
+        done = cache._calls.read(cache._call, _current_device(), _raw_stream(cache.device.index), slots, status)
+        if done is not NotImplemented:
+            return _taken(done, "mimo_cache_read")
     dev = cache.device
     index = _gpu(dev)
     if _current_device() != index:
@@ -410,6 +435,15 @@ def attend(q, cache, plan, scale=None, window=0, sink_tokens=0, sink_logits=None
     product with v, else 8: a decoding request beside a chunk differs by that rounding.  sink_logits fp32 [heads]: a logit
     that joins each row's softmax without a value.  Returns bf16 [N, heads, v_dim] (out, if given: contiguous bf16); rows of
     no request are 0."""
+    if cache._call is not None and not _capturing():
+        index = cache.device.index
+        stream = _raw_stream(index)
+        ws = _lib._ws.get((index, stream, "attend"))
+        if ws is not None:
+            done = cache._calls.attend(cache._call, _current_device(), stream, q, plan.starts, plan.lens, plan.table, plan.max_new,
+                                       plan.status, plan.page_size, scale, window, sink_tokens, sink_logits, out, ws)
+            if done is not NotImplemented:
+                return _taken(done, "mimo_cache_attend")
     if not (0 <= window <= INT32_MAX and 0 <= sink_tokens <= INT32_MAX):
         raise ValueError(f"window and sink_tokens must be from 0 to 2^31 - 1 (got {window}, {sink_tokens})")
     _same_pages(plan, cache)
