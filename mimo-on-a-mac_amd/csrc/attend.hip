@@ -51,6 +51,7 @@ namespace mimo {
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef int v2i __attribute__((ext_vector_type(2)));
+typedef int v8i __attribute__((ext_vector_type(8)));
 
 struct AttendArgs {
   const uint16_t* q;
@@ -86,6 +87,7 @@ constexpr int AT_START = 8;                               // units that a wide b
 template <int DK_, int DV_, int DTYPE, bool WIDE_> struct AtCfg {
   static constexpr int DK = DK_, DV = DV_;
   static constexpr bool F8 = DTYPE != MIMO_KV_BF16, BS = DTYPE == MIMO_KV_E4M3_BLOCKS, HS = F8 && !BS, WIDE = WIDE_;
+  static constexpr bool QP = BS && WIDE;                   // q as two E4M3 planes
   static constexpr int CBB = F8 ? 64 : 128;                // bytes of a row in one 64-element column block
   static constexpr int KCB = DK / 64, VCB = DV / 64;
   static constexpr int KEYS = WIDE ? 64 : 32;              // keys of one LDS tile (narrow: one wave's)
@@ -430,18 +432,61 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   c = zero ? 1.0f : fabsf(c);
   uint4 qraw[C::DK / 16];
   {
-    const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + qt) * a.q_stride + head * C::DK + (C::F8 ? 16 : 8) * h;
+    const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + qt) * a.q_stride + head * C::DK + (C::QP ? 32 : C::F8 ? 16 : 8) * h;
 #pragma unroll
     for (int s = 0; s < C::DK / 16; ++s) {
       qraw[s] = make_uint4(0, 0, 0, 0);
-      if (valid && !zero) qraw[s] = *reinterpret_cast<const uint4*>(qp + (C::F8 ? 32 * (s >> 1) + 8 * (s & 1) : 16 * s));
+      if (valid && !zero) qraw[s] = *reinterpret_cast<const uint4*>(qp + (C::QP ? 64 * (s >> 2) + 8 * (s & 3) : C::F8 ? 32 * (s >> 1) + 8 * (s & 1) : 16 * s));
     }
   }
-  bf16x8 Q[C::DK / 16];
+  bf16x8 Q[C::QP ? 1 : C::DK / 16];
+  // Wide, block scales: E4M3 products with scales (v_mfma_scale_f32_32x32x64_f8f6f4), whose K operand is the cache's codes and bytes as
+  // they are: 4096 tokens at 8192, 64/4 heads of 192/128 1611 us, 1721 with K turned into bf16 by every wave.  (Narrow tiles would
+  // wait for the planes: 128 windowed decodes 29.0 us instead of 23.5.)  q is two planes of E4M3, Qp[0] and Qp[1], the second what the first's rounding leaves, times 16: 8 bits in all,
+  // bf16's own, for values down to 2^-13 of the largest of their 64 dimensions (smaller ones are off by up to 2^-21 of that).
+  // q_by: bytes of the planes' scales.
+  v8i Qp[2][C::QP ? C::KCB : 1];
+  int q_by[C::QP ? C::KCB : 1];
+  bool q_odd = false;                                      // infinities or NaN: these planes do not hold them apart
   auto take_q = [&]() __attribute__((always_inline)) {     // once the first copies are on their way
+    if constexpr (C::QP) {
 #pragma unroll
-    for (int s = 0; s < C::DK / 16; ++s)
-      Q[s] = __builtin_bit_cast(bf16x8, make_uint4(qraw[s].x ^ flip, qraw[s].y ^ flip, qraw[s].z ^ flip, qraw[s].w ^ flip));
+      for (int b = 0; b < C::KCB; ++b) {
+        uint32_t most = 0;                                 // as bf16 bits
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 w = qraw[4 * b + i];
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) most = max(most, max(u[k] & 0x7FFFu, u[k] >> 16 & 0x7FFFu));
+        }
+        most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));   // one scale for a row's 64, whichever lane holds which
+        q_odd |= most >= 0x7F80u;
+        const int X = fp8_block_exp(__uint_as_float(most << 16));
+        const float by = exp2i(-max(X, -122));             // X - 4 is a byte too
+        q_by[b] = (max(X, -122) + 127) | (max(X, -122) + 123) << 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 w = qraw[4 * b + i];
+          const uint32_t u[4] = {w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip};
+#pragma unroll
+          for (int k = 0; k < 4; k += 2) {
+            const float x0 = __uint_as_float(u[k] << 16) * by, x1 = __uint_as_float(u[k] & 0xFFFF0000u) * by;
+            const float x2 = __uint_as_float(u[k + 1] << 16) * by, x3 = __uint_as_float(u[k + 1] & 0xFFFF0000u) * by;
+            int w0 = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
+            w0 = __builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, w0, true);
+            const v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8(w0, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w0, true);
+            int w1 = __builtin_amdgcn_cvt_pk_fp8_f32((x0 - lo.x) * 16.0f, (x1 - lo.y) * 16.0f, 0, false);
+            w1 = __builtin_amdgcn_cvt_pk_fp8_f32((x2 - hi.x) * 16.0f, (x3 - hi.y) * 16.0f, w1, true);
+            Qp[0][b][2 * i + k / 2] = w0, Qp[1][b][2 * i + k / 2] = w1;
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < C::DK / 16; ++s)
+        Q[s] = __builtin_bit_cast(bf16x8, make_uint4(qraw[s].x ^ flip, qraw[s].y ^ flip, qraw[s].z ^ flip, qraw[s].w ^ flip));
+    }
   };
   const int pos = base_pos + qt;                           // this lane's position
   const int w_first = C::WIDE ? 32 * wave / a.HT : 0, w_last = min(toks - 1, ((C::WIDE ? 32 * wave : 0) + 31) / a.HT);
@@ -470,9 +515,10 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   };
   // Block scales of the tile in hand: of this lane's key in each block of 32, and of each group of 16 keys.  Narrow tiles'
   // groups are the wave's own; of a wide tile each wave has loaded one group's bytes, and passes them on through LDS.
-  float k_by[C::NB], v_by[2 * C::NB];
+  uint32_t k_by[C::NB];                                    // wide: bytes, narrow: powers of two as bits
+  float v_by[2 * C::NB];
 #pragma unroll
-  for (int i = 0; i < C::NB; ++i) k_by[i] = v_by[2 * i] = v_by[2 * i + 1] = 1.0f;
+  for (int i = 0; i < C::NB; ++i) k_by[i] = __float_as_uint(1.0f), v_by[2 * i] = v_by[2 * i + 1] = 1.0f;
   constexpr int ES = C::F8 ? 1 : 2;
   auto issue_k = [&](uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
@@ -495,7 +541,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
 
   // operand addresses in a tile: K row r32, cell 2 s + h; V as the transposing reads want them
   const int i16 = lane & 15, d16 = (lane >> 4) & 1;
-  const int k_at = C::F8 ? r32 * 64 + 16 * (h ^ ((r32 >> 2) & 3)) : r32 * 128 + 16 * (h ^ ((r32 >> 1) & 7));
+  const int k_at = C::F8 ? r32 * 64 + 16 * ((C::QP ? 2 * h : h) ^ ((r32 >> 2) & 3)) : r32 * 128 + 16 * (h ^ ((r32 >> 1) & 7));
   const int v_row = C::F8 ? 4 * h + ((i16 >> 1) & 3) + 8 * (i16 >> 3) : 4 * h + (i16 >> 2);
   const int v_at = C::F8 ? v_row * 64 + 16 * (d16 ^ ((v_row >> 2) & 3)) + 8 * (i16 & 1)
                          : v_row * 128 + 16 * ((2 * d16 + ((i16 >> 1) & 1)) ^ (4 * ((v_row >> 1) & 1))) + 8 * (i16 & 1);
@@ -532,7 +578,32 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   bf16x8 P[C::NB][2], rest[C::WIDE ? 1 : C::NB][2];        // narrow: what the rounding of P leaves off, rounded
   // operands are read PX products ahead; the barriers keep the compiler from reading them all at once (spilled registers)
   constexpr int PX = 4;
+  auto scores_of_codes = [&](const uint8_t* st) __attribute__((always_inline)) {
+    constexpr int F = C::NB * C::KCB, AHEAD = 2;           // blocks of 64 dimensions and 32 keys; lane: 32 of a key's codes
+    v8i X[AHEAD];
+    auto read = [&](int f) __attribute__((always_inline)) {
+      const uint8_t* p = st + f / C::NB * (C::KEYS * 64) + f % C::NB * 32 * 64;
+      const uint4 x = *reinterpret_cast<const uint4*>(p + k_at), y = *reinterpret_cast<const uint4*>(p + (k_at ^ 16));
+      return v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+    };
+#pragma unroll
+    for (int f = 0; f < AHEAD && f < F; ++f) X[f] = read(f);
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const int kb = f % C::NB, b = f / C::NB;
+      __builtin_amdgcn_sched_barrier(0);
+      const v16f none = {0.0f};
+      S[kb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(X[f % AHEAD], Qp[0][b], b == 0 ? none : S[kb], 0, 0, 0, k_by[kb], 0, q_by[b]);
+      S[kb] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(X[f % AHEAD], Qp[1][b], S[kb], 0, 0, 0, k_by[kb], 1, q_by[b]);
+      if (f + AHEAD < F) X[f % AHEAD] = read(f + AHEAD);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // these products run 16 passes; the sums are read no sooner than 20 wait states after the last
+    asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
   auto scores = [&](const uint8_t* st) __attribute__((always_inline)) {
+    if constexpr (C::QP) return scores_of_codes(st);
     constexpr int PER = C::F8 ? 2 : 1, F = C::NB * C::DK / (16 * PER);   // products per read
     uint4 X[PX];
 #pragma unroll
@@ -544,8 +615,8 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       const v16f none = {0.0f};
       const uint4 x = X[f % PX];
       if constexpr (C::F8) {
-        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.x, x.y, k_by[kb]), Q[2 * s], s == 0 ? none : S[kb], 0, 0, 0);
-        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.z, x.w, k_by[kb]), Q[2 * s + 1], S[kb], 0, 0, 0);
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.x, x.y, __uint_as_float(k_by[kb])), Q[2 * s], s == 0 ? none : S[kb], 0, 0, 0);
+        S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(at_f8_bf16x8(x.z, x.w, __uint_as_float(k_by[kb])), Q[2 * s + 1], S[kb], 0, 0, 0);
       } else {
         S[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, x), Q[s], s == 0 ? none : S[kb], 0, 0, 0);
       }
@@ -635,14 +706,13 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       const int cur = (it - it0) & 1, g0 = it * UG;
       if (it + 1 < it1) look(it + 1);
       uint32_t* sc = reinterpret_cast<uint32_t*>(lds + C::SCALES) + 8 * cur;
-      if (C::BS && lane == 0) sc[wave] = next_scales[0].x << 23, sc[4 + wave] = next_scales[0].y << 23;
+      if (C::BS && lane == 0) sc[wave] = next_scales[0].x, sc[4 + wave] = next_scales[0].y << 23;
       at_wait_vm(0);
       __syncthreads();                                     // the tile has landed everywhere; the other one is free
       if constexpr (C::BS) {                               // on their way while the copies are asked for
-        const float* by = reinterpret_cast<const float*>(sc);
-        k_by[0] = by[r32 >> 4], k_by[1] = by[2 + (r32 >> 4)];
+        k_by[0] = sc[r32 >> 4], k_by[1] = sc[2 + (r32 >> 4)];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v_by[i] = by[4 + i];
+        for (int i = 0; i < 4; ++i) v_by[i] = __uint_as_float(sc[4 + i]);
       }
       if (it + 1 < it1) {
         rows_of();
@@ -671,7 +741,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       const bool more = it + 1 < end;
       if (more) look(it + 1);
       if constexpr (C::BS) {
-        k_by[0] = e8m0_f32(r32 < 16 ? next_scales[0].x : next_scales[1].x);
+        k_by[0] = (r32 < 16 ? next_scales[0].x : next_scales[1].x) << 23;
         v_by[0] = e8m0_f32(next_scales[0].y), v_by[1] = e8m0_f32(next_scales[1].y);
       }
       at_wait_vm(NV);
@@ -721,6 +791,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       }
       suspect = __ballot(odd) != 0;
     }
+    if constexpr (C::QP) suspect |= __ballot(busy && q_odd) != 0;
   }
   const float vs = C::HS ? static_cast<const float*>(a.v_scale)[kv] : 1.0f;
   // the wave's rows once more, one by one; done(row, place of the row, its head, O, m, l)

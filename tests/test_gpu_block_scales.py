@@ -613,3 +613,47 @@ def test_calls_on_another_stream(rng):
         got, again = attend(q, cache, plan, **kw), read(cache, i32(np.arange(0, 160, 3)))
     other.synchronize()
     assert torch.equal(got, want) and torch.equal(again[0].view(torch.int16), rows[0].view(torch.int16))
+
+
+@pytest.mark.parametrize("dims", list(DIMS))
+@pytest.mark.parametrize("what", ["nan", "inf", "-inf"])
+def test_attend_queries_that_are_not_finite(rng, dims, what):
+    """A query that holds a NaN or an infinity makes its own row what the formula makes it, and no other."""
+    q, cache, plan, kw = _attend_case(rng, [150, 40], [70, 33], 4, 2, *DIMS[dims], 16, window=30)
+    q[5, 1, 7] = q[80, 2, 63] = float(what)
+    x = torch.full((q.shape[0], 4, cache.v_dim), -1.0, dtype=BF, device="cuda")
+    attend(q, cache, plan, out=x, **kw)
+    plan.check()
+    clean = q.clone()
+    clean[5, 1, 7] = clean[80, 2, 63] = 0.0
+    want = attend(clean, cache, plan, **kw)
+    others = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+    others[5, 1] = others[80, 2] = False
+    # the rows beside it may be taken again in 32 bits: both within the rounding of weights and output of the same value
+    assert torch.isfinite(x[others]).all() and (x[others].float() - want[others].float()).abs().max() <= 2.0 ** -5
+    if what == "nan":
+        assert torch.isnan(x[5, 1]).all() and torch.isnan(x[80, 2]).all()
+    else:
+        k, v = _values(cache)
+        ref, _ = oa.attend(f64(q), k, v, plan.starts.cpu().numpy(), plan.lens.cpu().numpy(), plan.table.cpu().numpy(), cache.k_dim ** -0.5, 30)
+        got = f64(x)
+        for n, h in ((5, 1), (80, 2)):
+            assert np.array_equal(np.isnan(got[n, h]), np.isnan(ref[n, h]))
+
+
+@pytest.mark.parametrize("dims", list(DIMS))
+@pytest.mark.parametrize("new", [1, 50])
+def test_attend_queries_of_far_sizes(rng, dims, new):
+    """Dimensions of a query from 2^-12 of its largest up: every one counts, against keys that weigh the small ones more."""
+    q, cache, plan, kw = _attend_case(rng, [90], [new], 4, 2, *DIMS[dims], 16)
+    Dk = DIMS[dims][0]
+    small = 2.0 ** -rng.integers(0, 12, (q.shape[0], 4, Dk))
+    q.copy_(torch.from_numpy((rng.standard_normal(q.shape) * small).astype(np.float32)).to(BF))
+    _check(q, cache, plan, kw, scale=0.2, few=new == 1)
+    tiny = (q.float() * 2.0 ** -100).to(BF)                # the same far below 1, and a scale that takes it back
+    _check(tiny, cache, plan, kw, scale=0.2 * 2.0 ** 100, few=new == 1)
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_attend_scales_of_either_sign(rng, scale):
+    _check(*_attend_case(rng, [150, 40], [70, 33], 4, 2, 192, 128, 16), scale=scale)
