@@ -240,7 +240,7 @@ typedef struct mimo_kv_cache {
   void* k;                 /* [n_pages, kv_heads, page_size, k_dim] bf16 or E4M3 */
   void* v;                 /* [n_pages, kv_heads, page_size, v_dim] */
   const void* k_scale;     /* E4M3: fp32 [kv_heads]; E4M3_BLOCKS: bytes [n_pages, kv_heads, page_size / 16], 16-byte aligned, */
-  const void* v_scale;     /*   readable up to the next multiple of 4 bytes, written by append */
+  const void* v_scale;     /*   readable up to the next multiple of 4 bytes, written by append, apart from one another */
   int32_t dtype, n_pages, page_size, kv_heads, k_dim, v_dim;
 } mimo_kv_cache;
 
@@ -277,7 +277,7 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
 /* mimo_cache_append with the rotation in full (NULL: none): pairs (i, i + dim / 2), or (2 i, 2 i + 1) where interleaved is 1;
  * turns fp64 [dim / 2] as above (a host may stretch them for long contexts); rotated values times magnitude (finite; 1: as
  * they are).  Into a cache with block scales (either entry; N up to 2^23 - 17): the rows of one block of 16 slots have to
- * follow one another, as a step lays a request's tokens.  A call that writes a block's first slot begins the block anew,
+ * follow one another, as a step lays a request's tokens, with no other row between them, not even one of a slot below 0.  A call that writes a block's first slot begins the block anew,
  * whatever it held; else its byte grows if the new values need it, and what the block held is kept, in the new scale.  Values
  * past 448 * 2^119 saturate.  status also receives MIMO_ERR_SLOT for a slot that follows itself; if a block's rows do not stand
  * together that block's contents are undefined, and nothing else is touched. */

@@ -616,6 +616,9 @@ int check_cache(const mimo_kv_cache* c, const char* what) {
   MIMO_REQUIRE(aligned16(c->k) && aligned16(c->v), MIMO_ERR_ALIGN, "%s: 16-byte alignment", what);
   MIMO_REQUIRE(c->dtype != MIMO_KV_E4M3_BLOCKS || (aligned16(c->k_scale) && aligned16(c->v_scale)), MIMO_ERR_ALIGN,
                "%s: 16-byte alignment of the block scales", what);
+  const size_t scales = (size_t)c->n_pages * c->kv_heads * (c->page_size / 16);
+  MIMO_REQUIRE(c->dtype != MIMO_KV_E4M3_BLOCKS || !overlap(c->k_scale, scales, c->v_scale, scales), MIMO_ERR_ARG,
+               "%s: k_scale and v_scale overlap: a block scale belongs to K or to V", what);
   return MIMO_OK;
 }
 

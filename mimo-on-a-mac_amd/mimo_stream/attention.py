@@ -240,6 +240,8 @@ class KVCache:
                 raise ValueError("k_scale and v_scale of two kinds")
             if blocks[0]:
                 k_scale, v_scale = (_block_scales(s, k.device, (n_pages, heads, page // 16)) for s in (k_scale, v_scale))
+                if abs(k_scale.data_ptr() - v_scale.data_ptr()) < k_scale.numel():
+                    raise ValueError("k_scale and v_scale overlap: a block scale belongs to K or to V")
                 kind = _lib.KV_E4M3_BLOCKS
             else:
                 k_scale, v_scale = (torch.as_tensor(s, dtype=torch.float32, device=k.device).expand(heads).contiguous()
@@ -333,8 +335,8 @@ def append(cache, plan, k, v, q=None, rotary=None):
     out), k rotated to plan.positions; returns q [N, heads, k_dim] rotated likewise (None without q).  q, k and v may be
     views of one projection's rows; other types than bf16 are rounded to it first.  Slots are distinct.
 
-    Into a cache with block scales, the rows of one block of 16 slots follow one another, as in the plan of a step (a block
-    whose rows do not has undefined contents).  A call that writes a block's first slot begins the block anew; in another the
+    Into a cache with block scales, the rows of one block of 16 slots follow one another, as in the plan of a step, with no
+    other row between them, not even one that is left out (a block whose rows do not has undefined contents).  A call that writes a block's first slot begins the block anew; in another the
     scale of each head grows where the new values need it, and what the block holds is kept: exactly, but for values below
     2 ** -6 of the new scale, which are rounded to 2 ** -9 of it.  Values past 448 * 2 ** 119 saturate, infinities among
     them."""

@@ -29,6 +29,8 @@ def test_block_scaled_cache_arguments():
             KVCache(3, page, 2, 64, 64, dtype=E4M3, block_scales=True, device="cpu")
     with pytest.raises(ValueError, match="two kinds"):
         KVCache.of(c.k, c.v, c.k_scale, 1.0)
+    with pytest.raises(ValueError, match="overlap"):
+        KVCache.of(c.k, c.v, c.k_scale, c.k_scale)
     for bad in (c.k_scale[:, :, :1], c.k_scale.float(), c.k_scale.transpose(0, 1), torch.zeros(13, dtype=torch.uint8)[1:].view(3, 2, 2)):
         with pytest.raises(ValueError, match="block scales"):
             KVCache.of(c.k, c.v, bad, c.v_scale)
@@ -83,7 +85,7 @@ OUT = ADDR + 32768
 
 
 def _kv(**kw):
-    f = dict(k=ADDR, v=ADDR, k_scale=ADDR, v_scale=ADDR, dtype=2, n_pages=2, page_size=16, kv_heads=2, k_dim=64, v_dim=64)
+    f = dict(k=ADDR, v=ADDR, k_scale=ADDR, v_scale=ADDR + 16, dtype=2, n_pages=2, page_size=16, kv_heads=2, k_dim=64, v_dim=64)
     f.update(kw)
     return _lib.MimoKvCache(*(f[n] for n, _ in _lib.MimoKvCache._fields_))
 
@@ -104,7 +106,7 @@ def test_append_refusals(bad, code):
 
 
 BAD_CACHES = [(dict(k_scale=None), "ARG"), (dict(v_scale=None), "ARG"), (dict(dtype=3), "ARG"), (dict(dtype=-1), "ARG"), (dict(k_scale=ADDR + 4), "ALIGN"),
-              (dict(v_scale=ADDR + 1), "ALIGN"), (dict(page_size=8), "SHAPE"), (dict(v_dim=128), "SHAPE"), (dict(k=None), "ARG")]
+              (dict(v_scale=ADDR + 1), "ALIGN"), (dict(v_scale=ADDR), "ARG"), (dict(v_scale=ADDR + 16, n_pages=9), "ARG"), (dict(page_size=8), "SHAPE"), (dict(v_dim=128), "SHAPE"), (dict(k=None), "ARG")]
 
 
 def _read(cache=None, **kw):
