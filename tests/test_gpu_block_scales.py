@@ -658,3 +658,53 @@ def test_attend_queries_of_far_sizes(rng, dims, new):
 @pytest.mark.parametrize("scale", [-0.1, 0.0])
 def test_attend_scales_of_either_sign(rng, scale):
     _check(*_attend_case(rng, [150, 40], [70, 33], 4, 2, 192, 128, 16), scale=scale)
+
+
+@pytest.mark.parametrize("heads,N,piece", [(1, 40000, 997), (2, 5000, 613), (9, 2100, 250)])
+def test_long_calls_are_their_pieces(rng, heads, N, piece):
+    """Calls of every number of rows that a block of threads may look at, bit for bit as in pieces that do not end with a block
+    of slots; values whose codes stay in the normal range under any scale they meet."""
+    D, page = 64, 64
+
+    def rows():
+        x = 2.0 ** rng.uniform(-3, 2.99, (N, heads, D)) * rng.choice([-1.0, 1.0], (N, heads, D))
+        return torch.from_numpy(x.astype(np.float32)).to(BF).cuda()
+    k, v = rows(), rows()
+    ends = np.minimum(np.arange(piece, N + piece, piece), N)
+    held = []
+    for cuts in ([N], ends):
+        n_pages = oa.pages(N, page) + 1
+        cache, pt, at = _empty(n_pages, page, heads, D, D), PageTable(1, n_pages, n_pages, page), 0
+        for end in cuts:
+            plan = pt.step(i32([end]), int(end) - at)
+            append(cache, plan, k[at:end], v[at:end])
+            plan.check()
+            at = int(end)
+        held.append((cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale))
+    assert all(torch.equal(a, b) for a, b in zip(*held))
+    got = read(cache, pt.slots(0, N))
+    assert ((got[0].float() - k.float()).abs() <= 2.0 ** -4 * k.float().abs()).all()
+    assert ((got[1].float() - v.float()).abs() <= 2.0 ** -4 * v.float().abs()).all()
+
+
+def test_a_padded_step(rng):
+    """Rows behind a step's last token: not written, their attention is 0, and what the cache holds beside them stays."""
+    cache, pt = _random_cache(rng, 6, 16, KV, DK, DV, 119, 124), PageTable(2, 3, 6, 16)
+    before = [t.view(torch.uint8).clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)]
+    plan = pt.step(i32([5, 17]), 40)
+    q, k, v = (torch.from_numpy(rng.standard_normal((40, h, d)).astype(np.float32)).to(BF).cuda() for h, d in ((HEADS, DK), (KV, DK), (KV, DV)))
+    q = append(cache, plan, k, v, q=q, rotary=Rotary(64))
+    out = attend(q, cache, plan)
+    plan.check()
+    assert not out[22:].any() and bool(out[:22].any())
+    written = torch.zeros(6 * 16, dtype=torch.bool, device="cuda")
+    written[plan.slots[:22].long()] = True
+    for t, old in ((cache.k, before[0]), (cache.v, before[1])):
+        now = t.view(torch.uint8).transpose(1, 2).flatten(0, 1)
+        assert torch.equal(now[~written], old.transpose(1, 2).flatten(0, 1)[~written])
+    blocks = torch.zeros(6, dtype=torch.bool, device="cuda")
+    blocks[plan.slots[:22].long() // 16] = True
+    for t, old in ((cache.k_scale, before[2]), (cache.v_scale, before[3])):
+        assert torch.equal(t[~blocks], old[~blocks])
+    none = pt.step(i32([5, 17]), 3)
+    assert not attend(q[:3].contiguous(), cache, none).any()
