@@ -279,8 +279,8 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
  * they are).  Into a cache with block scales (either entry; N up to 2^23 - 17): the rows of one block of 16 slots have to
  * follow one another, as a step lays a request's tokens, with no other row between them, not even one of a slot below 0.  A call that writes a block's first slot begins the block anew,
  * whatever it held; else its byte grows if the new values need it, and what the block held is kept, in the new scale.  Values
- * past 448 * 2^119 saturate.  status also receives MIMO_ERR_SLOT for a slot that follows itself; if a block's rows do not stand
- * together that block's contents are undefined, and nothing else is touched. */
+ * past 448 * 2^119 saturate.  If a block's rows do not stand together, or one slot comes twice, that block's contents are
+ * undefined, and nothing else is touched; status receives MIMO_ERR_SLOT where 15 or fewer rows lie between. */
 typedef struct mimo_rotary {
   const double* turns;
   int32_t dim, interleaved;

@@ -548,6 +548,10 @@ __global__ void __launch_bounds__(256, 4) cache_append_scaled_kernel(AppendArgs 
   uint64_t first = __ballot(mine && slot >= 0 && slot < a.n_slots && slot >> SB_SHIFT != before >> SB_SHIFT);
   for (bool again = false; first; first &= first - 1, again = true) {
     const int l = __builtin_ctzll(first);
+    // rows of this block that other rows part from it are in somebody else's care at the same time
+    const uint64_t all = __ballot(slot >> SB_SHIFT == __builtin_amdgcn_readlane(slot, l) >> SB_SHIFT);
+    const bool parted = ((all >> l) & ((all >> l) + 1)) || (all & ((1ull << l) - 1));
+    if (parted && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;
     if (again) lds_barrier();                            // the last block's angles have been read
     ap_run<SIDE>(a, n0 - 1 + l, __shfl(slot, min(lane + l, 63), 64), b - x * parts, parts, room);
   }

@@ -336,7 +336,8 @@ def append(cache, plan, k, v, q=None, rotary=None):
     views of one projection's rows; other types than bf16 are rounded to it first.  Slots are distinct.
 
     Into a cache with block scales, the rows of one block of 16 slots follow one another, as in the plan of a step, with no
-    other row between them, not even one that is left out (a block whose rows do not has undefined contents).  A call that writes a block's first slot begins the block anew; in another the
+    other row between them, not even one that is left out (a block whose rows do not has undefined contents, and plan.check()
+    raises where 15 or fewer rows lie between).  A call that writes a block's first slot begins the block anew; in another the
     scale of each head grows where the new values need it, and what the block holds is kept: exactly, but for values below
     2 ** -6 of the new scale, which are rounded to 2 ** -9 of it.  Values past 448 * 2 ** 119 saturate, infinities among
     them."""

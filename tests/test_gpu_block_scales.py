@@ -298,6 +298,16 @@ def test_append_reports_slots(rng):
             plan.check()
         k = read(cache, i32([2, 5, 6]))[0]
         assert (k[0] == (1.0 if slots[0] == 16 else 0.0)).all()
+    for slots in ([5, 20, 5], [5, 20, 6], [5, -1, 6], [5] + list(range(32, 47)) + [7]):   # a block's rows that others part
+        cache = _empty(4, 16, 1, 64, 64)
+        z = torch.ones(len(slots), 1, 64, dtype=BF, device="cuda")
+        plan = StepPlan(slots=i32(slots), positions=i32([0] * len(slots)), status=word())
+        append(cache, plan, z, z)
+        with pytest.raises(ValueError, match="slot"):
+            plan.check()
+        others = [s for s in slots if s >= 16]
+        assert not others or (read(cache, i32(others))[0] == 1.0).all()
+        assert not cache.k[3].float().any()
     cache = _empty(2, 16, 1, 64, 64)
     y = torch.ones(20, 1, 64, dtype=BF, device="cuda")
     plan = StepPlan(slots=i32([3] * 20), positions=i32([0] * 20), status=word())
