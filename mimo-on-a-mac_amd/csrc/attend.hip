@@ -16,7 +16,11 @@
 //
 // K and V go from HBM to LDS without passing registers, 16 bytes a lane; in LDS a tile is [64-element column block][key][128
 // bytes, E4M3 64] with the 16-byte cells of a row permuted by its number, which keeps the operand reads free of bank conflicts.
-// E4M3 becomes bf16 (exactly) after the LDS read; the scales multiply c and the result.
+// E4M3 becomes bf16 (exactly) after the LDS read; a head's scales multiply c and the result.
+//
+// Block scales (cache.hip): a power of two for each 16 slots, the group in which keys are taken anyway.  V's, and K's in narrow
+// tiles, goes into the conversion to bf16, which has room for one; wide tiles multiply K's codes and bytes as they are, with q
+// as two E4M3 planes (at take_q).  A byte comes by scalar loads once its page is known, while the keys are copied.
 //
 // Masks.  A tile's loads touch only keys that some row of the tile sees: others (past the last position, between the first
 // tokens and the window) read a visible row again, and their weights are set to 0.  A key that one row sees and another does
@@ -35,9 +39,13 @@
 // of 64, which have the room, 0.59 against 0.70); row sums by a matrix product, operands read further ahead, wave priorities:
 // no change.  Heads of 64: the exponentials (16 cycles for 64 of them) and what is around them, 0.66-0.70 PFLOP/s.
 // No vector register is spilled; 9 to 14 (wide) and 48 to 52 (narrow) scalar ones are, to lanes of a vector register.
+// Block scales: the same chunk 1598-1611 us where a head's scales take 1649 and K turned into bf16 by every wave 1721 (on another
+// card 1678); chunks of heads of 64 in a window of 1111, 24 requests, 54 us (51 with a head's scales).
 // Narrow: HBM.  48 requests of 500 to 16384 keys (1.03 GB) 187 us, 5.5 TB/s; 32 of 1000 to 32768 in E4M3 (1.13 GB) 206 us, 5.4
 // TB/s, above a large copy's 4.9 (read and written); a call of few keys 9 us, a chain of round trips (starts and lengths,
-// the table, K and V, the waves' parts through LDS).
+// the table, K and V, the waves' parts through LDS).  Block scales: 48 requests of 500 to 16384 keys, 32/8 heads of 128 (825 MB)
+// 159 us, 5.2 TB/s (157 with a head's scales), one of 32768 21.0 (20.1), 128 in a window of 128 23.5 (22.5): of this, 2.2 us are
+// the blocks' start, 3.2 the work's search, and each of two tiles takes 2.4-3.3 for its first keys, 4 for two steps, 1.8 to join.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
