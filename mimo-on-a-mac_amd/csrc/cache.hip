@@ -552,13 +552,13 @@ __global__ void __launch_bounds__(256, 4) cache_append_scaled_kernel(AppendArgs 
     const uint64_t all = __ballot(slot >> SB_SHIFT == __builtin_amdgcn_readlane(slot, l) >> SB_SHIFT);
     const bool parted = ((all >> l) & ((all >> l) + 1)) || (all & ((1ull << l) - 1));
     if (parted && threadIdx.x == 0 && a.status) a.status[0] = MIMO_ERR_SLOT;
-    if (again) lds_barrier();                            // the last block's angles have been read
+    if (again) lds_barrier();                              // the last block's angles have been read
     ap_run<SIDE>(a, n0 - 1 + l, __shfl(slot, min(lane + l, 63), 64), b - x * parts, parts, room);
   }
 }
 
 // ------------------------------------------------------------------ read
-// Cached tokens as bf16 rows: code times scale, rounded once (with block scales exact).  A thread turns 8 values; a block of
+// Cached tokens as bf16 rows: code times scale in 32 bits, rounded to bf16 (with block scales exact).  A thread turns 8 values; a block of
 // 256 a few tokens one after another, whose rows of a head share cache lines.
 //
 // Bound by HBM: 32768 tokens of 4 heads of 192/128 with block scales (126 MB) 23.4 us a call, 5.4 TB/s; the rows are written past

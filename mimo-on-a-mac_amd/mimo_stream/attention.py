@@ -386,9 +386,9 @@ def append(cache, plan, k, v, q=None, rotary=None):
 
 def read(cache, slots, out=None, status=None):
     """Cached tokens as rows: (k [N, kv_heads, k_dim], v [N, kv_heads, v_dim]) in bf16 of int32 slots [N] (a plan's, or
-    PageTable.slots; in any order, any slot any number of times), stored values times their scales, rounded once; rows of
-    slot -1 are 0.  Keys are as append left them, rotated.  out: two contiguous bf16 tensors to write; status: int32 [1] that
-    receives a failure (a slot past the cache, whose row is 0) as plan.status does."""
+    PageTable.slots; in any order, any slot any number of times), stored values times their scales (in 32 bits, rounded to
+    bf16); rows of slot -1 are 0.  Keys are as append left them, rotated.  out: two contiguous bf16 tensors to write; status:
+    int32 [1] that receives a failure (a slot past the cache, whose row is 0) as plan.status does."""
     if cache._call is not None and out is None:
         done = cache._calls.read(cache._call, _current_device(), _raw_stream(cache.device.index), slots, status)
         if done is not NotImplemented:
