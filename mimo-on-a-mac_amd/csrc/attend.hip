@@ -2,7 +2,8 @@
 // engine/mimo_stream/mimo_v2.py:110-150, on one request's cache).
 //
 // Rows.  The queries that share a K/V head (its G heads, one after another, of consecutive tokens) are the rows of a tile, so
-// a key or value is read once for all of them: narrow tiles of 32 rows for requests with few rows (decode), wide tiles of 128.
+// a key or value is read once for all of them: narrow tiles of 32 rows, over block scales also of 16, for requests with few rows
+// (decode), wide tiles of 128.
 //
 // One pass over the keys with the running maximum m and sum l of each row (exp(x) = 2^(x log2 e) throughout):
 //   S^T = K Q^T      v_mfma_f32_32x32x16_bf16, K rows as the A operand: lane (r, h) = (l % 32, l / 32) then holds, for
@@ -44,8 +45,9 @@
 // Narrow: HBM.  48 requests of 500 to 16384 keys (1.03 GB) 187 us, 5.5 TB/s; 32 of 1000 to 32768 in E4M3 (1.13 GB) 206 us, 5.4
 // TB/s, above a large copy's 4.9 (read and written); a call of few keys 9 us, a chain of round trips (starts and lengths,
 // the table, K and V, the waves' parts through LDS).  Block scales: 48 requests of 500 to 16384 keys, 32/8 heads of 128 (825 MB)
-// 159 us, 5.2 TB/s (157 with a head's scales), one of 32768 21.0 (20.1), 128 in a window of 128 23.5 (22.5): of this, 2.2 us are
-// the blocks' start, 3.2 the work's search, and each of two tiles takes 2.4-3.3 for its first keys, 4 for two steps, 1.8 to join.
+// 155 us, 5.3 TB/s (157 with a head's scales, in tiles of 32 rows), one of 32768 19.1 (20.1), 128 in a window of 128 20.5 (22.5):
+// in tiles of 32 rows these took 23.5, of which 2.2 were the blocks' start, 3.2 the work's search, and each of two tiles took
+// 2.4-3.3 for its first keys, 4 for two steps and 1.8 to join.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -92,21 +94,20 @@ constexpr int AT_WIDE_TARGET = 512, AT_NARROW_TARGET = 512;
 constexpr int AT_WIDE_MIN = 4, AT_NARROW_MIN = 2;
 constexpr int AT_START = 8;                               // units that a wide block's start and a part's join cost
 
-template <int DK_, int DV_, int DTYPE, bool WIDE_> struct AtCfg {
-  static constexpr int DK = DK_, DV = DV_;
-  static constexpr bool F8 = DTYPE != MIMO_KV_BF16, BS = DTYPE == MIMO_KV_E4M3_BLOCKS, HS = F8 && !BS, WIDE = WIDE_;
+template <int DK_, int DV_, int DTYPE, int ROWS_> struct AtCfg {
+  static constexpr int DK = DK_, DV = DV_, ROWS = ROWS_;   // rows of a tile: 128 (wide), 32 or 16 (narrow)
+  static constexpr bool F8 = DTYPE != MIMO_KV_BF16, BS = DTYPE == MIMO_KV_E4M3_BLOCKS, HS = F8 && !BS, WIDE = ROWS == 128;
   static constexpr bool QP = BS && WIDE;                   // q as two E4M3 planes
   static constexpr int CBB = F8 ? 64 : 128;                // bytes of a row in one 64-element column block
   static constexpr int KCB = DK / 64, VCB = DV / 64;
   static constexpr int KEYS = WIDE ? 64 : 32;              // keys of one LDS tile (narrow: one wave's)
   static constexpr int NB = KEYS / 32;
   static constexpr int UNIT = WIDE ? 64 : 128;             // keys per iteration of the block
-  static constexpr int ROWS = WIDE ? 128 : 32;
   static constexpr int KBYTES = KEYS * CBB * KCB, VBYTES = KEYS * CBB * VCB;
   static constexpr int STAGE = KBYTES + VBYTES;
   static constexpr int GR = 1024 / CBB;                    // rows of one copy instruction (64 lanes of 16 bytes)
   static constexpr int LR = (WIDE ? 16 : 32) / GR;         // row groups that a wave copies per tile
-  static constexpr int MERGE = WIDE ? 0 : 4 * 32 * DV * 4 + 4 * 32 * 8;   // narrow: the waves' O, m, l joined at the end
+  static constexpr int MERGE = WIDE ? 0 : 4 * ROWS * DV * 4 + 4 * ROWS * 8;   // narrow: the waves' O, m, l joined at the end
   static constexpr int SCALES = (WIDE ? 2 : 4) * STAGE;    // wide: the two tiles' block scales stand behind them
   static constexpr int ROOM = SCALES + (BS && WIDE ? 2 * 8 * 4 : 0);
   static constexpr int LDS = ROOM > MERGE ? ROOM : MERGE;
@@ -144,12 +145,23 @@ __device__ __forceinline__ float at_swap_sum(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+// f(x of this lane, x of the lane of the neighbouring 16)
+template <class F> __device__ __forceinline__ float at_swap16(float x, F f) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // eight E4M3 codes times a power of two to bf16, exact
 __device__ __forceinline__ bf16x8 at_f8_bf16x8(uint32_t a, uint32_t b, float by) {
   const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, true);
   const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, true);
+  return bf16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
+}
+// the first four times one power of two, the others times another
+__device__ __forceinline__ bf16x8 at_f8_bf16x8(uint32_t a, float by_a, uint32_t b, float by_b) {
+  const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by_a, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by_a, true);
+  const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by_b, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by_b, true);
   return bf16x8{x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
 }
 
@@ -928,6 +940,305 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   }
 }
 
+// One item in tiles of 16 rows, over block scales: v_mfma_f32_16x16x32_bf16, so that requests of up to 16 rows leave no half of
+// the products, of the softmax and of the registers empty.  S^T = K Q^T: lane (c, g) = (l % 16, l / 16) holds, for query row c,
+// keys 4 g + i of each of the wave's two groups of 16, whose scales are one number each; P^T, as it stands, is the B operand of
+// the 32 keys in the order (g, group, i), in which the transposing reads of V fetch them.  Against tiles of 32 rows: one request
+// of 32768 keys, 64/4 heads of 192/128, 19.1 us (20.9), 48 of 500 to 16384, 32/8 of 128, 155 (159), 128 in a window of 128, 64/8
+// of 192/128, 20.5 (23.4), one of 40, 8/2 of 64, 6.0 (6.8).  The first three with more blocks a CU, 3: 20.6, 159, 21.5; 4: 26.5,
+// 199, 27.7 (spills); with a second tile on its way 20.1, 162, 20.5; with operands read 2 instead of 4 ahead 19.3, 156, 20.6.
+template <class C>
+__device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, const AtItem& item) {
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));                              // nothing per lane is kept in registers from one item to the next
+  const int lane = t & 63, r16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int b = __builtin_amdgcn_readfirstlane(item.b), hg = item.hh % a.HG, kv = item.hh / a.HG, ns = item.ns;
+  const int tok0 = item.tt * a.TQ, toks = min(a.TQ, item.n - tok0);
+  const int heads = min(a.HT, a.G - hg * a.HT);
+  const int qt = r16 / a.HT, qh = r16 - qt * a.HT;         // this lane's query row
+  const bool valid = qt < toks && qh < heads;
+  const int head = kv * a.G + hg * a.HT + qh;
+  const int base_pos = item.len - item.n + tok0;
+  if (a.meta && item.it0 == 0 && t < toks)
+    a.meta[(size_t)(item.s0 + tok0 + t) * a.Hh + item.hh] = make_int2(item.slot, ns | (t << 16));
+  if (item.len == 0) {                                     // a refused request
+    if (a.status && t == 0) a.status[0] = MIMO_ERR_SHAPE;
+    if (valid && wave == 0)
+      for (int d = 0; d < C::DV / 4; d += 8)
+        *reinterpret_cast<uint4*>(a.out + ((size_t)(item.s0 + tok0 + qt) * a.Hq + head) * C::DV + g4 * (C::DV / 4) + d) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const AtRange rg = at_range(base_pos, base_pos + toks - 1, a.window, a.sinks, C::UNIT);
+  const int it0 = item.it0, it1 = min(item.it1, rg.I);
+  constexpr int UG = C::UNIT / 16;
+  const int wg = 2 * wave;                                 // the wave's first group in a unit
+  AtKeys kg[2];
+  auto look = [&](int it) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) kg[x] = at_keys(a, rg, b, rg.key(it * UG + wg + x));
+  };
+  look(it0);                                               // the table is read while the queries are asked for
+
+  // queries: row r16, dimensions 64 e + 16 g4 .., two products' worth of each 64
+  float c = a.scale * kLog2e;
+  const uint32_t flip = c < 0.0f ? 0x80008000u : 0u;
+  const bool zero = c == 0.0f;
+  c = zero ? 1.0f : fabsf(c);
+  uint4 qraw[2 * C::KCB];
+  {
+    const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + qt) * a.q_stride + head * C::DK + 16 * g4;
+#pragma unroll
+    for (int s = 0; s < 2 * C::KCB; ++s) {
+      qraw[s] = make_uint4(0, 0, 0, 0);
+      if (valid && !zero) qraw[s] = *reinterpret_cast<const uint4*>(qp + 64 * (s >> 1) + 8 * (s & 1));
+    }
+  }
+  const int pos = base_pos + qt;
+  const int wp_min = base_pos, wp_max = base_pos + min(toks - 1, 15 / a.HT);
+
+  // Copies and reads as in at_tile, the cell at place p of row x being p ^ (x / 4) % 4 ^ 2 (x / 16): the last term keeps the
+  // rows of both groups, which one transposing read of V takes together, in different banks.
+  const int cr = lane / 4, cell = (lane & 3) ^ g4;
+  const uint32_t lds0 = lds_addr(lds) + wave * C::STAGE;
+  size_t crow[2];
+  uint2 scales[2];                                         // bytes of the tile that is being copied
+  auto rows_of = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int page = at_page(a, kg[x].id);
+      crow[x] = at_row(a, rg, kg[x], page, kv, cr);
+      scales[x] = at_scales(a, kg[x], page, kv);
+    }
+  };
+  auto issue = [&](const uint8_t* from, int dim, uint32_t stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const uint8_t* p = from + crow[x] * dim + 16 * (cell ^ (2 * x));
+#pragma unroll
+      for (int cb = 0; cb < dim / 64; ++cb) at_copy16(p + cb * 64, stage + cb * (C::KEYS * 64) + x * 1024);
+    }
+  };
+  auto issue_k = [&]() __attribute__((always_inline)) { issue(a.k, C::DK, lds0); };
+  auto issue_v = [&]() __attribute__((always_inline)) { issue(a.v, C::DV, lds0 + C::KBYTES); };
+  const uint8_t* st = lds + wave * C::STAGE;
+  const int k_at = r16 * 64 + 16 * (g4 ^ (r16 >> 2));
+  const int v_at = (4 * g4 + ((r16 >> 1) & 3) + 16 * (r16 >> 3)) * 64 + 16 * (g4 ^ (2 * (r16 >> 3))) + 8 * (r16 & 1);
+  auto k_read = [&](int f) __attribute__((always_inline)) {   // group f % 2, dimensions 64 (f / 2) + 16 g4 ..
+    return *reinterpret_cast<const uint4*>(st + (k_at ^ (32 * (f & 1))) + (f & 1) * 1024 + (f >> 1) * (C::KEYS * 64));
+  };
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wint-to-pointer-cast"   // LDS pointers are 32 bits on the device
+  auto v_read = [&](int d) __attribute__((always_inline)) {   // dimension 16 d + r16 of keys 4 g4 + i of both groups
+    typedef __attribute__((address_space(3))) v2i* lds2;
+    const uint8_t* p = st + C::KBYTES + (v_at ^ (16 * (d & 3))) + (d >> 2) * (C::KEYS * 64);
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds2)(uint32_t)(uintptr_t)p);
+  };
+#pragma clang diagnostic pop
+
+  constexpr int ND = C::DV / 16;
+  v4f O[ND], S[2];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) O[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  float m = -INFINITY, l = 0.0f;                           // l: this lane's keys
+  bf16x8 Q[2 * C::KCB], P, rest;
+  float k_by[2], v_by[2];
+  auto take_q = [&]() __attribute__((always_inline)) {     // once the first copies are on their way
+#pragma unroll
+    for (int s = 0; s < 2 * C::KCB; ++s)
+      Q[s] = __builtin_bit_cast(bf16x8, make_uint4(qraw[s].x ^ flip, qraw[s].y ^ flip, qraw[s].z ^ flip, qraw[s].w ^ flip));
+  };
+  auto scores = [&]() __attribute__((always_inline)) {
+    constexpr int F = 2 * C::KCB, AHEAD = 2 * C::KCB < 4 ? 2 * C::KCB : 4;
+    uint4 X[AHEAD];
+#pragma unroll
+    for (int f = 0; f < AHEAD; ++f) X[f] = k_read(f);
+#pragma unroll
+    for (int f = 0; f < F; ++f) {
+      const int x = f & 1, e = f >> 1;
+      __builtin_amdgcn_sched_barrier(0);
+      const v4f none = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint4 w = X[f % AHEAD];
+      S[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_f8_bf16x8(w.x, w.y, k_by[x]), Q[2 * e], e == 0 ? none : S[x], 0, 0, 0);
+      S[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(at_f8_bf16x8(w.z, w.w, k_by[x]), Q[2 * e + 1], S[x], 0, 0, 0);
+      if (f + AHEAD < F) X[f % AHEAD] = k_read(f + AHEAD);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const uint32_t span = a.window ? (uint32_t)a.window : 0x80000000u;
+  auto mask = [&](int g0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int j0 = rg.key(g0 + x) + 4 * g4;
+      const uint32_t back = (uint32_t)(pos - j0);
+      const int first = rg.key(g0 + x) < a.sinks ? min(a.sinks, pos + 1) - j0 : 0;   // first tokens that the row sees
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float s = S[x][i];
+        S[x][i] = back - (uint32_t)i < span || i < first ? s : -INFINITY;
+      }
+    }
+  };
+  auto softmax = [&]() __attribute__((always_inline)) {
+    float top = S[0][0];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, S[x][i]);
+    top = at_swap_max(at_swap16(top, [](float u, float v) { return fmaxf(u, v); })) * c;
+    if (__ballot(top > m + 8.0f || (m == -INFINITY && top > m))) {   // m may lag, as in at_tile
+      const float next = fmaxf(m, top), was = at_exp2(m - (next == -INFINITY ? 0.0f : next));
+      m = next;
+      l *= was;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) O[d] *= was;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float p = at_exp2(__builtin_fmaf(S[x][i], c, -ref));
+        l += p;
+        P[4 * x + i] = (__bf16)p;
+        rest[4 * x + i] = (__bf16)(p - (float)P[4 * x + i]);
+      }
+  };
+  auto values = [&]() __attribute__((always_inline)) {
+    constexpr int AHEAD = 4;
+    v2i X[AHEAD];
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) X[d] = v_read(d);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      __builtin_amdgcn_sched_barrier(0);
+      const bf16x8 w = at_f8_bf16x8(X[d % AHEAD][0], v_by[0], X[d % AHEAD][1], v_by[1]);
+      O[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, P, O[d], 0, 0, 0);
+      O[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, rest, O[d], 0, 0, 0);
+      if (d + AHEAD < ND) X[d % AHEAD] = v_read(d + AHEAD);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // every row sees all keys of the wave's tile from group g0 on
+  auto open = [&](int g0) {
+    const int j0 = rg.key(g0);
+    return g0 >= rg.sg && j0 + C::KEYS - 1 <= wp_min && (!a.window || j0 > wp_max - a.window);
+  };
+
+  constexpr int NK = 2 * C::KCB, NV = 2 * C::VCB;
+  const int end = min(it1, (rg.gt - wg + UG - 1) / UG);    // of the units that hold groups of this wave
+  if (it0 < end) {
+    rows_of();
+    issue_k();
+    issue_v();
+  }
+  take_q();
+  for (int it = it0; it < end; ++it) {
+    const int g0 = it * UG + wg;
+    const bool more = it + 1 < end;
+    if (more) look(it + 1);
+#pragma unroll
+    for (int x = 0; x < 2; ++x) k_by[x] = e8m0_f32(scales[x].x), v_by[x] = e8m0_f32(scales[x].y);
+    at_wait_vm(NV);
+    scores();
+    at_wait_lds();                                         // K has been read: its room takes the next keys
+    if (more) {
+      rows_of();
+      issue_k();
+    }
+    if (!open(g0)) mask(g0);
+    softmax();
+    if (more) at_wait_vm(NK);
+    else at_wait_vm(0);
+    values();
+    at_wait_lds();
+    if (more) issue_v();
+  }
+  // sums that are not finite, as in at_tile: another row's NaN value may have made them so
+  bool suspect = false;
+  if (rg.p_min != rg.p_max) {
+    float worst = 0.0f;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) worst += O[d][i] - O[d][i];   // 0, or NaN
+    if (__ballot(worst != 0.0f)) {
+      bool odd = false;
+#pragma unroll 1
+      for (int g = it0 * UG; g < min(rg.gt, it1 * UG); ++g) {
+        if (open(g & ~1)) continue;
+        const AtKeys k = at_keys(a, rg, b, rg.key(g));
+        const int page = at_page(a, k.id);
+#pragma unroll 1
+        for (int x = 0; x < 16; ++x) {
+          const size_t row = at_row(a, rg, k, page, kv, x) * C::DV;
+          const uint32_t w = lane < C::DV / 4 ? *reinterpret_cast<const uint32_t*>(a.v + row + 4 * lane) : 0u;
+          odd |= (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0;
+        }
+      }
+      suspect = __ballot(odd) != 0;
+    }
+  }
+  // the waves' parts, joined over LDS in wave order: row r at [wave][r][DV], 16-byte pieces turned by the row
+  float* po = reinterpret_cast<float*>(lds);
+  float* pm = po + 4 * 16 * C::DV;
+  constexpr int NP = C::DV / 4;
+  at_wait_vm(0);
+  __syncthreads();                                         // every wave is done with its tiles
+  if (suspect) {
+#pragma unroll 1
+    for (int r = 0; r < 16; ++r) {
+      const int rt = r / a.HT, rh = r - rt * a.HT;
+      if (rt >= toks || rh >= heads) continue;
+      float o[C::VCB], mr, lr;
+      at_slow<C>(a, rg, b, kv, it0, it1, wg, 2, a.q + (int64_t)(item.s0 + tok0 + rt) * a.q_stride + (kv * a.G + hg * a.HT + rh) * C::DK,
+                 base_pos + rt, a.scale * kLog2e, o, mr, lr);
+#pragma unroll
+      for (int e = 0; e < C::VCB; ++e) po[(wave * 16 + r) * C::DV + 4 * ((16 * e + lane / 4 + r) & (NP - 1)) + (lane & 3)] = o[e];
+      if (lane == 0) pm[2 * (16 * wave + r)] = mr, pm[2 * (16 * wave + r) + 1] = lr;
+    }
+  } else {
+    l = at_swap_sum(at_swap16(l, [](float u, float v) { return u + v; }));
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      *reinterpret_cast<float4*>(po + (wave * 16 + r16) * C::DV + 4 * ((4 * d + g4 + r16) & (NP - 1))) = make_float4(O[d][0], O[d][1], O[d][2], O[d][3]);
+    if (g4 == 0) pm[2 * (16 * wave + r16)] = m, pm[2 * (16 * wave + r16) + 1] = l;
+  }
+  __syncthreads();
+  for (int e = t; e < 16 * NP; e += AT_THREADS) {
+    const int row = e / NP, piece = e & (NP - 1), rt = row / a.HT, rh = row - rt * a.HT;
+    if (rt >= toks || rh >= heads) continue;
+    float mw[4], top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mw[w] = pm[2 * (16 * w + row)], top = fmaxf(top, mw[w]);
+    const int hd = kv * a.G + hg * a.HT + rh;
+    const float sink = ns == 1 && a.sink_logits ? a.sink_logits[hd] * kLog2e : -INFINITY;
+    const float all = fmaxf(top, sink), ref = all == -INFINITY ? 0.0f : all;
+    float tot = ns == 1 ? at_exp2(sink - ref) : 0.0f;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = at_exp2(mw[w] - ref);
+      const float4 o = *reinterpret_cast<const float4*>(po + (w * 16 + row) * C::DV + 4 * ((piece + row) & (NP - 1)));
+      tot += pm[2 * (16 * w + row) + 1] * f;
+      x[0] += o.x * f, x[1] += o.y * f, x[2] += o.z * f, x[3] += o.w * f;
+    }
+    if (ns > 1) {
+      const size_t pr = (size_t)item.slot * (a.TQ * a.HT) + row;
+      *reinterpret_cast<float4*>(a.part_o + pr * C::DV + 4 * piece) = make_float4(x[0], x[1], x[2], x[3]);
+      if (piece == 0) a.part_ml[2 * pr] = all, a.part_ml[2 * pr + 1] = tot;
+    } else {
+      const float w = tot == 0.0f ? 0.0f : 1.0f / tot;
+      uint2 y;
+      y.x = (uint32_t)f32_to_bf16(x[0] * w) | ((uint32_t)f32_to_bf16(x[1] * w) << 16);
+      y.y = (uint32_t)f32_to_bf16(x[2] * w) | ((uint32_t)f32_to_bf16(x[3] * w) << 16);
+      if (tot == 0.0f) y = make_uint2(0, 0);
+      *reinterpret_cast<uint2*>(a.out + ((size_t)(item.s0 + tok0 + rt) * a.Hq + hd) * C::DV + 4 * piece) = y;
+    }
+  }
+  __syncthreads();                                         // the next item's copies may come
+}
+
 // rows of no request
 __device__ __forceinline__ void at_clear(const AttendArgs& a, int row) {
   const int first = a.starts[0], last = a.starts[a.B], gap = first + a.N - last;
@@ -1041,7 +1352,10 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
         item.slot = 2 * (j * a.Hh + hh) + (start > u0 ? 1 : 0);
         item.it0 = off, item.it1 = (int)min((int64_t)real, u1 - start);
       }
-      if (item.it0 < item.it1) at_tile<C>(a, lds, item);
+      if (item.it0 < item.it1) {
+        if constexpr (C::ROWS == 16) at_tile16<C>(a, lds, item);
+        else at_tile<C>(a, lds, item);
+      }
       u = start + bound;
     }
   }
@@ -1259,17 +1573,20 @@ static int at_launch(AttendArgs a, bool join, hipStream_t st) {
   return check_launch("attend_join");
 }
 
-template <int DTYPE, bool WIDE>
+template <int DTYPE, int ROWS>
 static int at_dims(const AttendArgs& a, int dk, bool join, hipStream_t st) {
   switch (dk) {
-    case 64: return at_launch<AtCfg<64, 64, DTYPE, WIDE>>(a, join, st);
-    case 128: return at_launch<AtCfg<128, 128, DTYPE, WIDE>>(a, join, st);
-    default: return at_launch<AtCfg<192, 128, DTYPE, WIDE>>(a, join, st);
+    case 64: return at_launch<AtCfg<64, 64, DTYPE, ROWS>>(a, join, st);
+    case 128: return at_launch<AtCfg<128, 128, DTYPE, ROWS>>(a, join, st);
+    default: return at_launch<AtCfg<192, 128, DTYPE, ROWS>>(a, join, st);
   }
 }
 template <int DTYPE>
-static int at_width(const AttendArgs& a, int dk, bool wide, bool join, hipStream_t st) {
-  return wide ? at_dims<DTYPE, true>(a, dk, join, st) : at_dims<DTYPE, false>(a, dk, join, st);
+static int at_width(const AttendArgs& a, int dk, int rows, bool join, hipStream_t st) {
+  if (rows == 128) return at_dims<DTYPE, 128>(a, dk, join, st);
+  if constexpr (DTYPE == MIMO_KV_E4M3_BLOCKS)
+    if (rows == 16) return at_dims<DTYPE, 16>(a, dk, join, st);
+  return at_dims<DTYPE, 32>(a, dk, join, st);
 }
 
 }  // namespace mimo
@@ -1281,7 +1598,7 @@ extern "C" {
 size_t mimo_cache_attend_workspace_size(int N, int heads, int kv_heads, int v_dim) {
   if (N < 1 || heads < 1 || kv_heads < 1 || v_dim < 1 || heads % kv_heads) return 256;
   const AtRoom w = at_room(128, AT_WIDE_TARGET, N, heads, kv_heads, v_dim), n = at_room(32, AT_NARROW_TARGET, N, heads, kv_heads, v_dim);
-  return std::max(w.o + w.ml + w.meta, n.o + n.ml + n.meta);
+  return std::max(w.o + w.ml + w.meta, n.o + n.ml + n.meta);   // tiles of 16 rows need no more than those of 32
 }
 
 int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, const mimo_kv_cache* cache, int B,
@@ -1317,23 +1634,26 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   a.k_scale = cache->k_scale, a.v_scale = cache->v_scale, a.sink_logits = sink_logits;
   a.scale = scale, a.out = out, a.status = status;
   // narrow tiles hold the rows of a request in 32, wide ones are up to a quarter filled: at 5 to 8 rows of 8 heads the wide
-  // ones take 132-136 us for 32 requests of 4000 keys, two and more narrow tiles 136-139, and at 12 143 against 356
-  const bool wide = (int64_t)std::min(max_new, N) * (heads / cache->kv_heads) > 32;
-  at_tiles(wide ? 128 : 32, N, heads, cache->kv_heads, a);
+  // ones take 132-136 us for 32 requests of 4000 keys, two and more narrow tiles 136-139, and at 12 143 against 356.  Over block scales those of up to 16 rows have tiles of 16 (at_tile16), which also at 16 rows, 16 heads of 192/128 at 300
+  // keys, take 11.0 us against 12.1
+  const int64_t per_request = (int64_t)std::min(max_new, N) * (heads / cache->kv_heads);
+  const bool wide = per_request > 32;
+  const int rows = wide ? 128 : (cache->dtype == MIMO_KV_E4M3_BLOCKS && per_request <= 16 ? 16 : 32);
+  at_tiles(rows, N, heads, cache->kv_heads, a);
   a.target = wide ? AT_WIDE_TARGET : AT_NARROW_TARGET;
   // no tile can walk more units than the table or the window holds; where none has to be split there is no second launch
   const int most = at_most((int64_t)max_pages * cache->page_size, window, a.sinks, a.TQ, wide ? 64 : 128);
   const bool join = most > (wide ? AT_WIDE_MIN : AT_NARROW_MIN);
-  const AtRoom room = at_room(wide ? 128 : 32, a.target, N, heads, cache->kv_heads, cache->v_dim);
+  const AtRoom room = at_room(rows, a.target, N, heads, cache->kv_heads, cache->v_dim);
   char* w = static_cast<char*>(ws);
   a.part_o = reinterpret_cast<float*>(w);
   a.part_ml = reinterpret_cast<float*>(w + room.o);
   a.meta = join ? reinterpret_cast<int2*>(w + room.o + room.ml) : nullptr;
   hipStream_t st = as_stream(stream);
   switch (cache->dtype) {
-    case MIMO_KV_BF16: return at_width<MIMO_KV_BF16>(a, cache->k_dim, wide, join, st);
-    case MIMO_KV_E4M3: return at_width<MIMO_KV_E4M3>(a, cache->k_dim, wide, join, st);
-    default: return at_width<MIMO_KV_E4M3_BLOCKS>(a, cache->k_dim, wide, join, st);
+    case MIMO_KV_BF16: return at_width<MIMO_KV_BF16>(a, cache->k_dim, rows, join, st);
+    case MIMO_KV_E4M3: return at_width<MIMO_KV_E4M3>(a, cache->k_dim, rows, join, st);
+    default: return at_width<MIMO_KV_E4M3_BLOCKS>(a, cache->k_dim, rows, join, st);
   }
 }
 

@@ -487,6 +487,27 @@ def test_attend_values_that_only_later_rows_see(rng, dims, new):
     assert torch.isnan(out[-1, :, 3]).all() and torch.isfinite(out[:-1]).all()
 
 
+@pytest.mark.parametrize("dims", list(DIMS))
+@pytest.mark.parametrize("heads,new", [((5, 1), 3), ((8, 2), 4), ((1, 1), 16), ((16, 1), 1), ((14, 2), 2), ((34, 2), 1)])
+@pytest.mark.parametrize("window,sinks,page", [(0, 0, 16), (21, 3, 16), (100, 40, 64)])
+def test_attend_up_to_sixteen_rows(rng, dims, heads, new, window, sinks, page):
+    """Requests of several tokens that fill a tile of 16 rows, or leave some free; the last one has a row too many for it."""
+    lens = [new, new + 15, 64, 0, 129, 143, 500, 4001]
+    _check(*_attend_case(rng, lens, [new, new, 1, 0, new, new, new, new], *heads, *DIMS[dims], page, window, sinks, True, pad=2), few=True)
+
+
+@pytest.mark.parametrize("dims", list(DIMS))
+@pytest.mark.parametrize("window,sinks", [(0, 0), (30, 0), (30, 20)])
+def test_attend_few_rows_with_values_that_are_not_finite(rng, dims, window, sinks):
+    """NaN in keys' values at both ends of a window: only the rows that see them have it, tile by tile."""
+    q, cache, plan, kw = _attend_case(rng, [400, 70], [4, 4], 4, 1, *DIMS[dims], 16, window, sinks)
+    codes = cache.v.view(torch.uint8)
+    for b, at in [(0, 397), (0, 370), (0, 18), (1, 40), (1, 69)]:
+        codes[int(plan.table[b, at // 16]), :, at % 16, at % 7] = 0x7F
+    out = _check(q, cache, plan, kw, few=True)
+    assert torch.isnan(out).any() and torch.isfinite(out).any()
+
+
 def test_attend_scales_far_apart(rng):
     """Blocks whose values differ by 2^40: the large ones decide, and the small ones are there when they are alone."""
     q, cache, plan, kw = _attend_case(rng, [48, 16], [1, 1], 2, 1, 64, 64, 16)
