@@ -345,16 +345,22 @@ __device__ __forceinline__ int at_page(const AttendArgs& a, int id) {
   if (a.status && (threadIdx.x & 63) == 0) a.status[0] = MIMO_ERR_SLOT;
   return 0;
 }
-// the bytes of K and V of a group's block scale, by scalar loads of the dwords around them
-__device__ __forceinline__ uint2 at_scales(const AttendArgs& a, const AtKeys& g, int page, int kv) {
+// The bytes of K and V of a group's block scale, by scalar loads of the dwords around them.  They are taken out where they are
+// used: the copies, which come first, do not wait for them.
+struct AtScales {
+  uint32_t k, v;
+  int shift;
+  __device__ __forceinline__ uint32_t k_byte() const { return k >> shift & 0xFFu; }
+  __device__ __forceinline__ uint32_t v_byte() const { return v >> shift & 0xFFu; }
+};
+__device__ __forceinline__ AtScales at_scales(const AttendArgs& a, const AtKeys& g, int page, int kv) {
   typedef const __attribute__((address_space(4))) uint32_t* words;
   const int part = (g.g0 & ((1 << a.page_shift) - 1)) >> 4;
   const uint64_t at = (((uint64_t)(uint32_t)page * a.Hkv + kv) << (a.page_shift - 4)) + part;
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)at), hi = __builtin_amdgcn_readfirstlane((uint32_t)(at >> 32));
   const uint64_t word = (((uint64_t)hi << 32) | lo) >> 2;
-  const int shift = 8 * (lo & 3);
-  return make_uint2(reinterpret_cast<words>(reinterpret_cast<uintptr_t>(a.k_scale))[word] >> shift & 0xFFu,
-                    reinterpret_cast<words>(reinterpret_cast<uintptr_t>(a.v_scale))[word] >> shift & 0xFFu);
+  return AtScales{reinterpret_cast<words>(reinterpret_cast<uintptr_t>(a.k_scale))[word],
+                  reinterpret_cast<words>(reinterpret_cast<uintptr_t>(a.v_scale))[word], 8 * (int)(lo & 3)};
 }
 // cache row (of [page, head, row in page]) of key g0 + r
 __device__ __forceinline__ size_t at_row(const AttendArgs& a, const AtRange& r, const AtKeys& g, int page, int kv, int row) {
@@ -521,7 +527,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   const int cell_v = C::F8 ? cell_k : (lane & 7) ^ (4 * ((lane >> 4) & 1));
   const uint32_t lds0 = lds_addr(lds) + (C::WIDE ? 0 : wave * C::STAGE);
   size_t crow[C::LR];
-  uint2 next_scales[C::BS ? NG : 1];                       // the bytes of the tile that is being copied
+  AtScales next_scales[C::BS ? NG : 1];                    // of the tile that is being copied
   auto rows_of = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < C::LR; ++x) {
@@ -726,7 +732,7 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       const int cur = (it - it0) & 1, g0 = it * UG;
       if (it + 1 < it1) look(it + 1);
       uint32_t* sc = reinterpret_cast<uint32_t*>(lds + C::SCALES) + 8 * cur;
-      if (C::BS && lane == 0) sc[wave] = next_scales[0].x, sc[4 + wave] = next_scales[0].y << 23;
+      if (C::BS && lane == 0) sc[wave] = next_scales[0].k_byte(), sc[4 + wave] = next_scales[0].v_byte() << 23;
       at_wait_vm(0);
       __syncthreads();                                     // the tile has landed everywhere; the other one is free
       if constexpr (C::BS) {                               // on their way while the copies are asked for
@@ -761,8 +767,8 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       const bool more = it + 1 < end;
       if (more) look(it + 1);
       if constexpr (C::BS) {
-        k_by[0] = (r32 < 16 ? next_scales[0].x : next_scales[1].x) << 23;
-        v_by[0] = e8m0_f32(next_scales[0].y), v_by[1] = e8m0_f32(next_scales[1].y);
+        k_by[0] = (r32 < 16 ? next_scales[0].k_byte() : next_scales[1].k_byte()) << 23;
+        v_by[0] = e8m0_f32(next_scales[0].v_byte()), v_by[1] = e8m0_f32(next_scales[1].v_byte());
       }
       at_wait_vm(NV);
       scores(st);
@@ -1002,7 +1008,7 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
   const int cr = lane / 4, cell = (lane & 3) ^ g4;
   const uint32_t lds0 = lds_addr(lds) + wave * C::STAGE;
   size_t crow[2];
-  uint2 scales[2];                                         // bytes of the tile that is being copied
+  AtScales scales[2];                                      // of the tile that is being copied
   auto rows_of = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -1138,7 +1144,7 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
     const bool more = it + 1 < end;
     if (more) look(it + 1);
 #pragma unroll
-    for (int x = 0; x < 2; ++x) k_by[x] = e8m0_f32(scales[x].x), v_by[x] = e8m0_f32(scales[x].y);
+    for (int x = 0; x < 2; ++x) k_by[x] = e8m0_f32(scales[x].k_byte()), v_by[x] = e8m0_f32(scales[x].v_byte());
     at_wait_vm(NV);
     scores();
     at_wait_lds();                                         // K has been read: its room takes the next keys
@@ -1307,6 +1313,8 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
     total = __shfl(before, 63, 64);
     before -= mine;
   }
+  // known to be one number for the wave: all that follows from it stays in scalar registers
+  total = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(total >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)total));
   // blocks that share the work: a unit each at least, and one per CU while that leaves them no more than 8 units and the tiles
   // alone do not fill the card (one request of 32768 keys, 64/4 heads: 25.6 us with 256 blocks, 27.8 with 512; 8 of 4000: 24.1
   // and 25.5; a limit of 32 units changes neither)
