@@ -76,6 +76,7 @@ struct AttendArgs {
   int32_t* status;
   // rows of a tile: TQ tokens of HT heads (HG groups of HT heads cover G), Hh = Hkv * HG
   int TQ, HT, HG, Hh, target;
+  uint32_t by_ht, by_tq, by_hh;                            // reciprocals (at_tiles): 2^16 / HT, 2^32 / TQ, 2^32 / Hh
   // split tiles: per slot TQ * HT rows of O (fp32 [Dv]) and (m, l); per (token, head group) the first part's slot and
   // parts | token's place in its tile << 16.  Part i > 0 is in slot (first & ~part_mask) + i part_step.  meta is null when no
   // tile can be split.
@@ -135,6 +136,11 @@ __device__ __forceinline__ void at_copy16(const uint8_t* src, uint32_t lds) {
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory", "m0");
 }
+// the same from src (wave-uniform) + at
+__device__ __forceinline__ void at_copy16(const uint8_t* src, uint32_t at, uint32_t lds) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(src), "s"(m) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 __device__ __forceinline__ float at_swap_max(float x) {
@@ -186,14 +192,16 @@ __device__ __forceinline__ AtRange at_range(int p_min, int p_max, int window, in
   return r;
 }
 // the most units any row tile of a request of `len` tokens walks
-__host__ __device__ __forceinline__ int at_most(int64_t len, int window, int sinks, int TQ, int unit) {
+__host__ __device__ __forceinline__ int at_most(int len, int window, int sinks, int TQ, int unit) {
   if (len <= 0) return 0;
-  const int64_t all = (len - 1) / unit + 1;
+  const uint32_t all = (uint32_t)(len - 1) / unit + 1;
   if (!window) return (int)all;
-  const int64_t groups = ((sinks < len ? sinks : len) + 15) / 16 + ((int64_t)window + TQ + 13) / 16 + 1;
-  const int64_t w = (16 * groups + unit - 1) / unit;
+  const uint32_t groups = ((uint32_t)(sinks < len ? sinks : len) + 15) / 16 + ((uint32_t)window + TQ + 13) / 16 + 1;
+  const uint32_t w = (groups + unit / 16 - 1) / (unit / 16);
   return (int)(w < all ? w : all);
 }
+// x / d, given 2^32 / d + 1 (d = 1: 0); at_tiles says where this is the quotient
+__device__ __forceinline__ int at_div(uint32_t x, uint32_t by) { return by ? (int)__umulhi(x, by) : (int)x; }
 
 // One row tile of one request and head group, units it0 .. it1 - 1 of its I: part `split` of ns, kept in `slot` when ns > 1.
 struct AtItem {
@@ -959,12 +967,12 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
   asm volatile("" : "+v"(t));                              // nothing per lane is kept in registers from one item to the next
   const int lane = t & 63, r16 = lane & 15, g4 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int b = __builtin_amdgcn_readfirstlane(item.b), hg = item.hh % a.HG, kv = item.hh / a.HG, ns = item.ns;
+  const int b = __builtin_amdgcn_readfirstlane(item.b), kv = item.hh, ns = item.ns;   // G = HT heads: no groups
   const int tok0 = item.tt * a.TQ, toks = min(a.TQ, item.n - tok0);
-  const int heads = min(a.HT, a.G - hg * a.HT);
-  const int qt = r16 / a.HT, qh = r16 - qt * a.HT;         // this lane's query row
-  const bool valid = qt < toks && qh < heads;
-  const int head = kv * a.G + hg * a.HT + qh;
+  auto token = [&](int row) { return (int)((uint32_t)row * a.by_ht >> 16); };   // row / HT
+  const int qt = token(r16), qh = r16 - qt * a.HT;         // this lane's query row
+  const bool valid = qt < toks;
+  const int head = kv * a.G + qh;
   const int base_pos = item.len - item.n + tok0;
   if (a.meta && item.it0 == 0 && t < toks)
     a.meta[(size_t)(item.s0 + tok0 + t) * a.Hh + item.hh] = make_int2(item.slot, ns | (t << 16));
@@ -992,37 +1000,37 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
   const bool zero = c == 0.0f;
   c = zero ? 1.0f : fabsf(c);
   uint4 qraw[2 * C::KCB];
-  {
-    const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + qt) * a.q_stride + head * C::DK + 16 * g4;
+  {                                                        // lanes without a row take the last token's: no branches
+    const uint16_t* qp = a.q + (int64_t)(item.s0 + tok0 + min(qt, toks - 1)) * a.q_stride + head * C::DK + 16 * g4;
 #pragma unroll
-    for (int s = 0; s < 2 * C::KCB; ++s) {
-      qraw[s] = make_uint4(0, 0, 0, 0);
-      if (valid && !zero) qraw[s] = *reinterpret_cast<const uint4*>(qp + 64 * (s >> 1) + 8 * (s & 1));
-    }
+    for (int s = 0; s < 2 * C::KCB; ++s) qraw[s] = *reinterpret_cast<const uint4*>(qp + 64 * (s >> 1) + 8 * (s & 1));
   }
   const int pos = base_pos + qt;
-  const int wp_min = base_pos, wp_max = base_pos + min(toks - 1, 15 / a.HT);
+  const int wp_min = base_pos, wp_max = base_pos + toks - 1;
 
   // Copies and reads as in at_tile, the cell at place p of row x being p ^ (x / 4) % 4 ^ 2 (x / 16): the last term keeps the
   // rows of both groups, which one transposing read of V takes together, in different banks.
   const int cr = lane / 4, cell = (lane & 3) ^ g4;
   const uint32_t lds0 = lds_addr(lds) + wave * C::STAGE;
-  size_t crow[2];
+  size_t crow[2];                                          // rows of the groups' first keys, and this lane's key behind it:
+  uint32_t ckey[2];                                        // pages end where groups do, so it is in the group
   AtScales scales[2];                                      // of the tile that is being copied
   auto rows_of = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const int page = at_page(a, kg[x].id);
-      crow[x] = at_row(a, rg, kg[x], page, kv, cr);
+      const int page = __builtin_amdgcn_readfirstlane(at_page(a, kg[x].id)), j = kg[x].g0 + cr;
+      crow[x] = (((size_t)page * a.Hkv + kv) << a.page_shift) + (kg[x].g0 & ((1 << a.page_shift) - 1));
+      ckey[x] = j <= rg.p_max && (j >= rg.lo || j < rg.sinks) ? cr : kg[x].fb - kg[x].g0;
       scales[x] = at_scales(a, kg[x], page, kv);
     }
   };
   auto issue = [&](const uint8_t* from, int dim, uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const uint8_t* p = from + crow[x] * dim + 16 * (cell ^ (2 * x));
+      const uint8_t* p = from + crow[x] * dim;
+      const uint32_t at = ckey[x] * dim + 16 * (cell ^ (2 * x));
 #pragma unroll
-      for (int cb = 0; cb < dim / 64; ++cb) at_copy16(p + cb * 64, stage + cb * (C::KEYS * 64) + x * 1024);
+      for (int cb = 0; cb < dim / 64; ++cb) at_copy16(p + cb * 64, at, stage + cb * (C::KEYS * 64) + x * 1024);
     }
   };
   auto issue_k = [&]() __attribute__((always_inline)) { issue(a.k, C::DK, lds0); };
@@ -1049,10 +1057,12 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
   float m = -INFINITY, l = 0.0f;                           // l: this lane's keys
   bf16x8 Q[2 * C::KCB], P, rest;
   float k_by[2], v_by[2];
-  auto take_q = [&]() __attribute__((always_inline)) {     // once the first copies are on their way
+  const uint32_t keep = zero ? 0u : 0xFFFFFFFFu;
+  auto take_q = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int s = 0; s < 2 * C::KCB; ++s)
-      Q[s] = __builtin_bit_cast(bf16x8, make_uint4(qraw[s].x ^ flip, qraw[s].y ^ flip, qraw[s].z ^ flip, qraw[s].w ^ flip));
+      Q[s] = __builtin_bit_cast(bf16x8, make_uint4((qraw[s].x ^ flip) & keep, (qraw[s].y ^ flip) & keep, (qraw[s].z ^ flip) & keep,
+                                                   (qraw[s].w ^ flip) & keep));
   };
   auto scores = [&]() __attribute__((always_inline)) {
     constexpr int F = 2 * C::KCB, AHEAD = 2 * C::KCB < 4 ? 2 * C::KCB : 4;
@@ -1077,11 +1087,13 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
     for (int x = 0; x < 2; ++x) {
       const int j0 = rg.key(g0 + x) + 4 * g4;
       const uint32_t back = (uint32_t)(pos - j0);
-      const int first = rg.key(g0 + x) < a.sinks ? min(a.sinks, pos + 1) - j0 : 0;   // first tokens that the row sees
+      if (rg.key(g0 + x) >= a.sinks) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float s = S[x][i];
-        S[x][i] = back - (uint32_t)i < span || i < first ? s : -INFINITY;
+        for (int i = 0; i < 4; ++i) S[x][i] = back - (uint32_t)i < span ? S[x][i] : -INFINITY;
+      } else {
+        const int first = min(a.sinks, pos + 1) - j0;      // first tokens that the row sees
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[x][i] = back - (uint32_t)i < span || i < first ? S[x][i] : -INFINITY;
       }
     }
   };
@@ -1133,12 +1145,12 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
 
   constexpr int NK = 2 * C::KCB, NV = 2 * C::VCB;
   const int end = min(it1, (rg.gt - wg + UG - 1) / UG);    // of the units that hold groups of this wave
+  if (it0 < end) rows_of();
+  take_q();                                                // before the copies: the wait for q would be for them as well
   if (it0 < end) {
-    rows_of();
     issue_k();
     issue_v();
   }
-  take_q();
   for (int it = it0; it < end; ++it) {
     const int g0 = it * UG + wg;
     const bool more = it + 1 < end;
@@ -1194,10 +1206,10 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
   if (suspect) {
 #pragma unroll 1
     for (int r = 0; r < 16; ++r) {
-      const int rt = r / a.HT, rh = r - rt * a.HT;
-      if (rt >= toks || rh >= heads) continue;
+      const int rt = token(r), rh = r - rt * a.HT;
+      if (rt >= toks) continue;
       float o[C::VCB], mr, lr;
-      at_slow<C>(a, rg, b, kv, it0, it1, wg, 2, a.q + (int64_t)(item.s0 + tok0 + rt) * a.q_stride + (kv * a.G + hg * a.HT + rh) * C::DK,
+      at_slow<C>(a, rg, b, kv, it0, it1, wg, 2, a.q + (int64_t)(item.s0 + tok0 + rt) * a.q_stride + (kv * a.G + rh) * C::DK,
                  base_pos + rt, a.scale * kLog2e, o, mr, lr);
 #pragma unroll
       for (int e = 0; e < C::VCB; ++e) po[(wave * 16 + r) * C::DV + 4 * ((16 * e + lane / 4 + r) & (NP - 1)) + (lane & 3)] = o[e];
@@ -1212,12 +1224,12 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
   }
   __syncthreads();
   for (int e = t; e < 16 * NP; e += AT_THREADS) {
-    const int row = e / NP, piece = e & (NP - 1), rt = row / a.HT, rh = row - rt * a.HT;
-    if (rt >= toks || rh >= heads) continue;
+    const int row = e / NP, piece = e & (NP - 1), rt = token(row), rh = row - rt * a.HT;
+    if (rt >= toks) continue;
     float mw[4], top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; ++w) mw[w] = pm[2 * (16 * w + row)], top = fmaxf(top, mw[w]);
-    const int hd = kv * a.G + hg * a.HT + rh;
+    const int hd = kv * a.G + rh;
     const float sink = ns == 1 && a.sink_logits ? a.sink_logits[hd] * kLog2e : -INFINITY;
     const float all = fmaxf(top, sink), ref = all == -INFINITY ? 0.0f : all;
     float tot = ns == 1 ? at_exp2(sink - ref) : 0.0f;
@@ -1280,13 +1292,13 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_wide_kernel(AttendA
 template <class C>
 __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(AttendArgs a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  const int lane = threadIdx.x & 63, hh = blockIdx.x % a.Hh, j = blockIdx.x / a.Hh;
+  const int lane = threadIdx.x & 63, j = at_div(blockIdx.x, a.by_hh), hh = blockIdx.x - j * a.Hh;
   const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
   // without room for parts (no tile can have more than AT_NARROW_MIN units) a share is whole tiles, each counted as one
   int s0, n, len, nt, I;
   auto size = [&](int b) {
     const bool sound = at_request(a, b, s0, n, len);
-    nt = (n + a.TQ - 1) / a.TQ;
+    nt = at_div(n + a.TQ - 1, a.by_tq);
     I = a.meta ? max(1, at_most(len, a.window, a.sinks, a.TQ, C::UNIT)) : 1;
     return sound;
   };
@@ -1343,7 +1355,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
         int64_t x = u - at;
         for (int bit = 20; x >> 32; --bit)
           if (x >= (int64_t)I << bit) x -= (int64_t)I << bit, f_tt += 1 << bit;
-        const uint32_t q = (uint32_t)x / (uint32_t)I;
+        const uint32_t q = nt > 1 ? (uint32_t)x / (uint32_t)I : 0;
         f_b = b, f_tt += q, f_off = (uint32_t)x - q * I;
       }
       const int src = __builtin_ctzll(__ballot(here));
@@ -1512,6 +1524,11 @@ static void at_tiles(int rows, int N, int heads, int kv_heads, AttendArgs& a) {
   a.HG = (a.G + a.HT - 1) / a.HT;
   a.Hh = kv_heads * a.HG;
   a.TQ = std::max(1, std::min(rows / a.HT, N));
+  // Quotients by them are products: x / d is the integer part of x (1/d + e) while x e < 1/d; here e <= 2^-16 with x < 128, and
+  // e <= 2^-32 with x <= 2^20 + 128 and d <= 128, or x <= 2^16 and d <= 1024.  0 stands for 1 / 1.
+  a.by_ht = 65536 / a.HT + 1;
+  a.by_tq = a.TQ == 1 ? 0 : (uint32_t)(0x100000000ull / a.TQ + 1);
+  a.by_hh = a.Hh == 1 ? 0 : (uint32_t)(0x100000000ull / a.Hh + 1);
 }
 
 struct AtRoom {
@@ -1650,7 +1667,7 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   at_tiles(rows, N, heads, cache->kv_heads, a);
   a.target = wide ? AT_WIDE_TARGET : AT_NARROW_TARGET;
   // no tile can walk more units than the table or the window holds; where none has to be split there is no second launch
-  const int most = at_most((int64_t)max_pages * cache->page_size, window, a.sinks, a.TQ, wide ? 64 : 128);
+  const int most = at_most(max_pages * cache->page_size, window, a.sinks, a.TQ, wide ? 64 : 128);
   const bool join = most > (wide ? AT_WIDE_MIN : AT_NARROW_MIN);
   const AtRoom room = at_room(rows, a.target, N, heads, cache->kv_heads, cache->v_dim);
   char* w = static_cast<char*>(ws);
