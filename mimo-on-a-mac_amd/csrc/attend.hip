@@ -92,7 +92,11 @@ constexpr int AT_THREADS = 256;
 constexpr int AT_WIDE_TARGET = 512, AT_NARROW_TARGET = 512;
 // Parts of wide tiles have at least 4 units of 64 keys: 40 tokens of 32/8 heads at 3000 21.7 us; 27.3 with 2, 24.9 with 8.
 // Narrow tiles of up to 2 units of 128 keys (a window of 128) are not split, which saves the join's launch.
-constexpr int AT_WIDE_MIN = 4, AT_NARROW_MIN = 2;
+// Those of 16 rows neither up to 4 units (32 requests of 300 to 380 keys, 64/8 heads, 15.3 us split and 11.0 whole, one of 500 10.4
+// and 11.0, one of 1000 10.5 and 16.7), and up to 8 where there are 512 tiles, or 256 in a window, where as a rule all are full: 64
+// of 500 to 1000 36.9 and 28.8, 32 in a window of 512 17.6 and 13.8.  128 of 30 to 50 and one of 1000, 32/8 heads, 20.7 and
+// 21.9; with 32 requests, 64/8 heads, it would be 11.4 and 16.5 (but all of 600 to 1000 22.1 and 17.9).
+constexpr int AT_WIDE_MIN = 4, AT_NARROW_MIN = 2, AT_FEW_MIN = 4, AT_FULL_MIN = 8;
 constexpr int AT_START = 8;                               // units that a wide block's start and a part's join cost
 
 template <int DK_, int DV_, int DTYPE, int ROWS_> struct AtCfg {
@@ -1294,7 +1298,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, j = at_div(blockIdx.x, a.by_hh), hh = blockIdx.x - j * a.Hh;
   const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
-  // without room for parts (no tile can have more than AT_NARROW_MIN units) a share is whole tiles, each counted as one
+  // without room for parts (no tile can have more units than the host leaves whole) a share is whole tiles, each counted as one
   int s0, n, len, nt, I;
   auto size = [&](int b) {
     const bool sound = at_request(a, b, s0, n, len);
@@ -1668,7 +1672,8 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   a.target = wide ? AT_WIDE_TARGET : AT_NARROW_TARGET;
   // no tile can walk more units than the table or the window holds; where none has to be split there is no second launch
   const int most = at_most(max_pages * cache->page_size, window, a.sinks, a.TQ, wide ? 64 : 128);
-  const bool join = most > (wide ? AT_WIDE_MIN : AT_NARROW_MIN);
+  const bool full = N * a.Hh >= (window ? a.target / 2 : a.target);
+  const bool join = most > (wide ? AT_WIDE_MIN : rows == 32 ? AT_NARROW_MIN : full ? AT_FULL_MIN : AT_FEW_MIN);
   const AtRoom room = at_room(rows, a.target, N, heads, cache->kv_heads, cache->v_dim);
   char* w = static_cast<char*>(ws);
   a.part_o = reinterpret_cast<float*>(w);

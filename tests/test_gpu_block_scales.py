@@ -497,6 +497,15 @@ def test_attend_up_to_sixteen_rows(rng, dims, heads, new, window, sinks, page):
 
 
 @pytest.mark.parametrize("dims", list(DIMS))
+@pytest.mark.parametrize("reqs,heads,longest,window", [(130, (8, 4), 900, 0), (66, (4, 4), 2000, 480), (40, (4, 4), 480, 0), (129, (8, 4), 1100, 0)])
+def test_attend_many_tiles_whole_and_split(rng, dims, reqs, heads, longest, window):
+    """Tiles that fill the card and are not split, one as long as the table beside short ones, and some that are."""
+    lens = rng.integers(1, 60, reqs).tolist()
+    lens[reqs // 2], lens[-1] = longest, longest - 77
+    _check(*_attend_case(rng, lens, [1] * reqs, *heads, *DIMS[dims], 64, window, 0, True), few=True)
+
+
+@pytest.mark.parametrize("dims", list(DIMS))
 @pytest.mark.parametrize("window,sinks", [(0, 0), (30, 0), (30, 20)])
 def test_attend_few_rows_with_values_that_are_not_finite(rng, dims, window, sinks):
     """NaN in keys' values at both ends of a window: only the rows that see them have it, tile by tile."""
