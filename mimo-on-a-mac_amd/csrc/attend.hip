@@ -140,10 +140,22 @@ __device__ __forceinline__ void at_copy16(const uint8_t* src, uint32_t lds) {
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory", "m0");
 }
-// the same from src (wave-uniform) + at
-__device__ __forceinline__ void at_copy16(const uint8_t* src, uint32_t at, uint32_t lds) {
+// The same from src (wave-uniform) + at, + 64 and so on, CB times, to places 2048 bytes apart.  An instruction's offset counts
+// for both addresses.
+template <int CB> __device__ __forceinline__ void at_copies16(const uint8_t* src, uint32_t at, uint32_t lds) {
+  static_assert(CB >= 1 && CB <= 3);
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(src), "s"(m) : "memory", "m0");
+  if constexpr (CB == 1)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(src), "s"(m) : "memory", "m0");
+  else if constexpr (CB == 2)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
+                 "s_add_u32 m0, %2, 1984\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:64"
+                 ::"v"(at), "s"(src), "s"(m) : "memory", "m0", "scc");
+  else
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
+                 "s_add_u32 m0, %2, 1984\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:64\n\t"
+                 "s_add_u32 m0, %2, 3968\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:128"
+                 ::"v"(at), "s"(src), "s"(m) : "memory", "m0", "scc");
 }
 #pragma clang diagnostic pop
 
@@ -1028,17 +1040,17 @@ __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, con
       scales[x] = at_scales(a, kg[x], page, kv);
     }
   };
-  auto issue = [&](const uint8_t* from, int dim, uint32_t stage) __attribute__((always_inline)) {
+  static_assert(C::KEYS * 64 == 2048);
+  auto issue_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const uint8_t* p = from + crow[x] * dim;
-      const uint32_t at = ckey[x] * dim + 16 * (cell ^ (2 * x));
-#pragma unroll
-      for (int cb = 0; cb < dim / 64; ++cb) at_copy16(p + cb * 64, at, stage + cb * (C::KEYS * 64) + x * 1024);
-    }
+    for (int x = 0; x < 2; ++x)
+      at_copies16<C::KCB>(a.k + crow[x] * C::DK, ckey[x] * C::DK + 16 * (cell ^ (2 * x)), lds0 + x * 1024);
   };
-  auto issue_k = [&]() __attribute__((always_inline)) { issue(a.k, C::DK, lds0); };
-  auto issue_v = [&]() __attribute__((always_inline)) { issue(a.v, C::DV, lds0 + C::KBYTES); };
+  auto issue_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+      at_copies16<C::VCB>(a.v + crow[x] * C::DV, ckey[x] * C::DV + 16 * (cell ^ (2 * x)), lds0 + C::KBYTES + x * 1024);
+  };
   const uint8_t* st = lds + wave * C::STAGE;
   const int k_at = r16 * 64 + 16 * (g4 ^ (r16 >> 2));
   const int v_at = (4 * g4 + ((r16 >> 1) & 3) + 16 * (r16 >> 3)) * 64 + 16 * (g4 ^ (2 * (r16 >> 3))) + 8 * (r16 & 1);
@@ -1300,16 +1312,23 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
   const int per = (a.B + 63) / 64, b0 = min(a.B, lane * per), b1 = min(a.B, b0 + per);
   // without room for parts (no tile can have more units than the host leaves whole) a share is whole tiles, each counted as one
   int s0, n, len, nt, I;
-  auto size = [&](int b) {
+  auto read = [&](int b) {
     const bool sound = at_request(a, b, s0, n, len);
     nt = at_div(n + a.TQ - 1, a.by_tq);
     I = a.meta ? max(1, at_most(len, a.window, a.sinks, a.TQ, C::UNIT)) : 1;
     return sound;
   };
+  // the lane's first request, as a rule its only one, is kept
+  int first[5] = {0, 0, 0, 0, 0};
+  auto size = [&](int b) {
+    if (b == b0) s0 = first[0], n = first[1], len = first[2], nt = first[3], I = first[4];
+    else read(b);
+  };
   int64_t mine = 0;
   int tiles = 0;
   for (int b = b0; b < b1; ++b) {
-    const bool sound = size(b);
+    const bool sound = read(b);
+    if (b == b0) first[0] = s0, first[1] = n, first[2] = len, first[3] = nt, first[4] = I;
     mine += (int64_t)nt * I;
     tiles = sound ? min(tiles + nt, AT_REFUSED) : AT_REFUSED;
   }
@@ -1335,7 +1354,7 @@ __global__ void __launch_bounds__(AT_THREADS, C::WGS) attend_narrow_kernel(Atten
   // alone do not fill the card (one request of 32768 keys, 64/4 heads: 25.6 us with 256 blocks, 27.8 with 512; 8 of 4000: 24.1
   // and 25.5; a limit of 32 units changes neither)
   const bool few = total * a.Hh <= 8 * (a.target / 2) && (int64_t)tiles * a.Hh < a.target / 2;
-  const int most = max(1, (few ? a.target / 2 : a.target) / a.Hh);
+  const int most = max(1, at_div(few ? a.target / 2 : a.target, a.by_hh));
   const uint32_t shares = total >= most ? most : max(1, (int)total);
   // share x begins at unit (x coarse / shares) << sh, sh chosen so that 32 bits hold the products: no 64-bit division
   const int sh = max(0, 65 - __builtin_clzll(total | 1) - __builtin_clz(shares));
