@@ -39,15 +39,15 @@
 // 0.97 (sums moved between the register files); the next tile's products woven into the softmax by hand 0.58 (spills; heads
 // of 64, which have the room, 0.59 against 0.70); row sums by a matrix product, operands read further ahead, wave priorities:
 // no change.  Heads of 64: the exponentials (16 cycles for 64 of them) and what is around them, 0.66-0.70 PFLOP/s.
-// No vector register is spilled; 9 to 14 (wide) and 48 to 52 (narrow) scalar ones are, to lanes of a vector register.
-// Block scales: the same chunk 1598-1611 us where a head's scales take 1649 and K turned into bf16 by every wave 1721 (on another
+// No vector register is spilled; 9 to 20 (wide) and 56 to 81 (narrow) scalar ones are, to lanes of a vector register.
+// Block scales: the same chunk 1582-1616 us where a head's scales take 1649 and K turned into bf16 by every wave 1721 (on another
 // card 1678); chunks of heads of 64 in a window of 1111, 24 requests, 54 us (51 with a head's scales).
 // Narrow: HBM.  48 requests of 500 to 16384 keys (1.03 GB) 187 us, 5.5 TB/s; 32 of 1000 to 32768 in E4M3 (1.13 GB) 206 us, 5.4
 // TB/s, above a large copy's 4.9 (read and written); a call of few keys 9 us, a chain of round trips (starts and lengths,
 // the table, K and V, the waves' parts through LDS).  Block scales: 48 requests of 500 to 16384 keys, 32/8 heads of 128 (825 MB)
-// 155 us, 5.3 TB/s (157 with a head's scales, in tiles of 32 rows), one of 32768 19.1 (20.1), 128 in a window of 128 20.5 (22.5):
-// in tiles of 32 rows these took 23.5, of which 2.2 were the blocks' start, 3.2 the work's search, and each of two tiles took
-// 2.4-3.3 for its first keys, 4 for two steps and 1.8 to join.
+// 153 us, 5.4 TB/s (157 with a head's scales, in tiles of 32 rows), one of 32768 17.4 (20.1), 128 in a window of 128 18.6 (22.5):
+// of this, 2.2 us are the blocks' start, 3 the work's search, and each of two tiles takes 2-3 for its first keys, 3 for two
+// steps and 1.2 to join.
 #include <algorithm>
 #include <atomic>
 #include <mutex>
@@ -973,10 +973,14 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
 // One item in tiles of 16 rows, over block scales: v_mfma_f32_16x16x32_bf16, so that requests of up to 16 rows leave no half of
 // the products, of the softmax and of the registers empty.  S^T = K Q^T: lane (c, g) = (l % 16, l / 16) holds, for query row c,
 // keys 4 g + i of each of the wave's two groups of 16, whose scales are one number each; P^T, as it stands, is the B operand of
-// the 32 keys in the order (g, group, i), in which the transposing reads of V fetch them.  Against tiles of 32 rows: one request
-// of 32768 keys, 64/4 heads of 192/128, 19.1 us (20.9), 48 of 500 to 16384, 32/8 of 128, 155 (159), 128 in a window of 128, 64/8
-// of 192/128, 20.5 (23.4), one of 40, 8/2 of 64, 6.0 (6.8).  The first three with more blocks a CU, 3: 20.6, 159, 21.5; 4: 26.5,
-// 199, 27.7 (spills); with a second tile on its way 20.1, 162, 20.5; with operands read 2 instead of 4 ahead 19.3, 156, 20.6.
+// the 32 keys in the order (g, group, i), in which the transposing reads of V fetch them.
+// One request of 32768 keys, 64/4 heads of 192/128, 17.4 us, 48 of 500 to 16384, 32/8 of 128, 153, 128 in a window of 128, 64/8 of
+// 192/128, 18.6, one of 40, 8/2 of 64, 5.3.  In tiles of 32 rows these took 20.9, 159, 23.4 and 6.8, where the first tiles of 16
+// took 19.1, 155, 20.5 and 6.0.  Beside those the first three took, with more blocks a CU, 3: 20.6, 159, 21.5; 4: 26.5, 199, 27.7
+// (spills, whose loads wait for the copies too); with a second tile on its way 20.1, 162, 20.5; with operands read 2 instead of
+// 4 ahead 19.3, 156, 20.6; blocks of 6 waves 19.5, 158 and 27.6 (two do not fit on a CU).
+// What counts for the short ones is the number of instructions, some 5 cycles each with two waves on a SIMD: what a wave holds as
+// one number is kept in scalar registers, addresses are a scalar and a lane's 32 bits, quotients are products.
 template <class C>
 __device__ __forceinline__ void at_tile16(const AttendArgs& a, uint8_t* lds, const AtItem& item) {
   int t = threadIdx.x;
@@ -1683,7 +1687,7 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   a.scale = scale, a.out = out, a.status = status;
   // narrow tiles hold the rows of a request in 32, wide ones are up to a quarter filled: at 5 to 8 rows of 8 heads the wide
   // ones take 132-136 us for 32 requests of 4000 keys, two and more narrow tiles 136-139, and at 12 143 against 356.  Over block scales those of up to 16 rows have tiles of 16 (at_tile16), which also at 16 rows, 16 heads of 192/128 at 300
-  // keys, take 11.0 us against 12.1
+  // keys, took 11.0 us against 12.1
   const int64_t per_request = (int64_t)std::min(max_new, N) * (heads / cache->kv_heads);
   const bool wide = per_request > 32;
   const int rows = wide ? 128 : (cache->dtype == MIMO_KV_E4M3_BLOCKS && per_request <= 16 ? 16 : 32);
