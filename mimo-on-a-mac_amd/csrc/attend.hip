@@ -141,18 +141,18 @@ __device__ __forceinline__ void at_copy16(const uint8_t* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory", "m0");
 }
 // The same from src (wave-uniform) + at, + 64 and so on, CB times, to places 2048 bytes apart.  An instruction's offset counts
-// for both addresses.
+// for both addresses.  The first wait is for src too: a vector instruction that wrote it (a readlane) has to be 5 wait states back.
 template <int CB> __device__ __forceinline__ void at_copies16(const uint8_t* src, uint32_t at, uint32_t lds) {
   static_assert(CB >= 1 && CB <= 3);
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
   if constexpr (CB == 1)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(src), "s"(m) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(at), "s"(src), "s"(m) : "memory", "m0");
   else if constexpr (CB == 2)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
                  "s_add_u32 m0, %2, 1984\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:64"
                  ::"v"(at), "s"(src), "s"(m) : "memory", "m0", "scc");
   else
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1\n\t"
                  "s_add_u32 m0, %2, 1984\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:64\n\t"
                  "s_add_u32 m0, %2, 3968\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:128"
                  ::"v"(at), "s"(src), "s"(m) : "memory", "m0", "scc");
