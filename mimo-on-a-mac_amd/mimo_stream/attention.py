@@ -292,8 +292,8 @@ class Rotary:
             raise ValueError("the rotary dimension must be a multiple of 16 up to 256")
         if not theta > 0.0:
             raise ValueError("theta must be positive")
-        self.dim, self.interleaved, self.magnitude = int(dim), bool(interleaved), float(magnitude)
-        if not math.isfinite(self.magnitude) or abs(self.magnitude) > 3.4e38:
+        magnitude = float(magnitude)
+        if not math.isfinite(magnitude) or abs(magnitude) > 3.4e38:
             raise ValueError("magnitude must be a finite fp32")
         if frequencies is None:
             frequencies = float(theta) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
@@ -301,12 +301,26 @@ class Rotary:
             frequencies = torch.as_tensor(frequencies).detach().to(device="cpu", dtype=torch.float64)
             if frequencies.shape != (dim // 2,) or not bool(torch.isfinite(frequencies).all()):
                 raise ValueError(f"frequencies: need {dim // 2} finite numbers, got shape {tuple(frequencies.shape)}")
-        self._turns = (frequencies / (2.0 * math.pi)).to(_device(device))
-        self._struct = _lib.MimoRotary(self._turns.data_ptr(), self.dim, self.interleaved, self.magnitude)
-        self._at = ctypes.addressof(self._struct)
-        self._index = self._turns.device.index if self._turns.is_cuda else -1
+        self._bind((frequencies / (2.0 * math.pi)).to(_device(device)), int(dim), bool(interleaved), magnitude)
 
-    turns = property(lambda self: self._turns)               # fixed: the struct holds its address
+    def _bind(self, turns, dim, interleaved, magnitude):
+        self._turns, self._dim, self._interleaved, self._magnitude = turns, dim, interleaved, magnitude
+        self._struct = _lib.MimoRotary(turns.data_ptr(), dim, interleaved, magnitude)
+        self._at = ctypes.addressof(self._struct)
+        self._index = turns.device.index if turns.is_cuda else -1
+
+    # fixed: the struct holds them
+    turns = property(lambda self: self._turns)
+    dim = property(lambda self: self._dim)
+    interleaved = property(lambda self: self._interleaved)
+    magnitude = property(lambda self: self._magnitude)
+
+    # a copied or saved Rotary is its numbers; the struct, which holds an address, is made anew
+    def __getstate__(self):
+        return {"turns": self._turns, "dim": self._dim, "interleaved": self._interleaved, "magnitude": self._magnitude}
+
+    def __setstate__(self, state):
+        self._bind(state["turns"], state["dim"], state.get("interleaved", False), state.get("magnitude", 1.0))
 
 
 def _rows(x, dev, heads, dim, name):
@@ -341,7 +355,7 @@ def append(cache, plan, k, v, q=None, rotary=None):
     scale of each head grows where the new values need it, and what the block holds is kept: exactly, but for values below
     2 ** -6 of the new scale, which are rounded to 2 ** -9 of it.  Values past 448 * 2 ** 119 saturate, infinities among
     them."""
-    if cache._call is not None and (rotary is None or rotary.dim <= cache.k_dim):
+    if cache._call is not None and (rotary is None or rotary._dim <= cache.k_dim):
         done = cache._calls.append(cache._call, _current_device(), _raw_stream(cache.device.index), plan.slots, plan.positions, plan.status,
                                    plan.page_size, k, v, q, 0 if rotary is None else rotary._at, -1 if rotary is None else rotary._index)
         if done is not NotImplemented:

@@ -1,7 +1,9 @@
 """Refusals of the cache with block scales, of the rotary forms and of read, without a GPU."""
+import copy
 import ctypes
 import math
 import os
+import pickle
 
 import pytest
 import torch
@@ -55,6 +57,24 @@ def test_rotary_forms_arguments():
 def test_stretched_arguments(bad):
     with pytest.raises(ValueError):
         stretched(**{**dict(dim=64, theta=10000.0, factor=2.0, original=4096), **bad})
+
+
+@pytest.mark.parametrize("again", [copy.copy, copy.deepcopy, lambda r: pickle.loads(pickle.dumps(r))])
+def test_rotary_is_copied_and_saved(again):
+    r = Rotary(64, 5000.0, device="cpu", interleaved=True, magnitude=0.75)
+    c = again(r)
+    assert (c.dim, c.interleaved, c.magnitude) == (64, True, 0.75) and torch.equal(c.turns, r.turns)
+    s = c._struct                                          # what the kernels are given: the copy's own numbers
+    assert (s.turns, s.dim, s.interleaved, s.magnitude) == (c.turns.data_ptr(), 64, 1, 0.75) and c._at == ctypes.addressof(s)
+    before = Rotary.__new__(Rotary)                        # saved when there was one form
+    before.__setstate__({"dim": 64, "turns": r.turns})
+    assert (before.dim, before.interleaved, before.magnitude) == (64, False, 1.0)
+
+
+@pytest.mark.parametrize("name,value", [("dim", 32), ("interleaved", True), ("magnitude", 2.0), ("turns", torch.zeros(32))])
+def test_rotary_is_fixed(name, value):
+    with pytest.raises(AttributeError):                    # and not a change that the kernels would not see
+        setattr(Rotary(64, device="cpu"), name, value)
 
 
 def test_slots_of_a_request():
