@@ -293,7 +293,7 @@ int mimo_cache_append_rotary(const uint16_t* q, int64_t q_stride, int heads, con
 
 /* Cached tokens back as rows: k_out bf16 [N, kv_heads, k_dim] and v_out [N, kv_heads, v_dim], row n from slots[n] (in any order,
  * any slot any number of times), code times scale in 32 bits, rounded to bf16; a slot below 0 gives a row of 0.  The outputs may not overlap
- * the cache, the slots or one another.  N is below 2^24.  status (optional, not cleared) receives MIMO_ERR_SLOT for a slot past
+ * the cache, its scales, the slots or one another.  N is below 2^24.  status (optional, not cleared) receives MIMO_ERR_SLOT for a slot past
  * the cache, whose row is 0.  (The reference slices its cache arrays, engine/mimo_stream/mimo_v2.py:110-150.) */
 int mimo_cache_read(const mimo_kv_cache* cache, const int32_t* slots, int N, uint16_t* k_out, uint16_t* v_out,
                     int32_t* status, void* stream);

@@ -757,6 +757,12 @@ int mimo_cache_read(const mimo_kv_cache* cache, const int32_t* slots, int N, uin
     MIMO_REQUIRE(!overlap(outs[i], sizes[i], cache->k, rows * kn) && !overlap(outs[i], sizes[i], cache->v, rows * vn) &&
                      !overlap(outs[i], sizes[i], slots, (size_t)N * 4),
                  MIMO_ERR_ARG, "cache_read: outputs may not overlap the cache or the slots");
+  if (cache->dtype != MIMO_KV_BF16) {
+    const size_t scales = cache->dtype == MIMO_KV_E4M3 ? (size_t)cache->kv_heads * 4 : (size_t)cache->n_pages * cache->kv_heads * (cache->page_size / 16);
+    for (int i = 0; i < 2; ++i)
+      MIMO_REQUIRE(!overlap(outs[i], sizes[i], cache->k_scale, scales) && !overlap(outs[i], sizes[i], cache->v_scale, scales), MIMO_ERR_ARG,
+                   "cache_read: outputs may not overlap the scales");
+  }
   MIMO_REQUIRE(!overlap(k_out, sizes[0], v_out, sizes[1]), MIMO_ERR_ARG, "cache_read: k_out may not overlap v_out");
   ReadArgs a{static_cast<const uint8_t*>(cache->k), static_cast<const uint8_t*>(cache->v), cache->k_scale, cache->v_scale, slots,
              k_out, v_out, status, N, cache->kv_heads, cache->k_dim, cache->v_dim, __builtin_ctz(cache->page_size),

@@ -142,6 +142,12 @@ def test_read_refusals(bad, code):
     assert _read(**bad) == getattr(_lib, "ERR_" + code)
 
 
+@pytest.mark.parametrize("dtype", [_lib.KV_E4M3, _lib.KV_E4M3_BLOCKS])
+@pytest.mark.parametrize("scales", [dict(k_scale=OUT), dict(v_scale=OUT), dict(k_scale=OUT + 1024 + 240), dict(v_scale=OUT + 1024)])
+def test_read_refuses_outputs_over_scales(dtype, scales):
+    assert _read(_kv(dtype=dtype, **scales)) == _lib.ERR_ARG
+
+
 @pytest.mark.parametrize("bad,code", BAD_CACHES)
 def test_cache_refusals(bad, code):
     assert _append(_kv(**bad)) == getattr(_lib, "ERR_" + code)
