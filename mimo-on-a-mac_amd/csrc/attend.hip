@@ -1688,7 +1688,8 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   // narrow tiles hold the rows of a request in 32, wide ones are up to a quarter filled: at 5 to 8 rows of 8 heads the wide
   // ones take 132-136 us for 32 requests of 4000 keys, two and more narrow tiles 136-139, and at 12 143 against 356.  Over block scales those of up to 16 rows have tiles of 16 (at_tile16), which also at 16 rows, 16 heads of 192/128 at 300
   // keys, took 11.0 us against 12.1
-  const int64_t per_request = (int64_t)std::min(max_new, N) * (heads / cache->kv_heads);
+  // (never 0, whatever max_new says: a K/V head's queries have to fit tiles of 16, which know no groups of them)
+  const int64_t per_request = (int64_t)std::max(1, std::min(max_new, N)) * (heads / cache->kv_heads);
   const bool wide = per_request > 32;
   const int rows = wide ? 128 : (cache->dtype == MIMO_KV_E4M3_BLOCKS && per_request <= 16 ? 16 : 32);
   at_tiles(rows, N, heads, cache->kv_heads, a);

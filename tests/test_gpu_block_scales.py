@@ -497,6 +497,15 @@ def test_attend_up_to_sixteen_rows(rng, dims, heads, new, window, sinks, page):
 
 
 @pytest.mark.parametrize("dims", list(DIMS))
+@pytest.mark.parametrize("heads,new,said", [((17, 1), 1, 0), ((40, 2), 1, 0), ((64, 1), 2, 0), ((132, 2), 1, 0), ((4, 2), 3, 0), ((16, 1), 3, 1), ((8, 2), 9, 2)])
+def test_attend_with_more_new_tokens_than_said(rng, dims, heads, new, said):
+    """max_new picks the kernel and nothing else, also where it says that no request has new tokens."""
+    q, cache, plan, kw = _attend_case(rng, [new, 64, 150, 700], [new, 1, new, new], *heads, *DIMS[dims], 16, 0, 0, True, pad=1)
+    plan.max_new = said
+    _check(q, cache, plan, kw, few=max(said, 1) * heads[0] // heads[1] <= 32)
+
+
+@pytest.mark.parametrize("dims", list(DIMS))
 @pytest.mark.parametrize("reqs,heads,longest,window", [(130, (8, 4), 900, 0), (66, (4, 4), 2000, 480), (40, (4, 4), 480, 0), (129, (8, 4), 1100, 0)])
 def test_attend_many_tiles_whole_and_split(rng, dims, reqs, heads, longest, window):
     """Tiles that fill the card and are not split, one as long as the table beside short ones, and some that are."""
