@@ -269,7 +269,8 @@ def stretched(dim, theta, factor, original, few=1.0, many=32.0):
     """Frequencies fp64 [dim / 2] for contexts `factor` times as long as the `original` length that theta ** (-2 i / dim) was
     trained at: a pair that turns at least `many` times over the original length keeps its frequency, one of at most `few`
     turns has it divided by factor, and those between are blended in proportion to i, from the last whole pair number of
-    `many` turns to the first of `few`."""
+    `many` turns (0 at least) to the first of `few` (dim - 1 at most, past the last pair: where even that one turns more than
+    `few` times, none is divided by the whole factor)."""
     if dim < 2 or dim % 2 or not theta > 1.0 or not factor > 0.0 or not original > 0 or not 0.0 < few < many:
         raise ValueError(f"need an even dim, theta > 1, factor > 0, original > 0 and 0 < few < many (got {dim}, {theta}, {factor}, "
                          f"{original}, {few}, {many})")
@@ -277,8 +278,9 @@ def stretched(dim, theta, factor, original, few=1.0, many=32.0):
     freq = float(theta) ** (-2.0 * i / dim)
     # pair i turns original theta ** (-2 i / dim) / 2 pi times
     first, last = (0.5 * dim * math.log(original / (2.0 * math.pi * turns)) / math.log(theta) for turns in (many, few))
-    first, last = max(math.floor(first), 0), min(math.ceil(last), dim // 2 - 1)
-    slow = ((i - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)
+    first, last = max(math.floor(first), 0), min(math.ceil(last), dim - 1)
+    slow = ((i - first) / max(last - first, 1)).clamp(0.0, 1.0)
+    slow[i >= last] = 1.0                                    # pair 0 as well, where it has few turns already
     return freq * (1.0 - slow * (1.0 - 1.0 / factor))
 
 

@@ -108,10 +108,10 @@ def stretched(dim, theta, factor, original, few, many):
 
     def pair_of(turns):                                    # the real pair number whose frequency makes that many turns
         return dim * np.log(original / (2 * np.pi * turns)) / (2 * np.log(theta))
-    lo, hi = max(int(np.floor(pair_of(many))), 0), min(int(np.ceil(pair_of(few))), dim // 2 - 1)
+    lo, hi = max(int(np.floor(pair_of(many))), 0), min(int(np.ceil(pair_of(few))), dim - 1)
     out = []
     for i, f in enumerate(freq):
-        share = min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0)
+        share = 1.0 if i >= hi else 0.0 if i <= lo else (i - lo) / (hi - lo)
         out.append((1 - share) * f + share * f / factor)
     return np.array(out)
 
