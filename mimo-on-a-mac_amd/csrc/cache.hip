@@ -540,9 +540,10 @@ __global__ void __launch_bounds__(256, 4) cache_append_scaled_kernel(AppendArgs 
   }
   const int x = b / parts, n0 = x % C * SB_ROWS + x / C * W, lane = threadIdx.x & 63;
   if (n0 >= a.N) return;
-  // lane l: row n0 - 1 + l, up to the 16 rows behind the last
+  // lane l: row n0 - 1 + l, up to the 31 rows behind the last: a block's first piece (16 rows at most), up to 15 rows of others
+  // and the next piece's first row
   const int at = n0 - 1 + lane;
-  const int slot = lane <= W + SB_ROWS && at >= 0 && at < a.N ? a.slots[at] : -1, before = __shfl_up(slot, 1, 64);
+  const int slot = lane <= W + 2 * SB_ROWS - 1 && at >= 0 && at < a.N ? a.slots[at] : -1, before = __shfl_up(slot, 1, 64);
   const bool mine = lane >= 1 && lane <= W;
   if (mine && slot >= a.n_slots && threadIdx.x < 64 && a.status) a.status[0] = MIMO_ERR_SLOT;
   uint64_t first = __ballot(mine && slot >= 0 && slot < a.n_slots && slot >> SB_SHIFT != before >> SB_SHIFT);
