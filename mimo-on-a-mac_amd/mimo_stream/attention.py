@@ -29,7 +29,8 @@ INT32 = torch.int32
 
 STATUS_MESSAGES = {_lib.ERR_PAGES: "fewer free pages than the step needs",
                    _lib.ERR_SHAPE: "request lengths or starts outside the page table, the rows or max_new",
-                   _lib.ERR_SLOT: "a page or slot outside the cache"}
+                   _lib.ERR_SLOT: "a page or slot outside the cache, or, with block scales, a slot written twice or rows of a block of "
+                                  "16 slots that others part"}
 
 # A decode step makes one step call and two calls per layer, each of a few microseconds on the GPU: what they do on the host
 # is kept short.  append, read and attend hand a call to _lib.calls() first, which takes it in its ordinary form (csrc/calls.cpp)

@@ -156,3 +156,11 @@ def test_cache_refusals(bad, code):
 
 def test_empty_calls_need_no_gpu():
     assert _append(N=0) == 0 and _append(N=0, rotary=None) == 0 and _read(N=0) == 0
+
+
+def test_what_a_slot_failure_may_be():
+    """A plan whose slots are all inside the cache, but not together, is not told that one is outside alone."""
+    plan = StepPlan(status=torch.tensor([_lib.ERR_SLOT], dtype=torch.int32))
+    for part in ("outside the cache", "a slot written twice", "that others part"):
+        with pytest.raises(ValueError, match=part):
+            plan.check("append")
