@@ -67,6 +67,13 @@ bool same_pages(PyObject* o, const Cache* c) {
   return o == Py_None || (number(o, &page) && page == c->c.page_size);
 }
 
+// The entries run without the interpreter's lock, which an exception on its way out would have to have again: no tensor is looked
+// at meanwhile, since one without memory of its own (inside of torch.vmap) throws where its address is asked for.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // An exception on its way through C would end the process: an allocation that fails, above all.
 template <class F> PyObject* guarded(F f) {
   try {
@@ -130,11 +137,14 @@ PyObject* append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       heads = q->size(1);
       out = bf16({N, heads, c->c.k_dim}, c->device);
     }
-    int rc;
-    Py_BEGIN_ALLOW_THREADS;
-    rc = append_entry(q ? at_<uint16_t>(q) : nullptr, qs, (int)heads, at_<uint16_t>(k), ks, at_<uint16_t>(v), vs, (int)N, at_<int32_t>(positions),
-                      at_<int32_t>(slots), &c->c, turn, q ? at_<uint16_t>(&out) : nullptr, status, reinterpret_cast<void*>(stream));
-    Py_END_ALLOW_THREADS;
+    const uint16_t *at_q = q ? at_<uint16_t>(q) : nullptr, *at_k = at_<uint16_t>(k), *at_v = at_<uint16_t>(v);
+    const int32_t *at_positions = at_<int32_t>(positions), *at_slots = at_<int32_t>(slots);
+    uint16_t* at_out = q ? at_<uint16_t>(&out) : nullptr;
+    const int rc = [&] {
+      Unlocked u;
+      return append_entry(at_q, qs, (int)heads, at_k, ks, at_v, vs, (int)N, at_positions, at_slots, &c->c, turn, at_out, status,
+                          reinterpret_cast<void*>(stream));
+    }();
     if (rc) return PyLong_FromLong(rc);
     if (!q) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
@@ -153,10 +163,12 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!int32(slots) || slots->dim() != 1 || slots->size(0) < 1 || slots->size(0) > INT32_MAX || !status_of(a[4], c->device, &status)) return other();
     const int64_t N = slots->size(0);
     at::Tensor k = bf16({N, c->c.kv_heads, c->c.k_dim}, c->device), v = bf16({N, c->c.kv_heads, c->c.v_dim}, c->device);
-    int rc;
-    Py_BEGIN_ALLOW_THREADS;
-    rc = read_entry(&c->c, at_<int32_t>(slots), (int)N, at_<uint16_t>(&k), at_<uint16_t>(&v), status, reinterpret_cast<void*>(stream));
-    Py_END_ALLOW_THREADS;
+    const int32_t* at_slots = at_<int32_t>(slots);
+    uint16_t *at_k = at_<uint16_t>(&k), *at_v = at_<uint16_t>(&v);
+    const int rc = [&] {
+      Unlocked u;
+      return read_entry(&c->c, at_slots, (int)N, at_k, at_v, status, reinterpret_cast<void*>(stream));
+    }();
     if (rc) return PyLong_FromLong(rc);
     PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = pk ? THPVariable_Wrap(std::move(v)) : nullptr;
     PyObject* both = pv ? PyTuple_Pack(2, pk, pv) : nullptr;
@@ -209,11 +221,15 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     } else {
       made = bf16({N, heads, c->c.v_dim}, c->device);
     }
-    int rc;
-    Py_BEGIN_ALLOW_THREADS;
-    rc = attend_entry(at_<uint16_t>(q), qs, (int)N, (int)heads, &c->c, (int)B, at_<int32_t>(starts), at_<int32_t>(lens), at_<int32_t>(table), (int)width,
-                      (int)most, (float)scale, (int)window, (int)sinks, logits, at_<uint16_t>(out), status, ws->data_ptr(), bytes, reinterpret_cast<void*>(stream));
-    Py_END_ALLOW_THREADS;
+    const uint16_t* at_q = at_<uint16_t>(q);
+    const int32_t *at_starts = at_<int32_t>(starts), *at_lens = at_<int32_t>(lens), *at_table = at_<int32_t>(table);
+    uint16_t* at_out = at_<uint16_t>(out);
+    void* room = ws->data_ptr();
+    const int rc = [&] {
+      Unlocked u;
+      return attend_entry(at_q, qs, (int)N, (int)heads, &c->c, (int)B, at_starts, at_lens, at_table, (int)width, (int)most, (float)scale,
+                          (int)window, (int)sinks, logits, at_out, status, room, bytes, reinterpret_cast<void*>(stream));
+    }();
     if (rc) return PyLong_FromLong(rc);
     if (out != &made) {
       Py_INCREF(a[14]);
