@@ -285,6 +285,22 @@ def stretched(dim, theta, factor, original, few=1.0, many=32.0):
     return freq * (1.0 - slow * (1.0 - 1.0 / factor))
 
 
+def _rotary_number(name):
+    """One of a Rotary's numbers: fixed, since its struct holds them.  A class derived from it may set its own, which a call then takes
+    as they are (append)."""
+    def change(self, value):
+        if type(self) is Rotary:
+            raise AttributeError(f"a Rotary's {name} is fixed")
+        self.__dict__["_" + name] = value
+
+    def value(self):
+        try:
+            return self.__dict__["_" + name]
+        except KeyError:
+            raise AttributeError(name) from None
+    return property(value, change)
+
+
 class Rotary:
     """Rotary positions on the first `dim` dimensions of a head (a multiple of 16): pairs (i, i + dim / 2), or (2 i, 2 i + 1) if
     interleaved; frequencies theta ** (-2 i / dim), or the dim / 2 given ones (stretched makes them for long contexts), kept
@@ -312,18 +328,34 @@ class Rotary:
         self._at = ctypes.addressof(self._struct)
         self._index = turns.device.index if turns.is_cuda else -1
 
-    # fixed: the struct holds them
-    turns = property(lambda self: self._turns)
-    dim = property(lambda self: self._dim)
-    interleaved = property(lambda self: self._interleaved)
-    magnitude = property(lambda self: self._magnitude)
+    turns, dim, interleaved, magnitude = (_rotary_number(name) for name in ("turns", "dim", "interleaved", "magnitude"))
 
     # a copied or saved Rotary is its numbers; the struct, which holds an address, is made anew
     def __getstate__(self):
-        return {"turns": self._turns, "dim": self._dim, "interleaved": self._interleaved, "magnitude": self._magnitude}
+        own = ("_turns", "_dim", "_interleaved", "_magnitude")
+        state = {name: value for name, value in self.__dict__.items() if name not in own + ("_struct", "_at", "_index")}
+        return {**state, **{name[1:]: self.__dict__[name] for name in own if name in self.__dict__}}
 
     def __setstate__(self, state):
-        self._bind(state["turns"], state["dim"], state.get("interleaved", False), state.get("magnitude", 1.0))
+        state = dict(state)
+        self._bind(state.pop("turns"), state.pop("dim"), state.pop("interleaved", False), state.pop("magnitude", 1.0))
+        self.__dict__.update(state)
+
+
+def _turns_of(rotary, dev, k_dim):
+    """(struct mimo_rotary, turns to be held until the call is queued): a Rotary's own, or of whatever else has dim and turns (fp64,
+    the first dim / 2 of them) and may have interleaved and magnitude."""
+    dim, turns = rotary.dim, rotary.turns
+    if not 0 <= dim <= k_dim:
+        raise ValueError(f"rotary dimension {dim} past the head's {k_dim}")
+    if turns.device != dev:
+        raise ValueError(f"rotary on {turns.device}, expected {dev}")
+    if type(rotary) is Rotary:
+        return rotary._struct, turns
+    if turns.dtype != torch.float64 or turns.numel() < dim // 2 or not turns.is_contiguous():
+        raise ValueError(f"rotary turns: need contiguous float64 [{dim // 2}], got {turns.dtype} {tuple(turns.shape)}")
+    side, magnitude = getattr(rotary, "interleaved", False), getattr(rotary, "magnitude", 1.0)
+    return _lib.MimoRotary(turns.data_ptr(), int(dim), bool(side), float(magnitude)), turns
 
 
 def _rows(x, dev, heads, dim, name):
@@ -350,7 +382,8 @@ def _rows(x, dev, heads, dim, name):
 def append(cache, plan, k, v, q=None, rotary=None):
     """Write the new tokens' k [N, kv_heads, k_dim] and v [N, kv_heads, v_dim] to plan.slots (rows with slot -1 are left
     out), k rotated to plan.positions; returns q [N, heads, k_dim] rotated likewise (None without q).  q, k and v may be
-    views of one projection's rows; other types than bf16 are rounded to it first.  Slots are distinct.
+    views of one projection's rows; other types than bf16 are rounded to it first.  Slots are distinct.  rotary is a Rotary, or
+    has a dim and fp64 turns [dim / 2] on the cache's device, as one has (interleaved and magnitude if they are not False and 1).
 
     Into a cache with block scales, the rows of one block of 16 slots follow one another, as in the plan of a step, with no
     other row between them, not even one that is left out (a block whose rows do not has undefined contents, and plan.check()
@@ -358,7 +391,7 @@ def append(cache, plan, k, v, q=None, rotary=None):
     scale of each head grows where the new values need it, and what the block holds is kept: exactly, but for values below
     2 ** -6 of the new scale, which are rounded to 2 ** -9 of it.  Values past 448 * 2 ** 119 saturate, infinities among
     them."""
-    if cache._call is not None and (rotary is None or rotary._dim <= cache.k_dim):
+    if cache._call is not None and (rotary is None or (type(rotary) is Rotary and rotary._dim <= cache.k_dim)):
         done = cache._calls.append(cache._call, _current_device(), _raw_stream(cache.device.index), plan.slots, plan.positions, plan.status,
                                    plan.page_size, k, v, q, 0 if rotary is None else rotary._at, -1 if rotary is None else rotary._index)
         if done is not NotImplemented:
@@ -376,13 +409,7 @@ def append(cache, plan, k, v, q=None, rotary=None):
         raise ValueError(f"{N} tokens of k, {v.shape[0]} of v")
     at_slots = _int32(plan.slots, dev, (N,), "plan.slots")
     at_positions = _int32(plan.positions, dev, (N,), "plan.positions")
-    turn = None
-    if rotary is not None:
-        if rotary.dim > cache.k_dim:
-            raise ValueError(f"rotary dimension {rotary.dim} past the head's {cache.k_dim}")
-        if rotary._turns.device != dev:
-            raise ValueError(f"rotary on {rotary._turns.device}, expected {dev}")
-        turn = rotary._struct
+    turn, turns = (None, None) if rotary is None else _turns_of(rotary, dev, cache.k_dim)
     out, at_q, at_out, q_stride, heads = None, None, None, 0, 0
     if q is not None:
         q, at_q, q_stride = _rows(q, dev, None, cache.k_dim, "q")
