@@ -1,9 +1,10 @@
-"""Tensors that have no memory of their own (inside of torch.vmap) given to append, read and attend: an error, and the process goes on."""
+"""The short host path where it cannot serve: tensors that have no memory of their own (inside of torch.vmap) are an error, and the
+process goes on; without the module of the short path every call goes the long way."""
 import numpy as np
 import pytest
 import torch
 
-from mimo_stream import KVCache, PageTable, StepPlan, append, attend, read
+from mimo_stream import KVCache, PageTable, StepPlan, _lib, append, attend, read
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +58,14 @@ def test_attend(what):
     with pytest.raises(RuntimeError, match="data pointer|storage"):
         torch.vmap(call)(_twice(given[what]))
     assert torch.equal(attend(q, cache, plan), want)
+
+
+def test_without_the_module(monkeypatch):
+    *_, want = _state()
+
+    def missing():
+        raise RuntimeError("mimo_stream/_calls.so is not built")
+    monkeypatch.setattr(_lib, "calls", missing)
+    with pytest.warns(RuntimeWarning, match="_calls.so is not built"):
+        cache, plan, q, k, _, got = _state()
+    assert cache._call is None and torch.equal(got, want) and torch.equal(read(cache, plan.slots)[0], k)
