@@ -93,9 +93,12 @@ constexpr int AT_WIDE_TARGET = 512, AT_NARROW_TARGET = 512;
 // Parts of wide tiles have at least 4 units of 64 keys: 40 tokens of 32/8 heads at 3000 21.7 us; 27.3 with 2, 24.9 with 8.
 // Narrow tiles of up to 2 units of 128 keys (a window of 128) are not split, which saves the join's launch.
 // Those of 16 rows neither up to 4 units (32 requests of 300 to 380 keys, 64/8 heads, 15.3 us split and 11.0 whole, one of 500 10.4
-// and 11.0, one of 1000 10.5 and 16.7), and up to 8 where there are 512 tiles, or 256 in a window, where as a rule all are full: 64
-// of 500 to 1000 36.9 and 28.8, 32 in a window of 512 17.6 and 13.8.  128 of 30 to 50 and one of 1000, 32/8 heads, 20.7 and
-// 21.9; with 32 requests, 64/8 heads, it would be 11.4 and 16.5 (but all of 600 to 1000 22.1 and 17.9).
+// and 11.0, one of 1000 10.5 and 16.7), and up to 8 where there are 512 tokens times K/V heads, or 256 in a window, where as a rule
+// all tiles are full: 64 of 500 to 1000 36.9 and 28.8, 32 in a window of 512 17.6 and 13.8.  128 of 30 to 50 and one of 1000, 32/8
+// heads, 20.7 and 21.9; with 32 requests, 64/8 heads, it would be 11.4 and 16.5 (but all of 600 to 1000 22.1 and 17.9).  Where
+// tiles hold several tokens they have to be 128 at least: 8 requests of 16 new tokens at 800 to 1024 keys, 4/4 heads of 64, 32
+// tiles, 9.9 split and 12.8 whole, in a window of 512 11.0 and 11.3 (heads of 128); 32 of 4 tokens at 500 to 1024, 16/4 heads, 128
+// tiles, 16.7 and 15.6; 64 of them, 256 tiles, 21.5 and 16.3.
 constexpr int AT_WIDE_MIN = 4, AT_NARROW_MIN = 2, AT_FEW_MIN = 4, AT_FULL_MIN = 8;
 constexpr int AT_START = 8;                               // units that a wide block's start and a part's join cost
 
@@ -1689,14 +1692,18 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   // ones take 132-136 us for 32 requests of 4000 keys, two and more narrow tiles 136-139, and at 12 143 against 356.  Over block scales those of up to 16 rows have tiles of 16 (at_tile16), which also at 16 rows, 16 heads of 192/128 at 300
   // keys, took 11.0 us against 12.1
   // (never 0, whatever max_new says: a K/V head's queries have to fit tiles of 16, which know no groups of them)
-  const int64_t per_request = (int64_t)std::max(1, std::min(max_new, N)) * (heads / cache->kv_heads);
+  const int new_each = std::max(1, std::min(max_new, N));
+  const int64_t per_request = (int64_t)new_each * (heads / cache->kv_heads);
   const bool wide = per_request > 32;
   const int rows = wide ? 128 : (cache->dtype == MIMO_KV_E4M3_BLOCKS && per_request <= 16 ? 16 : 32);
   at_tiles(rows, N, heads, cache->kv_heads, a);
   a.target = wide ? AT_WIDE_TARGET : AT_NARROW_TARGET;
   // no tile can walk more units than the table or the window holds; where none has to be split there is no second launch
   const int most = at_most(max_pages * cache->page_size, window, a.sinks, a.TQ, wide ? 64 : 128);
-  const bool full = N * a.Hh >= (window ? a.target / 2 : a.target);
+  // a tile of 16 rows holds a request's new tokens, so with new_each of them a request there are this many tiles, if no rows are
+  // padding (at most B requests have any)
+  const int tiles = std::min(B, (N + new_each - 1) / new_each) * a.Hh, queries = (int)std::min<int64_t>(N, (int64_t)B * new_each) * a.Hh;
+  const bool full = queries >= (window ? a.target / 2 : a.target) && tiles >= a.target / 4;
   const bool join = most > (wide ? AT_WIDE_MIN : rows == 32 ? AT_NARROW_MIN : full ? AT_FULL_MIN : AT_FEW_MIN);
   const AtRoom room = at_room(rows, a.target, N, heads, cache->kv_heads, cache->v_dim);
   char* w = static_cast<char*>(ws);
