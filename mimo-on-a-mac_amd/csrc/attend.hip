@@ -177,7 +177,8 @@ template <class F> __device__ __forceinline__ float at_swap16(float x, F f) {
 }
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// eight E4M3 codes times a power of two to bf16, exact
+// eight E4M3 codes times a power of two to bf16: exact, subnormal results too, but for what lies between their steps of 2^-133 (under
+// block scales of bytes 1 and 2), which is rounded
 __device__ __forceinline__ bf16x8 at_f8_bf16x8(uint32_t a, uint32_t b, float by) {
   const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, true);
   const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, true);

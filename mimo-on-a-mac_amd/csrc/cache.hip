@@ -559,8 +559,9 @@ __global__ void __launch_bounds__(256, 4) cache_append_scaled_kernel(AppendArgs 
 }
 
 // ------------------------------------------------------------------ read
-// Cached tokens as bf16 rows: code times scale in 32 bits, rounded to bf16 (with block scales exact).  A thread turns 8 values; a block of
-// 256 a few tokens one after another, whose rows of a head share cache lines.
+// Cached tokens as bf16 rows: code times scale in 32 bits, rounded to bf16 (with block scales exact, but for products below bf16's
+// least step of 2^-133, which bytes 1 and 2 have).  A thread turns 8 values; a block of 256 a few tokens one after another, whose
+// rows of a head share cache lines.
 //
 // Bound by HBM: 32768 tokens of 4 heads of 192/128 with block scales (126 MB) 23.4 us a call, 5.4 TB/s; the rows are written past
 // the caches (31.0 us through them, call after call into the same rows; into rows that are new each time 24.1 and 25.0).  The
