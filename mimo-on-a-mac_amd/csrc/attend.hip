@@ -652,9 +652,6 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
       if (f + AHEAD < F) X[f % AHEAD] = read(f + AHEAD);
     }
     __builtin_amdgcn_sched_barrier(0);
-    // these products run 16 passes; the sums are read no sooner than 20 wait states after the last
-    asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
   };
   auto scores = [&](const uint8_t* st) __attribute__((always_inline)) {
     if constexpr (C::QP) return scores_of_codes(st);
