@@ -92,13 +92,13 @@ constexpr int AT_THREADS = 256;
 constexpr int AT_WIDE_TARGET = 512, AT_NARROW_TARGET = 512;
 // Parts of wide tiles have at least 4 units of 64 keys: 40 tokens of 32/8 heads at 3000 21.7 us; 27.3 with 2, 24.9 with 8.
 // Narrow tiles of up to 2 units of 128 keys (a window of 128) are not split, which saves the join's launch.
-// Those of 16 rows neither up to 4 units (32 requests of 300 to 380 keys, 64/8 heads, 15.3 us split and 11.0 whole, one of 500 10.4
-// and 11.0, one of 1000 10.5 and 16.7), and up to 8 where there are 512 tokens times K/V heads, or 256 in a window, where as a rule
-// all tiles are full: 64 of 500 to 1000 36.9 and 28.8, 32 in a window of 512 17.6 and 13.8.  128 of 30 to 50 and one of 1000, 32/8
-// heads, 20.7 and 21.9; with 32 requests, 64/8 heads, it would be 11.4 and 16.5 (but all of 600 to 1000 22.1 and 17.9).  Where
-// tiles hold several tokens they have to be 128 at least: 8 requests of 16 new tokens at 800 to 1024 keys, 4/4 heads of 64, 32
-// tiles, 9.9 split and 12.8 whole, in a window of 512 11.0 and 11.3 (heads of 128); 32 of 4 tokens at 500 to 1024, 16/4 heads, 128
-// tiles, 16.7 and 15.6; 64 of them, 256 tiles, 21.5 and 16.3.
+// Those of 16 rows neither up to 4 units (32 requests of 300 to 380 keys, 64/8 heads, 15.3 us split and 11.0 whole, one of
+// 500 10.4 and 11.0, one of 1000 10.5 and 16.7), and up to 8 where there are 512 tokens times K/V heads, or 256 in a window,
+// where as a rule all tiles are full: 64 of 500 to 1000 36.9 and 28.8, 32 in a window of 512 17.6 and 13.8.  128 of 30 to 50
+// and one of 1000, 32/8 heads, 20.7 and 21.9; with 32 requests, 64/8 heads, it would be 11.4 and 16.5 (but all of 600 to 1000
+// 22.1 and 17.9).  Where tiles hold several tokens they have to be 128 at least: 8 requests of 16 new tokens at 800 to 1024
+// keys, 4/4 heads of 64, 32 tiles, 9.9 split and 12.8 whole, in a window of 512 11.0 and 11.3 (heads of 128); 32 of 4 tokens
+// at 500 to 1024, 16/4 heads, 128 tiles, 16.7 and 15.6; 64 of them, 256 tiles, 21.5 and 16.3.
 constexpr int AT_WIDE_MIN = 4, AT_NARROW_MIN = 2, AT_FEW_MIN = 4, AT_FULL_MIN = 8;
 constexpr int AT_START = 8;                               // units that a wide block's start and a part's join cost
 
@@ -144,7 +144,8 @@ __device__ __forceinline__ void at_copy16(const uint8_t* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory", "m0");
 }
 // The same from src (wave-uniform) + at, + 64 and so on, CB times, to places 2048 bytes apart.  An instruction's offset counts
-// for both addresses.  The first wait is for src too: a vector instruction that wrote it (a readlane) has to be 5 wait states back.
+// for both addresses.  The first wait is for src too: a vector instruction that wrote it (a readlane) has to be 5 wait states
+// back.
 template <int CB> __device__ __forceinline__ void at_copies16(const uint8_t* src, uint32_t at, uint32_t lds) {
   static_assert(CB >= 1 && CB <= 3);
   const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
@@ -177,8 +178,8 @@ template <class F> __device__ __forceinline__ float at_swap16(float x, F f) {
 }
 __device__ __forceinline__ float at_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// eight E4M3 codes times a power of two to bf16: exact, subnormal results too, but for what lies between their steps of 2^-133 (under
-// block scales of bytes 1 and 2), which is rounded
+// eight E4M3 codes times a power of two to bf16: exact, subnormal results too, but for what lies between their steps of
+// 2^-133 (under block scales of bytes 1 and 2), which is rounded
 __device__ __forceinline__ bf16x8 at_f8_bf16x8(uint32_t a, uint32_t b, float by) {
   const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, by, true);
   const bf16x2 z = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, false), w = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, by, true);
@@ -494,11 +495,11 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
     }
   }
   bf16x8 Q[C::QP ? 1 : C::DK / 16];
-  // Wide, block scales: E4M3 products with scales (v_mfma_scale_f32_32x32x64_f8f6f4), whose K operand is the cache's codes and bytes as
-  // they are: 4096 tokens at 8192, 64/4 heads of 192/128 1611 us, 1721 with K turned into bf16 by every wave.  (Narrow tiles would
-  // wait for the planes: 128 windowed decodes 29.0 us instead of 23.5.)  q is two planes of E4M3, Qp[0] and Qp[1], the second what the first's rounding leaves, times 16: 8 bits in all,
-  // bf16's own, for values down to 2^-13 of the largest of their 64 dimensions (smaller ones are off by up to 2^-21 of that).
-  // q_by: bytes of the planes' scales.
+  // Wide, block scales: E4M3 products with scales (v_mfma_scale_f32_32x32x64_f8f6f4), whose K operand is the cache's codes
+  // and bytes as they are: 4096 tokens at 8192, 64/4 heads of 192/128 1611 us, 1721 with K turned into bf16 by every wave.
+  // (Narrow tiles would wait for the planes: 128 windowed decodes 29.0 us instead of 23.5.)  q is two planes of E4M3, Qp[0]
+  // and Qp[1], the second what the first's rounding leaves, times 16: 8 bits in all, bf16's own, for values down to 2^-13 of
+  // the largest of their 64 dimensions (smaller ones are off by up to 2^-21 of that). q_by: bytes of the planes' scales.
   v8i Qp[2][C::QP ? C::KCB : 1];
   int q_by[C::QP ? C::KCB : 1];
   bool q_odd = false;                                      // infinities or NaN: these planes do not hold them apart
@@ -1687,8 +1688,9 @@ int mimo_cache_attend(const uint16_t* q, int64_t q_stride, int N, int heads, con
   a.k_scale = cache->k_scale, a.v_scale = cache->v_scale, a.sink_logits = sink_logits;
   a.scale = scale, a.out = out, a.status = status;
   // narrow tiles hold the rows of a request in 32, wide ones are up to a quarter filled: at 5 to 8 rows of 8 heads the wide
-  // ones take 132-136 us for 32 requests of 4000 keys, two and more narrow tiles 136-139, and at 12 143 against 356.  Over block scales those of up to 16 rows have tiles of 16 (at_tile16), which also at 16 rows, 16 heads of 192/128 at 300
-  // keys, took 11.0 us against 12.1
+  // ones take 132-136 us for 32 requests of 4000 keys, two and more narrow tiles 136-139, and at 12 143 against 356.  Over
+  // block scales those of up to 16 rows have tiles of 16 (at_tile16), which also at 16 rows, 16 heads of 192/128 at 300 keys,
+  // took 11.0 us against 12.1
   // (never 0, whatever max_new says: a K/V head's queries have to fit tiles of 16, which know no groups of them)
   const int new_each = std::max(1, std::min(max_new, N));
   const int64_t per_request = (int64_t)new_each * (heads / cache->kv_heads);

@@ -167,7 +167,8 @@ __global__ void __launch_bounds__(256) cache_commit_kernel(const int32_t* from, 
 // ------------------------------------------------------------------ append
 // Bound by HBM for many tokens, by its launch for few.  4096 tokens of 64 q and 8 K/V heads (243 MB) 52 us, 4.7 TB/s, a large
 // copy's rate (39.4 us again and again on the same rows, which the last-level cache holds in part); 1777 tokens into E4M3 10.1
-// us (4 TB/s: 7 blocks on a CU in all, the start counts); 64 tokens 3.5 us.  One pass: q, k and v are read and written once, in 16-byte pieces (a pair of them where they rotate).
+// us (4 TB/s: 7 blocks on a CU in all, the start counts); 64 tokens 3.5 us.  One pass: q, k and v are read and written once,
+// in 16-byte pieces (a pair of them where they rotate).
 //
 // Angles are pos * turn_i turns in 64 bits (a position of 131072 times a first frequency of 1 / 2 pi leaves 32 bits with
 // no useful fraction), reduced to a fraction of a turn before the 32-bit sine and cosine; one rotation is
