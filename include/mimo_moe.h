@@ -252,7 +252,7 @@ typedef struct mimo_kv_cache {
  * of the step), slots [N] and positions [N] of the new tokens, rows behind the last one -1 and 0.  table entries of grown
  * requests and stack entries at and above n_free are written in place; they mean nothing under the old lengths, so a step
  * whose outputs are dropped leaves the state as it was (not what the cache holds, if new tokens were written: pages that one
- * request gives back are the first that others take in the same step).  commit_lens / commit_n_free (both or neither; lens
+ * request gives back are the first that others take in the same step, and block scales that new tokens raised stay raised).  commit_lens / commit_n_free (both or neither; lens
  * and n_free themselves, as a rule) receive the new lengths and count after everything else.  status [1] is overwritten: MIMO_OK,
  * MIMO_ERR_PAGES when too few pages are free, MIMO_ERR_SHAPE when a length is outside [0, max_pages * page_size] (at most
  * 2^31 - 2^16), a request grows by more than max_new, the new tokens are more than N (at most 2^20) or n_free and the lengths
@@ -264,11 +264,11 @@ int mimo_cache_step(const int32_t* lens, const int32_t* target, int B, int32_t* 
 
 /* Rotary positions on q and k (the first rotary_dim dimensions of a head, pairs (i, i + rotary_dim / 2); the reference's
  * partial RoPE, engine/mimo_stream/mimo_v2.py:66-150) and the write of k and v to their slots.  N is below 2^24.  q bf16
- * [N, heads, k_dim] (NULL: none), k [N, kv_heads, k_dim], v [N, kv_heads, v_dim], tokens *_stride elements apart (multiples of 8); turns fp64
- * [rotary_dim / 2]: turns per position of each pair (frequency / 2 pi).  q_out bf16 [N, heads, k_dim] may not overlap q, k
- * or v.  A slot below 0 writes no k and v; slots are distinct otherwise.  Rotated values are rounded once, to bf16 or (divided by their
- * head's scale, clamped to +-448) to E4M3.  status (optional) receives MIMO_ERR_SLOT for a slot past the cache, which is
- * skipped; it is not cleared. */
+ * [N, heads, k_dim] (NULL: none), k [N, kv_heads, k_dim], v [N, kv_heads, v_dim], tokens *_stride elements apart (multiples
+ * of 8); turns fp64 [rotary_dim / 2]: turns per position of each pair (frequency / 2 pi).  q_out bf16 [N, heads, k_dim] may
+ * not overlap q, k or v.  A slot below 0 writes no k and v; slots are distinct otherwise.  Rotated values are rounded once,
+ * to bf16 or (divided by their head's scale, clamped to +-448) to E4M3.  status (optional) receives MIMO_ERR_SLOT for a slot
+ * past the cache, which is skipped; it is not cleared. */
 int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k, int64_t k_stride,
                       const uint16_t* v, int64_t v_stride, int N, const int32_t* positions, const int32_t* slots,
                       const mimo_kv_cache* cache, int rotary_dim, const double* turns, uint16_t* q_out,
@@ -277,10 +277,11 @@ int mimo_cache_append(const uint16_t* q, int64_t q_stride, int heads, const uint
 /* mimo_cache_append with the rotation in full (NULL: none): pairs (i, i + dim / 2), or (2 i, 2 i + 1) where interleaved is 1;
  * turns fp64 [dim / 2] as above (a host may stretch them for long contexts); rotated values times magnitude (finite; 1: as
  * they are).  Into a cache with block scales (either entry; N up to 2^23 - 17): the rows of one block of 16 slots have to
- * follow one another, as a step lays a request's tokens, with no other row between them, not even one of a slot below 0.  A call that writes a block's first slot begins the block anew,
- * whatever it held; else its byte grows if the new values need it, and what the block held is kept, in the new scale.  Values
- * past 448 * 2^119 saturate.  If a block's rows do not stand together, or one slot comes twice, that block's contents are
- * undefined, and nothing else is touched; status receives MIMO_ERR_SLOT where 15 or fewer rows lie between. */
+ * follow one another, as a step lays a request's tokens, with no other row between them, not even one of a slot below 0.  A
+ * call that writes a block's first slot begins the block anew, whatever it held; else its byte grows if the new values need
+ * it, and what the block held is kept, in the new scale.  Values past 448 * 2^119 saturate.  If a block's rows do not stand
+ * together, or one slot comes twice, that block's contents are undefined, and nothing else is touched; status receives
+ * MIMO_ERR_SLOT where 15 or fewer rows lie between. */
 typedef struct mimo_rotary {
   const double* turns;
   int32_t dim, interleaved;
@@ -292,9 +293,10 @@ int mimo_cache_append_rotary(const uint16_t* q, int64_t q_stride, int heads, con
                              void* stream);
 
 /* Cached tokens back as rows: k_out bf16 [N, kv_heads, k_dim] and v_out [N, kv_heads, v_dim], row n from slots[n] (in any order,
- * any slot any number of times), code times scale in 32 bits, rounded to bf16; a slot below 0 gives a row of 0.  The outputs may not overlap
- * the cache, its scales, the slots or one another.  N is below 2^24.  status (optional, not cleared) receives MIMO_ERR_SLOT for a slot past
- * the cache, whose row is 0.  (The reference slices its cache arrays, engine/mimo_stream/mimo_v2.py:110-150.) */
+ * any slot any number of times), code times scale in 32 bits, rounded to bf16; a slot below 0 gives a row of 0.  The outputs
+ * may not overlap the cache, its scales, the slots or one another.  N is below 2^24.  status (optional, not cleared) receives
+ * MIMO_ERR_SLOT for a slot past the cache, whose row is 0.  (The reference slices its cache arrays,
+ * engine/mimo_stream/mimo_v2.py:110-150.) */
 int mimo_cache_read(const mimo_kv_cache* cache, const int32_t* slots, int N, uint16_t* k_out, uint16_t* v_out,
                     int32_t* status, void* stream);
 
@@ -322,9 +324,9 @@ size_t mimo_cache_attend_workspace_size(int N, int heads, int kv_heads, int v_di
 /* No counterpart in the reference: per-kernel timing for benchmarks.  While enabled, every kernel launch is
  * followed by a HIP event on its stream; the kernel's time runs from the previous kernel's event of the same
  * entry-point call (or from an event recorded just before it, for the first kernel of a call) to its own, so
- * back-to-back kernels add one event record each.  mimo_profile_enable also clears the records.  mimo_profile_read synchronises on the recorded events and returns the number of distinct
- * kernel names; for the first max_kernels of them it writes the name (64 bytes each, NUL-terminated, host
- * buffer), the total milliseconds and the launch count (host arrays). */
+ * back-to-back kernels add one event record each.  mimo_profile_enable also clears the records.  mimo_profile_read
+ * synchronises on the recorded events and returns the number of distinct kernel names; for the first max_kernels of them it
+ * writes the name (64 bytes each, NUL-terminated, host buffer), the total milliseconds and the launch count (host arrays). */
 int mimo_profile_enable(int on);
 int mimo_profile_read(int max_kernels, char* names, float* total_ms, int* launches);
 

@@ -139,9 +139,11 @@ class PageTable:
         n_tokens: rows of the step, at least the sum of new tokens (more: the rows behind are padding); max_new: at most
         this many new tokens on one request (default n_tokens).  With commit=False the page table keeps its lengths and
         free pages, and the step can be dropped or made again; after an append only if it gave no pages back (a request's
-        pages that end in a step are the first that others take in it, and then hold their tokens).  Returns a StepPlan; a
-        failure (too few free pages, lengths out of range) leaves the state as it was and is in plan.status (plan.check()
-        raises)."""
+        pages that end in a step are the first that others take in it, and then hold their tokens).  In a cache with block
+        scales an appended token leaves a trace even if its step is dropped or it is taken back: where it raised the scale of
+        a block of 16 slots that older tokens share, these stay rounded to that scale's steps, and later tokens of the block
+        get it too (KVCache).  Returns a StepPlan; a failure (too few free pages, lengths out of range) leaves the state as
+        it was and is in plan.status (plan.check() raises)."""
         if not 0 <= n_tokens <= 1 << 20 or (max_new is not None and not 0 <= max_new <= INT32_MAX):
             raise ValueError(f"n_tokens must be from 0 to 2^20 and max_new from 0 to 2^31 - 1 (got {n_tokens}, {max_new})")
         dev = self._lens.device
@@ -195,7 +197,11 @@ class KVCache:
     float8_e4m3fn with one fp32 scale per K/V head, k_scale and v_scale (a stored value stands for value * scale), which a
     user has to know beforehand: what is past 448 scales saturates;
     float8_e4m3fn with block_scales: k_scale and v_scale are bytes [n_pages, kv_heads, page_size / 16], and a value of a slot
-    stands for value * 2 ** (byte - 127).  append sets a block's byte by the values that it writes (mimo_stream.append)."""
+    stands for value * 2 ** (byte - 127).  append sets a block's byte by the values that it writes (mimo_stream.append); a
+    byte only grows until the block begins anew.  So what a request reads may depend on tokens that were rejected: a draft
+    whose values raised its block's byte has rounded the older tokens' values below 2 ** -6 of the new scale to 2 ** -9 of it,
+    and its byte stays when its step is dropped or its tokens are taken back, for the tokens that take their place as well.
+    A request whose length is taken back to the block's first slot, or before it, writes the block anew."""
 
     def __init__(self, n_pages, page_size, kv_heads, k_dim, v_dim, dtype=torch.bfloat16, k_scale=None, v_scale=None,
                  device="cuda", block_scales=False):

@@ -1,10 +1,10 @@
-"""append into a cache with block scales: what it reports of rows that do not stand together, and values that are not finite in
-blocks that several waves share."""
+"""append into a cache with block scales: what it reports of rows that do not stand together, and what drafts leave behind that are
+dropped."""
 import numpy as np
 import pytest
 import torch
 
-from mimo_stream import KVCache, StepPlan, append, read
+from mimo_stream import KVCache, PageTable, StepPlan, append, read
 
 pytestmark = pytest.mark.gpu
 
@@ -48,3 +48,35 @@ def test_a_parted_block_is_reported(N, piece):
                 order[first + piece + gap + 1:first + 64] = -1
             assert (status(order) != 0) == (gap > 0), (first, gap)
     assert (read(cache, i32(np.arange(16, 31)))[0] == 1.0).all()
+
+
+def test_a_dropped_step_leaves_its_scale(rng):
+    """Drafts of a step that is not committed: the lengths stay, the scale that the drafts raised too, with the older rows rounded to
+    it; a cache with a scale for each head holds what it held."""
+    old, new = (torch.from_numpy(rng.standard_normal((n, 1, 64)).astype(np.float32)).to(BF).cuda() for n in (5, 2))
+
+    def after(cache):
+        pt = PageTable(1, 1, 1, 16)
+        append(cache, pt.step(i32([5]), 5), old, old)
+        before = cache.k.view(torch.uint8).clone()
+        plan = pt.step(i32([7]), 2, commit=False)
+        append(cache, plan, new * 1024, new * 1024)
+        plan.check()
+        assert pt.lens.item() == 5
+        return before[0, 0, :5].cpu().view(E4M3), cache.k[0, 0, :5].cpu(), pt
+    cache = KVCache(1, 16, 1, 64, 64, dtype=E4M3, k_scale=1.0, v_scale=1.0)
+    before, now, _ = after(cache)
+    assert torch.equal(before.view(torch.uint8), now.view(torch.uint8))
+    cache = KVCache(1, 16, 1, 64, 64, dtype=E4M3, block_scales=True)
+    first = KVCache(1, 16, 1, 64, 64, dtype=E4M3, block_scales=True)
+    append(first, StepPlan(slots=i32(np.arange(5)), positions=i32(np.arange(5))), old, old)
+    before, now, pt = after(cache)
+    grown = cache.k_scale.item() - first.k_scale.item()
+    assert grown > 5 and torch.equal((before.float() * 2.0 ** -grown).to(E4M3).view(torch.uint8), now.view(torch.uint8))
+    # later tokens of the block have that scale too; a request that begins again has its own
+    top = cache.k_scale.item()
+    append(cache, pt.step(i32([6]), 1), old[:1], old[:1])
+    assert cache.k_scale.item() == top
+    pt.step(i32([0]), 0)
+    append(cache, pt.step(i32([5]), 5), old, old)
+    assert torch.equal(cache.k_scale, first.k_scale) and torch.equal(cache.k[0, 0, :5].view(torch.uint8), first.k[0, 0, :5].view(torch.uint8))
