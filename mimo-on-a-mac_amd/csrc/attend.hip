@@ -40,12 +40,12 @@
 // of 64, which have the room, 0.59 against 0.70); row sums by a matrix product, operands read further ahead, wave priorities:
 // no change.  Heads of 64: the exponentials (16 cycles for 64 of them) and what is around them, 0.66-0.70 PFLOP/s.
 // No vector register is spilled; 9 to 20 (wide) and 56 to 81 (narrow) scalar ones are, to lanes of a vector register.
-// Block scales: the same chunk 1582-1616 us where a head's scales take 1649 and K turned into bf16 by every wave 1721 (on another
-// card 1678); chunks of heads of 64 in a window of 1111, 24 requests, 54 us (51 with a head's scales).
+// Block scales: the same chunk 1530-1560 us (1721 with K turned into bf16 by every wave, where the planes of q took 1598); chunks of
+// heads of 64 in a window of 1111, 24 requests, 51 us in a row, 53 on three sets of tensors (49 and 51 with a head's scales).
 // Narrow: HBM.  48 requests of 500 to 16384 keys (1.03 GB) 187 us, 5.5 TB/s; 32 of 1000 to 32768 in E4M3 (1.13 GB) 206 us, 5.4
 // TB/s, above a large copy's 4.9 (read and written); a call of few keys 9 us, a chain of round trips (starts and lengths,
 // the table, K and V, the waves' parts through LDS).  Block scales: 48 requests of 500 to 16384 keys, 32/8 heads of 128 (825 MB)
-// 153 us, 5.4 TB/s (157 with a head's scales, in tiles of 32 rows), one of 32768 17.4 (20.1), 128 in a window of 128 18.6 (22.5):
+// 152 us, 5.4 TB/s (157 with a head's scales, in tiles of 32 rows), one of 32768 17.0 (20.1), 128 in a window of 128 18.2 (22.5):
 // of this, 2.2 us are the blocks' start, 3 the work's search, and each of two tiles takes 2-3 for its first keys, 3 for two
 // steps and 1.2 to join.
 #include <algorithm>
@@ -496,10 +496,10 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
   }
   bf16x8 Q[C::QP ? 1 : C::DK / 16];
   // Wide, block scales: E4M3 products with scales (v_mfma_scale_f32_32x32x64_f8f6f4), whose K operand is the cache's codes
-  // and bytes as they are: 4096 tokens at 8192, 64/4 heads of 192/128 1611 us, 1721 with K turned into bf16 by every wave.
+  // and bytes as they are: 4096 tokens at 8192, 64/4 heads of 192/128 1598 us, 1721 with K turned into bf16 by every wave.
   // (Narrow tiles would wait for the planes: 128 windowed decodes 29.0 us instead of 23.5.)  q is two planes of E4M3, Qp[0]
   // and Qp[1], the second what the first's rounding leaves, times 16: 8 bits in all, bf16's own, for values down to 2^-13 of
-  // the largest of their 64 dimensions (smaller ones are off by up to 2^-21 of that). q_by: bytes of the planes' scales.
+  // the largest of their 64 dimensions (smaller ones are off by up to 2^-21 of that).  q_by: bytes of the planes' scales.
   v8i Qp[2][C::QP ? C::KCB : 1];
   int q_by[C::QP ? C::KCB : 1];
   bool q_odd = false;                                      // infinities or NaN: these planes do not hold them apart
@@ -976,8 +976,8 @@ __device__ __forceinline__ void at_tile(const AttendArgs& a, uint8_t* lds, const
 // the products, of the softmax and of the registers empty.  S^T = K Q^T: lane (c, g) = (l % 16, l / 16) holds, for query row c,
 // keys 4 g + i of each of the wave's two groups of 16, whose scales are one number each; P^T, as it stands, is the B operand of
 // the 32 keys in the order (g, group, i), in which the transposing reads of V fetch them.
-// One request of 32768 keys, 64/4 heads of 192/128, 17.4 us, 48 of 500 to 16384, 32/8 of 128, 153, 128 in a window of 128, 64/8 of
-// 192/128, 18.6, one of 40, 8/2 of 64, 5.3.  In tiles of 32 rows these took 20.9, 159, 23.4 and 6.8, where the first tiles of 16
+// One request of 32768 keys, 64/4 heads of 192/128, 17.0 us, 48 of 500 to 16384, 32/8 of 128, 152, 128 in a window of 128, 64/8 of
+// 192/128, 18.2, one of 40, 8/2 of 64, 5.3.  In tiles of 32 rows these took 20.9, 159, 23.4 and 6.8, where the first tiles of 16
 // took 19.1, 155, 20.5 and 6.0.  Beside those the first three took, with more blocks a CU, 3: 20.6, 159, 21.5; 4: 26.5, 199, 27.7
 // (spills, whose loads wait for the copies too); with a second tile on its way 20.1, 162, 20.5; with operands read 2 instead of
 // 4 ahead 19.3, 156, 20.6; blocks of 6 waves 19.5, 158 and 27.6 (two do not fit on a CU).

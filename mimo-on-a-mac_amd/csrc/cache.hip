@@ -331,7 +331,8 @@ __global__ void __launch_bounds__(256) cache_append_kernel(AppendArgs a) {
 // One launch with the q rows, whose HBM time covers it: 4096 tokens of 64/8 heads (233 MB) 43.8 us, 5.3 TB/s, 37 without K and
 // V and 12 without q.  1687 tokens in pieces of 24 prompts, 32/8 heads 14.1 us (8.2 and 12.6): 130 blocks of slots for each of
 // 8 heads are a chain of round trips (slots, rows, stores), angles in 64 bits and the starts of 3400 blocks.  64 decoded tokens
-// 4.5 us.
+// 4.5 us (these times are of the same tensors again and again; on three sets in turn 45.2, 15.4 and 5.2), also where every one of
+// them raises its block's scales.
 constexpr int SB_SHIFT = 4, SB_ROWS = 1 << SB_SHIFT;       // slots that share a scale
 constexpr int SB_TOP = 246;
 // Blocks that look for work: each is given as few rows as that leaves (1687 tokens in pieces of 24 prompts 14.1 us; 1024
