@@ -282,9 +282,9 @@ def stretched(dim, theta, factor, original, few=1.0, many=32.0):
     turns has it divided by factor, and those between are blended in proportion to i, from the last whole pair number of
     `many` turns (0 at least) to the first of `few` (dim - 1 at most, past the last pair: where even that one turns more than
     `few` times, none is divided by the whole factor)."""
-    if dim < 2 or dim % 2 or not theta > 1.0 or not factor > 0.0 or not original > 0 or not 0.0 < few < many:
-        raise ValueError(f"need an even dim, theta > 1, factor > 0, original > 0 and 0 < few < many (got {dim}, {theta}, {factor}, "
-                         f"{original}, {few}, {many})")
+    if dim < 2 or dim % 2 or not 1.0 < theta < math.inf or not 0.0 < factor < math.inf or not 0 < original < math.inf or not 0.0 < few < many < math.inf:
+        raise ValueError(f"need an even dim, theta > 1, factor > 0, original > 0 and 0 < few < many, all finite (got {dim}, {theta}, "
+                         f"{factor}, {original}, {few}, {many})")
     i = torch.arange(dim // 2, dtype=torch.float64)
     freq = float(theta) ** (-2.0 * i / dim)
     # pair i turns original theta ** (-2 i / dim) / 2 pi times

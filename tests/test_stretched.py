@@ -56,6 +56,12 @@ def test_no_pair_of_few_turns_keeps_its_own(original):
         assert np.allclose(got, 0.25, rtol=1e-14, atol=0)
 
 
+@pytest.mark.parametrize("name", ["theta", "factor", "original", "many"])
+def test_numbers_without_an_end_are_refused(name):
+    with pytest.raises(ValueError, match="finite"):
+        stretched(**{**dict(dim=16, theta=10000.0, factor=2.0, original=4096), name: float("inf")})
+
+
 def test_between_few_and_many_from_pair_0_on():
     """theta 16, dim 16: 100 tokens are 15.9 turns of pair 0 and n(1) = 7.98, so pairs 0 to 7 of 8."""
     for got in both(16, 16.0, 4.0, 100):
