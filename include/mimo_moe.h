@@ -252,11 +252,12 @@ typedef struct mimo_kv_cache {
  * of the step), slots [N] and positions [N] of the new tokens, rows behind the last one -1 and 0.  table entries of grown
  * requests and stack entries at and above n_free are written in place; they mean nothing under the old lengths, so a step
  * whose outputs are dropped leaves the state as it was (not what the cache holds, if new tokens were written: pages that one
- * request gives back are the first that others take in the same step, and block scales that new tokens raised stay raised).  commit_lens / commit_n_free (both or neither; lens
- * and n_free themselves, as a rule) receive the new lengths and count after everything else.  status [1] is overwritten: MIMO_OK,
- * MIMO_ERR_PAGES when too few pages are free, MIMO_ERR_SHAPE when a length is outside [0, max_pages * page_size] (at most
- * 2^31 - 2^16), a request grows by more than max_new, the new tokens are more than N (at most 2^20) or n_free and the lengths
- * disagree; then starts are 0, slots -1, and lens_out / n_free_out the old state. */
+ * request gives back are the first that others take in the same step, and block scales that new tokens raised stay raised).
+ * commit_lens / commit_n_free (both or neither; lens and n_free themselves, as a rule) receive the new lengths and count
+ * after everything else.  status [1] is overwritten: MIMO_OK, MIMO_ERR_PAGES when too few pages are free, MIMO_ERR_SHAPE when
+ * a length is outside [0, max_pages * page_size] (at most 2^31 - 2^16), a request grows by more than max_new, the new tokens
+ * are more than N (at most 2^20) or n_free and the lengths disagree; then starts are 0, slots -1, and lens_out / n_free_out
+ * the old state. */
 int mimo_cache_step(const int32_t* lens, const int32_t* target, int B, int32_t* table, int max_pages,
                     int32_t* free_pages, const int32_t* n_free, int n_pages, int page_size, int N, int max_new,
                     int32_t* lens_out, int32_t* n_free_out, int32_t* starts, int32_t* slots, int32_t* positions,

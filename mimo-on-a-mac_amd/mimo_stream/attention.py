@@ -348,7 +348,8 @@ class Rotary:
 
     def __setstate__(self, state):
         state = dict(state)
-        self._bind(state.pop("turns"), state.pop("dim"), state.pop("interleaved", False), state.pop("magnitude", 1.0))
+        if "turns" in state and "dim" in state:              # a derived class may work them out instead
+            self._bind(state.pop("turns"), state.pop("dim"), state.pop("interleaved", False), state.pop("magnitude", 1.0))
         self.__dict__.update(state)
 
 

@@ -54,6 +54,21 @@ def test_a_derived_one_is_copied_whole(again):
     assert r.factor == 4.0 and r.dim == 32 and torch.equal(r.turns, Rotary(32, device="cpu").turns / 4.0)
 
 
+class Worked(Rotary):
+    """Has no numbers of its own: they are worked out from a factor."""
+    def __init__(self, factor):
+        self.factor = factor
+    dim = property(lambda self: 32)
+    turns = property(lambda self: Rotary(32, device="cpu").turns / self.factor)
+
+
+@pytest.mark.parametrize("again", [copy.copy, copy.deepcopy, lambda r: pickle.loads(pickle.dumps(r))])
+def test_a_derived_one_without_numbers_is_copied(again):
+    r = again(Worked(2.0))
+    s, turns = _turns_of(r, CPU, 64)
+    assert r.factor == 2.0 and s.turns == turns.data_ptr() and torch.equal(turns, Rotary(32, device="cpu").turns / 2.0)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["bf16", "blocks"])
 def test_append_takes_them(rng, kind):
