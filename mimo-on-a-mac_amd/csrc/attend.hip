@@ -40,7 +40,7 @@
 // of 64, which have the room, 0.59 against 0.70); row sums by a matrix product, operands read further ahead, wave priorities:
 // no change.  Heads of 64: the exponentials (16 cycles for 64 of them) and what is around them, 0.66-0.70 PFLOP/s.
 // No vector register is spilled; 9 to 20 (wide) and 56 to 81 (narrow) scalar ones are, to lanes of a vector register.
-// Block scales: the same chunk 1530-1560 us (1721 with K turned into bf16 by every wave, where the planes of q took 1598); chunks of
+// Block scales: the same chunk 1519-1563 us (1721 with K turned into bf16 by every wave, where the planes of q took 1598); chunks of
 // heads of 64 in a window of 1111, 24 requests, 51 us in a row, 53 on three sets of tensors (49 and 51 with a head's scales).
 // Narrow: HBM.  48 requests of 500 to 16384 keys (1.03 GB) 187 us, 5.5 TB/s; 32 of 1000 to 32768 in E4M3 (1.13 GB) 206 us, 5.4
 // TB/s, above a large copy's 4.9 (read and written); a call of few keys 9 us, a chain of round trips (starts and lengths,
